@@ -1,0 +1,499 @@
+// Attention of a batch's query tokens over a prefix that all of them see, in the 8-bit paged cache, on the 5th-generation tensor
+// cores: partial softmax states for attn_decode_q8.cu to join with each request's own tokens.
+//
+// The query rows of a KV head (requests x group, 128 to a block) are one operand for every key, so the prefix is read once per
+// block instead of once per request, and the work is bound by the products (4 rows tokens head_dim operations) as soon as there
+// are some ten requests. Items (KV head, block) times tiles of 64 tokens are a row of units that is cut evenly over the CTAs (two
+// to an SM); each leaves a piece per item.
+//
+//   warps 0-3   softmax: a thread per query row. They also bring their rows of Q into shared memory, as f16 with a power of two
+//               per row (see attn_decode_q8.cu).
+//   warp 4      tcgen05.mma: S(t+1) = Q K(t+1)^T is issued before P(t) is waited for; O += P(t) V(t) takes P from tensor memory
+//   warp 5, 6   keys / values: 8-bit numbers from their pages, a tile ahead in registers, to exact f16 in shared memory (128-byte
+//               swizzle; V stays token-major, an MN-major operand), and the tile's scales beside them
+//
+// Scores are S times the key's scale, in fp32. Weights are rounded to f16 times the value's scale relative to the largest one so
+// far, as in attn_decode_q8.cu; O is brought to a new reference where a row's maximum grows by 2^8 or that largest scale grows.
+#include "attn_q8.cuh"
+
+namespace nf {
+namespace {
+
+constexpr int kThreads = 224;
+constexpr int kTile = kPrefixTile;
+constexpr float kGap = 8.f, kHeadroom = 128.f;
+constexpr int kHalfBytes = kTile * 128;          // [64 tokens][64 elements]
+
+template <int HD>
+struct Pre {
+  static constexpr int NH = HD / 64;
+  static constexpr int kQ = 0;                                   // NH x [128 rows][64 elements]
+  static constexpr int kStage = NH * kHalfBytes;                 // a tile of K or V
+  static constexpr int kK = NH * 16384, kV = kK + 2 * kStage;
+  static constexpr int kScales = kV + 2 * kStage;                // [4 tiles][64] of keys, the same of values, [4] v_ref
+  static constexpr int kBars = kScales + 4 * kTile * 8 + 16;
+  static constexpr int kBytes = kBars + 256;
+};
+
+enum Bar : int {
+  Q_FULL = 0, K_FULL0, K_FULL1, K_EMPTY0, K_EMPTY1, V_FULL0, V_FULL1, V_EMPTY0, V_EMPTY1, S_FULL0, S_FULL1, P_FULL0, P_FULL1,
+  PV_DONE0, PV_DONE1, O_FREE, NUM_BARS
+};
+
+// MN-major operand in the 128-byte swizzle: 64 elements along N are one 128-byte row per k index, `lbo` bytes lead to the next 64,
+// `sbo` bytes to the next eight k indices.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16 |
+         static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
+}
+constexpr uint32_t kIdescBMnMajor = 1u << 16;
+// f16 x f16 -> fp32
+constexpr uint32_t idesc_f16(int m, int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24); }
+
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+// A CTA's share of the units, one item after the other.
+struct Share {
+  long long u, end;
+  int tiles, blocks;
+  int kvh, block, t0, n;     // the current part: tiles t0 .. t0 + n - 1 of item (kvh, block)
+  long long item;
+  __device__ __forceinline__ Share(const PrefixPlan& f, int kv_heads) {
+    const long long units = prefix_units(f, kv_heads);
+    u = range_begin(blockIdx.x, units, f.ctas);
+    end = range_begin(blockIdx.x + 1, units, f.ctas);
+    tiles = f.tiles;
+    blocks = f.blocks;
+  }
+  __device__ __forceinline__ bool next() {
+    if (u >= end) return false;
+    item = u / tiles;
+    t0 = static_cast<int>(u - item * tiles);
+    const long long left = end - u;
+    n = left < tiles - t0 ? static_cast<int>(left) : tiles - t0;
+    kvh = static_cast<int>(item / blocks);
+    block = static_cast<int>(item - static_cast<long long>(kvh) * blocks);
+    u += n;
+    return true;
+  }
+};
+
+// Keys (PART 0) or values (PART 1) of the CTA's tiles, by one warp.
+template <int HD, int KIND, int PART>
+__device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const PrefixPlan& f, uint32_t sb, float* scales, float* v_refs,
+                                            uint64_t* bars, volatile int* abort_flag) {
+  using C = Pre<HD>;
+  constexpr int LANES = HD / 16, AT_ONCE = 32 / LANES, NI = kTile / AT_ONCE;    // lanes of a token, tokens of a load, loads
+  const int lane = threadIdx.x & 31, c = lane % LANES, row = lane / LANES;
+  const uint8_t* pool = static_cast<const uint8_t*>(p.kv_pool);
+  const int n_pages = (p.prefix_len + kQ8Page - 1) / kQ8Page;
+  uint64_t* full = bars + (PART == 0 ? K_FULL0 : V_FULL0);
+  uint64_t* empty = bars + (PART == 0 ? K_EMPTY0 : V_EMPTY0);
+  uint4 raw[NI];
+  float sc[2];
+  // lane j < 4: the vectors of page j of the tile, -1 where there is none
+  auto page_of = [&](int kvh, int tile) {
+    long long at = -1;
+    const int slot = tile * (kTile / kQ8Page) + lane;
+    if (lane < kTile / kQ8Page && slot < n_pages) {
+      int page = p.prefix_pages[slot];
+      if (page < 0 || page >= p.num_pages) {
+        report_status(p.status, NF_ST_BAD_INDEX);
+        page = 0;
+      }
+      at = (static_cast<long long>(page) * 2 + PART) * p.kv_heads + kvh;
+    }
+    return at;
+  };
+  auto load = [&](int n, long long at) {
+    const int tok = n * AT_ONCE + row;
+    const long long head = __shfl_sync(0xffffffffu, at, tok / kQ8Page);
+    raw[n] = head < 0 ? make_uint4(0, 0, 0, 0)
+                      : *reinterpret_cast<const uint4*>(pool + (head * kQ8Page + tok % kQ8Page) * HD + c * 16);
+  };
+  auto load_scales = [&](long long at) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const long long head = __shfl_sync(0xffffffffu, at, 2 * k + lane / kQ8Page);
+      sc[k] = head < 0 ? 0.f : p.kv_scale[head * kQ8Page + lane % kQ8Page];
+    }
+  };
+  Share now(f, p.kv_heads), ahead = now;
+  int left = 0, tile_ahead = 0;                                  // the tile that is loaded next
+  auto advance = [&]() {                                         // false: none
+    if (left == 0) {
+      if (!ahead.next()) return false;
+      left = ahead.n;
+      tile_ahead = ahead.t0;
+    } else {
+      ++tile_ahead;
+    }
+    --left;
+    return true;
+  };
+  if (advance()) {
+    const long long at = page_of(ahead.kvh, tile_ahead);
+#pragma unroll
+    for (int n = 0; n < NI; ++n) load(n, at);
+    load_scales(at);
+  }
+  uint32_t g = 0;
+  while (now.next()) {
+    float v_ref = 7.8886091e-31f;                                // 2^-100
+    for (int t = 0; t < now.n; ++t, ++g) {
+      const int s = g & 1;
+      const int valid = p.prefix_len - (now.t0 + t) * kTile;     // tokens of the tile
+      const bool more = advance();
+      const long long at = more ? page_of(ahead.kvh, tile_ahead) : -1;
+      if (!__all_sync(0xffffffffu, wait_or_abort(&empty[s], ((g >> 1) & 1) ^ 1, abort_flag))) {
+        if (lane == 0) report_status(p.status, NF_ST_TIMEOUT_SMEM_EMPTY);
+        *abort_flag = 1;
+        return;
+      }
+      const uint32_t stage = sb + (PART == 0 ? C::kK : C::kV) + s * C::kStage;
+#pragma unroll
+      for (int n = 0; n < NI; ++n) {
+        const int tok = n * AT_ONCE + row;
+        uint32_t o[8];
+        q8_to_f16<KIND>(raw[n].x, o[0], o[1]);
+        q8_to_f16<KIND>(raw[n].y, o[2], o[3]);
+        q8_to_f16<KIND>(raw[n].z, o[4], o[5]);
+        q8_to_f16<KIND>(raw[n].w, o[6], o[7]);
+        // what lies behind the prefix may be anything: as values it would spoil every row (as keys it is masked)
+        if (PART == 1 && tok >= valid) o[0] = o[1] = o[2] = o[3] = o[4] = o[5] = o[6] = o[7] = 0u;
+        const uint32_t to = stage + (c >> 2) * kHalfBytes + tok * 128;
+        const uint32_t c0 = (2 * (c & 3)) ^ (tok & 7);
+        const bool swap = (c & 4) != 0;                          // the two halves' lanes on different banks
+        st_shared_v4(to + ((swap ? c0 ^ 1 : c0) << 4), swap ? o[4] : o[0], swap ? o[5] : o[1], swap ? o[6] : o[2], swap ? o[7] : o[3]);
+        st_shared_v4(to + ((swap ? c0 : c0 ^ 1) << 4), swap ? o[0] : o[4], swap ? o[1] : o[5], swap ? o[2] : o[6], swap ? o[3] : o[7]);
+        if (more) load(n, at);
+      }
+      float* dst = scales + (PART * 4 + (g & 3)) * kTile;
+      if (PART == 0) {
+        const float scale = p.sm_scale * kQ8Log2e;
+        dst[lane] = sc[0] * scale;
+        dst[lane + 32] = sc[1] * scale;
+      } else {
+        const float a = lane < valid ? sc[0] : 0.f, b = lane + 32 < valid ? sc[1] : 0.f;
+        float most = fmaxf(a, b);
+#pragma unroll
+        for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+        if (most > v_ref) v_ref = __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0xff800000u);   // the next power of two
+        const float unit = kHeadroom / v_ref;
+        dst[lane] = a * unit;
+        dst[lane + 32] = b * unit;
+        if (lane == 0) v_refs[g & 3] = v_ref;
+      }
+      if (more) load_scales(at);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&full[s]);
+    }
+  }
+}
+
+template <int HD, int KIND>
+__global__ void __launch_bounds__(kThreads, 2)
+attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, float* part_ml, float* part_o) {
+  using C = Pre<HD>;
+  constexpr int NH = C::NH;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sb = smem_u32(smem);
+  float* scales = reinterpret_cast<float*>(smem + C::kScales);
+  float* v_refs = scales + 8 * kTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NUM_BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  if ((sb & 1023u) != 0u) {                      // the operands' layouts need it; report instead of computing garbage
+    if (threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
+    return;
+  }
+  if (threadIdx.x == 0) {
+    for (int b = 0; b < NUM_BARS; ++b) mbar_init(&bars[b], b == Q_FULL || b == P_FULL0 || b == P_FULL1 || b == O_FREE ? 4 : 1);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(tmem_slot, 256);                  // S0: columns [0, 64), S1: [64, 128), O: [128, 128 + HD)
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  let_next_start();                              // what follows may begin with the requests' own tokens
+  const int group = p.q_heads / p.kv_heads;
+  auto fail = [&](unsigned int code) {
+    if (lane == 0) report_status(p.status, code);
+    *abort_flag = 1;
+  };
+  auto passed = [&](int bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, wait_or_abort(&bars[bar], parity, abort_flag)) != 0;
+  };
+
+  if (warp == 5) {
+    bring_tiles<HD, KIND, 0>(p, f, sb, scales, v_refs, bars, abort_flag);
+  } else if (warp == 6) {
+    bring_tiles<HD, KIND, 1>(p, f, sb, scales, v_refs, bars, abort_flag);
+  } else if (warp == 4) {
+    // ------------------------------------------------------------------ products (the warp walks, an elected lane issues)
+    const uint32_t idesc_s = idesc_f16(128, kTile), idesc_o = idesc_f16(128, HD) | kIdescBMnMajor;
+    const uint64_t q_desc = umma_desc_k_sw128(sb + C::kQ), k_desc = umma_desc_k_sw128(sb + C::kK);
+    const uint64_t v_desc = desc_mn_sw128(sb + C::kV, kHalfBytes, 1024);
+    uint32_t g = 0, parts = 0;
+    // S(gt) goes over P(gt - 2), which PV(gt - 2) reads: the latest PV issued must have completed
+    auto issue_s = [&](uint32_t gt, uint32_t pv_issued) {
+      const int s = gt & 1;
+      if (pv_issued > 0 && !passed(PV_DONE0 + ((pv_issued - 1) & 1), ((pv_issued - 1) >> 1) & 1)) return false;
+      if (!passed(K_FULL0 + s, (gt >> 1) & 1)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t kd = k_desc + static_cast<uint64_t>(s * (C::kStage >> 4));
+#pragma unroll
+        for (int h = 0; h < NH; ++h)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16_ss(tmem + s * kTile, q_desc + ((h * 16384 + k * 32) >> 4), kd + ((h * kHalfBytes + k * 32) >> 4), idesc_s, (h | k) ? 1u : 0u);
+        umma_commit(&bars[K_EMPTY0 + s]);
+        umma_commit(&bars[S_FULL0 + s]);
+      }
+      __syncwarp();
+      return true;
+    };
+    bool ok = true;
+    Share now(f, p.kv_heads);
+    while (ok && now.next()) {
+      if (!passed(Q_FULL, parts & 1) || !issue_s(g, g)) { fail(NF_ST_TIMEOUT_SMEM_FULL); break; }
+      for (int t = 0; t < now.n; ++t) {
+        const uint32_t gt = g + t;
+        const int s = gt & 1;
+        if (t + 1 < now.n && !issue_s(gt + 1, gt)) { fail(NF_ST_TIMEOUT_SMEM_FULL); ok = false; break; }
+        // the item before must have been read out of O
+        if (t == 0 && !passed(O_FREE, (parts & 1) ^ 1)) { fail(NF_ST_TIMEOUT_TMEM_EMPTY); ok = false; break; }
+        if (!passed(P_FULL0 + s, (gt >> 1) & 1) || !passed(V_FULL0 + s, (gt >> 1) & 1)) { fail(NF_ST_TIMEOUT_SMEM_FULL); ok = false; break; }
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t vd = v_desc + static_cast<uint64_t>(s * (C::kStage >> 4));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_bf16_ts(tmem + 2 * kTile, tmem + s * kTile + k * 8, vd + ((k * 2048) >> 4), idesc_o, (t | k) ? 1u : 0u);
+          umma_commit(&bars[V_EMPTY0 + s]);
+          umma_commit(&bars[PV_DONE0 + s]);
+        }
+        __syncwarp();
+      }
+      g += now.n;
+      ++parts;
+    }
+  } else {
+    // ------------------------------------------------------------------ softmax (a thread per query row)
+    const int row = warp * 32 + lane;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const uint32_t t_o = t_lane + 2 * kTile;
+    const int in_block = row / group, hh = row - in_block * group;
+    uint32_t g = 0;
+    bool ok = true;
+    Share now(f, p.kv_heads);
+    while (ok && now.next()) {
+      // ---- this thread's row of Q. The products of the item before have all been formed: its last scores have been read. ----
+      const int r = now.block * f.reqs_per_block + in_block;
+      int tok = -1;
+      if (in_block < f.reqs_per_block && r < p.req_count) {
+        tok = p.qo_indptr[p.req_begin + r];
+        if (tok < 0 || tok >= p.num_tokens) tok = -1;            // (reported where the row would be written)
+      }
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) +
+                                                        (static_cast<long long>(tok < 0 ? 0 : tok) * p.q_heads + now.kvh * group + (tok < 0 ? 0 : hh)) * HD);
+      uint32_t most = 0;
+#pragma unroll 4
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 v = tok < 0 ? make_uint4(0, 0, 0, 0) : src[c];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = max(most, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
+      }
+      float down, up;
+      q_powers(__uint_as_float(most), down, up);
+#pragma unroll 4
+      for (int c = 0; c < HD / 8; ++c) {
+        const uint4 v = tok < 0 ? make_uint4(0, 0, 0, 0) : src[c];
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = unpack_bf16x2(w[e]);
+          o[e] = pack_f16x2(x.x * down, x.y * down);
+        }
+        st_shared_v4(sb + C::kQ + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[Q_FULL]);
+
+      float ref = -INFINITY, l = 0.f, v_ref = 0.f;
+      for (int t = 0; t < now.n; ++t) {
+        const uint32_t gt = g + t;
+        const int s = gt & 1;
+        if (!passed(S_FULL0 + s, (gt >> 1) & 1) || !passed(V_FULL0 + s, (gt >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); ok = false; break; }
+        tc_fence_after();
+        const float4* k4 = reinterpret_cast<const float4*>(scales + (gt & 3) * kTile);
+        const float4* v4 = reinterpret_cast<const float4*>(scales + (4 + (gt & 3)) * kTile);
+        uint32_t r0[32], r1[32];
+        tmem_ld_32x32b_x32(t_lane + s * kTile, r0);
+        tmem_ld_32x32b_x32(t_lane + s * kTile + 32, r1);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 a = k4[j], b = k4[8 + j];
+          const float ka[4] = {a.x, a.y, a.z, a.w}, kb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            r0[4 * j + e] = __float_as_uint(__uint_as_float(r0[4 * j + e]) * ka[e]);
+            r1[4 * j + e] = __float_as_uint(__uint_as_float(r1[4 * j + e]) * kb[e]);
+          }
+        }
+        const int valid = p.prefix_len - (now.t0 + t) * kTile;
+        if (valid < kTile) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            if (j >= valid) r0[j] = 0xff800000u;
+            if (32 + j >= valid) r1[j] = 0xff800000u;
+          }
+        }
+        float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < 32; ++j) mq[j & 3] = fmaxf(mq[j & 3], fmaxf(__uint_as_float(r0[j]), __uint_as_float(r1[j])));
+        const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * up;
+        const float v_new = v_refs[gt & 3];
+        if (t == 0) {
+          ref = mx;
+          v_ref = v_new;
+        } else {
+          const bool grow = mx > ref + kGap;
+          if (__any_sync(0xffffffffu, grow || v_new != v_ref)) {
+            // O may be touched between two products only: PV(t - 1) is the last one issued (PV(t) needs this tile's P)
+            if (!passed(PV_DONE0 + ((gt - 1) & 1), ((gt - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); ok = false; break; }
+            tc_fence_after();
+            const float alpha = grow ? q8_exp2(ref - mx) : 1.f, by = alpha * (v_ref / v_new);
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t ov[16];
+              tmem_ld_32x32b_x16n(t_o + c * 16, ov);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 16; ++j) ov[j] = __float_as_uint(__uint_as_float(ov[j]) * by);
+              tmem_st_32x32b_x16(t_o + c * 16, ov);
+            }
+            tmem_st_wait();
+            l *= alpha;
+            if (grow) ref = mx;
+            v_ref = v_new;
+          }
+        }
+        const float ms = ref == -INFINITY ? 0.f : ref;
+        float rs = 0.f;
+        uint32_t pk[32];                                         // column j: tokens 2j, 2j + 1
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float4 a = v4[j], b = v4[8 + j];
+          const float va[4] = {a.x, a.y, a.z, a.w}, vb[4] = {b.x, b.y, b.z, b.w};
+          float x[4], y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[e] = q8_exp2(fmaf(__uint_as_float(r0[4 * j + e]), up, -ms));
+            y[e] = q8_exp2(fmaf(__uint_as_float(r1[4 * j + e]), up, -ms));
+            rs += x[e] + y[e];
+          }
+          pk[2 * j] = pack_f16x2(x[0] * va[0], x[1] * va[1]);
+          pk[2 * j + 1] = pack_f16x2(x[2] * va[2], x[3] * va[3]);
+          pk[16 + 2 * j] = pack_f16x2(y[0] * vb[0], y[1] * vb[1]);
+          pk[16 + 2 * j + 1] = pack_f16x2(y[2] * vb[2], y[3] * vb[3]);
+        }
+        l += rs;
+        tmem_st_32x32b_x32(t_lane + s * kTile, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars[P_FULL0 + s]);
+      }
+      if (!ok) break;
+      g += now.n;
+      if (!passed(PV_DONE0 + ((g - 1) & 1), ((g - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
+      tc_fence_after();
+      const long long at = (now.item + blockIdx.x) * kPrefixRows + row;
+      const float back = v_ref / kHeadroom;
+#pragma unroll 1
+      for (int c = 0; c < HD / 32; ++c) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(t_o + c * 32, v);
+        tmem_ld_wait();
+        if (tok >= 0) {
+          float4* dst = reinterpret_cast<float4*>(part_o + at * HD + c * 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            __stcg(dst + j, make_float4(__uint_as_float(v[4 * j]) * back, __uint_as_float(v[4 * j + 1]) * back, __uint_as_float(v[4 * j + 2]) * back,
+                                        __uint_as_float(v[4 * j + 3]) * back));
+        }
+      }
+      if (tok >= 0) __stcg(reinterpret_cast<float2*>(part_ml) + at, make_float2(ref, l));
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars[O_FREE]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+template <int HD, int KIND>
+int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, cudaStream_t stream) {
+  const auto kernel = attn_prefix_q8_kernel<HD, KIND>;
+  static bool attr_dev[kMaxDevices] = {false};
+  bool& attr = attr_dev[device_slot()];
+  if (!attr) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Pre<HD>::kBytes) != cudaSuccess) return NF_ERR_CUDA;
+    attr = true;
+  }
+  if (launch_kernel(false, kernel, f.ctas, kThreads, Pre<HD>::kBytes, stream, 1, p, f, const_cast<float*>(f.ml), const_cast<float*>(f.o)) == cudaSuccess)
+    return NF_OK;
+  (void)cudaGetLastError();
+  return NF_ERR_CUDA;
+}
+
+}  // namespace
+
+PrefixPlan prefix_plan(const nfk_attn_q8_params& p) {
+  PrefixPlan f = {};
+  if (p.prefix_len <= 0) return f;
+  f.reqs_per_block = kPrefixRows / (p.q_heads / p.kv_heads);
+  f.blocks = (p.req_count + f.reqs_per_block - 1) / f.reqs_per_block;
+  f.tiles = (p.prefix_len + kPrefixTile - 1) / kPrefixTile;
+  const long long units = prefix_units(f, p.kv_heads);
+  long long ctas = 2ll * device_sm_count();
+  if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
+  if (ctas > units) ctas = units;
+  f.ctas = static_cast<int>(ctas);
+  return f;
+}
+
+int launch_prefix_q8(const nfk_attn_q8_params& p, const PrefixPlan& f, cudaStream_t stream) {
+  if (p.head_dim == 128) return p.kind == NFK_Q8_E4M3 ? launch<128, NFK_Q8_E4M3>(p, f, stream) : launch<128, NFK_Q8_INT8>(p, f, stream);
+  return p.kind == NFK_Q8_E4M3 ? launch<64, NFK_Q8_E4M3>(p, f, stream) : launch<64, NFK_Q8_INT8>(p, f, stream);
+}
+
+}  // namespace nf

@@ -258,6 +258,71 @@ int nfk_attn_prefill_tc(const nfk_attn_params* p, cudaStream_t stream);
 int nfk_attn_prefill_ws(const nfk_attn_params* p, cudaStream_t stream);
 
 // ------------------------------------------------------------------------------------------------
+// KV cache in 8 bits (rope_append_q8.cu, attn_decode_q8.cu, attn_prefix_q8.cu)
+// ------------------------------------------------------------------------------------------------
+// kv_pool [num_pages][2][kv_heads][16][head_dim] numbers of 8 bits, kv_scale [num_pages][2][kv_heads][16] fp32: a cached value is
+// number * scale. head_dim 64 or 128.
+enum { NFK_Q8_E4M3 = 0, NFK_Q8_INT8 = 1 };
+// Counterpart of nfk_rope_append for that pool. q_norm / k_norm: RMS norm of every query / key head before the rotation.
+// A vector's scale is its largest magnitude / 448 (e4m3) or / 127 (whole numbers); vectors below 2^-80 are stored as zeros, a
+// vector that is not finite gets the scale NaN.
+typedef struct nfk_rope_append_q8_params {
+  const void* qkv;           // [T][ld_qkv] bf16
+  long long ld_qkv;
+  int q_off, k_off, v_off;   // first columns
+  void* q_out;               // [T][q_heads * head_dim] bf16
+  void* kv_pool;
+  float* kv_scale;
+  const float* inv_freq;     // [head_dim / 2]
+  const float* cos_sin;      // [T][head_dim / 2][2] as nfk_rope_table leaves it, null: angles are computed (in 64 bits)
+  const int* positions;      // [T]
+  const int* token_req;      // [T]
+  const int* kv_indptr;      // [num_reqs + 1]
+  const int* kv_indices;     // [num_indices]
+  const void* q_norm;        // [head_dim] bf16, null: none
+  const void* k_norm;
+  float eps;
+  int T, q_heads, kv_heads, head_dim, num_pages, num_reqs, num_indices, kind;
+  unsigned int* status;
+} nfk_rope_append_q8_params;
+int nfk_rope_append_q8(const nfk_rope_append_q8_params* p, cudaStream_t stream);
+
+// out[i] = the bf16 values of page page_ids[i], in the layout of a bf16 pool page.
+typedef struct nfk_kv_read_q8_params {
+  const void* kv_pool;
+  const float* kv_scale;
+  void* out;                 // [n_pages][2][kv_heads][16][head_dim] bf16
+  const int* page_ids;
+  int n_pages, kv_heads, head_dim, num_pages, kind;
+  unsigned int* status;
+} nfk_kv_read_q8_params;
+int nfk_kv_read_q8(const nfk_kv_read_q8_params* p, cudaStream_t stream);
+
+// One query token per request (row qo_indptr[b] of q) over its cached tokens; with prefix_len > 0 all requests also see the
+// prefix_len tokens of prefix_pages, in front of their own. Requests that see nothing get zeros.
+typedef struct nfk_attn_q8_params {
+  const void* q;             // [num_tokens][q_heads * head_dim] bf16
+  void* out;                 // [num_tokens][q_heads * head_dim] bf16
+  const void* kv_pool;
+  const float* kv_scale;
+  const int* qo_indptr;      // [>= req_begin + req_count]
+  const int* kv_indptr;      // [>= req_begin + req_count + 1]
+  const int* kv_indices;     // [num_indices]
+  const int* kv_last_page_len;
+  const int* prefix_pages;   // [ceil(prefix_len / 16)]
+  int q_heads, kv_heads, head_dim, num_pages, num_tokens, num_indices;
+  int req_begin, req_count, prefix_len, kind;
+  float sm_scale;
+  int num_ctas;              // CTA budget; 0 = as many as fit
+  void* workspace;           // nfk_attn_q8_workspace bytes, zero before the first use; launches that may run at the same time
+  long long workspace_bytes; // each need their own
+  unsigned int* status;
+} nfk_attn_q8_params;
+// Bytes of workspace for calls of up to these sizes (req_count, q_heads, kv_heads, head_dim, prefix_len); 0: sizes not built.
+long long nfk_attn_q8_workspace(const nfk_attn_q8_params* p);
+int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream);
+
+// ------------------------------------------------------------------------------------------------
 // Layer-list models: residual step, latent attention, mLSTM (residual_norm.cu, latent.cu, mlstm.cu)
 // ------------------------------------------------------------------------------------------------
 enum { NFK_NORM_NONE = 0, NFK_NORM_RMS = 1, NFK_NORM_LAYER = 2, NFK_NORM_SCALE = 3 };   // SCALE: only times the weights

@@ -726,3 +726,7 @@ def kv_move_pages(pool: torch.Tensor, staging: torch.Tensor, page_ids: torch.Ten
                                    c_longlong(page_bytes), c_int(num_pages),
                                    c_int(0 if to_staging else 1), c_int(num_ctas), _p(status),
                                    _stream()), "nfk_kv_move_pages")
+
+
+from .cache_q8 import (attn_decode_q8, attn_decode_shared_q8, decode_workspace_q8, kv_pool_q8, kv_read_q8,  # noqa: E402
+                       rope_append_q8)

@@ -399,3 +399,66 @@ def moe_route(logits, correction, top, groups, keep, scale, score="sigmoid", gro
     if score == "softmax_all":
         return idx, w * scale
     return idx, w / (w.sum(-1, keepdim=True) + 1e-20) * scale
+
+
+# ---- the 8-bit cache, in 64 bits ----
+Q8_LARGEST = {torch.float8_e4m3fn: 448.0, torch.int8: 127.0}
+Q8_SMALLEST = 2.0 ** -80
+
+
+def rope_append_q8(qkv, inv_freq, positions, *, q_heads, kv_heads, head_dim, q_off, k_off, v_off, q_norm=None, k_norm=None, eps=1e-6):
+    """(q, k, v) [T, heads, head_dim], normed and rotated, before anything is rounded."""
+    T, half = qkv.shape[0], head_dim // 2
+    angle = positions.double()[:, None] * inv_freq.double()
+    cos, sin = angle.cos()[:, None], angle.sin()[:, None]
+
+    def rows(off, heads, norm):
+        x = qkv[:, off:off + heads * head_dim].reshape(T, heads, head_dim).double()
+        if norm is not None:
+            x = x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * norm.double()
+        return x
+
+    def rotated(x):
+        a, b = x[..., :half], x[..., half:]
+        return torch.cat((a * cos - b * sin, b * cos + a * sin), -1)
+
+    return rotated(rows(q_off, q_heads, q_norm)), rotated(rows(k_off, kv_heads, k_norm)), rows(v_off, kv_heads, None)
+
+
+def quantise_q8(x, dtype):
+    """(numbers, scale) of vectors along the last dimension."""
+    most = x.abs().amax(-1)
+    scale = torch.where(most.isfinite(), torch.where(most < Q8_SMALLEST, 0.0, most / Q8_LARGEST[dtype]), torch.nan)
+    y = torch.where((scale > 0)[..., None], x / torch.where(scale > 0, scale, 1.0)[..., None], 0.0)
+    return (y.round() if dtype == torch.int8 else y.float()).to(dtype), scale.float()
+
+
+def kv_values_q8(kv_pool, kv_scale, page_ids):
+    """Cached values of the listed pages."""
+    at = page_ids.long().cpu()
+    return kv_pool.cpu().view(torch.int8)[at].view(kv_pool.dtype).double() * kv_scale.cpu()[at].double()[..., None]
+
+
+def attn_decode_q8(q, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *, q_heads, req_begin, req_count,
+                   sm_scale=None, prefix_pages=None, prefix_len=0):
+    """{row of q: [q_heads, head_dim]} of the listed requests, and beside it what errors go with: sum_j p_j |v_j| (weights rounded
+    relative to themselves), the largest sum_d |q_d k_jd| times the scale (the scores' sums), and the number of tokens times the
+    largest |v_jd| (weights rounded to a multiple of the smallest one)."""
+    kv_heads, head_dim = kv_pool.shape[2], kv_pool.shape[4]
+    group, scale = q_heads // kv_heads, head_dim ** -0.5 if sm_scale is None else sm_scale
+    gather = lambda pages, n: kv_values_q8(kv_pool, kv_scale, pages).permute(1, 2, 0, 3, 4).reshape(2, kv_heads, -1, head_dim)[:, :, :n]
+    front = gather(prefix_pages, prefix_len) if prefix_len else torch.zeros(2, kv_heads, 0, head_dim, dtype=torch.double)
+    out = {}
+    for b in range(req_begin, req_begin + req_count):
+        pages = kv_indices[int(kv_indptr[b]):int(kv_indptr[b + 1])]
+        own = gather(pages, (len(pages) - 1) * 16 + int(kv_last_page_len[b])) if len(pages) else front[:, :, :0]
+        k, v = torch.cat((front, own), 2)
+        x = q[int(qo_indptr[b])].double().cpu().view(kv_heads, group, head_dim)
+        if k.shape[1] == 0:
+            out[int(qo_indptr[b])] = (torch.zeros(q_heads, head_dim, dtype=torch.double),) * 2 + (torch.zeros(q_heads, 1),) * 2
+            continue
+        p = torch.softmax(x @ k.transpose(1, 2) * scale, -1)
+        size = (x.abs() @ k.abs().transpose(1, 2)).amax(-1, keepdim=True) * scale
+        most = k.shape[1] * v.abs().amax((1, 2))[:, None, None].expand_as(size)
+        out[int(qo_indptr[b])] = tuple(t.reshape(q_heads, -1) for t in (p @ v, p @ v.abs(), size, most))
+    return out
