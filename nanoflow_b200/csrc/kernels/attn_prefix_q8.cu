@@ -63,25 +63,20 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
 
 // A CTA's share of the units, one item after the other.
 struct Share {
-  long long u, end;
-  int tiles, blocks;
-  int kvh, block, t0, n;     // the current part: tiles t0 .. t0 + n - 1 of item (kvh, block)
-  long long item;
-  __device__ __forceinline__ Share(const PrefixPlan& f, int kv_heads) {
-    const long long units = prefix_units(f, kv_heads);
-    u = range_begin(blockIdx.x, units, f.ctas);
-    end = range_begin(blockIdx.x + 1, units, f.ctas);
-    tiles = f.tiles;
-    blocks = f.blocks;
+  int u, end, tiles, blocks;
+  int item, kvh, block, t0, n;         // the current part: tiles t0 .. t0 + n - 1 of item (kvh, block)
+  __device__ __forceinline__ Share(const PrefixPlan& f, int kv_heads) : tiles(f.tiles), blocks(f.blocks) {
+    const Ranges ranges(prefix_units(f, kv_heads), f.ctas);
+    u = ranges.begin(blockIdx.x);
+    end = ranges.begin(blockIdx.x + 1);
   }
   __device__ __forceinline__ bool next() {
     if (u >= end) return false;
     item = u / tiles;
-    t0 = static_cast<int>(u - item * tiles);
-    const long long left = end - u;
-    n = left < tiles - t0 ? static_cast<int>(left) : tiles - t0;
-    kvh = static_cast<int>(item / blocks);
-    block = static_cast<int>(item - static_cast<long long>(kvh) * blocks);
+    t0 = u - item * tiles;
+    n = min(end - u, tiles - t0);
+    kvh = item / blocks;
+    block = item - kvh * blocks;
     u += n;
     return true;
   }
@@ -430,7 +425,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, float* part_ml, float*
       g += now.n;
       if (!passed(PV_DONE0 + ((g - 1) & 1), ((g - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
       tc_fence_after();
-      const long long at = (now.item + blockIdx.x) * kPrefixRows + row;
+      const long long at = static_cast<long long>(now.item + blockIdx.x) * kPrefixRows + row;
       const float back = v_ref / kHeadroom;
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
@@ -483,11 +478,11 @@ PrefixPlan prefix_plan(const nfk_attn_q8_params& p) {
   f.reqs_per_block = kPrefixRows / (p.q_heads / p.kv_heads);
   f.blocks = (p.req_count + f.reqs_per_block - 1) / f.reqs_per_block;
   f.tiles = (p.prefix_len + kPrefixTile - 1) / kPrefixTile;
-  const long long units = prefix_units(f, p.kv_heads);
-  long long ctas = 2ll * device_sm_count();
+  const int units = prefix_units(f, p.kv_heads);
+  int ctas = 2 * device_sm_count();
   if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
   if (ctas > units) ctas = units;
-  f.ctas = static_cast<int>(ctas);
+  f.ctas = ctas;
   return f;
 }
 

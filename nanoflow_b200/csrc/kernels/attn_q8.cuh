@@ -11,11 +11,16 @@ namespace nf {
 constexpr int kQ8Page = 16;
 constexpr float kQ8Log2e = 1.4426950408889634f;
 
-__host__ __device__ __forceinline__ long long range_begin(long long w, long long units, long long workers) { return w * units / workers; }
-// The worker whose range holds unit u (each has at least one: workers <= units).
-__host__ __device__ __forceinline__ long long range_of(long long u, long long units, long long workers) {
-  return ((u + 1) * workers + units - 1) / units - 1;
-}
+// A row of n units in w ranges (w <= n): the first n % w ranges have one more than the others.
+struct Ranges {
+  int per, extra;
+  __host__ __device__ __forceinline__ Ranges(int n, int w) : per(w > 0 ? n / w : 0), extra(n - per * w) {}
+  __host__ __device__ __forceinline__ int begin(int w) const { return w * per + (w < extra ? w : extra); }
+  __host__ __device__ __forceinline__ int of(int u) const {             // the range that holds unit u
+    const int longer = extra * (per + 1);
+    return u < longer ? u / (per + 1) : extra + (u - longer) / per;
+  }
+};
 
 // The shared prefix: the query rows of a KV head (requests x group) are cut into blocks of at most 128 rows, whole requests each.
 // An item is (KV head, block), its units the prefix's tiles of 64 tokens. The piece of item i by CTA c has number i + c: along
@@ -26,14 +31,14 @@ struct PrefixPlan {
   const float* o;            // [pieces][128 rows][head_dim], not divided by the sum
   const float* ml;           // [pieces][128 rows][2]: reference (of exponents to base 2), sum
 };
-__host__ __device__ __forceinline__ long long prefix_units(const PrefixPlan& f, int kv_heads) {
-  return static_cast<long long>(kv_heads) * f.blocks * f.tiles;
-}
+__host__ __device__ __forceinline__ int prefix_units(const PrefixPlan& f, int kv_heads) { return kv_heads * f.blocks * f.tiles; }
 
-// Where things lie in the workspace, in this order: counts and partial rows of the decode kernel's CTAs, then the prefix's.
-constexpr int kDecodeCtasPerSm = 4;      // at most
+constexpr int kDecodeCtasPerSm = 4, kDecodeWarps = 4;      // of the decode kernel: at most, of so many warps
+
+// Where things lie in the workspace, in this order: counts of pieces that have been left, partial rows of the decode kernel's CTAs
+// (two requests each), rows that its warps keep (two requests each), the prefix's pieces.
 struct Q8Workspace {
-  long long counts, ml, o, prefix_ml, prefix_o, bytes;
+  long long counts, ml, o, kept, prefix_ml, prefix_o, bytes;
 };
 inline Q8Workspace q8_workspace(int group, int head_dim, long long prefix_pieces) {
   Q8Workspace w;
@@ -42,7 +47,8 @@ inline Q8Workspace q8_workspace(int group, int head_dim, long long prefix_pieces
   w.counts = 0;
   w.ml = up(ctas * 4);
   w.o = w.ml + up(ctas * 2 * group * 8);
-  w.prefix_ml = w.o + up(ctas * 2 * group * head_dim * 4ll);
+  w.kept = w.o + up(ctas * 2 * group * head_dim * 4ll);
+  w.prefix_ml = w.kept + up(2 * ctas * kDecodeWarps * group * (head_dim + 2) * 4ll);
   w.prefix_o = w.prefix_ml + up(prefix_pieces * kPrefixRows * 8);
   w.bytes = w.prefix_o + prefix_pieces * kPrefixRows * head_dim * 4;
   return w;
