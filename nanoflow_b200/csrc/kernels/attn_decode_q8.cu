@@ -14,6 +14,10 @@
 //
 // A warp keeps a reference per head instead of a running maximum: it moves only where a score exceeds it by 8 (in exponents to
 // base 2), so that the common page has one vote and no reduction across lanes; sums stay per lane until a request ends.
+//
+// All pages of all requests, one KV head after the other, are a row that is cut into ranges for single warps, without regard to where
+// a request ends (attn_q8.cuh). A warp writes the rows of requests that lie within one of its ranges; of others it leaves states in
+// the workspace, and a second kernel joins them, and the shared prefix's where there is one. Warps wait for nothing but their pages.
 #include "attn_q8.cuh"
 #include "attn_mma.cuh"
 
@@ -77,25 +81,6 @@ struct Row {
     for (int i = 0; i < N; ++i) o[i] = o[i] * a + y.o[i] * b;
     m = top;
   }
-  // A piece as the warps write it: rows of HD, behind them a (reference, sum) for each.
-  __device__ __forceinline__ void read(const float* piece, int group, int h) {
-    const int lane = threadIdx.x & 31;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-      const float2 v = *reinterpret_cast<const float2*>(piece + h * HD + lane * N + i);
-      o[i] = v.x;
-      o[i + 1] = v.y;
-    }
-    const float2 s = *reinterpret_cast<const float2*>(piece + group * HD + 2 * h);
-    m = s.x;
-    l = s.y;
-  }
-  __device__ __forceinline__ void store(float* ml, float* row) const {
-    const int lane = threadIdx.x & 31;
-    if constexpr (HD == 128) __stcg(reinterpret_cast<float4*>(row) + lane, make_float4(o[0], o[1], o[2], o[3]));
-    else __stcg(reinterpret_cast<float2*>(row) + lane, make_float2(o[0], o[1]));
-    if (lane == 0) __stcg(reinterpret_cast<float2*>(ml), make_float2(m, l));
-  }
   __device__ __forceinline__ void finish(__nv_bfloat16* out) const {
     const int lane = threadIdx.x & 31;
     const float inv = l == 0.f ? 0.f : 1.f / l;                // (a sum that is NaN stays visible)
@@ -106,29 +91,30 @@ struct Row {
   }
 };
 
-// Sum of n states in the workspace, the i-th in row at(i), in their order. Lanes fetch 32 references and sums at a time, so that
-// the rows are requested without waiting for one another.
+// A state in the workspace.
+struct State {
+  const float* ml;
+  const float* o;
+};
+// Sum of n states, the i-th being at(i), in their order. Lanes fetch 32 references and sums at a time and 16 rows are requested
+// without waiting for one another.
 template <int HD, class At>
-__device__ __forceinline__ Row<HD> sum_rows(const float* ml, const float* o, int n, At at) {
+__device__ __forceinline__ Row<HD> sum_states(int n, At at) {
+  constexpr int N = Row<HD>::N, AHEAD = 16;
   const int lane = threadIdx.x & 31;
   Row<HD> all;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int here = min(32, n - i0);
-    const long long mine = at(i0 + min(lane, here - 1));
-    const float2 s = __ldcg(reinterpret_cast<const float2*>(ml) + mine);
+    const State mine = at(i0 + min(lane, here - 1));
+    const float2 s = __ldcg(reinterpret_cast<const float2*>(mine.ml));
     Row<HD> part;
-    part.m = s.x;
+    float w = 0.f;
+    for (int i = 0; i < here; i += AHEAD) {
+      float x[AHEAD][N];
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) part.m = fmaxf(part.m, __shfl_xor_sync(0xffffffffu, part.m, off));
-    const float w = lane < here ? q8_exp2(s.x - (part.m == -INFINITY ? 0.f : part.m)) : 0.f;
-    part.l = lane < here ? s.y * w : 0.f;
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) part.l += __shfl_xor_sync(0xffffffffu, part.l, off);
-    for (int i = 0; i < here; i += 8) {
-      float x[8][Row<HD>::N];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {                            // (rows behind the last: that one again, times zero)
-        const float* row = o + __shfl_sync(0xffffffffu, mine, min(i + k, here - 1)) * HD;
+      for (int k = 0; k < AHEAD; ++k) {
+        if (i + k >= here) break;
+        const float* row = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine.o), i + k));
         if constexpr (HD == 128) {
           const float4 v = __ldcg(reinterpret_cast<const float4*>(row) + lane);
           x[k][0] = v.x; x[k][1] = v.y; x[k][2] = v.z; x[k][3] = v.w;
@@ -137,12 +123,21 @@ __device__ __forceinline__ Row<HD> sum_rows(const float* ml, const float* o, int
           x[k][0] = v.x; x[k][1] = v.y;
         }
       }
+      if (i == 0) {                                            // (while the first rows are on their way)
+        part.m = s.x;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float by = i + k < here ? __shfl_sync(0xffffffffu, w, i + k) : 0.f;
-        if (i + k < here)
+        for (int off = 16; off > 0; off >>= 1) part.m = fmaxf(part.m, __shfl_xor_sync(0xffffffffu, part.m, off));
+        w = lane < here ? q8_exp2(s.x - (part.m == -INFINITY ? 0.f : part.m)) : 0.f;
+        part.l = lane < here ? s.y * w : 0.f;
 #pragma unroll
-          for (int e = 0; e < Row<HD>::N; ++e) part.o[e] += by * x[k][e];
+        for (int off = 16; off > 0; off >>= 1) part.l += __shfl_xor_sync(0xffffffffu, part.l, off);
+      }
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        if (i + k >= here) break;
+        const float by = __shfl_sync(0xffffffffu, w, i + k);
+#pragma unroll
+        for (int e = 0; e < N; ++e) part.o[e] += by * x[k][e];
       }
     }
     if (i0 == 0) all = part;
@@ -151,69 +146,45 @@ __device__ __forceinline__ Row<HD> sum_rows(const float* ml, const float* o, int
   return all;
 }
 
-// What the shared prefix gives for head `h` of KV head `kvh` of request `r`.
-template <int HD>
-__device__ __forceinline__ Row<HD> prefix_row(const PrefixPlan& f, int kv_heads, int group, int kvh, int r, int h) {
-  const Ranges ranges(prefix_units(f, kv_heads), f.ctas);
-  const int item = kvh * f.blocks + r / f.reqs_per_block, row = r % f.reqs_per_block * group + h;
-  const int c0 = ranges.of(item * f.tiles), c1 = ranges.of((item + 1) * f.tiles - 1);
-  return sum_rows<HD>(f.ml, f.o, c1 - c0 + 1, [&](int i) { return static_cast<long long>(item + c0 + i) * kPrefixRows + row; });
-}
-
-// A piece that a warp leaves for its CTA: what its range holds of a request for a KV head.
-struct Piece {
-  int kvh, r, tok, begin, end;     // request (from req_begin), its row of q, its pages in the row of pages
-  int flags;                       // 1 there is one, 2 the request starts in it, 4 ends in it
-};
-// A request of which a CTA holds a part only: the first of the CTAs that do and their number; `last`: the others' parts are left.
-struct Part {
-  int kvh, r, tok, first, n, last;
+// Where states go: [..][group or heads] (reference, sum) and rows of head_dim.
+struct States {
+  float* ml;
+  float* o;
+  template <int HD>
+  __device__ __forceinline__ State at(long long i) const { return State{ml + i * 2, o + i * HD}; }
 };
 
 template <int HD, int NT, int KIND, bool SHARED>
-__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : 3)
-attn_decode_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, unsigned int* counts, float* part_ml, float* part_o, float* kept) {
+__global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : HD == 64 ? 3 : 2)
+attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* records, States parts, States wholes) {
   using D = Dec<HD>;
   constexpr int KS = HD / 16, MT = HD / 16, VB = HD / 8;      // steps of Q K^T, row tiles of V^T, bytes of a token's values per lane
   constexpr int ST = D::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ Piece pieces[2 * kWarps];
-  __shared__ Part parts[2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int group = p.q_heads / p.kv_heads, ctas = gridDim.x;
+  const int group = p.q_heads / p.kv_heads;
   const int* indptr = p.kv_indptr + p.req_begin;
   const int base = indptr[0];
   const long long listed = static_cast<long long>(indptr[p.req_count]) - base;
   bool listed_well = base >= 0 && listed >= 0 && base + listed <= p.num_indices;       // else nothing is read
   const int pages_all = listed_well ? static_cast<int>(listed) : 0;
-  const int units = pages_all * p.kv_heads, workers = min(units, ctas * kWarps);
-  const Ranges ranges(units, workers);
+  const int n_ranges = decode_ranges(pages_all * p.kv_heads, gridDim.x);
+  const Ranges ranges(pages_all * p.kv_heads, n_ranges);
   const float scale = p.sm_scale * kQ8Log2e;
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out);
+  let_next_start();
 
-  auto row_of = [&](int r) {                                   // the request's row of q and out
-    const int tok = p.qo_indptr[p.req_begin + r];
-    if (tok >= 0 && tok < p.num_tokens) return tok;
-    if (lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
-    return -1;
-  };
-
-  // A warp's places for pieces: of its range's last run over its pipeline, which is done by then; of the first run in the workspace,
-  // and behind those of all warps that of a request which lies within the range and waits for the prefix's share.
-  static_assert(D::kWarpBytes >= 8 * NT * (HD + 2) * 4, "a piece lies over its warp's pipeline");
-  const int piece_floats = group * (HD + 2);
+  // ---- loads: the pages of this warp's range ----
+  const int range = blockIdx.x * kWarps + warp, u0 = ranges.begin(range);
+  const int n = range < n_ranges ? ranges.begin(range + 1) - u0 : 0;
+  int kvh = n > 0 ? u0 / pages_all : 0, at = n > 0 ? u0 - kvh * pages_all : 0;         // of the next page to work on: KV head, place in the row
   const uint32_t pipe = smem_u32(smem) + warp * D::kWarpBytes;
-  auto piece_at = [&](int k) {                                 // warp k / 2, its first (0) or last (1) run
-    return (k & 1) ? reinterpret_cast<float*>(smem + (k >> 1) * D::kWarpBytes)
-                   : kept + (static_cast<long long>(blockIdx.x) * kWarps + (k >> 1)) * piece_floats;
-  };
-
-  // ---- loads: unit i of the range is page (u0 + i) % pages_all of KV head (u0 + i) / pages_all ----
-  int n = 0, kvh = 0, at = 0;                                  // units of the range; KV head and place in the row of pages of the next one
-  int i_kvh = 0, i_page = 0, ids = 0, ids_left = 0;            // of the next one to load; page numbers, one per lane, 32 at a time
   const uint8_t* pool = reinterpret_cast<const uint8_t*>(p.kv_pool);
-  auto issue = [&](int i) {
-    if (i < n) {
+  int i_left = n, i_kvh = kvh, i_page = at;                    // of the next one to load; pages that are left
+  int ids = 0, ids_left = 0;                                   // page numbers, one per lane, 32 at a time
+  uint32_t to = pipe;                                          // the stage that is loaded next
+  auto issue = [&]() {
+    if (i_left > 0) {
       if (ids_left == 0) {
         ids_left = min(32, pages_all - i_page);
         ids = lane < ids_left ? p.kv_indices[base + i_page + lane] : 0;
@@ -228,21 +199,23 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, unsigned int* counts, 
       const long long head = static_cast<long long>(page) * 2 * p.kv_heads + i_kvh;
       const uint8_t* k = pool + head * D::kKeyBytes;
       const uint8_t* v = k + static_cast<long long>(p.kv_heads) * D::kKeyBytes;
-      const uint32_t st = pipe + i % ST * D::kStageBytes;
-      // eight (head_dim 64: four) neighbouring lanes take a token's row: a sector asked for by itself comes at half the rate
+      // Eight (head_dim 64: four) neighbouring lanes take a token's row. With a sector to each quarter of the warp L2 had twice as
+      // many requests to answer: 683 requests of 1024 to 1536 tokens, 378 us instead of 318.
 #pragma unroll
       for (int y = 0; y < HD / 32; ++y) {
         const int tok = y * (512 / HD) + lane / (HD / 16), c = lane % (HD / 16);
-        cp_async16(st + D::key_at(tok, c), k + tok * HD + c * 16);
-        cp_async16(st + D::kKeyBytes + D::value_at((tok & 1) + (tok >> 3) * 2, (tok >> 1) & 3, c), v + tok * HD + c * 16);
+        cp_async16(to + D::key_at(tok, c), k + tok * HD + c * 16);
+        cp_async16(to + D::kKeyBytes + D::value_at((tok & 1) + (tok >> 3) * 2, (tok >> 1) & 3, c), v + tok * HD + c * 16);
       }
-      if (lane < 8) cp_async16(st + 2 * D::kKeyBytes + lane * 16, p.kv_scale + (head + (lane >> 2) * p.kv_heads) * kQ8Page + (lane & 3) * 4);
+      if (lane < 8) cp_async16(to + 2 * D::kKeyBytes + lane * 16, p.kv_scale + (head + (lane >> 2) * p.kv_heads) * kQ8Page + (lane & 3) * 4);
+      --i_left;
       if (++i_page == pages_all) {
         i_page = 0;
         ++i_kvh;
         ids_left = 0;
       }
     }
+    to = to + D::kStageBytes == pipe + D::kWarpBytes ? pipe : to + D::kStageBytes;
     cp_async_commit();
   };
   // The request that a place in the row of pages belongs to: the last whose pages start at or before it, 32 candidates at a time.
@@ -258,367 +231,383 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, unsigned int* counts, 
     return lo;
   };
 
-  const int w = blockIdx.x * kWarps + warp;
-  if (w < workers) {
-    const int u0 = ranges.begin(w);
-    n = ranges.begin(w + 1) - u0;
-    i_kvh = kvh = u0 / pages_all;
-    i_page = at = u0 - kvh * pages_all;
+  auto row_of = [&](int r) {                                   // the request's row of q and out
+    const int tok = p.qo_indptr[p.req_begin + r];
+    if (tok >= 0 && tok < p.num_tokens) return tok;
+    if (lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
+    return -1;
+  };
+
 #pragma unroll
-    for (int s = 0; s < ST - 1; ++s) issue(s);
-  }
-  // (while the first pages are on their way)
-  int seen = 0;
+  for (int s = 0; s < ST - 1; ++s) issue();
+  // (while the first pages are on their way: the lists must go up, or runs of pages would have no end)
+  bool falls = false, none = false;
   for (int r = threadIdx.x; r < p.req_count; r += kThreads) {
     const int own = indptr[r + 1] - indptr[r];
-    seen |= own < 0 ? 1 : own == 0 ? 2 : 0;
+    falls = falls || own < 0;
+    none = none || own == 0;
   }
-  if (lane < 2) pieces[warp * 2 + lane].flags = 0;
-  if (threadIdx.x < 2) parts[threadIdx.x].n = 0;
-  listed_well = __syncthreads_or(seen & 1) == 0 && listed_well;
-  const bool some_empty = __syncthreads_or(seen & 2) != 0 || pages_all == 0 || !listed_well;
-  if (!listed_well) {
-    if (threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
-    n = 0;
+  listed_well = __syncthreads_or(falls ? 1 : 0) == 0 && listed_well;
+  // requests without pages: zeros (with a prefix the other kernel's)
+  if (!SHARED && (__syncthreads_or(none ? 1 : 0) != 0 || !listed_well))
+    for (int e = range; e < p.req_count * p.q_heads; e += gridDim.x * kWarps) {
+      const int er = e / p.q_heads, tok = !listed_well || indptr[er + 1] == indptr[er] ? row_of(er) : -1;
+      if (tok >= 0) Row<HD>().finish(out + (static_cast<long long>(tok) * p.q_heads + e - er * p.q_heads) * HD);
+    }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *bad_lists = listed_well ? 0 : 1;
+    if (!listed_well) report_status(p.status, NF_ST_BAD_INDEX);
   }
 
-  int r = n > 0 ? find(at) : 0;
-  for (int i = 0; i < n;) {
-    // ---- a request's run of pages in this range ----
-    const int r_begin = indptr[r] - base, r_end = indptr[r + 1] - base;
-    const int count = min(n - i, r_end - at);
-    const bool starts = at == r_begin, ends = at + count == r_end;
-    const int last_len = p.kv_last_page_len[p.req_begin + r];
-    const int tok = row_of(r);
-    uint32_t qb[NT][KS][2];
-    float q_up[NT][2];
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int h = nt * 8 + g;
-      const bool on = tok >= 0 && h < group;
-      const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) +
-                                                        (static_cast<long long>(on ? tok : 0) * p.q_heads + kvh * group + (on ? h : 0)) * HD) + t * 2;
-      uint4 raw[KS / 2];
-      uint32_t most = 0;
-#pragma unroll
-      for (int x = 0; x < KS / 2; ++x) {
-        raw[x] = on ? src[(x >> 1) * 8 + (x & 1)] : make_uint4(0, 0, 0, 0);
-        const uint32_t q4[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) most = max(most, max(q4[e] << 16 & 0x7fffffffu, q4[e] & 0x7fff0000u));
-      }
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
-      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      float down, up;
-      q_powers(__uint_as_float(most), down, up);
-#pragma unroll
-      for (int x = 0; x < KS / 2; ++x) {
-        const uint32_t q4[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 q2 = unpack_bf16x2(q4[e]);
-          qb[nt][x * 2 + (e >> 1)][e & 1] = pack_f16x2(q2.x * down, q2.y * down);
-        }
-      }
-      up *= scale;
-      q_up[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t);     // of the columns that this lane's scores are in
-      q_up[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
-    }
-    float o[NT][MT][4], ref[NT][2], l[NT][2], v_ref = 7.8886091e-31f, v_unit = kHeadroom / 7.8886091e-31f;      // 2^-100
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      ref[nt][0] = ref[nt][1] = -INFINITY;
-      l[nt][0] = l[nt][1] = 0.f;
-#pragma unroll
-      for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
-    }
-
-    for (int c = 0; c < count; ++c, ++i) {
-      cp_async_wait<ST - 2>();
-      __syncwarp();                                          // the page is there, and no lane looks at the one before any more
-      issue(i + ST - 1);
-      const uint32_t st = pipe + i % ST * D::kStageBytes;
-      float s[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
-#pragma unroll
-      for (int x = 0; x < HD / 64; ++x) {
-        const uint4 a = ld_shared_v4(st + D::key_at(g, x * 4 + t)), b = ld_shared_v4(st + D::key_at(g + 8, x * 4 + t));
-        const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t a0, a1, a2, a3;
-          q8_to_f16<KIND>(aw[e], a0, a2);
-          q8_to_f16<KIND>(bw[e], a1, a3);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qb[nt][x * 4 + e][0], qb[nt][x * 4 + e][1]);
-        }
-      }
-      const uint32_t sc = st + 2 * D::kKeyBytes;
-      const int valid = ends && c == count - 1 ? last_len : kQ8Page;
-      const bool on0 = g < valid, on1 = g + 8 < valid;
-      const float k0 = ld_shared_f32(sc + g * 4), k1 = ld_shared_f32(sc + g * 4 + 32);
-      const float v0 = on0 ? ld_shared_f32(sc + 64 + g * 4) : 0.f, v1 = on1 ? ld_shared_f32(sc + 96 + g * 4) : 0.f;
-      bool grow = v0 > v_ref || v1 > v_ref;
+  DecodeRecord record = {0, 0, 0, 0};
+  if (listed_well && n > 0) {
+    uint32_t st = pipe;                                        // the stage that is worked on
+    int r = find(at);
+    for (int i = 0; i < n;) {
+      // ---- a request's run of pages in this range ----
+      const int r_begin = indptr[r] - base, r_end = indptr[r + 1] - base;
+      const int count = min(n - i, r_end - at);
+      const bool starts = at == r_begin, ends = at + count == r_end;
+      const int last_len = p.kv_last_page_len[p.req_begin + r];
+      const int tok = row_of(r);
+      uint32_t qb[NT][KS][2];
+      float q_up[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
+        const int h = nt * 8 + g;
+        const bool on = tok >= 0 && h < group;
+        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) +
+                                                          (static_cast<long long>(on ? tok : 0) * p.q_heads + kvh * group + (on ? h : 0)) * HD) + t * 2;
+        uint4 raw[KS / 2];
+        uint32_t most = 0;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          s[nt][e] = on0 ? s[nt][e] * k0 * q_up[nt][e] : -INFINITY;
-          s[nt][2 + e] = on1 ? s[nt][2 + e] * k1 * q_up[nt][e] : -INFINITY;
-          grow = grow || fmaxf(s[nt][e], s[nt][2 + e]) > ref[nt][e] + kGap;
+        for (int x = 0; x < KS / 2; ++x) {
+          raw[x] = on ? src[(x >> 1) * 8 + (x & 1)] : make_uint4(0, 0, 0, 0);
+          const uint32_t q4[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) most = max(most, max(q4[e] << 16 & 0x7fffffffu, q4[e] & 0x7fff0000u));
         }
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-        float most = fmaxf(v_ref, fmaxf(v0, v1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+        float down, up;
+        q_powers(__uint_as_float(most), down, up);
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-        most = __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0xff800000u);          // the next power of two
-        const float shrink = v_ref / most;
-        v_ref = most;
-        v_unit = kHeadroom / most;
+        for (int x = 0; x < KS / 2; ++x) {
+          const uint32_t q4[4] = {raw[x].x, raw[x].y, raw[x].z, raw[x].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 q2 = unpack_bf16x2(q4[e]);
+            qb[nt][x * 2 + (e >> 1)][e & 1] = pack_f16x2(q2.x * down, q2.y * down);
+          }
+        }
+        up *= scale;
+        q_up[nt][0] = __shfl_sync(0xffffffffu, up, 8 * t);     // of the columns that this lane's scores are in
+        q_up[nt][1] = __shfl_sync(0xffffffffu, up, 8 * t + 4);
+      }
+      float o[NT][MT][4], ref[NT][2], l[NT][2], v_ref = 7.8886091e-31f, v_unit = kHeadroom / 7.8886091e-31f;      // 2^-100
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        ref[nt][0] = ref[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+      }
+
+
+      for (int c = 0; c < count; ++c, ++i) {
+        cp_async_wait<ST - 2>();
+        __syncwarp();                                          // the page is there, and no lane looks at the one before any more
+        issue();
+        float s[NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+#pragma unroll
+        for (int x = 0; x < HD / 64; ++x) {
+          const uint4 a = ld_shared_v4(st + D::key_at(g, x * 4 + t)), b = ld_shared_v4(st + D::key_at(g + 8, x * 4 + t));
+          const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            uint32_t a0, a1, a2, a3;
+            q8_to_f16<KIND>(aw[e], a0, a2);
+            q8_to_f16<KIND>(bw[e], a1, a3);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qb[nt][x * 4 + e][0], qb[nt][x * 4 + e][1]);
+          }
+        }
+        const uint32_t sc = st + 2 * D::kKeyBytes;
+        const int valid = ends && c == count - 1 ? last_len : kQ8Page;
+        const bool on0 = g < valid, on1 = g + 8 < valid;
+        const float k0 = ld_shared_f32(sc + g * 4), k1 = ld_shared_f32(sc + g * 4 + 32);
+        const float v0 = on0 ? ld_shared_f32(sc + 64 + g * 4) : 0.f, v1 = on1 ? ld_shared_f32(sc + 96 + g * 4) : 0.f;
+        bool grow = v0 > v_ref || v1 > v_ref;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-          float by[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(s[nt][e], s[nt][2 + e]);
-#pragma unroll
-            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-            const float top = mx > ref[nt][e] + kGap ? mx : ref[nt][e];
-            const float alpha = top == ref[nt][e] ? 1.f : q8_exp2(ref[nt][e] - top);
-            ref[nt][e] = top;
-            l[nt][e] *= alpha;
-            by[e] = alpha * shrink;
-          }
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            o[nt][j][0] *= by[0]; o[nt][j][1] *= by[1]; o[nt][j][2] *= by[0]; o[nt][j][3] *= by[1];
+            s[nt][e] = on0 ? s[nt][e] * k0 * q_up[nt][e] : -INFINITY;
+            s[nt][2 + e] = on1 ? s[nt][2 + e] * k1 * q_up[nt][e] : -INFINITY;
+            grow = grow || fmaxf(s[nt][e], s[nt][2 + e]) > ref[nt][e] + kGap;
           }
         }
-      }
-      const float w0 = v0 * v_unit, w1 = v1 * v_unit;
-      uint32_t pb[NT][2];
+        if (__any_sync(0xffffffffu, grow)) {
+          float most = fmaxf(v_ref, fmaxf(v0, v1));
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        float e0[2], e1[2];
+          for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+          most = __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0xff800000u);          // the next power of two
+          const float shrink = v_ref / most;
+          v_ref = most;
+          v_unit = kHeadroom / most;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float safe = ref[nt][e] == -INFINITY ? 0.f : ref[nt][e];
-          e0[e] = q8_exp2(s[nt][e] - safe);
-          e1[e] = q8_exp2(s[nt][2 + e] - safe);
-          l[nt][e] += e0[e] + e1[e];
+          for (int nt = 0; nt < NT; ++nt) {
+            float by[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float mx = fmaxf(s[nt][e], s[nt][2 + e]);
+#pragma unroll
+              for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+              const float top = mx > ref[nt][e] + kGap ? mx : ref[nt][e];
+              const float alpha = top == ref[nt][e] ? 1.f : q8_exp2(ref[nt][e] - top);
+              ref[nt][e] = top;
+              l[nt][e] *= alpha;
+              by[e] = alpha * shrink;
+            }
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+              o[nt][j][0] *= by[0]; o[nt][j][1] *= by[1]; o[nt][j][2] *= by[0]; o[nt][j][3] *= by[1];
+            }
+          }
         }
-        pb[nt][0] = transpose_8x8(pack_f16x2(e0[0] * w0, e0[1] * w0));
-        pb[nt][1] = transpose_8x8(pack_f16x2(e1[0] * w1, e1[1] * w1));
-      }
-      uint32_t vw[4][VB / 4];
+        const float w0 = v0 * v_unit, w1 = v1 * v_unit;
+        uint32_t pb[NT][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t from = st + D::kKeyBytes + (HD == 128 ? D::value_at(j, t, g) : D::value_at(j, t, g >> 1) + (g & 1) * 8);
-        if constexpr (HD == 128) {
-          const uint4 v = ld_shared_v4(from);
-          vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
-        } else {
-          const uint2 v = ld_shared_v2(from);
-          vw[j][0] = v.x; vw[j][1] = v.y;
+        for (int nt = 0; nt < NT; ++nt) {
+          float e0[2], e1[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float safe = ref[nt][e] == -INFINITY ? 0.f : ref[nt][e];
+            e0[e] = q8_exp2(s[nt][e] - safe);
+            e1[e] = q8_exp2(s[nt][2 + e] - safe);
+            l[nt][e] += e0[e] + e1[e];
+          }
+          pb[nt][0] = transpose_8x8(pack_f16x2(e0[0] * w0, e0[1] * w0));
+          pb[nt][1] = transpose_8x8(pack_f16x2(e1[0] * w1, e1[1] * w1));
         }
+        uint32_t vw[4][VB / 4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t from = st + D::kKeyBytes + (HD == 128 ? D::value_at(j, t, g) : D::value_at(j, t, g >> 1) + (g & 1) * 8);
+          if constexpr (HD == 128) {
+            const uint4 v = ld_shared_v4(from);
+            vw[j][0] = v.x; vw[j][1] = v.y; vw[j][2] = v.z; vw[j][3] = v.w;
+          } else {
+            const uint2 v = ld_shared_v2(from);
+            vw[j][0] = v.x; vw[j][1] = v.y;
+          }
+        }
+        if (valid < kQ8Page)                                   // what lies behind the last token may be anything, NaN among it
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int e = 0; e < VB / 4; ++e) vw[j][e] = 2 * t + (j & 1) + 8 * (j >> 1) < valid ? vw[j][e] : 0u;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {                         // elements 2j (rows g) and 2j + 1 (rows g + 8) of the lane's
+          const uint32_t sel = (j & 1) ? 0x7362u : 0x5140u;
+          uint32_t a0, a1, a2, a3;
+          q8_to_f16<KIND>(__byte_perm(vw[0][j >> 1], vw[1][j >> 1], sel), a0, a1);
+          q8_to_f16<KIND>(__byte_perm(vw[2][j >> 1], vw[3][j >> 1], sel), a2, a3);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][j], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+        }
+        st = st + D::kStageBytes == pipe + D::kWarpBytes ? pipe : st + D::kStageBytes;
       }
-      if (valid < kQ8Page)                                   // what lies behind the last token may be anything, NaN among it
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-          for (int e = 0; e < VB / 4; ++e) vw[j][e] = 2 * t + (j & 1) + 8 * (j >> 1) < valid ? vw[j][e] : 0u;
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {                         // elements 2j (rows g) and 2j + 1 (rows g + 8) of the lane's
-        const uint32_t sel = (j & 1) ? 0x7362u : 0x5140u;
-        uint32_t a0, a1, a2, a3;
-        q8_to_f16<KIND>(__byte_perm(vw[0][j >> 1], vw[1][j >> 1], sel), a0, a1);
-        q8_to_f16<KIND>(__byte_perm(vw[2][j >> 1], vw[3][j >> 1], sel), a2, a3);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][j], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
-      }
-    }
 
-    // ---- the run's end: the final row where it is the whole request, else a piece ----
-    const bool whole = starts && ends, last_run = i == n;
-    const float v_back = v_ref / kHeadroom;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
-    auto leave = [&](float* piece) {
+      // ---- the run's end: the final row where it is the whole request and no prefix joins it, else its state ----
+      const float v_back = v_ref / kHeadroom;
+      const bool final = starts && ends && !SHARED;
+      // states of this run's heads: of a whole request by its number; of a piece by the range's, those of a request that began before
+      // it first
+      const States& states = starts && ends ? wholes : parts;
+      const long long first = starts && ends ? static_cast<long long>(r) * p.q_heads + kvh * group
+                                             : (static_cast<long long>(range) * 2 + (starts ? 1 : 0)) * group;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int off = 4; off < 32; off <<= 1) l[nt][e] += __shfl_xor_sync(0xffffffffu, l[nt][e], off);
           const int h = nt * 8 + 2 * t + e;
           if (h >= group) continue;
-          if (g == 0) *reinterpret_cast<float2*>(piece + group * HD + 2 * h) = make_float2(ref[nt][e], l[nt][e]);
+          if (final) {
+            if (tok < 0) continue;
+            const float inv = l[nt][e] == 0.f ? 0.f : v_back / l[nt][e];
+            uint4* dst = reinterpret_cast<uint4*>(out + (static_cast<long long>(tok) * p.q_heads + kvh * group + h) * HD + g * VB);
 #pragma unroll
-          for (int j = 0; j < MT; ++j)
-            *reinterpret_cast<float2*>(piece + h * HD + g * VB + 2 * j) = make_float2(o[nt][j][e] * v_back, o[nt][j][2 + e] * v_back);
+            for (int j = 0; j < MT; j += 4)
+              dst[j / 4] = make_uint4(pack_bf16x2(o[nt][j][e] * inv, o[nt][j][2 + e] * inv), pack_bf16x2(o[nt][j + 1][e] * inv, o[nt][j + 1][2 + e] * inv),
+                                      pack_bf16x2(o[nt][j + 2][e] * inv, o[nt][j + 2][2 + e] * inv), pack_bf16x2(o[nt][j + 3][e] * inv, o[nt][j + 3][2 + e] * inv));
+          } else {
+            if (g == 0) *reinterpret_cast<float2*>(states.ml + (first + h) * 2) = make_float2(ref[nt][e], l[nt][e]);
+            float4* dst = reinterpret_cast<float4*>(states.o + (first + h) * HD + g * VB);
+#pragma unroll
+            for (int j = 0; j < MT; j += 2)
+              dst[j / 2] = make_float4(o[nt][j][e] * v_back, o[nt][j][2 + e] * v_back, o[nt][j + 1][e] * v_back, o[nt][j + 1][2 + e] * v_back);
+          }
         }
-    };
-    if (whole && !SHARED) {
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int h = nt * 8 + 2 * t + e;
-          if (h >= group || tok < 0) continue;
-          const float inv = l[nt][e] == 0.f ? 0.f : v_back / l[nt][e];
-          uint4* dst = reinterpret_cast<uint4*>(out + (static_cast<long long>(tok) * p.q_heads + kvh * group + h) * HD + g * VB);
-#pragma unroll
-          for (int j = 0; j < MT; j += 4)
-            dst[j / 4] = make_uint4(pack_bf16x2(o[nt][j][e] * inv, o[nt][j][2 + e] * inv), pack_bf16x2(o[nt][j + 1][e] * inv, o[nt][j + 1][2 + e] * inv),
-                                    pack_bf16x2(o[nt][j + 2][e] * inv, o[nt][j + 2][2 + e] * inv), pack_bf16x2(o[nt][j + 3][e] * inv, o[nt][j + 3][2 + e] * inv));
-        }
-    } else if (whole && !last_run) {                         // the warp joins it with the prefix itself
-      float* piece = kept + (static_cast<long long>(ctas + blockIdx.x) * kWarps + warp) * piece_floats;
-      leave(piece);
-      await_previous();
-      __syncwarp();
-      for (int h = 0; h < group; ++h) {
-        Row<HD> row;
-        row.read(piece, group, h);
-        row.add(prefix_row<HD>(f, p.kv_heads, group, kvh, r, h));
-        if (tok >= 0) row.finish(out + (static_cast<long long>(tok) * p.q_heads + kvh * group + h) * HD);
-      }
-      __syncwarp();
-    } else {                                                 // a run that is neither whole nor the last is the first
-      const int k = warp * 2 + (last_run ? 1 : 0);
-      if (last_run) __syncwarp();                            // no lane looks at its last page any more
-      leave(piece_at(k));
-      if (lane == 0) pieces[k] = Piece{kvh, r, tok, r_begin, r_end, 1 | (starts ? 2 : 0) | (ends ? 4 : 0)};
-    }
 
-    // ---- the next request that has pages ----
-    at += count;
-    if (i < n) {
-      if (at == pages_all) {
-        at = 0;
-        ++kvh;
+      if (starts && !ends) record = DecodeRecord{kvh, r, tok, ranges.of(kvh * pages_all + r_end - 1) - range + 1};
+
+      // ---- the next request that has pages ----
+      at += count;
+      if (i < n) {
+        if (at == pages_all) {
+          at = 0;
+          ++kvh;
+        }
+        r = r + 1 < p.req_count && at > 0 && indptr[r + 1] - base <= at && indptr[r + 2] - base > at ? r + 1 : find(at);
       }
-      r = r + 1 < p.req_count && at > 0 && indptr[r + 1] - base <= at && indptr[r + 2] - base > at ? r + 1 : find(at);
     }
   }
+  if (lane == 0) records[range] = record;
   cp_async_wait<0>();
   if (SHARED) await_previous();
-  __syncthreads();
+}
 
-  // ---- requests without pages of their own: zeros, or the prefix alone ----
-  if (some_empty)
-    for (int e = blockIdx.x * kWarps + warp; e < p.req_count * p.q_heads; e += ctas * kWarps) {
-      const int er = e / p.q_heads, head = e - er * p.q_heads;
-      if (listed_well && indptr[er + 1] > indptr[er]) continue;
-      const int tok = row_of(er);
-      Row<HD> row;
-      if (SHARED) row = prefix_row<HD>(f, p.kv_heads, group, head / group, er, head % group);
-      if (tok >= 0) row.finish(out + (static_cast<long long>(tok) * p.q_heads + head) * HD);
-    }
+// Joins the states of requests that lie in more than one range, a warp to each (range that one begins in, head).
+template <int HD>
+__global__ void __launch_bounds__(128) attn_join_parts_q8_kernel(nfk_attn_q8_params p, const DecodeRecord* records, States parts, int n_ranges) {
+  const int e = blockIdx.x * 4 + (threadIdx.x >> 5), group = p.q_heads / p.kv_heads, range = e / group, h = e - range * group;
+  await_previous();
+  if (range >= n_ranges) return;
+  const int4 raw = __ldcg(reinterpret_cast<const int4*>(records) + range);
+  const DecodeRecord rec = {raw.x, raw.y, raw.z, raw.w};
+  if (rec.n == 0) return;
+  const Row<HD> row = sum_states<HD>(rec.n, [&](int i) { return parts.at<HD>((static_cast<long long>(range + i) * 2 + (i == 0 ? 1 : 0)) * group + h); });
+  if (rec.tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(rec.tok) * p.q_heads + rec.kvh * group + h) * HD);
+}
 
-  // ---- pieces of the CTA's warps, joined request by request. Of a request that goes on in another CTA a part is left in the
-  // workspace: at most one that began before this CTA's pages (side 0) and one that begins in them (side 1). ----
-  bool left = false;
-  for (int first = 0; first < 2 * kWarps; ++first) {
-    const Piece piece = pieces[first];
-    if (piece.flags == 0) continue;
-    int last = first;
-    for (int k = first + 1; k < 2 * kWarps; ++k)
-      if (pieces[k].flags != 0) {
-        if (pieces[k].kvh != piece.kvh || pieces[k].r != piece.r) break;
-        last = k;
-      }
-    const bool starts = (piece.flags & 2) != 0, ends = (pieces[last].flags & 4) != 0, inside = starts && ends;
-    if (!inside && threadIdx.x == kThreads - 1) {            // the CTAs that hold parts of the request follow from the ranges
-      const int c0 = ranges.of(piece.kvh * pages_all + piece.begin) / kWarps, c1 = ranges.of(piece.kvh * pages_all + piece.end - 1) / kWarps;
-      parts[starts ? 1 : 0] = Part{piece.kvh, piece.r, piece.tok, c0, c1 - c0 + 1, 0};
+// The same row by row, with the shared prefix's states where there is one, and WARPS warps to a row: a context of 900 tokens is 29
+// pieces for each of 32 heads, one of 100000 tokens 296.
+template <int HD, int WARPS>
+__global__ void __launch_bounds__(128)
+attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_lists, States parts, States wholes, int decode_ctas) {
+  __shared__ float shared_ml[4][2];
+  __shared__ float shared_o[4][HD];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = warp % WARPS;
+  const int group = p.q_heads / p.kv_heads;
+  const int* indptr = p.kv_indptr + p.req_begin;
+  // lists and their cut while the kernels before this one still run: they do not write them
+  const int e = blockIdx.x * (4 / WARPS) + warp / WARPS;
+  const bool on = e < p.req_count * p.q_heads;
+  const int r = on ? e / p.q_heads : 0, head = on ? e - r * p.q_heads : 0, kvh = head / group, h = head - kvh * group;
+  const int base = indptr[0], pages_all = indptr[p.req_count] - base, begin = indptr[r] - base, end = indptr[r + 1] - base;
+  int tok = p.qo_indptr[p.req_begin + r];
+  const bool tok_ok = tok >= 0 && tok < p.num_tokens;
+  if (!tok_ok) tok = -1;
+  const Ranges ranges(pages_all * p.kv_heads, decode_ranges(pages_all * p.kv_heads, decode_ctas));
+  int k0 = 0, n_own = 0, c0 = 0, n_all = 0, item = 0, in_block = 0;
+  await_previous();
+  if (on) {
+    if (!tok_ok && lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
+    if (*bad_lists == 0 && end > begin) {
+      k0 = ranges.of(kvh * pages_all + begin);
+      n_own = ranges.of(kvh * pages_all + end - 1) - k0 + 1;
     }
-    left = left || !inside;
-    for (int h = warp; h < group; h += kWarps) {
-      Row<HD> row;
-      for (int k = first; k <= last; ++k) {
-        if (pieces[k].flags == 0) continue;
-        Row<HD> one;
-        one.read(piece_at(k), group, h);
-        row.add(one);
-      }
-      if (inside) {
-        if (SHARED) row.add(prefix_row<HD>(f, p.kv_heads, group, piece.kvh, piece.r, h));
-        if (piece.tok >= 0) row.finish(out + (static_cast<long long>(piece.tok) * p.q_heads + piece.kvh * group + h) * HD);
-      } else {
-        const long long to = (static_cast<long long>(blockIdx.x) * 2 + (starts ? 1 : 0)) * group + h;
-        row.store(part_ml + to * 2, part_o + to * HD);
-      }
-    }
-    first = last;
-  }
-  if (left) {
-    __syncthreads();
-    if (threadIdx.x < 2 && parts[threadIdx.x].n > 0) {
-      Part& part = parts[threadIdx.x];
-      __threadfence();
-      if (atomicAdd(counts + part.first, 1u) == static_cast<unsigned int>(part.n - 1)) {
-        counts[part.first] = 0u;
-        part.last = 1;
-        __threadfence();
-      }
-    }
-    __syncthreads();
-    // the last of a request's parts to be left: all of them, in their order
-    for (int side = 0; side < 2; ++side) {
-      const Part part = parts[side];
-      if (part.n == 0 || part.last == 0) continue;
-      for (int h = warp; h < group; h += kWarps) {
-        Row<HD> row = sum_rows<HD>(part_ml, part_o, part.n,
-                                   [&](int i) { return (static_cast<long long>(part.first + i) * 2 + (i == 0 ? 1 : 0)) * group + h; });
-        if (SHARED) row.add(prefix_row<HD>(f, p.kv_heads, group, part.kvh, part.r, h));
-        if (part.tok >= 0) row.finish(out + (static_cast<long long>(part.tok) * p.q_heads + part.kvh * group + h) * HD);
-      }
+    n_all = n_own;
+    if (p.prefix_len > 0) {
+      const Ranges prefix(prefix_units(f, p.kv_heads), f.ctas);
+      const int in = r / f.reqs_per_block;
+      item = kvh * f.blocks + in;
+      in_block = (r - in * f.reqs_per_block) * group + h;
+      c0 = prefix.of(item * f.tiles);
+      n_all += prefix.of((item + 1) * f.tiles - 1) - c0 + 1;
     }
   }
+  if (p.prefix_len == 0 && n_own <= 1) tok = -1, n_all = 0;    // the row has been written
+  // all states of the row, WARPS shares of them one after the other
+  const int a = static_cast<int>(static_cast<long long>(n_all) * which / WARPS), b = static_cast<int>(static_cast<long long>(n_all) * (which + 1) / WARPS);
+  Row<HD> row = sum_states<HD>(b - a, [&](int i) {
+    const int k = a + i;
+    if (k >= n_own) return State{f.ml + (static_cast<long long>(item + c0 + k - n_own) * kPrefixRows + in_block) * 2,
+                                 f.o + (static_cast<long long>(item + c0 + k - n_own) * kPrefixRows + in_block) * HD};
+    if (n_own == 1) return wholes.at<HD>(e);
+    return parts.at<HD>((static_cast<long long>(k0 + k) * 2 + (k == 0 ? 1 : 0)) * group + h);
+  });
+  if (WARPS > 1) {
+#pragma unroll
+    for (int i = 0; i < Row<HD>::N; ++i) shared_o[warp][lane * Row<HD>::N + i] = row.o[i];
+    if (lane == 0) {
+      shared_ml[warp][0] = row.m;
+      shared_ml[warp][1] = row.l;
+    }
+    __syncthreads();
+    if (which == 0)
+      for (int k = 1; k < WARPS; ++k) {
+        Row<HD> other;
+        other.m = shared_ml[warp + k][0];
+        other.l = shared_ml[warp + k][1];
+#pragma unroll
+        for (int i = 0; i < Row<HD>::N; ++i) other.o[i] = shared_o[warp + k][lane * Row<HD>::N + i];
+        row.add(other);
+      }
+  }
+  if (which == 0 && tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(tok) * p.q_heads + head) * HD);
+}
+
+// CTAs of an SM that fit, for a kernel with `bytes` of shared memory; 0: an error.
+int fitting(const void* kernel, int threads, int bytes) {
+  int per_sm = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, bytes) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return 0;
+  }
+  return per_sm;
 }
 
 template <int HD, int NT, int KIND, bool SHARED>
-int launch_decode(const nfk_attn_q8_params& p, const PrefixPlan& f, const Q8Workspace& ws, cudaStream_t stream) {
+int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, int* bad_lists, DecodeRecord* records, const States& parts, const States& wholes,
+           cudaStream_t stream) {
   constexpr int bytes = kWarps * Dec<HD>::kWarpBytes;
-  static int fit_dev[kMaxDevices] = {0};                       // CTAs that fit an SM
-  int& fit = fit_dev[device_slot()];
   const auto kernel = attn_decode_q8_kernel<HD, NT, KIND, SHARED>;
-  if (fit == 0) {
-    int per_sm = 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess ||
-        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kThreads, bytes) != cudaSuccess || per_sm < 1) {
-      (void)cudaGetLastError();
+  static int fit_dev[kMaxDevices] = {0};
+  int& fit = fit_dev[device_slot()];
+  if (fit == 0) fit = fitting(reinterpret_cast<const void*>(kernel), kThreads, bytes);
+  if (fit == 0) return NF_ERR_CUDA;
+  const int sms = device_sm_count(), room = (fit < kDecodeCtasPerSm ? fit : kDecodeCtasPerSm) * sms;
+  const int useful = decode_ranges(p.num_indices * p.kv_heads, room);
+  int ctas = (useful + kWarps - 1) / kWarps;
+  if (ctas < 1) ctas = 1;
+  if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
+  const auto done = [](cudaError_t e) {
+    if (e == cudaSuccess) return true;
+    (void)cudaGetLastError();
+    return false;
+  };
+  if (!done(launch_kernel(SHARED, kernel, ctas, kThreads, bytes, stream, 1, p, bad_lists, records, parts, wholes))) return NF_ERR_CUDA;
+  // Few rows: four warps to each, since there are many pieces to a row then. With a prefix every row has states to join. Else the
+  // pieces lead to the rows, of which most lie in one range.
+  const int rows = p.req_count * p.q_heads;
+  if (rows <= 8 * sms) {
+    if (!done(launch_kernel(true, attn_join_rows_q8_kernel<HD, 4>, rows, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, ctas))) return NF_ERR_CUDA;
+  } else if (SHARED) {
+    if (!done(launch_kernel(true, attn_join_rows_q8_kernel<HD, 1>, (rows + 3) / 4, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, ctas)))
       return NF_ERR_CUDA;
-    }
-    fit = per_sm < kDecodeCtasPerSm ? per_sm : kDecodeCtasPerSm;
+  } else {
+    const int group = p.q_heads / p.kv_heads;
+    if (!done(launch_kernel(true, attn_join_parts_q8_kernel<HD>, ctas * group, 128, 0, stream, 1, p, records, parts, ctas * kWarps))) return NF_ERR_CUDA;
   }
-  const long long room = static_cast<long long>(fit) * device_sm_count();
-  long long ctas = p.num_ctas > 0 && p.num_ctas < room ? p.num_ctas : room;
-  const long long work = static_cast<long long>(p.num_indices) * p.kv_heads + static_cast<long long>(p.req_count) * p.q_heads;
-  const long long useful = (work + kWarps - 1) / kWarps;
-  if (ctas > useful) ctas = useful;
-  char* base = static_cast<char*>(p.workspace);
-  if (launch_kernel(SHARED, kernel, static_cast<int>(ctas), kThreads, bytes, stream, 1, p, f, reinterpret_cast<unsigned int*>(base + ws.counts),
-                    reinterpret_cast<float*>(base + ws.ml), reinterpret_cast<float*>(base + ws.o), reinterpret_cast<float*>(base + ws.kept)) == cudaSuccess)
-    return NF_OK;
-  (void)cudaGetLastError();
-  return NF_ERR_CUDA;
+  return NF_OK;
 }
 
-template <int HD, int NT, int KIND>
-int launch_decode(const nfk_attn_q8_params& p, const PrefixPlan& f, const Q8Workspace& ws, cudaStream_t stream) {
-  return p.prefix_len > 0 ? launch_decode<HD, NT, KIND, true>(p, f, ws, stream) : launch_decode<HD, NT, KIND, false>(p, f, ws, stream);
+template <int HD, int NT, int KIND, class... A>
+int launch(const nfk_attn_q8_params& p, const A&... a) {
+  return p.prefix_len > 0 ? launch<HD, NT, KIND, true>(p, a...) : launch<HD, NT, KIND, false>(p, a...);
 }
-template <int HD>
-int launch_decode(const nfk_attn_q8_params& p, const PrefixPlan& f, const Q8Workspace& ws, cudaStream_t stream) {
+template <int HD, class... A>
+int launch(const nfk_attn_q8_params& p, const A&... a) {
   const bool wide = p.q_heads / p.kv_heads > 8;
-  if (p.kind == NFK_Q8_E4M3) return wide ? launch_decode<HD, 2, NFK_Q8_E4M3>(p, f, ws, stream) : launch_decode<HD, 1, NFK_Q8_E4M3>(p, f, ws, stream);
-  return wide ? launch_decode<HD, 2, NFK_Q8_INT8>(p, f, ws, stream) : launch_decode<HD, 1, NFK_Q8_INT8>(p, f, ws, stream);
+  if (p.kind == NFK_Q8_E4M3) return wide ? launch<HD, 2, NFK_Q8_E4M3>(p, a...) : launch<HD, 1, NFK_Q8_E4M3>(p, a...);
+  return wide ? launch<HD, 2, NFK_Q8_INT8>(p, a...) : launch<HD, 1, NFK_Q8_INT8>(p, a...);
 }
 
 bool sizes_built(const nfk_attn_q8_params& p) {
@@ -633,8 +622,7 @@ bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 
 extern "C" long long nfk_attn_q8_workspace(const nfk_attn_q8_params* p) {
   using namespace nf;
   if (p == nullptr || !sizes_built(*p) || p->req_count < 0 || p->prefix_len < 0) return 0;
-  const PrefixPlan f = prefix_plan(*p);
-  return q8_workspace(p->q_heads / p->kv_heads, p->head_dim, static_cast<long long>(p->kv_heads) * f.blocks + f.ctas).bytes;
+  return q8_workspace(*p, prefix_plan(*p)).bytes;
 }
 
 extern "C" int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream) {
@@ -649,13 +637,19 @@ extern "C" int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stre
       !aligned16(p->kv_scale) || (reinterpret_cast<uintptr_t>(p->workspace) & 255) != 0)
     return NF_ERR_BAD_ARG;
   PrefixPlan f = prefix_plan(*p);
-  const Q8Workspace ws = q8_workspace(p->q_heads / p->kv_heads, p->head_dim, static_cast<long long>(p->kv_heads) * f.blocks + f.ctas);
+  const Q8Workspace ws = q8_workspace(*p, f);
   if (p->workspace_bytes < ws.bytes) return NF_ERR_BAD_ARG;
-  f.ml = reinterpret_cast<const float*>(static_cast<const char*>(p->workspace) + ws.prefix_ml);
-  f.o = reinterpret_cast<const float*>(static_cast<const char*>(p->workspace) + ws.prefix_o);
+  char* base = static_cast<char*>(p->workspace);
+  const auto at = [&](long long offset) { return reinterpret_cast<float*>(base + offset); };
+  f.ml = at(ws.prefix_ml);
+  f.o = at(ws.prefix_o);
   if (p->prefix_len > 0) {
     const int rc = launch_prefix_q8(*p, f, stream);
     if (rc != NF_OK) return rc;
   }
-  return p->head_dim == 128 ? launch_decode<128>(*p, f, ws, stream) : launch_decode<64>(*p, f, ws, stream);
+  int* bad_lists = reinterpret_cast<int*>(base);
+  DecodeRecord* records = reinterpret_cast<DecodeRecord*>(base + ws.records);
+  const States parts = {at(ws.ml), at(ws.o)}, wholes = {at(ws.whole_ml), at(ws.whole_o)};
+  return p->head_dim == 128 ? launch<128>(*p, f, bad_lists, records, parts, wholes, stream)
+                            : launch<64>(*p, f, bad_lists, records, parts, wholes, stream);
 }

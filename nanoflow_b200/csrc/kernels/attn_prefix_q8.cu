@@ -198,7 +198,7 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
 
 template <int HD, int KIND>
 __global__ void __launch_bounds__(kThreads, 2)
-attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, float* part_ml, float* part_o) {
+attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
   using C = Pre<HD>;
   constexpr int NH = C::NH;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -433,14 +433,14 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, float* part_ml, float*
         tmem_ld_32x32b_x32(t_o + c * 32, v);
         tmem_ld_wait();
         if (tok >= 0) {
-          float4* dst = reinterpret_cast<float4*>(part_o + at * HD + c * 32);
+          float4* dst = reinterpret_cast<float4*>(f.o + at * HD + c * 32);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             __stcg(dst + j, make_float4(__uint_as_float(v[4 * j]) * back, __uint_as_float(v[4 * j + 1]) * back, __uint_as_float(v[4 * j + 2]) * back,
                                         __uint_as_float(v[4 * j + 3]) * back));
         }
       }
-      if (tok >= 0) __stcg(reinterpret_cast<float2*>(part_ml) + at, make_float2(ref, l));
+      if (tok >= 0) __stcg(reinterpret_cast<float2*>(f.ml) + at, make_float2(ref, l));
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[O_FREE]);
@@ -464,7 +464,7 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, cudaStream_t stream
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Pre<HD>::kBytes) != cudaSuccess) return NF_ERR_CUDA;
     attr = true;
   }
-  if (launch_kernel(false, kernel, f.ctas, kThreads, Pre<HD>::kBytes, stream, 1, p, f, const_cast<float*>(f.ml), const_cast<float*>(f.o)) == cudaSuccess)
+  if (launch_kernel(false, kernel, f.ctas, kThreads, Pre<HD>::kBytes, stream, 1, p, f) == cudaSuccess)
     return NF_OK;
   (void)cudaGetLastError();
   return NF_ERR_CUDA;

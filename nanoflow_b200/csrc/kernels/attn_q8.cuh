@@ -28,29 +28,42 @@ struct Ranges {
 constexpr int kPrefixTile = 64, kPrefixRows = 128;
 struct PrefixPlan {
   int reqs_per_block, blocks, tiles, ctas;
-  const float* o;            // [pieces][128 rows][head_dim], not divided by the sum
-  const float* ml;           // [pieces][128 rows][2]: reference (of exponents to base 2), sum
+  float* ml;                 // states, [pieces][128 rows]: reference (of exponents to base 2) and sum,
+  float* o;                  // [pieces][128 rows][head_dim], not divided by the sum
 };
 __host__ __device__ __forceinline__ int prefix_units(const PrefixPlan& f, int kv_heads) { return kv_heads * f.blocks * f.tiles; }
 
-constexpr int kDecodeCtasPerSm = 4, kDecodeWarps = 4;      // of the decode kernel: at most, of so many warps
-
-// Where things lie in the workspace, in this order: counts of pieces that have been left, partial rows of the decode kernel's CTAs
-// (two requests each), rows that its warps keep (two requests each), the prefix's pieces.
-struct Q8Workspace {
-  long long counts, ml, o, kept, prefix_ml, prefix_o, bytes;
+// The row of pages of the decode kernel is cut into a range for each of its warps, of two pages at least.
+constexpr int kDecodeCtasPerSm = 4, kDecodeWarps = 4;      // at most, of so many warps
+__host__ __device__ __forceinline__ int decode_ranges(int units, int ctas) {
+  const int most = ctas * kDecodeWarps, useful = (units + 1) / 2;
+  return useful < most ? useful : most;
+}
+// What a range leaves for the kernel that joins states: the request that begins in it and goes on behind it, if there is one.
+struct DecodeRecord {
+  int kvh, r, tok, n;        // n: ranges that hold parts of it; 0: no such request
 };
-inline Q8Workspace q8_workspace(int group, int head_dim, long long prefix_pieces) {
+
+// Where things lie in the workspace: a word that says whether the page lists are none, a record for each range, states of the
+// decode kernel's pieces (two a range), of whole requests that wait for the prefix's share, and the prefix's.
+struct Q8Workspace {
+  long long records, ml, o, whole_ml, whole_o, prefix_ml, prefix_o, bytes;
+};
+inline Q8Workspace q8_workspace(const nfk_attn_q8_params& p, const PrefixPlan& f) {
   Q8Workspace w;
-  const long long ctas = static_cast<long long>(kDecodeCtasPerSm) * device_sm_count();
+  const int group = p.q_heads / p.kv_heads;
+  const long long ranges = static_cast<long long>(kDecodeCtasPerSm) * kDecodeWarps * device_sm_count(), pieces = 2 * ranges * group;
+  const long long whole = p.prefix_len > 0 ? static_cast<long long>(p.req_count) * p.q_heads : 0;
+  const long long prefix = (static_cast<long long>(p.kv_heads) * f.blocks + f.ctas) * kPrefixRows;
   const auto up = [](long long x) { return (x + 255) / 256 * 256; };
-  w.counts = 0;
-  w.ml = up(ctas * 4);
-  w.o = w.ml + up(ctas * 2 * group * 8);
-  w.kept = w.o + up(ctas * 2 * group * head_dim * 4ll);
-  w.prefix_ml = w.kept + up(2 * ctas * kDecodeWarps * group * (head_dim + 2) * 4ll);
-  w.prefix_o = w.prefix_ml + up(prefix_pieces * kPrefixRows * 8);
-  w.bytes = w.prefix_o + prefix_pieces * kPrefixRows * head_dim * 4;
+  w.records = 256;
+  w.ml = w.records + up(ranges * static_cast<long long>(sizeof(DecodeRecord)));
+  w.o = w.ml + up(pieces * 8);
+  w.whole_ml = w.o + up(pieces * p.head_dim * 4);
+  w.whole_o = w.whole_ml + up(whole * 8);
+  w.prefix_ml = w.whole_o + up(whole * p.head_dim * 4);
+  w.prefix_o = w.prefix_ml + up(prefix * 8);
+  w.bytes = w.prefix_o + prefix * p.head_dim * 4;
   return w;
 }
 PrefixPlan prefix_plan(const nfk_attn_q8_params& p);

@@ -228,7 +228,6 @@ def test_decode(kind, heads, kv_heads, dim, lengths):
         _check_rows(out, ref.attn_decode_q8(q, pool, scale, qo, ptr, idx, last, q_heads=heads, req_begin=0, req_count=len(n)), dim)
     other = [r for r in range(len(n) + 2) if r not in rows.tolist()]
     assert bool((out[other] == 3).all())
-    assert not bool(ws[:4 * 592].any())
 
 
 @pytest.mark.parametrize("ctas", [1, 3, 37])
