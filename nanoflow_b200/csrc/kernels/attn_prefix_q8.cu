@@ -9,8 +9,8 @@
 //   warps 0-3   softmax: a thread per query row. They also bring their rows of Q into shared memory, as f16 with a power of two
 //               per row (see attn_decode_q8.cu).
 //   warp 4      tcgen05.mma: S(t+1) = Q K(t+1)^T is issued before P(t) is waited for; O += P(t) V(t) takes P from tensor memory
-//   warp 5, 6   keys / values: 8-bit numbers from their pages, a tile ahead in registers, to exact f16 in shared memory (128-byte
-//               swizzle; V stays token-major, an MN-major operand), and the tile's scales beside them
+//   warps 5-8   two for keys, two for values, half a tile each: 8-bit numbers from their pages, a tile ahead in registers, to exact
+//               f16 in shared memory (128-byte swizzle; V stays token-major, an MN-major operand), and the tile's scales beside them
 //
 // Scores are S times the key's scale, in fp32. Weights are rounded to f16 times the value's scale relative to the largest one so
 // far, as in attn_decode_q8.cu; O is brought to a new reference where a row's maximum grows by 2^8 or that largest scale grows.
@@ -19,7 +19,7 @@
 namespace nf {
 namespace {
 
-constexpr int kThreads = 224;
+constexpr int kThreads = 288;
 constexpr int kTile = kPrefixTile;
 constexpr float kGap = 8.f, kHeadroom = 128.f;
 constexpr int kHalfBytes = kTile * 128;          // [64 tokens][64 elements]
@@ -82,13 +82,16 @@ struct Share {
   }
 };
 
-// Keys (PART 0) or values (PART 1) of the CTA's tiles, by one warp.
+// Keys (PART 0) or values (PART 1) of the CTA's tiles: tokens 32 half .. 32 half + 31 of each, by one warp.
 template <int HD, int KIND, int PART>
-__device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const PrefixPlan& f, uint32_t sb, float* scales, float* v_refs,
+__device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const PrefixPlan& f, int half, uint32_t sb, float* scales, float* v_refs,
                                             uint64_t* bars, volatile int* abort_flag) {
   using C = Pre<HD>;
-  constexpr int LANES = HD / 16, AT_ONCE = 32 / LANES, NI = kTile / AT_ONCE;    // lanes of a token, tokens of a load, loads
-  const int lane = threadIdx.x & 31, c = lane % LANES, row = lane / LANES;
+  constexpr int LANES = HD / 16, AT_ONCE = 32 / LANES, NI = 32 / AT_ONCE;       // lanes of a token, tokens of a load, loads
+  const int lane = threadIdx.x & 31, c = lane % LANES;
+  // head_dim 128: the lanes of the row's second half take the neighbouring token's, so that the two halves (which lie 8 KB apart)
+  // are stored to different banks
+  const int row = half * 32 + ((lane / LANES) ^ (c >> 2));
   const uint8_t* pool = static_cast<const uint8_t*>(p.kv_pool);
   const int n_pages = (p.prefix_len + kQ8Page - 1) / kQ8Page;
   uint64_t* full = bars + (PART == 0 ? K_FULL0 : V_FULL0);
@@ -154,7 +157,7 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
         *abort_flag = 1;
         return;
       }
-      const uint32_t stage = sb + (PART == 0 ? C::kK : C::kV) + s * C::kStage;
+      const uint32_t stage = sb + (PART == 0 ? C::kK : C::kV) + s * C::kStage + (c >> 2) * kHalfBytes;
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
         const int tok = n * AT_ONCE + row;
@@ -165,28 +168,22 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
         q8_to_f16<KIND>(raw[n].w, o[6], o[7]);
         // what lies behind the prefix may be anything: as values it would spoil every row (as keys it is masked)
         if (PART == 1 && tok >= valid) o[0] = o[1] = o[2] = o[3] = o[4] = o[5] = o[6] = o[7] = 0u;
-        const uint32_t to = stage + (c >> 2) * kHalfBytes + tok * 128;
-        const uint32_t c0 = (2 * (c & 3)) ^ (tok & 7);
-        const bool swap = (c & 4) != 0;                          // the two halves' lanes on different banks
-        st_shared_v4(to + ((swap ? c0 ^ 1 : c0) << 4), swap ? o[4] : o[0], swap ? o[5] : o[1], swap ? o[6] : o[2], swap ? o[7] : o[3]);
-        st_shared_v4(to + ((swap ? c0 : c0 ^ 1) << 4), swap ? o[0] : o[4], swap ? o[1] : o[5], swap ? o[2] : o[6], swap ? o[3] : o[7]);
+        const uint32_t to = stage + tok * 128, c0 = (2 * (c & 3)) ^ (tok & 7);
+        st_shared_v4(to + (c0 << 4), o[0], o[1], o[2], o[3]);
+        st_shared_v4(to + ((c0 ^ 1) << 4), o[4], o[5], o[6], o[7]);
         if (more) load(n, at);
       }
-      float* dst = scales + (PART * 4 + (g & 3)) * kTile;
+      float* dst = scales + (PART * 4 + (g & 3)) * kTile + half * 32;
       if (PART == 0) {
-        const float scale = p.sm_scale * kQ8Log2e;
-        dst[lane] = sc[0] * scale;
-        dst[lane + 32] = sc[1] * scale;
+        dst[lane] = sc[half] * (p.sm_scale * kQ8Log2e);
       } else {
         const float a = lane < valid ? sc[0] : 0.f, b = lane + 32 < valid ? sc[1] : 0.f;
         float most = fmaxf(a, b);
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
         if (most > v_ref) v_ref = __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0xff800000u);   // the next power of two
-        const float unit = kHeadroom / v_ref;
-        dst[lane] = a * unit;
-        dst[lane + 32] = b * unit;
-        if (lane == 0) v_refs[g & 3] = v_ref;
+        dst[lane] = (half == 0 ? a : b) * (kHeadroom / v_ref);
+        if (lane == 0 && half == 0) v_refs[g & 3] = v_ref;
       }
       if (more) load_scales(at);
       fence_proxy_async_smem();
@@ -214,7 +211,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     return;
   }
   if (threadIdx.x == 0) {
-    for (int b = 0; b < NUM_BARS; ++b) mbar_init(&bars[b], b == Q_FULL || b == P_FULL0 || b == P_FULL1 || b == O_FREE ? 4 : 1);
+    for (int b = 0; b < NUM_BARS; ++b) mbar_init(&bars[b], b == Q_FULL || b == P_FULL0 || b == P_FULL1 || b == O_FREE ? 4 : b == K_FULL0 || b == K_FULL1 || b == V_FULL0 || b == V_FULL1 ? 2 : 1);
     *abort_flag = 0;
     mbar_fence_init();
   }
@@ -236,10 +233,10 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     return __all_sync(0xffffffffu, wait_or_abort(&bars[bar], parity, abort_flag)) != 0;
   };
 
-  if (warp == 5) {
-    bring_tiles<HD, KIND, 0>(p, f, sb, scales, v_refs, bars, abort_flag);
-  } else if (warp == 6) {
-    bring_tiles<HD, KIND, 1>(p, f, sb, scales, v_refs, bars, abort_flag);
+  if (warp == 5 || warp == 6) {
+    bring_tiles<HD, KIND, 0>(p, f, warp - 5, sb, scales, v_refs, bars, abort_flag);
+  } else if (warp >= 7) {
+    bring_tiles<HD, KIND, 1>(p, f, warp - 7, sb, scales, v_refs, bars, abort_flag);
   } else if (warp == 4) {
     // ------------------------------------------------------------------ products (the warp walks, an elected lane issues)
     const uint32_t idesc_s = idesc_f16(128, kTile), idesc_o = idesc_f16(128, HD) | kIdescBMnMajor;
@@ -397,25 +394,23 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
         }
         const float ms = ref == -INFINITY ? 0.f : ref;
         float rs = 0.f;
-        uint32_t pk[32];                                         // column j: tokens 2j, 2j + 1
+        auto weights = [&](const uint32_t (&x)[32], const float4* v, uint32_t to) {
+          uint32_t pk[16];                                       // column j: tokens 2j, 2j + 1
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 a = v4[j], b = v4[8 + j];
-          const float va[4] = {a.x, a.y, a.z, a.w}, vb[4] = {b.x, b.y, b.z, b.w};
-          float x[4], y[4];
+          for (int j = 0; j < 8; ++j) {
+            const float4 unit = v[j];
+            float e[4];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[e] = q8_exp2(fmaf(__uint_as_float(r0[4 * j + e]), up, -ms));
-            y[e] = q8_exp2(fmaf(__uint_as_float(r1[4 * j + e]), up, -ms));
-            rs += x[e] + y[e];
+            for (int k = 0; k < 4; ++k) e[k] = q8_exp2(fmaf(__uint_as_float(x[4 * j + k]), up, -ms));
+            rs += (e[0] + e[1]) + (e[2] + e[3]);
+            pk[2 * j] = pack_f16x2(e[0] * unit.x, e[1] * unit.y);
+            pk[2 * j + 1] = pack_f16x2(e[2] * unit.z, e[3] * unit.w);
           }
-          pk[2 * j] = pack_f16x2(x[0] * va[0], x[1] * va[1]);
-          pk[2 * j + 1] = pack_f16x2(x[2] * va[2], x[3] * va[3]);
-          pk[16 + 2 * j] = pack_f16x2(y[0] * vb[0], y[1] * vb[1]);
-          pk[16 + 2 * j + 1] = pack_f16x2(y[2] * vb[2], y[3] * vb[3]);
-        }
+          tmem_st_32x32b_x16(to, pk);
+        };
+        weights(r0, v4, t_lane + s * kTile);
+        weights(r1, v4 + 8, t_lane + s * kTile + 16);
         l += rs;
-        tmem_st_32x32b_x32(t_lane + s * kTile, pk);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
