@@ -1,8 +1,9 @@
 """In-tree build of the native code: the sm_100a kernel library and the C++ executor module.
 
 ``python -m nanoflow_b200.ops.build`` compiles every ``csrc/kernels/*.cu`` with
-``nvcc -gencode arch=compute_100a,code=sm_100a`` into ``nanoflow_b200/ops/libnanoflow_kernels.so``
-and ``csrc/executor/*.cpp`` into ``nanoflow_b200/runtime/_executor*.so``. Objects are cached under
+``nvcc -gencode arch=compute_100a,code=sm_100a`` into ``nanoflow_b200/ops/libnanoflow_kernels.so``,
+``csrc/executor/*.cpp`` into ``nanoflow_b200/runtime/_executor*.so`` and ``csrc/calls/*.cpp`` (calls that check torch
+tensors in C++) into ``nanoflow_b200/ops/_*.so``. Objects are cached under
 ``build/`` and rebuilt only when a source or header is newer. nvcc cross-compiles without a GPU.
 
 The reference builds with CMake for sm_80 (pipeline/CMakeLists.txt:5-8, gemv/CMakeLists.txt:8);
@@ -21,6 +22,7 @@ PKG = Path(__file__).resolve().parent.parent
 ROOT = PKG.parent
 KERNEL_DIR = PKG / "csrc" / "kernels"
 EXEC_DIR = PKG / "csrc" / "executor"
+CALLS_DIR = PKG / "csrc" / "calls"
 BUILD_DIR = ROOT / "build"
 KERNEL_LIB = PKG / "ops" / "libnanoflow_kernels.so"
 
@@ -126,8 +128,24 @@ def build_executor_host(verbose: bool = False, sanitize: str = "") -> Path:
     return out
 
 
+def build_calls(verbose: bool = False) -> None:
+    """``csrc/calls/<name>.cpp`` -> the extension module ``nanoflow_b200.ops._<name>``, against the installed torch."""
+    import torch
+
+    home = Path(torch.__file__).parent
+    suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
+    for src in sorted(CALLS_DIR.glob("*.cpp")):
+        out = PKG / "ops" / f"_{src.stem}{suffix}"
+        if _newer(out, [src, KERNEL_DIR / "kernels.h"]):
+            _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+                  f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", sysconfig.get_paths()["include"],
+                  "-I", home / "include", "-I", home / "include" / "torch" / "csrc" / "api" / "include",
+                  "-I", "/usr/local/cuda/include", "-I", KERNEL_DIR, src, "-o", out, "-L", home / "lib",
+                  "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"], verbose)
+
+
 def build_runtime(verbose: bool = False) -> None:
-    """What running a model needs: the kernel library and the executor, if they are missing or out of date. A
+    """What running a model needs: the kernel library, the executor and the calls, if they are missing or out of date. A
     lock file keeps processes that start together from compiling twice."""
     import fcntl
 
@@ -136,12 +154,14 @@ def build_runtime(verbose: bool = False) -> None:
         fcntl.flock(lock, fcntl.LOCK_EX)
         build_kernels(verbose)
         build_executor(verbose)
+        build_calls(verbose)
 
 
 def build_all(verbose: bool = False) -> None:
     build_kernels(verbose)
     build_executor(verbose)
     build_executor_host(verbose)
+    build_calls(verbose)
 
 
 if __name__ == "__main__":
