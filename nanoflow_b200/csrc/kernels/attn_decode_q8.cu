@@ -96,11 +96,11 @@ struct State {
   const float* ml;
   const float* o;
 };
-// Sum of n states, the i-th being at(i), in their order. Lanes fetch 32 references and sums at a time and 16 rows are requested
+// Sum of n states, the i-th being at(i), in their order. Lanes fetch 32 references and sums at a time and AHEAD rows are requested
 // without waiting for one another.
-template <int HD, class At>
+template <int HD, int AHEAD, class At>
 __device__ __forceinline__ Row<HD> sum_states(int n, At at) {
-  constexpr int N = Row<HD>::N, AHEAD = 16;
+  constexpr int N = Row<HD>::N;
   const int lane = threadIdx.x & 31;
   Row<HD> all;
   for (int i0 = 0; i0 < n; i0 += 32) {
@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(128) attn_join_parts_q8_kernel(nfk_attn_q8_par
   const int4 raw = __ldcg(reinterpret_cast<const int4*>(records) + range);
   const DecodeRecord rec = {raw.x, raw.y, raw.z, raw.w};
   if (rec.n == 0) return;
-  const Row<HD> row = sum_states<HD>(rec.n, [&](int i) { return parts.at<HD>((static_cast<long long>(range + i) * 2 + (i == 0 ? 1 : 0)) * group + h); });
+  const Row<HD> row = sum_states<HD, 8>(rec.n, [&](int i) { return parts.at<HD>((static_cast<long long>(range + i) * 2 + (i == 0 ? 1 : 0)) * group + h); });
   if (rec.tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(rec.tok) * p.q_heads + rec.kvh * group + h) * HD);
 }
 
@@ -525,10 +525,10 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   if (p.prefix_len == 0 && n_own <= 1) tok = -1, n_all = 0;    // the row has been written
   // all states of the row, WARPS shares of them one after the other
   const int a = static_cast<int>(static_cast<long long>(n_all) * which / WARPS), b = static_cast<int>(static_cast<long long>(n_all) * (which + 1) / WARPS);
-  Row<HD> row = sum_states<HD>(b - a, [&](int i) {
+  Row<HD> row = sum_states<HD, WARPS == 1 ? 8 : 16>(b - a, [&](int i) {
     const int k = a + i;
-    if (k >= n_own) return State{f.ml + (static_cast<long long>(item + c0 + k - n_own) * kPrefixRows + in_block) * 2,
-                                 f.o + (static_cast<long long>(item + c0 + k - n_own) * kPrefixRows + in_block) * HD};
+    if (k >= n_own) return State{f.ml + (static_cast<long long>(item + c0 + k - n_own) * f.rows + in_block) * 2,
+                                 f.o + (static_cast<long long>(item + c0 + k - n_own) * f.rows + in_block) * HD};
     if (n_own == 1) return wholes.at<HD>(e);
     return parts.at<HD>((static_cast<long long>(k0 + k) * 2 + (k == 0 ? 1 : 0)) * group + h);
   });

@@ -6,11 +6,13 @@
 // are some ten requests. Items (KV head, block) times tiles of 64 tokens are a row of units that is cut evenly over the CTAs (two
 // to an SM); each leaves a piece per item.
 //
-//   warps 0-3   softmax: a thread per query row. They also bring their rows of Q into shared memory, as f16 with a power of two
-//               per row (see attn_decode_q8.cu).
-//   warp 4      tcgen05.mma: S(t+1) = Q K(t+1)^T is issued before P(t) is waited for; O += P(t) V(t) takes P from tensor memory
-//   warps 5-8   two for keys, two for values, half a tile each: 8-bit numbers from their pages, a tile ahead in registers, to exact
-//               f16 in shared memory (128-byte swizzle; V stays token-major, an MN-major operand), and the tile's scales beside them
+// A block has one or two slots of 128 rows: with two, which share the tiles, a CTA has the SM, with one there are two CTAs.
+//
+//   4 warps a slot  softmax: a thread per query row. They also bring their rows of Q into shared memory, as f16 with a power of two
+//                   per row (see attn_decode_q8.cu).
+//   1 warp          tcgen05.mma: S(t+1) = Q K(t+1)^T is issued before P(t) is waited for; O += P(t) V(t) takes P from tensor memory
+//   2 + 2 warps     keys and values, half a tile each: 8-bit numbers from their pages, a tile ahead in registers, to exact f16 in
+//                   shared memory (128-byte swizzle; V stays token-major, an MN-major operand), and the tile's scales beside them
 //
 // Scores are S times the key's scale, in fp32. Weights are rounded to f16 times the value's scale relative to the largest one so
 // far, as in attn_decode_q8.cu; O is brought to a new reference where a row's maximum grows by 2^8 or that largest scale grows.
@@ -19,25 +21,25 @@
 namespace nf {
 namespace {
 
-constexpr int kThreads = 288;
 constexpr int kTile = kPrefixTile;
 constexpr float kGap = 8.f, kHeadroom = 128.f;
 constexpr int kHalfBytes = kTile * 128;          // [64 tokens][64 elements]
 
-template <int HD>
+template <int HD, int SLOTS>
 struct Pre {
   static constexpr int NH = HD / 64;
-  static constexpr int kQ = 0;                                   // NH x [128 rows][64 elements]
+  static constexpr int kThreads = SLOTS * 128 + 160;
+  static constexpr int kStages = SLOTS == 2 ? 4 : 2, kRing = 2 * kStages;       // tiles of K and of V; of their scales (see there)
+  static constexpr int kQ = 0, kSlot = NH * 16384;               // SLOTS x NH x [128 rows][64 elements]
   static constexpr int kStage = NH * kHalfBytes;                 // a tile of K or V
-  static constexpr int kK = NH * 16384, kV = kK + 2 * kStage;
-  static constexpr int kScales = kV + 2 * kStage;                // [4 tiles][64] of keys, the same of values, [4] v_ref
-  static constexpr int kBars = kScales + 4 * kTile * 8 + 16;
+  static constexpr int kK = SLOTS * kSlot, kV = kK + kStages * kStage;
+  static constexpr int kScales = kV + kStages * kStage;          // [kRing][64] of keys, the same of values, [kRing] v_ref
+  static constexpr int kBars = kScales + kRing * (kTile * 8 + 4);
   static constexpr int kBytes = kBars + 256;
-};
-
-enum Bar : int {
-  Q_FULL = 0, K_FULL0, K_FULL1, K_EMPTY0, K_EMPTY1, V_FULL0, V_FULL1, V_EMPTY0, V_EMPTY1, S_FULL0, S_FULL1, P_FULL0, P_FULL1,
-  PV_DONE0, PV_DONE1, O_FREE, NUM_BARS
+  // barriers
+  static constexpr int Q_FULL = 0, O_FREE = 1, K_FULL = 2, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages, V_EMPTY = V_FULL + kStages,
+                       S_FULL = V_EMPTY + kStages, P_FULL = S_FULL + 2 * SLOTS, PV_DONE = P_FULL + 2 * SLOTS, kNumBars = PV_DONE + 2 * SLOTS;
+  static_assert(kBars % 8 == 0 && kNumBars * 8 + 8 <= 256, "room for the barriers");
 };
 
 // MN-major operand in the 128-byte swizzle: 64 elements along N are one 128-byte row per k index, `lbo` bytes lead to the next 64,
@@ -59,6 +61,39 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+
+// Two fp32 operations by one instruction.
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 halves(f32x2 x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // A CTA's share of the units, one item after the other.
@@ -83,10 +118,10 @@ struct Share {
 };
 
 // Keys (PART 0) or values (PART 1) of the CTA's tiles: tokens 32 half .. 32 half + 31 of each, by one warp.
-template <int HD, int KIND, int PART>
+template <int HD, int SLOTS, int KIND, int PART>
 __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const PrefixPlan& f, int half, uint32_t sb, float* scales, float* v_refs,
                                             uint64_t* bars, volatile int* abort_flag) {
-  using C = Pre<HD>;
+  using C = Pre<HD, SLOTS>;
   constexpr int LANES = HD / 16, AT_ONCE = 32 / LANES, NI = 32 / AT_ONCE;       // lanes of a token, tokens of a load, loads
   const int lane = threadIdx.x & 31, c = lane % LANES;
   // head_dim 128: the lanes of the row's second half take the neighbouring token's, so that the two halves (which lie 8 KB apart)
@@ -94,8 +129,8 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
   const int row = half * 32 + ((lane / LANES) ^ (c >> 2));
   const uint8_t* pool = static_cast<const uint8_t*>(p.kv_pool);
   const int n_pages = (p.prefix_len + kQ8Page - 1) / kQ8Page;
-  uint64_t* full = bars + (PART == 0 ? K_FULL0 : V_FULL0);
-  uint64_t* empty = bars + (PART == 0 ? K_EMPTY0 : V_EMPTY0);
+  uint64_t* full = bars + (PART == 0 ? C::K_FULL : C::V_FULL);
+  uint64_t* empty = bars + (PART == 0 ? C::K_EMPTY : C::V_EMPTY);
   uint4 raw[NI];
   float sc[2];
   // lane j < 4: the vectors of page j of the tile, -1 where there is none
@@ -138,21 +173,24 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
     --left;
     return true;
   };
+  // numbers are requested a tile ahead, page numbers two
   if (advance()) {
-    const long long at = page_of(ahead.kvh, tile_ahead);
+    const long long first = page_of(ahead.kvh, tile_ahead);
 #pragma unroll
-    for (int n = 0; n < NI; ++n) load(n, at);
-    load_scales(at);
+    for (int n = 0; n < NI; ++n) load(n, first);
+    load_scales(first);
   }
+  bool more = advance();
+  long long at = more ? page_of(ahead.kvh, tile_ahead) : -1;
   uint32_t g = 0;
   while (now.next()) {
     float v_ref = 7.8886091e-31f;                                // 2^-100
     for (int t = 0; t < now.n; ++t, ++g) {
-      const int s = g & 1;
+      const int s = g % C::kStages, ring = g % C::kRing;
       const int valid = p.prefix_len - (now.t0 + t) * kTile;     // tokens of the tile
-      const bool more = advance();
-      const long long at = more ? page_of(ahead.kvh, tile_ahead) : -1;
-      if (!__all_sync(0xffffffffu, wait_or_abort(&empty[s], ((g >> 1) & 1) ^ 1, abort_flag))) {
+      const bool more_then = more && advance();
+      const long long at_then = more_then ? page_of(ahead.kvh, tile_ahead) : -1;
+      if (!__all_sync(0xffffffffu, wait_or_abort(&empty[s], (g / C::kStages & 1) ^ 1, abort_flag))) {
         if (lane == 0) report_status(p.status, NF_ST_TIMEOUT_SMEM_EMPTY);
         *abort_flag = 1;
         return;
@@ -173,7 +211,7 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
         st_shared_v4(to + ((c0 ^ 1) << 4), o[4], o[5], o[6], o[7]);
         if (more) load(n, at);
       }
-      float* dst = scales + (PART * 4 + (g & 3)) * kTile + half * 32;
+      float* dst = scales + (PART * C::kRing + ring) * kTile + half * 32;
       if (PART == 0) {
         dst[lane] = sc[half] * (p.sm_scale * kQ8Log2e);
       } else {
@@ -183,9 +221,11 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
         for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
         if (most > v_ref) v_ref = __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0xff800000u);   // the next power of two
         dst[lane] = (half == 0 ? a : b) * (kHeadroom / v_ref);
-        if (lane == 0 && half == 0) v_refs[g & 3] = v_ref;
+        if (lane == 0 && half == 0) v_refs[ring] = v_ref;
       }
       if (more) load_scales(at);
+      more = more_then;
+      at = at_then;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[s]);
@@ -193,17 +233,17 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
   }
 }
 
-template <int HD, int KIND>
-__global__ void __launch_bounds__(kThreads, 2)
+template <int HD, int SLOTS, int KIND>
+__global__ void __launch_bounds__(SLOTS * 128 + 160, SLOTS == 2 ? 1 : 2)
 attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
-  using C = Pre<HD>;
-  constexpr int NH = C::NH;
+  using C = Pre<HD, SLOTS>;
+  constexpr int NH = C::NH, ST = C::kStages, MMA_WARP = 4 * SLOTS;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sb = smem_u32(smem);
   float* scales = reinterpret_cast<float*>(smem + C::kScales);
-  float* v_refs = scales + 8 * kTile;
+  float* v_refs = scales + 2 * C::kRing * kTile;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kBars);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NUM_BARS);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   if ((sb & 1023u) != 0u) {                      // the operands' layouts need it; report instead of computing garbage
@@ -211,12 +251,15 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     return;
   }
   if (threadIdx.x == 0) {
-    for (int b = 0; b < NUM_BARS; ++b) mbar_init(&bars[b], b == Q_FULL || b == P_FULL0 || b == P_FULL1 || b == O_FREE ? 4 : b == K_FULL0 || b == K_FULL1 || b == V_FULL0 || b == V_FULL1 ? 2 : 1);
+    for (int b = 0; b < C::kNumBars; ++b) {
+      const bool bring = (b >= C::K_FULL && b < C::K_EMPTY) || (b >= C::V_FULL && b < C::V_EMPTY), weights = b >= C::P_FULL && b < C::PV_DONE;
+      mbar_init(&bars[b], b <= C::O_FREE ? 4 * SLOTS : weights ? 4 : bring ? 2 : 1);
+    }
     *abort_flag = 0;
     mbar_fence_init();
   }
-  if (warp == 4) {
-    tmem_alloc(tmem_slot, 256);                  // S0: columns [0, 64), S1: [64, 128), O: [128, 128 + HD)
+  if (warp == MMA_WARP) {
+    tmem_alloc(tmem_slot, 256 * SLOTS);          // of each slot: S0 in columns [0, 64), S1 in [64, 128), O in [128, 128 + HD)
     tmem_relinquish();
   }
   tc_fence_before();
@@ -233,11 +276,11 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     return __all_sync(0xffffffffu, wait_or_abort(&bars[bar], parity, abort_flag)) != 0;
   };
 
-  if (warp == 5 || warp == 6) {
-    bring_tiles<HD, KIND, 0>(p, f, warp - 5, sb, scales, v_refs, bars, abort_flag);
-  } else if (warp >= 7) {
-    bring_tiles<HD, KIND, 1>(p, f, warp - 7, sb, scales, v_refs, bars, abort_flag);
-  } else if (warp == 4) {
+  if (warp > MMA_WARP && warp <= MMA_WARP + 2) {
+    bring_tiles<HD, SLOTS, KIND, 0>(p, f, warp - MMA_WARP - 1, sb, scales, v_refs, bars, abort_flag);
+  } else if (warp > MMA_WARP + 2) {
+    bring_tiles<HD, SLOTS, KIND, 1>(p, f, warp - MMA_WARP - 3, sb, scales, v_refs, bars, abort_flag);
+  } else if (warp == MMA_WARP) {
     // ------------------------------------------------------------------ products (the warp walks, an elected lane issues)
     const uint32_t idesc_s = idesc_f16(128, kTile), idesc_o = idesc_f16(128, HD) | kIdescBMnMajor;
     const uint64_t q_desc = umma_desc_k_sw128(sb + C::kQ), k_desc = umma_desc_k_sw128(sb + C::kK);
@@ -245,52 +288,60 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     uint32_t g = 0, parts = 0;
     // S(gt) goes over P(gt - 2), which PV(gt - 2) reads: the latest PV issued must have completed
     auto issue_s = [&](uint32_t gt, uint32_t pv_issued) {
-      const int s = gt & 1;
-      if (pv_issued > 0 && !passed(PV_DONE0 + ((pv_issued - 1) & 1), ((pv_issued - 1) >> 1) & 1)) return false;
-      if (!passed(K_FULL0 + s, (gt >> 1) & 1)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t kd = k_desc + static_cast<uint64_t>(s * (C::kStage >> 4));
+      if (!passed(C::K_FULL + gt % ST, gt / ST & 1)) return false;
+      const uint64_t kd = k_desc + static_cast<uint64_t>(gt % ST * (C::kStage >> 4));
 #pragma unroll
-        for (int h = 0; h < NH; ++h)
+      for (int slot = 0; slot < SLOTS; ++slot) {
+        if (pv_issued > 0 && !passed(C::PV_DONE + slot * 2 + ((pv_issued - 1) & 1), ((pv_issued - 1) >> 1) & 1)) return false;
+        tc_fence_after();
+        if (elect_one()) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16_ss(tmem + s * kTile, q_desc + ((h * 16384 + k * 32) >> 4), kd + ((h * kHalfBytes + k * 32) >> 4), idesc_s, (h | k) ? 1u : 0u);
-        umma_commit(&bars[K_EMPTY0 + s]);
-        umma_commit(&bars[S_FULL0 + s]);
+          for (int h = 0; h < NH; ++h)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_bf16_ss(tmem + slot * 256 + (gt & 1) * kTile, q_desc + ((slot * C::kSlot + h * 16384 + k * 32) >> 4),
+                           kd + ((h * kHalfBytes + k * 32) >> 4), idesc_s, (h | k) ? 1u : 0u);
+          umma_commit(&bars[C::S_FULL + slot * 2 + (gt & 1)]);
+          if (slot == SLOTS - 1) umma_commit(&bars[C::K_EMPTY + gt % ST]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
       return true;
     };
     bool ok = true;
     Share now(f, p.kv_heads);
     while (ok && now.next()) {
-      if (!passed(Q_FULL, parts & 1) || !issue_s(g, g)) { fail(NF_ST_TIMEOUT_SMEM_FULL); break; }
-      for (int t = 0; t < now.n; ++t) {
+      if (!passed(C::Q_FULL, parts & 1) || !issue_s(g, g)) { fail(NF_ST_TIMEOUT_SMEM_FULL); break; }
+      for (int t = 0; ok && t < now.n; ++t) {
         const uint32_t gt = g + t;
-        const int s = gt & 1;
         if (t + 1 < now.n && !issue_s(gt + 1, gt)) { fail(NF_ST_TIMEOUT_SMEM_FULL); ok = false; break; }
         // the item before must have been read out of O
-        if (t == 0 && !passed(O_FREE, (parts & 1) ^ 1)) { fail(NF_ST_TIMEOUT_TMEM_EMPTY); ok = false; break; }
-        if (!passed(P_FULL0 + s, (gt >> 1) & 1) || !passed(V_FULL0 + s, (gt >> 1) & 1)) { fail(NF_ST_TIMEOUT_SMEM_FULL); ok = false; break; }
-        tc_fence_after();
-        if (elect_one()) {
-          const uint64_t vd = v_desc + static_cast<uint64_t>(s * (C::kStage >> 4));
+        if (t == 0 && !passed(C::O_FREE, (parts & 1) ^ 1)) { fail(NF_ST_TIMEOUT_TMEM_EMPTY); ok = false; break; }
+        if (!passed(C::V_FULL + gt % ST, gt / ST & 1)) { fail(NF_ST_TIMEOUT_SMEM_FULL); ok = false; break; }
+        const uint64_t vd = v_desc + static_cast<uint64_t>(gt % ST * (C::kStage >> 4));
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_bf16_ts(tmem + 2 * kTile, tmem + s * kTile + k * 8, vd + ((k * 2048) >> 4), idesc_o, (t | k) ? 1u : 0u);
-          umma_commit(&bars[V_EMPTY0 + s]);
-          umma_commit(&bars[PV_DONE0 + s]);
+        for (int slot = 0; slot < SLOTS; ++slot) {
+          if (!passed(C::P_FULL + slot * 2 + (gt & 1), (gt >> 1) & 1)) { fail(NF_ST_TIMEOUT_SMEM_FULL); ok = false; break; }
+          tc_fence_after();
+          if (elect_one()) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              umma_bf16_ts(tmem + slot * 256 + 2 * kTile, tmem + slot * 256 + (gt & 1) * kTile + k * 8, vd + ((k * 2048) >> 4), idesc_o,
+                           (t | k) ? 1u : 0u);
+            umma_commit(&bars[C::PV_DONE + slot * 2 + (gt & 1)]);
+            if (slot == SLOTS - 1) umma_commit(&bars[C::V_EMPTY + gt % ST]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
       }
       g += now.n;
       ++parts;
     }
   } else {
     // ------------------------------------------------------------------ softmax (a thread per query row)
-    const int row = warp * 32 + lane;
-    const uint32_t t_lane = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+    const int row = warp * 32 + lane, slot = warp >> 2;
+    const uint32_t t_lane = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + slot * 256;
+    const uint32_t q_row = sb + C::kQ + slot * C::kSlot + (row & 127) * 128;
     const uint32_t t_o = t_lane + 2 * kTile;
     const int in_block = row / group, hh = row - in_block * group;
     uint32_t g = 0;
@@ -326,47 +377,53 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
           const float2 x = unpack_bf16x2(w[e]);
           o[e] = pack_f16x2(x.x * down, x.y * down);
         }
-        st_shared_v4(sb + C::kQ + (c >> 3) * 16384 + row * 128 + (((c & 7) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
+        st_shared_v4(q_row + (c >> 3) * 16384 + (((c & 7) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
       }
       fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[Q_FULL]);
+      if (lane == 0) mbar_arrive(&bars[C::Q_FULL]);
 
       float ref = -INFINITY, l = 0.f, v_ref = 0.f;
       for (int t = 0; t < now.n; ++t) {
         const uint32_t gt = g + t;
         const int s = gt & 1;
-        if (!passed(S_FULL0 + s, (gt >> 1) & 1) || !passed(V_FULL0 + s, (gt >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); ok = false; break; }
+        if (!passed(C::S_FULL + slot * 2 + s, (gt >> 1) & 1) || !passed(C::V_FULL + gt % ST, gt / ST & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); ok = false; break; }
         tc_fence_after();
-        const float4* k4 = reinterpret_cast<const float4*>(scales + (gt & 3) * kTile);
-        const float4* v4 = reinterpret_cast<const float4*>(scales + (4 + (gt & 3)) * kTile);
-        uint32_t r0[32], r1[32];
-        tmem_ld_32x32b_x32(t_lane + s * kTile, r0);
-        tmem_ld_32x32b_x32(t_lane + s * kTile + 32, r1);
-        tmem_ld_wait();
+        const ulonglong2* k4 = reinterpret_cast<const ulonglong2*>(scales + gt % C::kRing * kTile);
+        const ulonglong2* v4 = reinterpret_cast<const ulonglong2*>(scales + (C::kRing + gt % C::kRing) * kTile);
+        f32x2 x0[16], x1[16];                                    // scores of tokens 2j, 2j + 1 (and of 32 tokens further)
+        {
+          uint32_t r0[32], r1[32];
+          tmem_ld_32x32b_x32(t_lane + s * kTile, r0);
+          tmem_ld_32x32b_x32(t_lane + s * kTile + 32, r1);
+          tmem_ld_wait();
+          const int valid = p.prefix_len - (now.t0 + t) * kTile;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float4 a = k4[j], b = k4[8 + j];
-          const float ka[4] = {a.x, a.y, a.z, a.w}, kb[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            r0[4 * j + e] = __float_as_uint(__uint_as_float(r0[4 * j + e]) * ka[e]);
-            r1[4 * j + e] = __float_as_uint(__uint_as_float(r1[4 * j + e]) * kb[e]);
+          for (int j = 0; j < 8; ++j) {
+            const ulonglong2 a = k4[j], b = k4[8 + j];
+            x0[2 * j] = mul2(pair(__uint_as_float(r0[4 * j]), __uint_as_float(r0[4 * j + 1])), a.x);
+            x0[2 * j + 1] = mul2(pair(__uint_as_float(r0[4 * j + 2]), __uint_as_float(r0[4 * j + 3])), a.y);
+            x1[2 * j] = mul2(pair(__uint_as_float(r1[4 * j]), __uint_as_float(r1[4 * j + 1])), b.x);
+            x1[2 * j + 1] = mul2(pair(__uint_as_float(r1[4 * j + 2]), __uint_as_float(r1[4 * j + 3])), b.y);
           }
-        }
-        const int valid = p.prefix_len - (now.t0 + t) * kTile;
-        if (valid < kTile) {
+          if (valid < kTile) {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            if (j >= valid) r0[j] = 0xff800000u;
-            if (32 + j >= valid) r1[j] = 0xff800000u;
+            for (int j = 0; j < 16; ++j) {
+              const float2 a = halves(x0[j]), b = halves(x1[j]);
+              x0[j] = pair(2 * j >= valid ? -INFINITY : a.x, 2 * j + 1 >= valid ? -INFINITY : a.y);
+              x1[j] = pair(32 + 2 * j >= valid ? -INFINITY : b.x, 33 + 2 * j >= valid ? -INFINITY : b.y);
+            }
           }
         }
         float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int j = 0; j < 32; ++j) mq[j & 3] = fmaxf(mq[j & 3], fmaxf(__uint_as_float(r0[j]), __uint_as_float(r1[j])));
+        for (int j = 0; j < 16; ++j) {
+          const float2 a = halves(x0[j]), b = halves(x1[j]);
+          mq[j & 1] = max3(mq[j & 1], a.x, a.y);
+          mq[2 + (j & 1)] = max3(mq[2 + (j & 1)], b.x, b.y);
+        }
         const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * up;
-        const float v_new = v_refs[gt & 3];
+        const float v_new = v_refs[gt % C::kRing];
         if (t == 0) {
           ref = mx;
           v_ref = v_new;
@@ -374,7 +431,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
           const bool grow = mx > ref + kGap;
           if (__any_sync(0xffffffffu, grow || v_new != v_ref)) {
             // O may be touched between two products only: PV(t - 1) is the last one issued (PV(t) needs this tile's P)
-            if (!passed(PV_DONE0 + ((gt - 1) & 1), ((gt - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); ok = false; break; }
+            if (!passed(C::PV_DONE + slot * 2 + ((gt - 1) & 1), ((gt - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); ok = false; break; }
             tc_fence_after();
             const float alpha = grow ? q8_exp2(ref - mx) : 1.f, by = alpha * (v_ref / v_new);
 #pragma unroll 1
@@ -393,34 +450,33 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
           }
         }
         const float ms = ref == -INFINITY ? 0.f : ref;
-        float rs = 0.f;
-        auto weights = [&](const uint32_t (&x)[32], const float4* v, uint32_t to) {
+        const f32x2 up2 = pair(up, up), ms2 = pair(-ms, -ms);
+        f32x2 rs = pair(0.f, 0.f);
+        auto weights = [&](const f32x2 (&x)[16], const ulonglong2* v, uint32_t to) {
           uint32_t pk[16];                                       // column j: tokens 2j, 2j + 1
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float4 unit = v[j];
-            float e[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) e[k] = q8_exp2(fmaf(__uint_as_float(x[4 * j + k]), up, -ms));
-            rs += (e[0] + e[1]) + (e[2] + e[3]);
-            pk[2 * j] = pack_f16x2(e[0] * unit.x, e[1] * unit.y);
-            pk[2 * j + 1] = pack_f16x2(e[2] * unit.z, e[3] * unit.w);
+          for (int j = 0; j < 16; ++j) {
+            const float2 y = halves(fma2(x[j], up2, ms2));
+            const f32x2 e = pair(q8_exp2(y.x), q8_exp2(y.y));
+            rs = add2(rs, e);
+            const float2 w = halves(mul2(e, (j & 1) ? v[j >> 1].y : v[j >> 1].x));
+            pk[j] = pack_f16x2(w.x, w.y);
           }
           tmem_st_32x32b_x16(to, pk);
         };
-        weights(r0, v4, t_lane + s * kTile);
-        weights(r1, v4 + 8, t_lane + s * kTile + 16);
-        l += rs;
+        weights(x0, v4, t_lane + s * kTile);
+        weights(x1, v4 + 8, t_lane + s * kTile + 16);
+        l += halves(rs).x + halves(rs).y;
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[P_FULL0 + s]);
+        if (lane == 0) mbar_arrive(&bars[C::P_FULL + slot * 2 + s]);
       }
       if (!ok) break;
       g += now.n;
-      if (!passed(PV_DONE0 + ((g - 1) & 1), ((g - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
+      if (!passed(C::PV_DONE + slot * 2 + ((g - 1) & 1), ((g - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
       tc_fence_after();
-      const long long at = static_cast<long long>(now.item + blockIdx.x) * kPrefixRows + row;
+      const long long at = static_cast<long long>(now.item + blockIdx.x) * (128 * SLOTS) + row;
       const float back = v_ref / kHeadroom;
 #pragma unroll 1
       for (int c = 0; c < HD / 32; ++c) {
@@ -438,31 +494,35 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       if (tok >= 0) __stcg(reinterpret_cast<float2*>(f.ml) + at, make_float2(ref, l));
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&bars[O_FREE]);
+      if (lane == 0) mbar_arrive(&bars[C::O_FREE]);
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == MMA_WARP) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, 256 * SLOTS);
   }
 }
 
-template <int HD, int KIND>
+template <int HD, int SLOTS, int KIND>
 int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, cudaStream_t stream) {
-  const auto kernel = attn_prefix_q8_kernel<HD, KIND>;
+  using C = Pre<HD, SLOTS>;
+  const auto kernel = attn_prefix_q8_kernel<HD, SLOTS, KIND>;
   static bool attr_dev[kMaxDevices] = {false};
   bool& attr = attr_dev[device_slot()];
   if (!attr) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Pre<HD>::kBytes) != cudaSuccess) return NF_ERR_CUDA;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes) != cudaSuccess) return NF_ERR_CUDA;
     attr = true;
   }
-  if (launch_kernel(false, kernel, f.ctas, kThreads, Pre<HD>::kBytes, stream, 1, p, f) == cudaSuccess)
-    return NF_OK;
+  if (launch_kernel(false, kernel, f.ctas, C::kThreads, C::kBytes, stream, 1, p, f) == cudaSuccess) return NF_OK;
   (void)cudaGetLastError();
   return NF_ERR_CUDA;
+}
+template <int HD, int SLOTS>
+int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, cudaStream_t stream) {
+  return p.kind == NFK_Q8_E4M3 ? launch<HD, SLOTS, NFK_Q8_E4M3>(p, f, stream) : launch<HD, SLOTS, NFK_Q8_INT8>(p, f, stream);
 }
 
 }  // namespace
@@ -470,11 +530,13 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, cudaStream_t stream
 PrefixPlan prefix_plan(const nfk_attn_q8_params& p) {
   PrefixPlan f = {};
   if (p.prefix_len <= 0) return f;
-  f.reqs_per_block = kPrefixRows / (p.q_heads / p.kv_heads);
+  const int group = p.q_heads / p.kv_heads, slots = static_cast<long long>(p.req_count) * group > 128 ? 2 : 1;
+  f.rows = 128 * slots;
+  f.reqs_per_block = f.rows / group;
   f.blocks = (p.req_count + f.reqs_per_block - 1) / f.reqs_per_block;
   f.tiles = (p.prefix_len + kPrefixTile - 1) / kPrefixTile;
   const int units = prefix_units(f, p.kv_heads);
-  int ctas = 2 * device_sm_count();
+  int ctas = (slots == 2 ? 1 : 2) * device_sm_count();
   if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
   if (ctas > units) ctas = units;
   f.ctas = ctas;
@@ -482,8 +544,8 @@ PrefixPlan prefix_plan(const nfk_attn_q8_params& p) {
 }
 
 int launch_prefix_q8(const nfk_attn_q8_params& p, const PrefixPlan& f, cudaStream_t stream) {
-  if (p.head_dim == 128) return p.kind == NFK_Q8_E4M3 ? launch<128, NFK_Q8_E4M3>(p, f, stream) : launch<128, NFK_Q8_INT8>(p, f, stream);
-  return p.kind == NFK_Q8_E4M3 ? launch<64, NFK_Q8_E4M3>(p, f, stream) : launch<64, NFK_Q8_INT8>(p, f, stream);
+  if (p.head_dim == 128) return f.rows == 256 ? launch<128, 2>(p, f, stream) : launch<128, 1>(p, f, stream);
+  return f.rows == 256 ? launch<64, 2>(p, f, stream) : launch<64, 1>(p, f, stream);
 }
 
 }  // namespace nf

@@ -22,14 +22,14 @@ struct Ranges {
   }
 };
 
-// The shared prefix: the query rows of a KV head (requests x group) are cut into blocks of at most 128 rows, whole requests each.
-// An item is (KV head, block), its units the prefix's tiles of 64 tokens. The piece of item i by CTA c has number i + c: along
-// the row of units every new piece raises one of the two.
-constexpr int kPrefixTile = 64, kPrefixRows = 128;
+// The shared prefix: the query rows of a KV head (requests x group) are cut into blocks of at most `rows` (128 or 256) rows, whole
+// requests each. An item is (KV head, block), its units the prefix's tiles of 64 tokens. The piece of item i by CTA c has number
+// i + c: along the row of units every new piece raises one of the two.
+constexpr int kPrefixTile = 64;
 struct PrefixPlan {
-  int reqs_per_block, blocks, tiles, ctas;
-  float* ml;                 // states, [pieces][128 rows]: reference (of exponents to base 2) and sum,
-  float* o;                  // [pieces][128 rows][head_dim], not divided by the sum
+  int rows, reqs_per_block, blocks, tiles, ctas;
+  float* ml;                 // states, [pieces][rows]: reference (of exponents to base 2) and sum,
+  float* o;                  // [pieces][rows][head_dim], not divided by the sum
 };
 __host__ __device__ __forceinline__ int prefix_units(const PrefixPlan& f, int kv_heads) { return kv_heads * f.blocks * f.tiles; }
 
@@ -54,7 +54,7 @@ inline Q8Workspace q8_workspace(const nfk_attn_q8_params& p, const PrefixPlan& f
   const int group = p.q_heads / p.kv_heads;
   const long long ranges = static_cast<long long>(kDecodeCtasPerSm) * kDecodeWarps * device_sm_count(), pieces = 2 * ranges * group;
   const long long whole = p.prefix_len > 0 ? static_cast<long long>(p.req_count) * p.q_heads : 0;
-  const long long prefix = (static_cast<long long>(p.kv_heads) * f.blocks + f.ctas) * kPrefixRows;
+  const long long prefix = (static_cast<long long>(p.kv_heads) * f.blocks + f.ctas) * f.rows;
   const auto up = [](long long x) { return (x + 255) / 256 * 256; };
   w.records = 256;
   w.ml = w.records + up(ranges * static_cast<long long>(sizeof(DecodeRecord)));
