@@ -55,6 +55,11 @@ constexpr uint32_t idesc_f16(int m, int n) { return (1u << 4) | (static_cast<uin
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ float4 ld_shared_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
@@ -126,16 +131,16 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
   const int lane = threadIdx.x & 31, c = lane % LANES;
   // head_dim 128: the lanes of the row's second half take the neighbouring token's, so that the two halves (which lie 8 KB apart)
   // are stored to different banks
-  const int row = half * 32 + ((lane / LANES) ^ (c >> 2));
-  const uint8_t* pool = static_cast<const uint8_t*>(p.kv_pool);
+  const int row = (lane / LANES) ^ (c >> 2);
   const int n_pages = (p.prefix_len + kQ8Page - 1) / kQ8Page;
+  const uint8_t* pool = static_cast<const uint8_t*>(p.kv_pool) + row * HD + c * 16;
   uint64_t* full = bars + (PART == 0 ? C::K_FULL : C::V_FULL);
   uint64_t* empty = bars + (PART == 0 ? C::K_EMPTY : C::V_EMPTY);
   uint4 raw[NI];
   float sc[2];
   // lane j < 4: the vectors of page j of the tile, -1 where there is none
   auto page_of = [&](int kvh, int tile) {
-    long long at = -1;
+    int at = -1;
     const int slot = tile * (kTile / kQ8Page) + lane;
     if (lane < kTile / kQ8Page && slot < n_pages) {
       int page = p.prefix_pages[slot];
@@ -143,21 +148,24 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
         report_status(p.status, NF_ST_BAD_INDEX);
         page = 0;
       }
-      at = (static_cast<long long>(page) * 2 + PART) * p.kv_heads + kvh;
+      at = page;
     }
     return at;
   };
-  auto load = [&](int n, long long at) {
-    const int tok = n * AT_ONCE + row;
-    const long long head = __shfl_sync(0xffffffffu, at, tok / kQ8Page);
-    raw[n] = head < 0 ? make_uint4(0, 0, 0, 0)
-                      : *reinterpret_cast<const uint4*>(pool + (head * kQ8Page + tok % kQ8Page) * HD + c * 16);
-  };
-  auto load_scales = [&](long long at) {
+  // numbers of the warp's two pages, and the tile's scales
+  auto load = [&](int at, int kvh) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int page = __shfl_sync(0xffffffffu, at, half * 2 + j);
+      const uint8_t* from = pool + ((static_cast<long long>(page) * 2 + PART) * p.kv_heads + kvh) * (kQ8Page * HD);
+#pragma unroll
+      for (int n = 0; n < NI / 2; ++n)
+        raw[j * (NI / 2) + n] = page < 0 ? make_uint4(0, 0, 0, 0) : *reinterpret_cast<const uint4*>(from + n * AT_ONCE * HD);
+    }
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const long long head = __shfl_sync(0xffffffffu, at, 2 * k + lane / kQ8Page);
-      sc[k] = head < 0 ? 0.f : p.kv_scale[head * kQ8Page + lane % kQ8Page];
+      const int page = __shfl_sync(0xffffffffu, at, 2 * k + lane / kQ8Page);
+      sc[k] = page < 0 ? 0.f : p.kv_scale[((static_cast<long long>(page) * 2 + PART) * p.kv_heads + kvh) * kQ8Page + lane % kQ8Page];
     }
   };
   Share now(f, p.kv_heads), ahead = now;
@@ -174,14 +182,9 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
     return true;
   };
   // numbers are requested a tile ahead, page numbers two
-  if (advance()) {
-    const long long first = page_of(ahead.kvh, tile_ahead);
-#pragma unroll
-    for (int n = 0; n < NI; ++n) load(n, first);
-    load_scales(first);
-  }
+  if (advance()) load(page_of(ahead.kvh, tile_ahead), ahead.kvh);
   bool more = advance();
-  long long at = more ? page_of(ahead.kvh, tile_ahead) : -1;
+  int at = more ? page_of(ahead.kvh, tile_ahead) : -1, kvh = ahead.kvh;
   uint32_t g = 0;
   while (now.next()) {
     float v_ref = 7.8886091e-31f;                                // 2^-100
@@ -189,27 +192,28 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
       const int s = g % C::kStages, ring = g % C::kRing;
       const int valid = p.prefix_len - (now.t0 + t) * kTile;     // tokens of the tile
       const bool more_then = more && advance();
-      const long long at_then = more_then ? page_of(ahead.kvh, tile_ahead) : -1;
+      const int kvh_then = ahead.kvh, at_then = more_then ? page_of(kvh_then, tile_ahead) : -1;
       if (!__all_sync(0xffffffffu, wait_or_abort(&empty[s], (g / C::kStages & 1) ^ 1, abort_flag))) {
         if (lane == 0) report_status(p.status, NF_ST_TIMEOUT_SMEM_EMPTY);
         *abort_flag = 1;
         return;
       }
-      const uint32_t stage = sb + (PART == 0 ? C::kK : C::kV) + s * C::kStage + (c >> 2) * kHalfBytes;
+      // what lies behind the prefix may be anything: as values it would spoil every row (as keys it is masked)
+      if (PART == 1 && valid < kTile)
+#pragma unroll
+        for (int n = 0; n < NI; ++n)
+          if (half * 32 + n * AT_ONCE + row >= valid) raw[n] = make_uint4(0, 0, 0, 0);
+      const uint32_t stage = sb + (PART == 0 ? C::kK : C::kV) + s * C::kStage + (c >> 2) * kHalfBytes + (half * 32 + row) * 128;
 #pragma unroll
       for (int n = 0; n < NI; ++n) {
-        const int tok = n * AT_ONCE + row;
         uint32_t o[8];
         q8_to_f16<KIND>(raw[n].x, o[0], o[1]);
         q8_to_f16<KIND>(raw[n].y, o[2], o[3]);
         q8_to_f16<KIND>(raw[n].z, o[4], o[5]);
         q8_to_f16<KIND>(raw[n].w, o[6], o[7]);
-        // what lies behind the prefix may be anything: as values it would spoil every row (as keys it is masked)
-        if (PART == 1 && tok >= valid) o[0] = o[1] = o[2] = o[3] = o[4] = o[5] = o[6] = o[7] = 0u;
-        const uint32_t to = stage + tok * 128, c0 = (2 * (c & 3)) ^ (tok & 7);
+        const uint32_t to = stage + n * AT_ONCE * 128, c0 = (2 * (c & 3)) ^ ((n * AT_ONCE + row) & 7);
         st_shared_v4(to + (c0 << 4), o[0], o[1], o[2], o[3]);
         st_shared_v4(to + ((c0 ^ 1) << 4), o[4], o[5], o[6], o[7]);
-        if (more) load(n, at);
       }
       float* dst = scales + (PART * C::kRing + ring) * kTile + half * 32;
       if (PART == 0) {
@@ -223,9 +227,10 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
         dst[lane] = (half == 0 ? a : b) * (kHeadroom / v_ref);
         if (lane == 0 && half == 0) v_refs[ring] = v_ref;
       }
-      if (more) load_scales(at);
+      if (more) load(at, kvh);
       more = more_then;
       at = at_then;
+      kvh = kvh_then;
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[s]);
@@ -357,20 +362,21 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       }
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.q) +
                                                         (static_cast<long long>(tok < 0 ? 0 : tok) * p.q_heads + now.kvh * group + (tok < 0 ? 0 : hh)) * HD);
+      uint4 raw[HD / 8];
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c) raw[c] = tok < 0 ? make_uint4(0, 0, 0, 0) : src[c];
       uint32_t most = 0;
-#pragma unroll 4
+#pragma unroll
       for (int c = 0; c < HD / 8; ++c) {
-        const uint4 v = tok < 0 ? make_uint4(0, 0, 0, 0) : src[c];
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) most = max(most, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
       }
       float down, up;
       q_powers(__uint_as_float(most), down, up);
-#pragma unroll 4
+#pragma unroll
       for (int c = 0; c < HD / 8; ++c) {
-        const uint4 v = tok < 0 ? make_uint4(0, 0, 0, 0) : src[c];
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        const uint32_t w[4] = {raw[c].x, raw[c].y, raw[c].z, raw[c].w};
         uint32_t o[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -478,20 +484,32 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       tc_fence_after();
       const long long at = static_cast<long long>(now.item + blockIdx.x) * (128 * SLOTS) + row;
       const float back = v_ref / kHeadroom;
-#pragma unroll 1
+      // by way of the warp's own rows of Q, which no product reads any more, so that stores are of whole rows (a thread's own row by
+      // itself took 5300 cycles, half as long as 8 tiles)
+      float* const rows_o = f.o + (at - lane) * HD;
+      const uint32_t own = q_row - lane * 128;
+#pragma unroll
       for (int c = 0; c < HD / 32; ++c) {
         uint32_t v[32];
         tmem_ld_32x32b_x32(t_o + c * 32, v);
         tmem_ld_wait();
-        if (tok >= 0) {
-          float4* dst = reinterpret_cast<float4*>(f.o + at * HD + c * 32);
+        const uint32_t via = own + c % NH * 16384;
+        __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            __stcg(dst + j, make_float4(__uint_as_float(v[4 * j]) * back, __uint_as_float(v[4 * j + 1]) * back, __uint_as_float(v[4 * j + 2]) * back,
-                                        __uint_as_float(v[4 * j + 3]) * back));
+        for (int j = 0; j < 8; ++j)
+          st_shared_v4(via + lane * 128 + ((j ^ (lane & 7)) << 4), __float_as_uint(__uint_as_float(v[4 * j]) * back),
+                       __float_as_uint(__uint_as_float(v[4 * j + 1]) * back), __float_as_uint(__uint_as_float(v[4 * j + 2]) * back),
+                       __float_as_uint(__uint_as_float(v[4 * j + 3]) * back));
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int r = i * 4 + (lane >> 3), j = lane & 7;
+          const float4 x = ld_shared_f32x4(via + r * 128 + ((j ^ (r & 7)) << 4));
+          __stcg(reinterpret_cast<float4*>(rows_o + r * HD + c * 32 + j * 4), x);
         }
       }
-      if (tok >= 0) __stcg(reinterpret_cast<float2*>(f.ml) + at, make_float2(ref, l));
+      __syncwarp();
+      __stcg(reinterpret_cast<float2*>(f.ml) + at, make_float2(ref, l));
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[C::O_FREE]);
