@@ -14,14 +14,14 @@ namespace {
 constexpr int kQ8Page = 16;
 constexpr int kAppendThreads = 128;
 
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+__device__ __forceinline__ void unpack8(const uint4& v, f32x2 (&f)[4]) {
   const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 x = unpack_bf16x2(w[j]);
-    f[2 * j] = x.x;
-    f[2 * j + 1] = x.y;
-  }
+  for (int j = 0; j < 4; ++j) f[j] = pair(__uint_as_float(w[j] << 16), __uint_as_float(w[j] & 0xffff0000u));
+}
+__device__ __forceinline__ uint4 pack8(const f32x2 (&f)[4]) {
+  const float2 a = halves(f[0]), b = halves(f[1]), c = halves(f[2]), d = halves(f[3]);
+  return make_uint4(pack_bf16x2(a.x, a.y), pack_bf16x2(b.x, b.y), pack_bf16x2(c.x, c.y), pack_bf16x2(d.x, d.y));
 }
 
 // cos and sin of pos * f. The product is formed in 64 bits and brought to one turn there: in fp32 the angle of position 100000
@@ -34,12 +34,13 @@ __device__ __forceinline__ float2 turn(int pos, float f) {
 }
 
 // A CTA per token; HD / 16 threads per head, each with eight elements of either half, so that a thread holds both elements of its
-// eight pairs, and the same pairs for every head that it takes: its cosines and sines stay in registers. What bounds it is latency:
-// a thread requests its elements of BATCH heads before the CTA works out the token's angles and page.
+// eight pairs, and the same pairs for every head that it takes: its cosines and sines stay in registers. What bounds it is the issue
+// of instructions, and latency: arithmetic is two elements at a time, and a thread requests its elements of BATCH heads before the
+// CTA works out the token's angles and page.
 template <int HD, int KIND>
 __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_rope_append_q8_params p) {
   constexpr int HALF = HD / 2, LPH = HD / 16, AT_ONCE = kAppendThreads / LPH, BATCH = 3;
-  __shared__ float2 table[HALF];
+  __shared__ __align__(16) float cosines[HALF], sines[HALF], weights[2][HD];        // weights of the norms of queries and of keys
   const int l = threadIdx.x % LPH, h0 = threadIdx.x / LPH, t = blockIdx.x;
   const int heads = p.q_heads + 2 * p.kv_heads;
   const __nv_bfloat16* row = reinterpret_cast<const __nv_bfloat16*>(p.qkv) + t * p.ld_qkv + 8 * l;
@@ -59,17 +60,28 @@ __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_r
   const int pos = p.positions[t], req = p.token_req[t];
   const bool req_ok = req >= 0 && req < p.num_reqs && pos >= 0;
   const int begin = p.kv_indptr[req_ok ? req : 0], end = p.kv_indptr[req_ok ? req + 1 : 0];        // (not looked at before they are needed)
-  if (threadIdx.x < HALF)
-    table[threadIdx.x] = p.cos_sin != nullptr ? reinterpret_cast<const float2*>(p.cos_sin)[static_cast<long long>(t) * HALF + threadIdx.x]
-                                              : turn(pos, p.inv_freq[threadIdx.x]);
+  if (threadIdx.x < HALF) {
+    const float2 cs = p.cos_sin != nullptr ? reinterpret_cast<const float2*>(p.cos_sin)[static_cast<long long>(t) * HALF + threadIdx.x]
+                                           : turn(pos, p.inv_freq[threadIdx.x]);
+    cosines[threadIdx.x] = cs.x;
+    sines[threadIdx.x] = cs.y;
+  }
+  if (threadIdx.x < HD) {
+    if (p.q_norm != nullptr) weights[0][threadIdx.x] = __bfloat162float(static_cast<const __nv_bfloat16*>(p.q_norm)[threadIdx.x]);
+    if (p.k_norm != nullptr) weights[1][threadIdx.x] = __bfloat162float(static_cast<const __nv_bfloat16*>(p.k_norm)[threadIdx.x]);
+  }
   __syncthreads();
   const long long entry = static_cast<long long>(begin) + pos / kQ8Page;
   const bool entry_ok = req_ok && begin >= 0 && entry < end && entry < p.num_indices;
   const int page = entry_ok ? p.kv_indices[entry] : -1;
-  float2 cs[8];
+  const bool page_ok = page >= 0 && page < p.num_pages;
+  f32x2 co[4], si[4], minus_si[4];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) cs[j] = table[8 * l + j];
-  const bool norms = p.q_norm != nullptr || p.k_norm != nullptr;
+  for (int j = 0; j < 4; ++j) {
+    co[j] = reinterpret_cast<const f32x2*>(cosines + 8 * l)[j];
+    si[j] = reinterpret_cast<const f32x2*>(sines + 8 * l)[j];
+    minus_si[j] = si[j] ^ 0x8000000080000000ull;
+  }
   for (int first = 0; first < heads; first += BATCH * AT_ONCE) {
     if (first > 0) load(first);
 #pragma unroll
@@ -77,68 +89,74 @@ __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_r
       if (first + i * AT_ONCE >= heads) break;                // (the same for all threads: sums cross lanes)
       const int h = first + i * AT_ONCE + h0;
       const bool on = h < heads, is_q = h < p.q_heads, is_k = !is_q && h < p.q_heads + p.kv_heads;
-      const int hh = is_q ? h : is_k ? h - p.q_heads : h - p.q_heads - p.kv_heads;
-      float a[8] = {}, b[8] = {};
-      if (on) {
-        unpack8(lo[i], a);
-        unpack8(hi[i], b);
-      }
-      const void* norm = is_q ? p.q_norm : is_k ? p.k_norm : nullptr;
-      if (norms) {
-        float ss = 0.f;
+      f32x2 a[4], b[4];
+      unpack8(on ? lo[i] : make_uint4(0, 0, 0, 0), a);
+      unpack8(on ? hi[i] : make_uint4(0, 0, 0, 0), b);
+      const bool norm = is_q ? p.q_norm != nullptr : is_k && p.k_norm != nullptr;
+      if (__any_sync(0xffffffffu, norm)) {
+        f32x2 ss = mul2(a[0], a[0]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += a[j] * a[j] + b[j] * b[j];
+        for (int j = 1; j < 4; ++j) ss = fma2(a[j], a[j], ss);
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (on && norm != nullptr) {
-          const float inv = rsqrtf(ss / HD + p.eps);
-          float wa[8], wb[8];
-          unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(norm) + 8 * l), wa);
-          unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(norm) + HALF + 8 * l), wb);
+        for (int j = 0; j < 4; ++j) ss = fma2(b[j], b[j], ss);
+        float sum = halves(ss).x + halves(ss).y;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            a[j] *= inv * wa[j];
-            b[j] *= inv * wb[j];
+        for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (norm) {
+          const float inv = rsqrtf(sum * (1.f / HD) + p.eps);
+          const f32x2 inv2 = pair(inv, inv);
+          const f32x2* w = reinterpret_cast<const f32x2*>(weights[is_q ? 0 : 1] + 8 * l);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            a[j] = mul2(a[j], mul2(inv2, w[j]));
+            b[j] = mul2(b[j], mul2(inv2, w[HALF / 2 + j]));
           }
         }
       }
       if (is_q || is_k) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float x = a[j], y = b[j];
-          a[j] = x * cs[j].x - y * cs[j].y;
-          b[j] = y * cs[j].x + x * cs[j].y;
+        for (int j = 0; j < 4; ++j) {
+          const f32x2 x = a[j], y = b[j];
+          a[j] = fma2(y, minus_si[j], mul2(x, co[j]));
+          b[j] = fma2(x, si[j], mul2(y, co[j]));
         }
       }
-      if (on && is_q) {
-        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.q_out) + (static_cast<long long>(t) * p.q_heads + hh) * HD + 8 * l;
-        *reinterpret_cast<uint4*>(dst) = make_uint4(pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(a[4], a[5]), pack_bf16x2(a[6], a[7]));
-        *reinterpret_cast<uint4*>(dst + HALF) = make_uint4(pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3]), pack_bf16x2(b[4], b[5]), pack_bf16x2(b[6], b[7]));
+      if (is_q) {
+        __nv_bfloat16* dst = reinterpret_cast<__nv_bfloat16*>(p.q_out) + (static_cast<long long>(t) * p.q_heads + h) * HD + 8 * l;
+        *reinterpret_cast<uint4*>(dst) = pack8(a);
+        *reinterpret_cast<uint4*>(dst + HALF) = pack8(b);
       }
-      // Largest magnitude; as bits, so that infinities and NaN come out on top.
       if (__all_sync(0xffffffffu, is_q)) continue;
-      uint32_t most = 0;
+      float most = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        most = max(most, max(__float_as_uint(a[j]) & 0x7fffffffu, __float_as_uint(b[j]) & 0x7fffffffu));
+      for (int j = 0; j < 4; ++j) {
+        most = max3_magnitude(most, halves(a[j]).x, halves(a[j]).y);
+        most = max3_magnitude(most, halves(b[j]).x, halves(b[j]).y);
+      }
 #pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-      const bool page_ok = page >= 0 && page < p.num_pages;
-      if (on && !is_q && !page_ok && l == 0) report_status(p.status, NF_ST_BAD_INDEX);
-      if (on && !is_q && page_ok) {
-        float scale = __uint_as_float(most) / q8_largest<KIND>(), inv = 1.f / scale;
-        if (most >= 0x7f800000u) scale = __uint_as_float(0x7fc00000u), inv = 0.f;
-        else if (__uint_as_float(most) < kQ8Smallest) scale = 0.f, inv = 0.f;
-        if (inv == 0.f) {
+      for (int o = LPH / 2; o > 0; o >>= 1) most = max3_magnitude(most, __shfl_xor_sync(0xffffffffu, most, o), 0.f);
+      if (on && !is_q) {
+        const int hh = is_k ? h - p.q_heads : h - p.q_heads - p.kv_heads;
+        float scale = most * (1.f / q8_largest<KIND>()), inv = __fdividef(q8_largest<KIND>(), most);
+        if (!(most >= kQ8Smallest && most <= 3.402823466e38f)) {       // nothing to speak of, or not finite
+          scale = most < kQ8Smallest ? 0.f : __uint_as_float(0x7fc00000u);
+          inv = 0.f;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) a[j] = b[j] = 0.f;
+          for (int j = 0; j < 4; ++j) a[j] = b[j] = 0ull;
+        }
+        if (!page_ok) {
+          if (l == 0) report_status(p.status, NF_ST_BAD_INDEX);
+          continue;
         }
         const long long vec = ((static_cast<long long>(page) * 2 + (is_k ? 0 : 1)) * p.kv_heads + hh) * kQ8Page + pos % kQ8Page;
         uint8_t* dst = reinterpret_cast<uint8_t*>(p.kv_pool) + vec * HD + 8 * l;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(q8_from_f32<KIND>(a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv),
-                                                    q8_from_f32<KIND>(a[4] * inv, a[5] * inv, a[6] * inv, a[7] * inv));
-        *reinterpret_cast<uint2*>(dst + HALF) = make_uint2(q8_from_f32<KIND>(b[0] * inv, b[1] * inv, b[2] * inv, b[3] * inv),
-                                                           q8_from_f32<KIND>(b[4] * inv, b[5] * inv, b[6] * inv, b[7] * inv));
+        const f32x2 inv2 = pair(inv, inv);
+        const auto numbers = [&](const f32x2 (&x)[4]) {
+          const float2 u = halves(mul2(x[0], inv2)), v = halves(mul2(x[1], inv2)), y = halves(mul2(x[2], inv2)), z = halves(mul2(x[3], inv2));
+          return make_uint2(q8_from_f32<KIND>(u.x, u.y, v.x, v.y), q8_from_f32<KIND>(y.x, y.y, z.x, z.y));
+        };
+        *reinterpret_cast<uint2*>(dst) = numbers(a);
+        *reinterpret_cast<uint2*>(dst + HALF) = numbers(b);
         if (l == 0) p.kv_scale[vec] = scale;
       }
     }
