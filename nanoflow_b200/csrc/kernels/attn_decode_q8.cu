@@ -25,6 +25,7 @@ namespace nf {
 namespace {
 
 constexpr int kWarps = kDecodeWarps, kThreads = 32 * kWarps;
+constexpr int kListed = 1000;
 constexpr float kGap = 8.f, kHeadroom = 128.f;      // weights are below 2^8 * 2^7, f16 ends at 65504
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -161,10 +162,13 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   constexpr int KS = HD / 16, MT = HD / 16, VB = HD / 8;      // steps of Q K^T, row tiles of V^T, bytes of a token's values per lane
   constexpr int ST = D::kStages;
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int starts[kListed + 1];                          // places of the requests' first pages in the row, for up to kListed requests
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = p.q_heads / p.kv_heads;
   const int* indptr = p.kv_indptr + p.req_begin;
   const int base = indptr[0];
+  const bool in_shared = p.req_count <= kListed;
+  auto start_of = [&](int r) { return in_shared ? starts[r] : indptr[r] - base; };
   const long long listed = static_cast<long long>(indptr[p.req_count]) - base;
   bool listed_well = base >= 0 && listed >= 0 && base + listed <= p.num_indices;       // else nothing is read
   const int pages_all = listed_well ? static_cast<int>(listed) : 0;
@@ -224,7 +228,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
     while (hi - lo > 1) {
       const int step = (hi - lo + 31) / 32;
       const int r = lo + lane * step;
-      const unsigned int before = __ballot_sync(0xffffffffu, r < hi && indptr[r] - base <= place);
+      const unsigned int before = __ballot_sync(0xffffffffu, r < hi && start_of(r) <= place);
       lo += (31 - __clz(before)) * step;                       // (lane 0's is one: lo starts at or before the place)
       hi = min(hi, lo + step);
     }
@@ -243,15 +247,17 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   // (while the first pages are on their way: the lists must go up, or runs of pages would have no end)
   bool falls = false, none = false;
   for (int r = threadIdx.x; r < p.req_count; r += kThreads) {
-    const int own = indptr[r + 1] - indptr[r];
+    const int start = indptr[r], own = indptr[r + 1] - start;
+    if (in_shared) starts[r] = start - base;
     falls = falls || own < 0;
     none = none || own == 0;
   }
+  if (in_shared && threadIdx.x == 0) starts[p.req_count] = pages_all;
   listed_well = __syncthreads_or(falls ? 1 : 0) == 0 && listed_well;
   // requests without pages: zeros (with a prefix the other kernel's)
   if (!SHARED && (__syncthreads_or(none ? 1 : 0) != 0 || !listed_well))
     for (int e = range; e < p.req_count * p.q_heads; e += gridDim.x * kWarps) {
-      const int er = e / p.q_heads, tok = !listed_well || indptr[er + 1] == indptr[er] ? row_of(er) : -1;
+      const int er = e / p.q_heads, tok = !listed_well || start_of(er + 1) == start_of(er) ? row_of(er) : -1;
       if (tok >= 0) Row<HD>().finish(out + (static_cast<long long>(tok) * p.q_heads + e - er * p.q_heads) * HD);
     }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
@@ -265,11 +271,11 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
     int r = find(at);
     for (int i = 0; i < n;) {
       // ---- a request's run of pages in this range ----
-      const int r_begin = indptr[r] - base, r_end = indptr[r + 1] - base;
-      const int count = min(n - i, r_end - at);
-      const bool starts = at == r_begin, ends = at + count == r_end;
       const int last_len = p.kv_last_page_len[p.req_begin + r];
       const int tok = row_of(r);
+      const int r_begin = start_of(r), r_end = start_of(r + 1);
+      const int count = min(n - i, r_end - at);
+      const bool begins = at == r_begin, ends = at + count == r_end;
       uint32_t qb[NT][KS][2];
       float q_up[NT][2];
 #pragma unroll
@@ -423,12 +429,12 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
 
       // ---- the run's end: the final row where it is the whole request and no prefix joins it, else its state ----
       const float v_back = v_ref / kHeadroom;
-      const bool final = starts && ends && !SHARED;
+      const bool final = begins && ends && !SHARED;
       // states of this run's heads: of a whole request by its number; of a piece by the range's, those of a request that began before
       // it first
-      const States& states = starts && ends ? wholes : parts;
-      const long long first = starts && ends ? static_cast<long long>(r) * p.q_heads + kvh * group
-                                             : (static_cast<long long>(range) * 2 + (starts ? 1 : 0)) * group;
+      const States& states = begins && ends ? wholes : parts;
+      const long long first = begins && ends ? static_cast<long long>(r) * p.q_heads + kvh * group
+                                             : (static_cast<long long>(range) * 2 + (begins ? 1 : 0)) * group;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -454,7 +460,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
           }
         }
 
-      if (starts && !ends) record = DecodeRecord{kvh, r, tok, ranges.of(kvh * pages_all + r_end - 1) - range + 1};
+      if (begins && !ends) record = DecodeRecord{kvh, r, tok, ranges.of(kvh * pages_all + r_end - 1) - range + 1};
 
       // ---- the next request that has pages ----
       at += count;
@@ -463,7 +469,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
           at = 0;
           ++kvh;
         }
-        r = r + 1 < p.req_count && at > 0 && indptr[r + 1] - base <= at && indptr[r + 2] - base > at ? r + 1 : find(at);
+        r = r + 1 < p.req_count && at > 0 && start_of(r + 2) > at ? r + 1 : find(at);
       }
     }
   }
@@ -504,24 +510,23 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   const bool tok_ok = tok >= 0 && tok < p.num_tokens;
   if (!tok_ok) tok = -1;
   const Ranges ranges(pages_all * p.kv_heads, decode_ranges(pages_all * p.kv_heads, decode_ctas));
-  int k0 = 0, n_own = 0, c0 = 0, n_all = 0, item = 0, in_block = 0;
-  await_previous();
-  if (on) {
-    if (!tok_ok && lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
-    if (*bad_lists == 0 && end > begin) {
-      k0 = ranges.of(kvh * pages_all + begin);
-      n_own = ranges.of(kvh * pages_all + end - 1) - k0 + 1;
-    }
-    n_all = n_own;
-    if (p.prefix_len > 0) {
-      const Ranges prefix(prefix_units(f, p.kv_heads), f.ctas);
-      const int in = r / f.reqs_per_block;
-      item = kvh * f.blocks + in;
-      in_block = (r - in * f.reqs_per_block) * group + h;
-      c0 = prefix.of(item * f.tiles);
-      n_all += prefix.of((item + 1) * f.tiles - 1) - c0 + 1;
-    }
+  int k0 = 0, n_own = 0, c0 = 0, n_prefix = 0, item = 0, in_block = 0;
+  if (on && end > begin) {
+    k0 = ranges.of(kvh * pages_all + begin);
+    n_own = ranges.of(kvh * pages_all + end - 1) - k0 + 1;
   }
+  if (on && p.prefix_len > 0) {
+    const Ranges prefix(prefix_units(f, p.kv_heads), f.ctas);
+    const int in = r / f.reqs_per_block;
+    item = kvh * f.blocks + in;
+    in_block = (r - in * f.reqs_per_block) * group + h;
+    c0 = prefix.of(item * f.tiles);
+    n_prefix = prefix.of((item + 1) * f.tiles - 1) - c0 + 1;
+  }
+  await_previous();
+  if (on && !tok_ok && lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
+  if (*bad_lists != 0) n_own = 0;
+  int n_all = n_own + n_prefix;
   if (p.prefix_len == 0 && n_own <= 1) tok = -1, n_all = 0;    // the row has been written
   // all states of the row, WARPS shares of them one after the other
   const int a = static_cast<int>(static_cast<long long>(n_all) * which / WARPS), b = static_cast<int>(static_cast<long long>(n_all) * (which + 1) / WARPS);
