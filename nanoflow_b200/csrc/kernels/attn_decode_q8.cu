@@ -56,6 +56,10 @@ __device__ __forceinline__ float ld_shared_f32(uint32_t a) {
 }
 
 // Lanes are (g, t) = (lane / 4, lane % 4), as the products' layouts have it.
+// Who writes rows of requests: the first kernel those in one range, the second one the others (PLAIN); the second one all, with the
+// prefix's share (SHARED_PREFIX); the first one all (FEW, for small batches).
+enum { PLAIN = 0, SHARED_PREFIX = 1, FEW = 2 };
+
 template <int HD>
 struct Dec {
   static constexpr int kKeyBytes = 16 * HD, kStageBytes = 2 * kKeyBytes + 128;    // keys, values, 16 scales of each
@@ -155,12 +159,20 @@ struct States {
   __device__ __forceinline__ State at(long long i) const { return State{ml + i * 2, o + i * HD}; }
 };
 
-template <int HD, int NT, int KIND, bool SHARED>
+__device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+// FEW: the warps of a cluster take equal shares of one request's pages for one KV head, and join in distributed shared memory.
+template <int HD, int NT, int KIND, int MODE>
 __global__ void __launch_bounds__(kThreads, NT == 1 ? 4 : HD == 64 ? 3 : 2)
 attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* records, States parts, States wholes) {
   using D = Dec<HD>;
   constexpr int KS = HD / 16, MT = HD / 16, VB = HD / 8;      // steps of Q K^T, row tiles of V^T, bytes of a token's values per lane
   constexpr int ST = D::kStages;
+  constexpr bool SHARED = MODE == SHARED_PREFIX;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int starts[kListed + 1];                          // places of the requests' first pages in the row, for up to kListed requests
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -179,14 +191,31 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   let_next_start();
 
   // ---- loads: the pages of this warp's range ----
-  const int range = blockIdx.x * kWarps + warp, u0 = ranges.begin(range);
-  const int n = range < n_ranges ? ranges.begin(range + 1) - u0 : 0;
-  int kvh = n > 0 ? u0 / pages_all : 0, at = n > 0 ? u0 - kvh * pages_all : 0;         // of the next page to work on: KV head, place in the row
+  const int range = blockIdx.x * kWarps + warp;
+  int n = 0, kvh = 0, at = 0, r = 0;                           // pages; of the next one to work on: KV head, place in the row, request
+  if (MODE == FEW) {
+    const int size = gridDim.x / (p.req_count * p.kv_heads), which = blockIdx.x / size;
+    r = which / p.kv_heads;
+    kvh = which - r * p.kv_heads;
+    const int begin = indptr[r] - base, own = indptr[r + 1] - base - begin, share = static_cast<int>(cluster_ctarank()) * kWarps + warp;
+    if (begin >= 0 && own > 0 && begin + own <= pages_all) {
+      const Ranges shares(own, size * kWarps);
+      at = begin + shares.begin(share);
+      n = begin + shares.begin(share + 1) - at;
+    }
+  } else if (range < n_ranges) {
+    const int u0 = ranges.begin(range);
+    n = ranges.begin(range + 1) - u0;
+    kvh = u0 / pages_all;
+    at = u0 - kvh * pages_all;
+  }
   const uint32_t pipe = smem_u32(smem) + warp * D::kWarpBytes;
   const uint8_t* pool = reinterpret_cast<const uint8_t*>(p.kv_pool);
   int i_left = n, i_kvh = kvh, i_page = at;                    // of the next one to load; pages that are left
   int ids = 0, ids_left = 0;                                   // page numbers, one per lane, 32 at a time
   uint32_t to = pipe;                                          // the stage that is loaded next
+  const States own_states = {reinterpret_cast<float*>(smem + warp * D::kWarpBytes) + group * HD, reinterpret_cast<float*>(smem + warp * D::kWarpBytes)};
+  static_assert(D::kWarpBytes >= 8 * NT * (HD + 2) * 4, "a state of all heads lies over the pipeline");
   auto issue = [&]() {
     if (i_left > 0) {
       if (ids_left == 0) {
@@ -255,20 +284,20 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   if (in_shared && threadIdx.x == 0) starts[p.req_count] = pages_all;
   listed_well = __syncthreads_or(falls ? 1 : 0) == 0 && listed_well;
   // requests without pages: zeros (with a prefix the other kernel's)
-  if (!SHARED && (__syncthreads_or(none ? 1 : 0) != 0 || !listed_well))
+  if (MODE == PLAIN && (__syncthreads_or(none ? 1 : 0) != 0 || !listed_well))
     for (int e = range; e < p.req_count * p.q_heads; e += gridDim.x * kWarps) {
       const int er = e / p.q_heads, tok = !listed_well || start_of(er + 1) == start_of(er) ? row_of(er) : -1;
       if (tok >= 0) Row<HD>().finish(out + (static_cast<long long>(tok) * p.q_heads + e - er * p.q_heads) * HD);
     }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    *bad_lists = listed_well ? 0 : 1;
+    if (MODE != FEW) *bad_lists = listed_well ? 0 : 1;
     if (!listed_well) report_status(p.status, NF_ST_BAD_INDEX);
   }
 
   DecodeRecord record = {0, 0, 0, 0};
   if (listed_well && n > 0) {
     uint32_t st = pipe;                                        // the stage that is worked on
-    int r = find(at);
+    if (MODE != FEW) r = find(at);
     for (int i = 0; i < n;) {
       // ---- a request's run of pages in this range ----
       const int last_len = p.kv_last_page_len[p.req_begin + r];
@@ -324,9 +353,11 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
         cp_async_wait<ST - 2>();
         __syncwarp();                                          // the page is there, and no lane looks at the one before any more
         issue();
-        float s[NT][4];
+        float s[NT][4], s_odd[NT][4];                          // sums of even and of odd steps: half as long a chain of products
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] = s_odd[nt][e] = 0.f;
 #pragma unroll
         for (int x = 0; x < HD / 64; ++x) {
           const uint4 a = ld_shared_v4(st + D::key_at(g, x * 4 + t)), b = ld_shared_v4(st + D::key_at(g + 8, x * 4 + t));
@@ -337,9 +368,13 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
             q8_to_f16<KIND>(aw[e], a0, a2);
             q8_to_f16<KIND>(bw[e], a1, a3);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(s[nt], a0, a1, a2, a3, qb[nt][x * 4 + e][0], qb[nt][x * 4 + e][1]);
+            for (int nt = 0; nt < NT; ++nt) mma_f16((e & 1) ? s_odd[nt] : s[nt], a0, a1, a2, a3, qb[nt][x * 4 + e][0], qb[nt][x * 4 + e][1]);
           }
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[nt][e] += s_odd[nt][e];
         const uint32_t sc = st + 2 * D::kKeyBytes;
         const int valid = ends && c == count - 1 ? last_len : kQ8Page;
         const bool on0 = g < valid, on1 = g + 8 < valid;
@@ -429,12 +464,17 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
 
       // ---- the run's end: the final row where it is the whole request and no prefix joins it, else its state ----
       const float v_back = v_ref / kHeadroom;
-      const bool final = begins && ends && !SHARED;
+      const bool final = begins && ends && MODE == PLAIN;
       // states of this run's heads: of a whole request by its number; of a piece by the range's, those of a request that began before
-      // it first
-      const States& states = begins && ends ? wholes : parts;
-      const long long first = begins && ends ? static_cast<long long>(r) * p.q_heads + kvh * group
-                                             : (static_cast<long long>(range) * 2 + (begins ? 1 : 0)) * group;
+      // it first; in a cluster over the warp's own pipeline, which is done
+      States states = begins && ends ? wholes : parts;
+      long long first = begins && ends ? static_cast<long long>(r) * p.q_heads + kvh * group
+                                       : (static_cast<long long>(range) * 2 + (begins ? 1 : 0)) * group;
+      if (MODE == FEW) {
+        states = own_states;
+        first = 0;
+        __syncwarp();
+      }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -473,9 +513,46 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
       }
     }
   }
-  if (lane == 0) records[range] = record;
-  cp_async_wait<0>();
-  if (SHARED) await_previous();
+  if (MODE == FEW) {
+    cp_async_wait<0>();
+    __syncwarp();
+    if (!listed_well || n == 0)                                // no share of the pages: an empty state
+      for (int e = lane; e < group * (HD + 2); e += 32) own_states.o[e] = e >= group * HD && (e & 1) == 0 ? -INFINITY : 0.f;
+    cluster_sync_all();
+    const int size = gridDim.x / (p.req_count * p.kv_heads), states = size * kWarps, tok = row_of(r);
+    for (int h = static_cast<int>(cluster_ctarank()) * kWarps + warp; h < group; h += states) {
+      // state i: of warp i % kWarps in CTA i / kWarps
+      const auto state = [&](int i) { return mapa_shared(smem_u32(smem) + i % kWarps * D::kWarpBytes, i / kWarps); };
+      const float2 s = ld_cluster_f32x2(state(min(lane, states - 1)) + (group * HD + 2 * h) * 4);
+      float m = s.x;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+      const float w = lane < states ? q8_exp2(s.x - (m == -INFINITY ? 0.f : m)) : 0.f;
+      Row<HD> row;
+      row.m = m;
+      row.l = lane < states ? s.y * w : 0.f;
+#pragma unroll
+      for (int off = 16; off > 0; off >>= 1) row.l += __shfl_xor_sync(0xffffffffu, row.l, off);
+      for (int i = 0; i < states; i += kWarps)
+#pragma unroll
+        for (int k = 0; k < kWarps; ++k) {
+          const float by = __shfl_sync(0xffffffffu, w, i + k);
+          const uint32_t from = state(i + k) + (h * HD + lane * Row<HD>::N) * 4;
+#pragma unroll
+          for (int e = 0; e < Row<HD>::N; e += 2) {
+            const float2 x = ld_cluster_f32x2(from + e * 4);
+            row.o[e] += by * x.x;
+            row.o[e + 1] += by * x.y;
+          }
+        }
+      if (tok >= 0) row.finish(out + (static_cast<long long>(tok) * p.q_heads + kvh * group + h) * HD);
+    }
+    cluster_sync_all();                                        // no CTA's shared memory goes before all have read it
+  } else {
+    if (lane == 0) records[range] = record;
+    cp_async_wait<0>();
+    if (SHARED) await_previous();
+  }
 }
 
 // Joins the states of requests that lie in more than one range, a warp to each (range that one begins in, head).
@@ -558,6 +635,18 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   if (which == 0 && tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(tok) * p.q_heads + head) * HD);
 }
 
+// CTAs that share a request's pages for one KV head in a small batch, 0 where the general form is at least as fast: one launch instead
+// of two, but as slow as the request with the most pages makes it, which the host does not know (0.5 us for each page of a warp). One
+// token 4.6 us instead of 7.2, 100 tokens 5.1 instead of 7.9, nine requests of 10 to 100 6.0 (with clusters of four 8.1) instead of
+// 8.3; one of 900 8.4 with four CTAs (with one 11.9, two 9.6, eight 8.7), 8.3 in the general form, whose call costs the host 2 us more.
+int few_cluster(const nfk_attn_q8_params& p) {
+  const int pages = p.num_indices, likely = p.req_count == 1 ? pages : pages < 2 * (pages / p.req_count + 1) ? pages : 2 * (pages / p.req_count + 1);
+  const int size = likely <= 5 * kWarps ? 1 : 4;
+  const long long ctas = static_cast<long long>(p.req_count) * p.kv_heads * size;
+  const bool fits = ctas <= 4ll * device_sm_count() && (p.num_ctas == 0 || ctas <= p.num_ctas);
+  return fits && p.prefix_len == 0 && likely <= size * kWarps * 5 && pages <= size * kWarps * 10 ? size : 0;
+}
+
 // CTAs of an SM that fit, for a kernel with `bytes` of shared memory; 0: an error.
 int fitting(const void* kernel, int threads, int bytes) {
   int per_sm = 0;
@@ -569,25 +658,31 @@ int fitting(const void* kernel, int threads, int bytes) {
   return per_sm;
 }
 
-template <int HD, int NT, int KIND, bool SHARED>
+template <int HD, int NT, int KIND, int MODE>
 int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, int* bad_lists, DecodeRecord* records, const States& parts, const States& wholes,
            cudaStream_t stream) {
   constexpr int bytes = kWarps * Dec<HD>::kWarpBytes;
-  const auto kernel = attn_decode_q8_kernel<HD, NT, KIND, SHARED>;
+  constexpr bool SHARED = MODE == SHARED_PREFIX;
+  const auto kernel = attn_decode_q8_kernel<HD, NT, KIND, MODE>;
   static int fit_dev[kMaxDevices] = {0};
   int& fit = fit_dev[device_slot()];
   if (fit == 0) fit = fitting(reinterpret_cast<const void*>(kernel), kThreads, bytes);
   if (fit == 0) return NF_ERR_CUDA;
-  const int sms = device_sm_count(), room = (fit < kDecodeCtasPerSm ? fit : kDecodeCtasPerSm) * sms;
-  const int useful = decode_ranges(p.num_indices * p.kv_heads, room);
-  int ctas = (useful + kWarps - 1) / kWarps;
-  if (ctas < 1) ctas = 1;
-  if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
   const auto done = [](cudaError_t e) {
     if (e == cudaSuccess) return true;
     (void)cudaGetLastError();
     return false;
   };
+  if (MODE == FEW) {
+    const int size = few_cluster(p);
+    return done(launch_kernel(false, kernel, p.req_count * p.kv_heads * size, kThreads, bytes, stream, size, p, bad_lists, records, parts, wholes))
+               ? NF_OK : NF_ERR_CUDA;
+  }
+  const int sms = device_sm_count(), room = (fit < kDecodeCtasPerSm ? fit : kDecodeCtasPerSm) * sms;
+  const int useful = decode_ranges(p.num_indices * p.kv_heads, room);
+  int ctas = (useful + kWarps - 1) / kWarps;
+  if (ctas < 1) ctas = 1;
+  if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
   if (!done(launch_kernel(SHARED, kernel, ctas, kThreads, bytes, stream, 1, p, bad_lists, records, parts, wholes))) return NF_ERR_CUDA;
   // Few rows: four warps to each, since there are many pieces to a row then. With a prefix every row has states to join. Else the
   // pieces lead to the rows, of which most lie in one range.
@@ -606,7 +701,8 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, int* bad_lists, Dec
 
 template <int HD, int NT, int KIND, class... A>
 int launch(const nfk_attn_q8_params& p, const A&... a) {
-  return p.prefix_len > 0 ? launch<HD, NT, KIND, true>(p, a...) : launch<HD, NT, KIND, false>(p, a...);
+  return p.prefix_len > 0 ? launch<HD, NT, KIND, SHARED_PREFIX>(p, a...) : few_cluster(p) > 0 ? launch<HD, NT, KIND, FEW>(p, a...)
+                                                                         : launch<HD, NT, KIND, PLAIN>(p, a...);
 }
 template <int HD, class... A>
 int launch(const nfk_attn_q8_params& p, const A&... a) {

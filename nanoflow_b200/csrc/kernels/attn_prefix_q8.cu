@@ -523,7 +523,11 @@ PrefixPlan prefix_plan(const nfk_attn_q8_params& p) {
   const int units = prefix_units(f, p.kv_heads);
   int ctas = (slots == 2 ? 1 : 2) * device_sm_count();
   if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
-  if (ctas > units) ctas = units;
+  // Some tiles to a CTA where the prefix is long: every CTA leaves a piece of each row, and the rows' joins are bound by their number (8
+  // requests of one KV head behind 30000 tokens: 31 us with a tile or two, 19 with four, 22 with eight; 16 of 8 behind 2000: 16.0 with
+  // one, 14.4 with two, 14.8 with four; behind 500 12.5 with one, 12.9 with two).
+  const int least = f.tiles >= 128 ? 4 : f.tiles >= 32 ? 2 : 1;
+  if (ctas > (units + least - 1) / least) ctas = (units + least - 1) / least;
   f.ctas = ctas;
   return f;
 }
