@@ -55,11 +55,11 @@ __device__ __forceinline__ float ld_shared_f32(uint32_t a) {
   return v;
 }
 
-// Lanes are (g, t) = (lane / 4, lane % 4), as the products' layouts have it.
 // Who writes rows of requests: the first kernel those in one range, the second one the others (PLAIN); the second one all, with the
 // prefix's share (SHARED_PREFIX); the first one all (FEW, for small batches).
 enum { PLAIN = 0, SHARED_PREFIX = 1, FEW = 2 };
 
+// Lanes are (g, t) = (lane / 4, lane % 4), as the products' layouts have it.
 template <int HD>
 struct Dec {
   static constexpr int kKeyBytes = 16 * HD, kStageBytes = 2 * kKeyBytes + 128;    // keys, values, 16 scales of each
@@ -348,7 +348,6 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
         for (int j = 0; j < MT; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       }
 
-
       for (int c = 0; c < count; ++c, ++i) {
         cp_async_wait<ST - 2>();
         __syncwarp();                                          // the page is there, and no lane looks at the one before any more
@@ -380,7 +379,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
         const bool on0 = g < valid, on1 = g + 8 < valid;
         const float k0 = ld_shared_f32(sc + g * 4), k1 = ld_shared_f32(sc + g * 4 + 32);
         const float v0 = on0 ? ld_shared_f32(sc + 64 + g * 4) : 0.f, v1 = on1 ? ld_shared_f32(sc + 96 + g * 4) : 0.f;
-        bool grow = v0 > v_ref || v1 > v_ref;
+        bool grow = fabsf(v0) > v_ref || fabsf(v1) > v_ref;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -391,7 +390,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
           }
         }
         if (__any_sync(0xffffffffu, grow)) {
-          float most = fmaxf(v_ref, fmaxf(v0, v1));
+          float most = fmaxf(v_ref, fmaxf(fabsf(v0), fabsf(v1)));
 #pragma unroll
           for (int off = 4; off < 32; off <<= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
           most = __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0xff800000u);          // the next power of two
@@ -715,6 +714,13 @@ bool sizes_built(const nfk_attn_q8_params& p) {
   return (p.head_dim == 64 || p.head_dim == 128) && p.kv_heads > 0 && p.q_heads > 0 && p.q_heads % p.kv_heads == 0 &&
          p.q_heads / p.kv_heads <= 16;
 }
+// All units, and all places in their rows, are counted in 32 bits.
+bool counts_fit(const nfk_attn_q8_params& p, const PrefixPlan& f) {
+  const long long most = 0x7ffffff0ll;
+  return static_cast<long long>(p.num_indices) * p.kv_heads <= most && static_cast<long long>(p.req_count) * p.q_heads <= most &&
+         static_cast<long long>(p.kv_heads) * f.blocks <= most / (f.tiles > 0 ? f.tiles : 1) &&
+         static_cast<long long>(p.req_begin) + p.req_count <= most;
+}
 bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }
 
 }  // namespace
@@ -723,7 +729,8 @@ bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 
 extern "C" long long nfk_attn_q8_workspace(const nfk_attn_q8_params* p) {
   using namespace nf;
   if (p == nullptr || !sizes_built(*p) || p->req_count < 0 || p->prefix_len < 0) return 0;
-  return q8_workspace(*p, prefix_plan(*p)).bytes;
+  const PrefixPlan f = prefix_plan(*p);
+  return counts_fit(*p, f) ? q8_workspace(*p, f).bytes : 0;
 }
 
 extern "C" int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream) {
@@ -733,11 +740,10 @@ extern "C" int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stre
   if (p->req_count == 0) return NF_OK;
   if (!p->q || !p->out || !p->kv_pool || !p->kv_scale || !p->qo_indptr || !p->kv_indptr || !p->kv_last_page_len || !p->workspace ||
       (p->num_indices > 0 && !p->kv_indices) || (p->prefix_len > 0 && !p->prefix_pages) || p->num_pages <= 0 || p->num_tokens <= 0 ||
-      p->num_indices < 0 || static_cast<long long>(p->num_indices) * p->kv_heads > 0x7fffffffll ||
-      static_cast<long long>(p->req_count) * p->q_heads > 0x7fffffffll || p->num_ctas < 0 || !aligned16(p->q) || !aligned16(p->out) || !aligned16(p->kv_pool) ||
-      !aligned16(p->kv_scale) || (reinterpret_cast<uintptr_t>(p->workspace) & 255) != 0)
+      p->num_indices < 0 || p->num_ctas < 0 || !aligned16(p->q) || !aligned16(p->out) || !aligned16(p->kv_pool) || !aligned16(p->kv_scale) || (reinterpret_cast<uintptr_t>(p->workspace) & 255) != 0)
     return NF_ERR_BAD_ARG;
   PrefixPlan f = prefix_plan(*p);
+  if (!counts_fit(*p, f)) return NF_ERR_BAD_ARG;
   const Q8Workspace ws = q8_workspace(*p, f);
   if (p->workspace_bytes < ws.bytes) return NF_ERR_BAD_ARG;
   char* base = static_cast<char*>(p->workspace);

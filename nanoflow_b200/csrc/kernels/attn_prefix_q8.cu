@@ -187,7 +187,7 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
         dst[lane] = sc[half] * (p.sm_scale * kQ8Log2e);
       } else {
         const float a = lane < valid ? sc[0] : 0.f, b = lane + 32 < valid ? sc[1] : 0.f;
-        float most = fmaxf(a, b);
+        float most = fmaxf(fabsf(a), fabsf(b));
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
         if (most > v_ref) v_ref = __uint_as_float((__float_as_uint(most) + 0x7fffffu) & 0xff800000u);   // the next power of two
@@ -518,16 +518,16 @@ PrefixPlan prefix_plan(const nfk_attn_q8_params& p) {
   const int group = p.q_heads / p.kv_heads, slots = static_cast<long long>(p.req_count) * group > 128 ? 2 : 1;
   f.rows = 128 * slots;
   f.reqs_per_block = f.rows / group;
-  f.blocks = (p.req_count + f.reqs_per_block - 1) / f.reqs_per_block;
-  f.tiles = (p.prefix_len + kPrefixTile - 1) / kPrefixTile;
-  const int units = prefix_units(f, p.kv_heads);
+  f.blocks = static_cast<int>((static_cast<long long>(p.req_count) + f.reqs_per_block - 1) / f.reqs_per_block);
+  f.tiles = static_cast<int>((static_cast<long long>(p.prefix_len) + kPrefixTile - 1) / kPrefixTile);
+  const long long units = static_cast<long long>(p.kv_heads) * f.blocks * f.tiles;         // (whether they fit 32 bits is asked afterwards)
   int ctas = (slots == 2 ? 1 : 2) * device_sm_count();
   if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
   // Some tiles to a CTA where the prefix is long: every CTA leaves a piece of each row, and the rows' joins are bound by their number (8
   // requests of one KV head behind 30000 tokens: 31 us with a tile or two, 19 with four, 22 with eight; 16 of 8 behind 2000: 16.0 with
   // one, 14.4 with two, 14.8 with four; behind 500 12.5 with one, 12.9 with two).
   const int least = f.tiles >= 128 ? 4 : f.tiles >= 32 ? 2 : 1;
-  if (ctas > (units + least - 1) / least) ctas = (units + least - 1) / least;
+  if (ctas > (units + least - 1) / least) ctas = static_cast<int>((units + least - 1) / least);
   f.ctas = ctas;
   return f;
 }

@@ -108,7 +108,7 @@ def decode_workspace_q8(*, requests: int, q_heads: int, kv_heads: int, head_dim:
     else:
         n = fn(byref(p))
     if n <= 0:
-        raise RuntimeError("decode_workspace_q8: unsupported configuration (head_dim 64 or 128, up to 16 query heads per KV head)")
+        raise RuntimeError("decode_workspace_q8: unsupported sizes (head_dim 64 or 128, up to 16 query heads per KV head, counts of 32 bits)")
     return torch.zeros(n, dtype=torch.uint8, device=device)
 
 
@@ -116,8 +116,9 @@ def attn_decode_q8(q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, 
                    req_count: int, workspace: torch.Tensor, sm_scale: Optional[float] = None, num_ctas: int = 0,
                    status: Optional[torch.Tensor] = None) -> torch.Tensor:
     """:func:`nanoflow_b200.ops.attn_decode` over the 8-bit cache: single-query attention for requests [req_begin, req_begin +
-    req_count). Contexts are cut over the CTAs by their pages, whatever their lengths. Requests without pages get zeros; rows of
-    other requests are left as they were. ``workspace``: :func:`decode_workspace_q8`. ``num_ctas``: CTA budget, 0 = all that fit."""
+    req_count), each with a row of ``q`` of its own. Contexts are cut over the CTAs by their pages, whatever their lengths. Requests
+    without pages get zeros; rows of other requests are left as they were. Page numbers, rows and page lists that are none are
+    reported in ``status``. ``workspace``: :func:`decode_workspace_q8`. ``num_ctas``: CTA budget, 0 = all that fit."""
     _calls().decode("attn_decode_q8", q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, None, 0, q_heads,
                     req_begin, req_count, sm_scale, num_ctas, workspace, status)
     return out

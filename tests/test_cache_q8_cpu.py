@@ -44,7 +44,9 @@ def _attn(**kw):
     (dict(head_dim=96), 3), (dict(head_dim=256), 3), (dict(q_heads=7), 3), (dict(q_heads=34), 3), (dict(kind=2), 3), (dict(kv_heads=0), 3),
     (dict(req_count=-1), 1), (dict(req_begin=-1), 1), (dict(prefix_len=-1), 1), (dict(q=0), 1), (dict(kv_scale=0), 1), (dict(kv_indices=0), 1),
     (dict(workspace=0), 1), (dict(workspace=4100), 1), (dict(workspace_bytes=1000), 1), (dict(q=4104), 1), (dict(kv_pool=4100), 1),
-    (dict(num_pages=0), 1), (dict(num_tokens=0), 1), (dict(prefix_len=5, prefix_pages=0), 1), (dict(num_ctas=-2), 1), (dict(req_count=0), 0)])
+    (dict(num_pages=0), 1), (dict(num_tokens=0), 1), (dict(prefix_len=5, prefix_pages=0), 1), (dict(num_ctas=-2), 1),
+    (dict(num_indices=2 ** 30), 1), (dict(req_count=2 ** 28), 1), (dict(prefix_len=2 ** 30, req_count=2 ** 20), 1), (dict(req_begin=2 ** 31 - 2), 1),
+    (dict(req_count=0), 0)])
 def test_attention_refuses_before_any_launch(change, rc):
     assert ops.lib().nfk_attn_decode_q8(byref(_attn(**change)), c_void_p(0)) == rc
 
@@ -80,6 +82,8 @@ def test_workspace_grows_with_the_sizes_and_covers_smaller_calls():
         last = now
     with pytest.raises(RuntimeError, match="unsupported"):
         size(q_heads=9)
+    with pytest.raises(RuntimeError, match="unsupported"):
+        size(requests=2 ** 24, prefix_len=2 ** 24)
 
 
 def test_quantising_in_the_plain_form():

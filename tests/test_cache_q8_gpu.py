@@ -332,6 +332,21 @@ def test_shared_prefix(kind, heads, kv_heads, dim, requests, prefix, own):
     assert torch.equal(same[:requests], out[:requests])
 
 
+@pytest.mark.parametrize("prefix", [0, 100])
+def test_more_requests_than_a_block_lists(prefix):
+    own = [(37 * i) % 23 for i in range(1100)]
+    pages = sum(-(-x // 16) for x in own) + 7
+    pool, scale = _cache(pages, 2, 64, INT8)
+    ptr, idx, last = _lists(own, pages - 7, 5)
+    front = torch.arange(pages - 7, pages, dtype=torch.int32, device="cuda")
+    q = torch.randn(1100, 2 * 64, device="cuda").to(torch.bfloat16)
+    out = torch.empty_like(q)
+    args = (pool, scale, torch.arange(1101, dtype=torch.int32, device="cuda"), ptr, idx, last)
+    ws = ops.decode_workspace_q8(requests=1100, q_heads=2, kv_heads=2, head_dim=64, prefix_len=prefix)
+    ops.attn_decode_shared_q8(q, out, *args, front, prefix, q_heads=2, req_begin=0, req_count=1100, workspace=ws)
+    _check_rows(out, ref.attn_decode_q8(q, *args, q_heads=2, req_begin=0, req_count=1100, prefix_pages=front, prefix_len=prefix), 64)
+
+
 def test_no_prefix_is_plain_decode():
     pool, scale = _cache(40, 2, 128, E4M3)
     ptr, idx, last = _lists([100, 7, 333], 40, 3)
