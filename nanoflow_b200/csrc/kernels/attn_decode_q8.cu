@@ -96,22 +96,32 @@ struct Row {
   }
 };
 
-// A state in the workspace.
-struct State {
-  const float* ml;
-  const float* o;
+// States in the workspace, [..][group or heads]: (reference, sum) and rows of head_dim.
+struct States {
+  float* ml;
+  float* o;
 };
+// One of them: its reference and sum, and the place of its row, counted in 16 bytes from the workspace's begin.
+struct State {
+  float2 ml;
+  unsigned int row;
+};
+template <int HD>
+__device__ __forceinline__ State state_at(const void* workspace, const float* ml, const float* o, unsigned int i) {
+  return State{__ldcg(reinterpret_cast<const float2*>(ml) + i),
+               static_cast<unsigned int>((reinterpret_cast<const char*>(o) - static_cast<const char*>(workspace)) >> 4) + i * (HD / 4)};
+}
 // Sum of n states, the i-th being at(i), in their order. Lanes fetch 32 references and sums at a time and AHEAD rows are requested
 // without waiting for one another.
 template <int HD, int AHEAD, class At>
-__device__ __forceinline__ Row<HD> sum_states(int n, At at) {
+__device__ __forceinline__ Row<HD> sum_states(const void* workspace, int n, At at) {
   constexpr int N = Row<HD>::N;
   const int lane = threadIdx.x & 31;
+  const char* base = static_cast<const char*>(workspace) + lane * (N * 4);
   Row<HD> all;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int here = min(32, n - i0);
     const State mine = at(i0 + min(lane, here - 1));
-    const float2 s = __ldcg(reinterpret_cast<const float2*>(mine.ml));
     Row<HD> part;
     float w = 0.f;
     for (int i = 0; i < here; i += AHEAD) {
@@ -119,21 +129,21 @@ __device__ __forceinline__ Row<HD> sum_states(int n, At at) {
 #pragma unroll
       for (int k = 0; k < AHEAD; ++k) {
         if (i + k >= here) break;
-        const float* row = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine.o), i + k));
+        const char* row = base + (static_cast<unsigned long long>(__shfl_sync(0xffffffffu, mine.row, i + k)) << 4);
         if constexpr (HD == 128) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(row) + lane);
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(row));
           x[k][0] = v.x; x[k][1] = v.y; x[k][2] = v.z; x[k][3] = v.w;
         } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(row) + lane);
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(row));
           x[k][0] = v.x; x[k][1] = v.y;
         }
       }
       if (i == 0) {                                            // (while the first rows are on their way)
-        part.m = s.x;
+        part.m = mine.ml.x;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) part.m = fmaxf(part.m, __shfl_xor_sync(0xffffffffu, part.m, off));
-        w = lane < here ? q8_exp2(s.x - (part.m == -INFINITY ? 0.f : part.m)) : 0.f;
-        part.l = lane < here ? s.y * w : 0.f;
+        w = lane < here ? q8_exp2(mine.ml.x - (part.m == -INFINITY ? 0.f : part.m)) : 0.f;
+        part.l = mine.ml.y * w;
 #pragma unroll
         for (int off = 16; off > 0; off >>= 1) part.l += __shfl_xor_sync(0xffffffffu, part.l, off);
       }
@@ -150,14 +160,6 @@ __device__ __forceinline__ Row<HD> sum_states(int n, At at) {
   }
   return all;
 }
-
-// Where states go: [..][group or heads] (reference, sum) and rows of head_dim.
-struct States {
-  float* ml;
-  float* o;
-  template <int HD>
-  __device__ __forceinline__ State at(long long i) const { return State{ml + i * 2, o + i * HD}; }
-};
 
 __device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t a) {
   float2 v;
@@ -556,14 +558,17 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
 
 // Joins the states of requests that lie in more than one range, a warp to each (range that one begins in, head).
 template <int HD>
-__global__ void __launch_bounds__(128) attn_join_parts_q8_kernel(nfk_attn_q8_params p, const DecodeRecord* records, States parts, int n_ranges) {
-  const int e = blockIdx.x * 4 + (threadIdx.x >> 5), group = p.q_heads / p.kv_heads, range = e / group, h = e - range * group;
+__global__ void __launch_bounds__(128)
+attn_join_parts_q8_kernel(nfk_attn_q8_params p, const DecodeRecord* records, States parts, unsigned int group, unsigned int n_ranges) {
+  const unsigned int e = blockIdx.x * 4 + (threadIdx.x >> 5), range = e / group, h = e - range * group;
   await_previous();
   if (range >= n_ranges) return;
   const int4 raw = __ldcg(reinterpret_cast<const int4*>(records) + range);
   const DecodeRecord rec = {raw.x, raw.y, raw.z, raw.w};
   if (rec.n == 0) return;
-  const Row<HD> row = sum_states<HD, 8>(rec.n, [&](int i) { return parts.at<HD>((static_cast<long long>(range + i) * 2 + (i == 0 ? 1 : 0)) * group + h); });
+  const Row<HD> row = sum_states<HD, 8>(p.workspace, rec.n, [&](int i) {
+    return state_at<HD>(p.workspace, parts.ml, parts.o, ((range + i) * 2 + (i == 0 ? 1 : 0)) * group + h);
+  });
   if (rec.tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(rec.tok) * p.q_heads + rec.kvh * group + h) * HD);
 }
 
@@ -571,33 +576,31 @@ __global__ void __launch_bounds__(128) attn_join_parts_q8_kernel(nfk_attn_q8_par
 // pieces for each of 32 heads, one of 100000 tokens 296.
 template <int HD, int WARPS>
 __global__ void __launch_bounds__(128)
-attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_lists, States parts, States wholes, int decode_ctas) {
+attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_lists, States parts, States wholes, unsigned int group, int decode_ctas) {
   __shared__ float shared_ml[4][2];
   __shared__ float shared_o[4][HD];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = warp % WARPS;
-  const int group = p.q_heads / p.kv_heads;
   const int* indptr = p.kv_indptr + p.req_begin;
   // lists and their cut while the kernels before this one still run: they do not write them
-  const int e = blockIdx.x * (4 / WARPS) + warp / WARPS;
-  const bool on = e < p.req_count * p.q_heads;
-  const int r = on ? e / p.q_heads : 0, head = on ? e - r * p.q_heads : 0, kvh = head / group, h = head - kvh * group;
+  const unsigned int e = blockIdx.x * (4 / WARPS) + warp / WARPS, q_heads = p.q_heads;
+  const bool on = e < p.req_count * q_heads;
+  const unsigned int r = on ? e / q_heads : 0, head = on ? e - r * q_heads : 0, kvh = head / group, h = head - kvh * group;
   const int base = indptr[0], pages_all = indptr[p.req_count] - base, begin = indptr[r] - base, end = indptr[r + 1] - base;
   int tok = p.qo_indptr[p.req_begin + r];
   const bool tok_ok = tok >= 0 && tok < p.num_tokens;
   if (!tok_ok) tok = -1;
   const Ranges ranges(pages_all * p.kv_heads, decode_ranges(pages_all * p.kv_heads, decode_ctas));
-  int k0 = 0, n_own = 0, c0 = 0, n_prefix = 0, item = 0, in_block = 0;
+  int k0 = 0, n_own = 0, n_prefix = 0;
+  unsigned int front = 0;                                      // the prefix's first state of this row
   if (on && end > begin) {
     k0 = ranges.of(kvh * pages_all + begin);
     n_own = ranges.of(kvh * pages_all + end - 1) - k0 + 1;
   }
   if (on && p.prefix_len > 0) {
-    const Ranges prefix(prefix_units(f, p.kv_heads), f.ctas);
-    const int in = r / f.reqs_per_block;
-    item = kvh * f.blocks + in;
-    in_block = (r - in * f.reqs_per_block) * group + h;
-    c0 = prefix.of(item * f.tiles);
-    n_prefix = prefix.of((item + 1) * f.tiles - 1) - c0 + 1;
+    const unsigned int in = r / static_cast<unsigned int>(f.reqs_per_block), item = kvh * f.blocks + in;
+    const int c0 = f.cut.of(item * f.tiles);
+    n_prefix = f.cut.of((item + 1) * f.tiles - 1) - c0 + 1;
+    front = (item + c0) * f.rows + (r - in * f.reqs_per_block) * group + h;
   }
   await_previous();
   if (on && !tok_ok && lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
@@ -605,13 +608,12 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   int n_all = n_own + n_prefix;
   if (p.prefix_len == 0 && n_own <= 1) tok = -1, n_all = 0;    // the row has been written
   // all states of the row, WARPS shares of them one after the other
-  const int a = static_cast<int>(static_cast<long long>(n_all) * which / WARPS), b = static_cast<int>(static_cast<long long>(n_all) * (which + 1) / WARPS);
-  Row<HD> row = sum_states<HD, WARPS == 1 ? 8 : 16>(b - a, [&](int i) {
+  const int a = n_all * which / WARPS, b = n_all * (which + 1) / WARPS;
+  Row<HD> row = sum_states<HD, WARPS == 1 ? 8 : 16>(p.workspace, b - a, [&](int i) {
     const int k = a + i;
-    if (k >= n_own) return State{f.ml + (static_cast<long long>(item + c0 + k - n_own) * f.rows + in_block) * 2,
-                                 f.o + (static_cast<long long>(item + c0 + k - n_own) * f.rows + in_block) * HD};
-    if (n_own == 1) return wholes.at<HD>(e);
-    return parts.at<HD>((static_cast<long long>(k0 + k) * 2 + (k == 0 ? 1 : 0)) * group + h);
+    const bool is_front = k >= n_own, whole = n_own == 1;
+    const unsigned int at = is_front ? front + (k - n_own) * f.rows : whole ? e : ((k0 + k) * 2 + (k == 0 ? 1 : 0)) * group + h;
+    return state_at<HD>(p.workspace, is_front ? f.ml : whole ? wholes.ml : parts.ml, is_front ? f.o : whole ? wholes.o : parts.o, at);
   });
   if (WARPS > 1) {
 #pragma unroll
@@ -631,7 +633,7 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
         row.add(other);
       }
   }
-  if (which == 0 && tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(tok) * p.q_heads + head) * HD);
+  if (which == 0 && tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(tok) * q_heads + head) * HD);
 }
 
 // CTAs that share a request's pages for one KV head in a small batch, 0 where the general form is at least as fast: one launch instead
@@ -685,15 +687,15 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, int* bad_lists, Dec
   if (!done(launch_kernel(SHARED, kernel, ctas, kThreads, bytes, stream, 1, p, bad_lists, records, parts, wholes))) return NF_ERR_CUDA;
   // Few rows: four warps to each, since there are many pieces to a row then. With a prefix every row has states to join. Else the
   // pieces lead to the rows, of which most lie in one range.
-  const int rows = p.req_count * p.q_heads;
+  const int rows = p.req_count * p.q_heads, group = p.q_heads / p.kv_heads;
   if (rows <= 8 * sms) {
-    if (!done(launch_kernel(true, attn_join_rows_q8_kernel<HD, 4>, rows, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, ctas))) return NF_ERR_CUDA;
+    if (!done(launch_kernel(true, attn_join_rows_q8_kernel<HD, 4>, rows, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, group, ctas))) return NF_ERR_CUDA;
   } else if (SHARED) {
-    if (!done(launch_kernel(true, attn_join_rows_q8_kernel<HD, 1>, (rows + 3) / 4, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, ctas)))
+    if (!done(launch_kernel(true, attn_join_rows_q8_kernel<HD, 1>, (rows + 3) / 4, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, group, ctas)))
       return NF_ERR_CUDA;
   } else {
-    const int group = p.q_heads / p.kv_heads;
-    if (!done(launch_kernel(true, attn_join_parts_q8_kernel<HD>, ctas * group, 128, 0, stream, 1, p, records, parts, ctas * kWarps))) return NF_ERR_CUDA;
+    if (!done(launch_kernel(true, attn_join_parts_q8_kernel<HD>, ctas * group, 128, 0, stream, 1, p, records, parts, group, ctas * kWarps)))
+      return NF_ERR_CUDA;
   }
   return NF_OK;
 }
@@ -730,7 +732,8 @@ extern "C" long long nfk_attn_q8_workspace(const nfk_attn_q8_params* p) {
   using namespace nf;
   if (p == nullptr || !sizes_built(*p) || p->req_count < 0 || p->prefix_len < 0) return 0;
   const PrefixPlan f = prefix_plan(*p);
-  return counts_fit(*p, f) ? q8_workspace(*p, f).bytes : 0;
+  const long long bytes = counts_fit(*p, f) ? q8_workspace(*p, f).bytes : 0;
+  return bytes <= (1ll << 35) ? bytes : 0;                     // (rows of the workspace are counted in 16 bytes, in 32 bits)
 }
 
 extern "C" int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream) {
@@ -745,7 +748,7 @@ extern "C" int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stre
   PrefixPlan f = prefix_plan(*p);
   if (!counts_fit(*p, f)) return NF_ERR_BAD_ARG;
   const Q8Workspace ws = q8_workspace(*p, f);
-  if (p->workspace_bytes < ws.bytes) return NF_ERR_BAD_ARG;
+  if (p->workspace_bytes < ws.bytes || ws.bytes > (1ll << 35)) return NF_ERR_BAD_ARG;
   char* base = static_cast<char*>(p->workspace);
   const auto at = [&](long long offset) { return reinterpret_cast<float*>(base + offset); };
   f.ml = at(ws.prefix_ml);

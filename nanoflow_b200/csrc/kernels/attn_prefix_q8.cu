@@ -72,10 +72,9 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
 struct Share {
   int u, end, tiles, blocks;
   int item, kvh, block, t0, n;         // the current part: tiles t0 .. t0 + n - 1 of item (kvh, block)
-  __device__ __forceinline__ Share(const PrefixPlan& f, int kv_heads) : tiles(f.tiles), blocks(f.blocks) {
-    const Ranges ranges(prefix_units(f, kv_heads), f.ctas);
-    u = ranges.begin(blockIdx.x);
-    end = ranges.begin(blockIdx.x + 1);
+  __device__ __forceinline__ explicit Share(const PrefixPlan& f) : tiles(f.tiles), blocks(f.blocks) {
+    u = f.cut.begin(blockIdx.x);
+    end = f.cut.begin(blockIdx.x + 1);
   }
   __device__ __forceinline__ bool next() {
     if (u >= end) return false;
@@ -135,7 +134,7 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
       sc[k] = page < 0 ? 0.f : p.kv_scale[((static_cast<long long>(page) * 2 + PART) * p.kv_heads + kvh) * kQ8Page + lane % kQ8Page];
     }
   };
-  Share now(f, p.kv_heads), ahead = now;
+  Share now(f), ahead = now;
   int left = 0, tile_ahead = 0;                                  // the tile that is loaded next
   auto advance = [&]() {                                         // false: none
     if (left == 0) {
@@ -281,7 +280,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       return true;
     };
     bool ok = true;
-    Share now(f, p.kv_heads);
+    Share now(f);
     while (ok && now.next()) {
       if (!passed(C::Q_FULL, parts & 1) || !issue_s(g, g)) { fail(NF_ST_TIMEOUT_SMEM_FULL); break; }
       for (int t = 0; ok && t < now.n; ++t) {
@@ -318,7 +317,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     const int in_block = row / group, hh = row - in_block * group;
     uint32_t g = 0;
     bool ok = true;
-    Share now(f, p.kv_heads);
+    Share now(f);
     while (ok && now.next()) {
       // ---- this thread's row of Q. The products of the item before have all been formed: its last scores have been read. ----
       const int r = now.block * f.reqs_per_block + in_block;
@@ -529,6 +528,7 @@ PrefixPlan prefix_plan(const nfk_attn_q8_params& p) {
   const int least = f.tiles >= 128 ? 4 : f.tiles >= 32 ? 2 : 1;
   if (ctas > (units + least - 1) / least) ctas = static_cast<int>((units + least - 1) / least);
   f.ctas = ctas;
+  if (units <= 0x7fffffff) f.cut = Ranges(static_cast<int>(units), ctas);
   return f;
 }
 

@@ -14,11 +14,13 @@ constexpr float kQ8Log2e = 1.4426950408889634f;
 // A row of n units in w ranges (w <= n): the first n % w ranges have one more than the others.
 struct Ranges {
   int per, extra;
+  Ranges() = default;
   __host__ __device__ __forceinline__ Ranges(int n, int w) : per(w > 0 ? n / w : 0), extra(n - per * w) {}
   __host__ __device__ __forceinline__ int begin(int w) const { return w * per + (w < extra ? w : extra); }
   __host__ __device__ __forceinline__ int of(int u) const {             // the range that holds unit u
-    const int longer = extra * (per + 1);
-    return u < longer ? u / (per + 1) : extra + (u - longer) / per;
+    const unsigned int longer = static_cast<unsigned int>(extra) * (per + 1u), v = u;
+    const bool in_longer = v < longer;
+    return static_cast<int>((in_longer ? v : v - longer) / (in_longer ? per + 1u : static_cast<unsigned int>(per)) + (in_longer ? 0u : extra));
   }
 };
 
@@ -28,10 +30,10 @@ struct Ranges {
 constexpr int kPrefixTile = 64;
 struct PrefixPlan {
   int rows, reqs_per_block, blocks, tiles, ctas;
+  Ranges cut;                // of the units
   float* ml;                 // states, [pieces][rows]: reference (of exponents to base 2) and sum,
   float* o;                  // [pieces][rows][head_dim], not divided by the sum
 };
-__host__ __device__ __forceinline__ int prefix_units(const PrefixPlan& f, int kv_heads) { return kv_heads * f.blocks * f.tiles; }
 
 // The row of pages of the decode kernel is cut into a range for each of its warps, of two pages at least.
 constexpr int kDecodeCtasPerSm = 4, kDecodeWarps = 4;      // at most, of so many warps
