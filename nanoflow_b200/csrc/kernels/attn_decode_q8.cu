@@ -731,7 +731,8 @@ bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 
 extern "C" long long nfk_attn_q8_workspace(const nfk_attn_q8_params* p) {
   using namespace nf;
   if (p == nullptr || !sizes_built(*p) || p->req_count < 0 || p->prefix_len < 0) return 0;
-  const PrefixPlan f = prefix_plan(*p);
+  PrefixPlan f = prefix_plan(*p);
+  f.ctas = f.most_ctas;                                        // a shorter prefix may be cut finer
   const long long bytes = counts_fit(*p, f) ? q8_workspace(*p, f).bytes : 0;
   return bytes <= (1ll << 35) ? bytes : 0;                     // (rows of the workspace are counted in 16 bytes, in 32 bits)
 }

@@ -522,6 +522,7 @@ PrefixPlan prefix_plan(const nfk_attn_q8_params& p) {
   const long long units = static_cast<long long>(p.kv_heads) * f.blocks * f.tiles;         // (whether they fit 32 bits is asked afterwards)
   int ctas = (slots == 2 ? 1 : 2) * device_sm_count();
   if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
+  f.most_ctas = units < ctas ? static_cast<int>(units) : ctas;
   // Some tiles to a CTA where the prefix is long: every CTA leaves a piece of each row, and the rows' joins are bound by their number (8
   // requests of one KV head behind 30000 tokens: 31 us with a tile or two, 19 with four, 22 with eight; 16 of 8 behind 2000: 16.0 with
   // one, 14.4 with two, 14.8 with four; behind 500 12.5 with one, 12.9 with two).

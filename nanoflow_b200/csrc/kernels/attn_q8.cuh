@@ -30,6 +30,7 @@ struct Ranges {
 constexpr int kPrefixTile = 64;
 struct PrefixPlan {
   int rows, reqs_per_block, blocks, tiles, ctas;
+  int most_ctas;             // that this prefix or a part of it is cut over
   Ranges cut;                // of the units
   float* ml;                 // states, [pieces][rows]: reference (of exponents to base 2) and sum,
   float* o;                  // [pieces][rows][head_dim], not divided by the sum

@@ -86,6 +86,18 @@ def test_workspace_grows_with_the_sizes_and_covers_smaller_calls():
         size(requests=2 ** 24, prefix_len=2 ** 24)
 
 
+@pytest.mark.parametrize("kv_heads,group,dim", [(1, 4, 128), (1, 16, 64), (2, 3, 128), (8, 4, 128)])
+def test_workspace_covers_shorter_prefixes_and_fewer_requests(kv_heads, group, dim):
+    """Shorter prefixes are cut into smaller shares, fewer requests into other blocks of rows: the larger call's workspace holds them."""
+    size = lambda r, n: ops.decode_workspace_q8(requests=r, q_heads=kv_heads * group, kv_heads=kv_heads, head_dim=dim, prefix_len=n, device="cpu").numel()
+    lengths = [0, 1, 64, 65, 1984, 1985, 2048, 8000, 8128, 8129, 8192, 19000, 40000]
+    for counts in zip(lengths, lengths[1:]):
+        assert size(8, counts[0]) <= size(8, counts[1])
+    for n in lengths:
+        sizes = [size(r, n) for r in (1, 7, 8, 9, 31, 32, 33, 42, 43, 85, 86, 500)]
+        assert sizes == sorted(sizes)
+
+
 def test_quantising_in_the_plain_form():
     x = torch.tensor([[1.0, -2.0, 0.0], [0, 0, 0], [1e-30, 0, 0], [float("inf"), 1, 1], [2.0 ** -79, 0, 0]], dtype=torch.double)
     for dtype, largest in ref.Q8_LARGEST.items():
