@@ -159,7 +159,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.v_off = whole(a[14], what, "v_off");
     p.eps = real(a[17], what, "eps");
     if (qkv.scalar_type() != at::kBFloat16 || qkv.dim() != 2 || qkv.device() != c.device || (qkv.size(1) > 1 && qkv.stride(1) != 1) ||
-        qkv.size(0) > INT32_MAX)
+        qkv.size(0) > INT32_MAX || qkv.size(1) > INT32_MAX)
       refuse(what, "qkv must be a bfloat16 [T, columns] with unit inner stride on " + c.device.str());
     if (c.kv_heads != p.kv_heads || c.head_dim != p.head_dim || p.q_heads < 1 || p.q_heads > 65536) refuse(what, "kv_pool does not have these heads");
     const int64_t T = qkv.size(0), columns = qkv.size(1), hd = p.head_dim;
@@ -214,6 +214,8 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor& out = checked(what, "out", a[3], at::kBFloat16, c.device);
     if (out.dim() != 5 || out.size(0) != page_ids.numel() || out.sizes().slice(1) != c.pool.sizes().slice(1))
       refuse(what, "out must be [pages, 2, kv_heads, 16, head_dim]");
+    apart(what, c.pool, out);
+    apart(what, c.scale, out);
     nfk_kv_read_q8_params p = {};
     p.kv_pool = c.pool.data_ptr();
     p.kv_scale = static_cast<const float*>(c.scale.data_ptr());

@@ -314,11 +314,12 @@ typedef struct nfk_attn_q8_params {
   int req_begin, req_count, prefix_len, kind;
   float sm_scale;
   int num_ctas;              // CTA budget; 0 = as many as fit
-  void* workspace;           // nfk_attn_q8_workspace bytes, zero before the first use; launches that may run at the same time
-  long long workspace_bytes; // each need their own
+  void* workspace;           // nfk_attn_q8_workspace bytes at 256, whatever they hold; calls that may run at the same time each
+  long long workspace_bytes; // need their own
   unsigned int* status;
 } nfk_attn_q8_params;
-// Bytes of workspace for calls of up to these sizes (req_count, q_heads, kv_heads, head_dim, prefix_len); 0: sizes not built.
+// Bytes of workspace for calls with these heads (q_heads, kv_heads, head_dim), of up to req_count requests and prefix_len tokens; 0:
+// sizes not built.
 long long nfk_attn_q8_workspace(const nfk_attn_q8_params* p);
 int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream);
 

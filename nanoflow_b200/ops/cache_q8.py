@@ -96,8 +96,9 @@ def kv_read_q8(kv_pool: torch.Tensor, kv_scale: torch.Tensor, page_ids: torch.Te
 
 def decode_workspace_q8(*, requests: int, q_heads: int, kv_heads: int, head_dim: int, prefix_len: int = 0,
                         device="cuda") -> torch.Tensor:
-    """Workspace of ``attn_decode_q8`` and ``attn_decode_shared_q8`` calls of up to these sizes: zeros, which calls leave ready
-    for the next one. Calls that may run at the same time (two streams, two captured graphs) each need their own."""
+    """Workspace of ``attn_decode_q8`` and ``attn_decode_shared_q8`` calls with these heads, of up to ``requests`` requests and
+    ``prefix_len`` tokens of prefix. What it holds before a call does not matter. Calls that may run at the same time (two streams,
+    two captured graphs) each need their own."""
     p = AttnQ8Params(q_heads=q_heads, kv_heads=kv_heads, head_dim=head_dim, req_count=requests, prefix_len=prefix_len)
     fn = lib().nfk_attn_q8_workspace
     fn.restype = c_longlong
@@ -109,7 +110,7 @@ def decode_workspace_q8(*, requests: int, q_heads: int, kv_heads: int, head_dim:
         n = fn(byref(p))
     if n <= 0:
         raise RuntimeError("decode_workspace_q8: unsupported sizes (head_dim 64 or 128, up to 16 query heads per KV head, counts of 32 bits)")
-    return torch.zeros(n, dtype=torch.uint8, device=device)
+    return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def attn_decode_q8(q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *, q_heads: int, req_begin: int,

@@ -359,6 +359,24 @@ def test_no_prefix_is_plain_decode():
     assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("prefix,lengths", [(0, [3]), (0, [900, 0, 35, 1]), (0, [4000] * 5 + [17]), (130, [40, 0, 200]), (9000, [0])])
+def test_workspace_may_hold_anything(prefix, lengths):
+    """NaN and large words in the workspace, and one made for more requests and a longer prefix: the same rows."""
+    pool, scale = _cache(2000, 2, 128, E4M3)
+    ptr, idx, last = _lists(lengths, 2000, 3)
+    n = len(lengths)
+    q = torch.randn(n, 8 * 128, device="cuda").to(torch.bfloat16)
+    front = torch.arange(-(-prefix // 16), dtype=torch.int32, device="cuda")
+    sizes = dict(q_heads=8, kv_heads=2, head_dim=128)
+    made = [ops.decode_workspace_q8(requests=r, prefix_len=p, **sizes) for r, p in ((n, prefix), (n, prefix), (n + 60, prefix + 70))]
+    outs = []
+    for ws, byte in zip(made, (0, 255, 127)):
+        ws.fill_(byte)
+        outs.append(ops.attn_decode_shared_q8(q, torch.empty_like(q), pool, scale, torch.arange(n + 1, dtype=torch.int32, device="cuda"), ptr, idx,
+                                              last, front, prefix, q_heads=8, req_begin=0, req_count=n, workspace=ws))
+    assert bool(outs[0].isfinite().all()) and torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+
+
 def test_lists_that_are_none_are_reported():
     """Page numbers, rows and page lists out of range: a status, finite rows, and a workspace that still serves."""
     pool, scale = _cache(40, 2, 128, E4M3)
@@ -518,3 +536,60 @@ def test_prompt_and_decode_steps_on_one_cache(kind):
             ops.attn_decode_shared_q8(q, two, pool, scale, *lists, front, 80, q_heads=heads, req_begin=0, req_count=1, workspace=ws, status=st)
             ops.check_status(st)
             assert bool(((one[0] - two[0]).abs().float() <= 0.02 * one[0].abs().float() + 0.01 * one[0].abs().max()).all())
+
+
+def _refusal_arguments():
+    pool, scale = _cache(6, 2, 64, INT8)
+    ptr, idx, last = _lists([20, 30], 6, 1, extra=1)
+    x = torch.randn(2, 8 * 64, device="cuda").to(torch.bfloat16)
+    append = dict(qkv=x, q_out=torch.zeros(2, 4 * 64, dtype=torch.bfloat16, device="cuda"), kv_pool=pool, kv_scale=scale,
+                  inv_freq=torch.ones(32, device="cuda"), positions=_i32([3, 4]), token_req=_i32([0, 1]), kv_indptr=ptr, kv_indices=idx, q_heads=4,
+                  kv_heads=2, head_dim=64, q_off=0, k_off=256, v_off=384, status=None)
+    read = dict(kv_pool=pool, kv_scale=scale, page_ids=_i32([1, 2]), out=torch.zeros(2, 2, 2, 16, 64, dtype=torch.bfloat16, device="cuda"))
+    q = x[:, :256].contiguous()
+    decode = dict(q=q, out=torch.zeros_like(q), kv_pool=pool, kv_scale=scale, qo_indptr=_i32([0, 1]), kv_indptr=ptr, kv_indices=idx,
+                  kv_last_page_len=last, prefix_pages=_i32([0, 1]), prefix_len=20, q_heads=4, req_begin=0, req_count=2,
+                  workspace=ops.decode_workspace_q8(requests=2, q_heads=4, kv_heads=2, head_dim=64, prefix_len=20))
+    return {"append": (ops.rope_append_q8, append, "q_out"), "read": (ops.kv_read_q8, read, "out"), "decode": (ops.attn_decode_shared_q8, decode, "out")}
+
+
+@pytest.mark.parametrize("op,change,why", [
+    ("append", lambda a: dict(qkv=a["qkv"].float()), "bfloat16"), ("append", lambda a: dict(qkv=a["qkv"].t()), "unit inner stride"),
+    ("append", lambda a: dict(qkv=a["qkv"].cpu()), "on cuda"), ("append", lambda a: dict(q_out=a["q_out"][:1]), "q_out"),
+    ("append", lambda a: dict(q_out=a["qkv"][:, :256].contiguous().t().contiguous().t()), "q_out"),
+    ("append", lambda a: dict(q_out=a["qkv"].view(-1)[256:768].view(2, 256)), "overlap"),
+    ("append", lambda a: dict(k_off=-8), "columns"), ("append", lambda a: dict(v_off=392), "columns"), ("append", lambda a: dict(k_off=260), "alignment"),
+    ("append", lambda a: dict(q_heads=2 ** 31), "32 bits"), ("append", lambda a: dict(kv_heads=4), "these heads"),
+    ("append", lambda a: dict(head_dim=128), "these heads"), ("append", lambda a: dict(kv_scale=a["kv_scale"].view(-1)), "kv_scale"),
+    ("append", lambda a: dict(kv_pool=a["kv_pool"].view(torch.uint8)), "kv_pool"), ("append", lambda a: dict(positions=a["positions"].long()), "int32"),
+    ("append", lambda a: dict(token_req=a["token_req"][:1]), "per token"), ("append", lambda a: dict(kv_indptr=a["kv_indptr"][:1]), "per request"),
+    ("append", lambda a: dict(inv_freq=a["inv_freq"][:16]), "inv_freq"), ("append", lambda a: dict(q_norm=torch.ones(32, dtype=torch.bfloat16, device="cuda")), "norms"),
+    ("append", lambda a: dict(k_norm=torch.ones(64, device="cuda")), "bfloat16"), ("append", lambda a: dict(cos_sin=a["inv_freq"]), "cos_sin"),
+    ("append", lambda a: dict(eps="small"), "number"), ("append", lambda a: dict(status=a["positions"][:0]), "status"),
+    ("read", lambda a: dict(out=a["out"][:1]), "pages"), ("read", lambda a: dict(out=a["out"].half()), "bfloat16"),
+    ("read", lambda a: dict(page_ids=a["page_ids"].long()), "int32"), ("read", lambda a: dict(page_ids=[1, 2]), "tensor"),
+    ("read", lambda a: dict(kv_pool=a["kv_pool"][:, :, :, :, :32]), "kv_pool"), ("read", lambda a: dict(kv_scale=a["kv_scale"][:3]), "kv_scale"),
+    ("read", lambda a: dict(out=a["kv_pool"].view(-1).view(torch.bfloat16)[:4096].view(1, 2, 2, 16, 64), page_ids=a["page_ids"][:1]), "overlap"),
+    ("decode", lambda a: dict(q_heads=3), "KV head"), ("decode", lambda a: dict(q_heads=34), "KV head"), ("decode", lambda a: dict(q_heads=0), "KV head"),
+    ("decode", lambda a: dict(q_heads=2), "q and out"), ("decode", lambda a: dict(out=a["out"][:1]), "q and out"), ("decode", lambda a: dict(out=a["q"]), "overlap"),
+    ("decode", lambda a: dict(q=a["q"].half()), "bfloat16"), ("decode", lambda a: dict(req_count=3), "listed"), ("decode", lambda a: dict(req_begin=1), "listed"),
+    ("decode", lambda a: dict(req_begin=-1), "listed"), ("decode", lambda a: dict(kv_last_page_len=a["kv_last_page_len"][:1]), "listed"),
+    ("decode", lambda a: dict(prefix_len=-1), "negative"), ("decode", lambda a: dict(prefix_len=33), "prefix_pages"),
+    ("decode", lambda a: dict(prefix_pages=None), "prefix_pages"), ("decode", lambda a: dict(workspace=None), "workspace"),
+    ("decode", lambda a: dict(workspace=a["workspace"][256:]), "bad argument"), ("decode", lambda a: dict(workspace=a["workspace"][1:]), "bad argument"),
+    ("decode", lambda a: dict(num_ctas=-1), "bad argument"), ("decode", lambda a: dict(sm_scale="small"), "number"),
+    ("decode", lambda a: dict(kv_indices=a["kv_indices"].cpu()), "on cuda")])
+def test_calls_refuse(op, change, why):
+    """Arguments that do not fit are refused by the host, and nothing is written."""
+    call, args, written = _refusal_arguments()[op]
+    before = [args[k].clone() for k in (written, "kv_scale")]
+    with pytest.raises(RuntimeError, match=why):
+        call(**{**args, **change(args)})
+    torch.cuda.synchronize()
+    assert all(torch.equal(args[k], b) for k, b in zip((written, "kv_scale"), before))
+
+
+def test_the_calls_behind_the_refusals_serve():
+    for call, args, written in _refusal_arguments().values():
+        call(**args)
+        assert bool(args[written].any()) and bool(args[written].isfinite().all())
