@@ -144,9 +144,9 @@ PyObject* guarded(Py_ssize_t have, Py_ssize_t want, F f) {
 }
 
 // qkv, q_out, kv_pool, kv_scale, inv_freq, positions, token_req, kv_indptr, kv_indices, q_heads, kv_heads, head_dim, q_off, k_off,
-// v_off, q_norm, k_norm, eps, cos_sin, status
+// v_off, q_norm, k_norm, eps, cos_sin, status, early_start
 PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 20, [&] {
+  return guarded(n, 21, [&] {
     const char* what = "rope_append_q8";
     const Cache c = cache(what, a[2], a[3]);
     const Tensor& qkv = tensor(what, "qkv", a[0]);
@@ -201,13 +201,14 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.num_indices = count(what, kv_indices, "kv_indices");
     p.kind = c.kind;
     p.status = status_word(what, a[19], c.device);
+    p.early_start = whole(a[20], what, "early_start");
     if (T > 0) launch("nfk_rope_append_q8", entries.append, p, c.device);
   });
 }
 
-// kv_pool, kv_scale, page_ids, out, status
+// kv_pool, kv_scale, page_ids, out, status, early_start
 PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 5, [&] {
+  return guarded(n, 6, [&] {
     const char* what = "kv_read_q8";
     const Cache c = cache(what, a[0], a[1]);
     const Tensor& page_ids = checked(what, "page_ids", a[2], at::kInt, c.device);
@@ -227,14 +228,15 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.num_pages = c.pages;
     p.kind = c.kind;
     p.status = status_word(what, a[4], c.device);
+    p.early_start = whole(a[5], what, "early_start");
     if (p.n_pages > 0) launch("nfk_kv_read_q8", entries.read, p, c.device);
   });
 }
 
 // what, q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, prefix_pages, prefix_len, q_heads, req_begin,
-// req_count, sm_scale, num_ctas, workspace, status
+// req_count, sm_scale, num_ctas, workspace, status, early_start
 PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 18, [&] {
+  return guarded(n, 19, [&] {
     const char* what = PyUnicode_AsUTF8(a[0]);
     if (what == nullptr) {
       PyErr_Clear();
@@ -287,6 +289,7 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.workspace = workspace.data_ptr();
     p.workspace_bytes = workspace.numel();
     p.status = status_word(what, a[17], c.device);
+    p.early_start = whole(a[18], what, "early_start");
     if (p.req_count > 0) launch(what, entries.decode, p, c.device);
   });
 }

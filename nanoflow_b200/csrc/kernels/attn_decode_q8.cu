@@ -180,6 +180,10 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = p.q_heads / p.kv_heads;
   const int* indptr = p.kv_indptr + p.req_begin;
+  // The lists are complete before the kernel that joins states may start, which looks at them at once. (With a prefix, its kernel
+  // starts this one behind them.)
+  if (!SHARED) await_previous();
+  let_next_start();
   const int base = indptr[0];
   const bool in_shared = p.req_count <= kListed;
   auto start_of = [&](int r) { return in_shared ? starts[r] : indptr[r] - base; };
@@ -190,7 +194,6 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   const Ranges ranges(pages_all * p.kv_heads, n_ranges);
   const float scale = p.sm_scale * kQ8Log2e;
   __nv_bfloat16* out = reinterpret_cast<__nv_bfloat16*>(p.out);
-  let_next_start();
 
   // ---- loads: the pages of this warp's range ----
   const int range = blockIdx.x * kWarps + warp;
@@ -676,7 +679,7 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, int* bad_lists, Dec
   };
   if (MODE == FEW) {
     const int size = few_cluster(p);
-    return done(launch_kernel(false, kernel, p.req_count * p.kv_heads * size, kThreads, bytes, stream, size, p, bad_lists, records, parts, wholes))
+    return done(launch_kernel(early_first(p.early_start), kernel, p.req_count * p.kv_heads * size, kThreads, bytes, stream, size, p, bad_lists, records, parts, wholes))
                ? NF_OK : NF_ERR_CUDA;
   }
   const int sms = device_sm_count(), room = (fit < kDecodeCtasPerSm ? fit : kDecodeCtasPerSm) * sms;
@@ -684,17 +687,17 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, int* bad_lists, Dec
   int ctas = (useful + kWarps - 1) / kWarps;
   if (ctas < 1) ctas = 1;
   if (p.num_ctas > 0 && p.num_ctas < ctas) ctas = p.num_ctas;
-  if (!done(launch_kernel(SHARED, kernel, ctas, kThreads, bytes, stream, 1, p, bad_lists, records, parts, wholes))) return NF_ERR_CUDA;
+  if (!done(launch_kernel(SHARED ? early_further(p.early_start) : early_first(p.early_start), kernel, ctas, kThreads, bytes, stream, 1, p, bad_lists, records, parts, wholes))) return NF_ERR_CUDA;
   // Few rows: four warps to each, since there are many pieces to a row then. With a prefix every row has states to join. Else the
   // pieces lead to the rows, of which most lie in one range.
   const int rows = p.req_count * p.q_heads, group = p.q_heads / p.kv_heads;
   if (rows <= 8 * sms) {
-    if (!done(launch_kernel(true, attn_join_rows_q8_kernel<HD, 4>, rows, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, group, ctas))) return NF_ERR_CUDA;
+    if (!done(launch_kernel(early_further(p.early_start), attn_join_rows_q8_kernel<HD, 4>, rows, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, group, ctas))) return NF_ERR_CUDA;
   } else if (SHARED) {
-    if (!done(launch_kernel(true, attn_join_rows_q8_kernel<HD, 1>, (rows + 3) / 4, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, group, ctas)))
+    if (!done(launch_kernel(early_further(p.early_start), attn_join_rows_q8_kernel<HD, 1>, (rows + 3) / 4, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, group, ctas)))
       return NF_ERR_CUDA;
   } else {
-    if (!done(launch_kernel(true, attn_join_parts_q8_kernel<HD>, ctas * group, 128, 0, stream, 1, p, records, parts, group, ctas * kWarps)))
+    if (!done(launch_kernel(early_further(p.early_start), attn_join_parts_q8_kernel<HD>, ctas * group, 128, 0, stream, 1, p, records, parts, group, ctas * kWarps)))
       return NF_ERR_CUDA;
   }
   return NF_OK;

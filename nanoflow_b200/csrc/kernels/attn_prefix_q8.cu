@@ -217,6 +217,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNumBars);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  await_previous();                              // (before tensor memory is taken, which the kernel before may need)
   if ((sb & 1023u) != 0u) {                      // the operands' layouts need it; report instead of computing garbage
     if (threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
     return;
@@ -500,7 +501,7 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, cudaStream_t stream
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes) != cudaSuccess) return NF_ERR_CUDA;
     attr = true;
   }
-  if (launch_kernel(false, kernel, f.ctas, C::kThreads, C::kBytes, stream, 1, p, f) == cudaSuccess) return NF_OK;
+  if (launch_kernel(early_first(p.early_start), kernel, f.ctas, C::kThreads, C::kBytes, stream, 1, p, f) == cudaSuccess) return NF_OK;
   (void)cudaGetLastError();
   return NF_ERR_CUDA;
 }

@@ -283,6 +283,7 @@ typedef struct nfk_rope_append_q8_params {
   const void* k_norm;
   float eps;
   int T, q_heads, kv_heads, head_dim, num_pages, num_reqs, num_indices, kind;
+  int early_start;           // see nfk_gemm_params
   unsigned int* status;
 } nfk_rope_append_q8_params;
 int nfk_rope_append_q8(const nfk_rope_append_q8_params* p, cudaStream_t stream);
@@ -294,6 +295,7 @@ typedef struct nfk_kv_read_q8_params {
   void* out;                 // [n_pages][2][kv_heads][16][head_dim] bf16
   const int* page_ids;
   int n_pages, kv_heads, head_dim, num_pages, kind;
+  int early_start;           // see nfk_gemm_params
   unsigned int* status;
 } nfk_kv_read_q8_params;
 int nfk_kv_read_q8(const nfk_kv_read_q8_params* p, cudaStream_t stream);
@@ -314,6 +316,7 @@ typedef struct nfk_attn_q8_params {
   int req_begin, req_count, prefix_len, kind;
   float sm_scale;
   int num_ctas;              // CTA budget; 0 = as many as fit
+  int early_start;           // see nfk_gemm_params
   void* workspace;           // nfk_attn_q8_workspace bytes at 256, whatever they hold; calls that may run at the same time each
   long long workspace_bytes; // need their own
   unsigned int* status;

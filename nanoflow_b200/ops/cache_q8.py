@@ -3,6 +3,9 @@
 The cache of a layer is a pool ``[num_pages, 2, kv_heads, 16, head_dim]`` of ``float8_e4m3fn`` or ``int8`` numbers and a scale
 for every vector, ``[num_pages, 2, kv_heads, 16]`` in fp32; a cached value is number * scale. Pages, page lists and the calls
 have the form of the bf16 cache (:func:`nanoflow_b200.ops.rope_append`, :func:`nanoflow_b200.ops.attn_decode`), at half the bytes.
+
+``early_start`` (EARLY_*) of the calls: their kernels may be launched while the one before them on the stream still runs, and wait
+for it there; 0 keeps the SMs free until then, for another stream's kernels beside it.
 """
 from __future__ import annotations
 
@@ -12,7 +15,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import lib
+from . import EARLY_FIRST, EARLY_FURTHER, lib
 
 PAGE = 16
 KINDS = {torch.float8_e4m3fn: 0, torch.int8: 1}
@@ -24,12 +27,13 @@ class RopeAppendQ8Params(Structure):
                 ("cos_sin", c_void_p), ("positions", c_void_p), ("token_req", c_void_p), ("kv_indptr", c_void_p),
                 ("kv_indices", c_void_p), ("q_norm", c_void_p), ("k_norm", c_void_p), ("eps", c_float), ("T", c_int),
                 ("q_heads", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("num_pages", c_int), ("num_reqs", c_int),
-                ("num_indices", c_int), ("kind", c_int), ("status", c_void_p)]
+                ("num_indices", c_int), ("kind", c_int), ("early_start", c_int), ("status", c_void_p)]
 
 
 class KvReadQ8Params(Structure):
     _fields_ = [("kv_pool", c_void_p), ("kv_scale", c_void_p), ("out", c_void_p), ("page_ids", c_void_p), ("n_pages", c_int),
-                ("kv_heads", c_int), ("head_dim", c_int), ("num_pages", c_int), ("kind", c_int), ("status", c_void_p)]
+                ("kv_heads", c_int), ("head_dim", c_int), ("num_pages", c_int), ("kind", c_int),
+                ("early_start", c_int), ("status", c_void_p)]
 
 
 class AttnQ8Params(Structure):
@@ -37,7 +41,7 @@ class AttnQ8Params(Structure):
                 ("kv_indptr", c_void_p), ("kv_indices", c_void_p), ("kv_last_page_len", c_void_p), ("prefix_pages", c_void_p),
                 ("q_heads", c_int), ("kv_heads", c_int), ("head_dim", c_int), ("num_pages", c_int), ("num_tokens", c_int),
                 ("num_indices", c_int), ("req_begin", c_int), ("req_count", c_int), ("prefix_len", c_int), ("kind", c_int),
-                ("sm_scale", c_float), ("num_ctas", c_int), ("workspace", c_void_p), ("workspace_bytes", c_longlong),
+                ("sm_scale", c_float), ("num_ctas", c_int), ("early_start", c_int), ("workspace", c_void_p), ("workspace_bytes", c_longlong),
                 ("status", c_void_p)]
 
 
@@ -72,7 +76,7 @@ def rope_append_q8(qkv: torch.Tensor, q_out: torch.Tensor, kv_pool: torch.Tensor
                    positions: torch.Tensor, token_req: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor, *,
                    q_heads: int, kv_heads: int, head_dim: int, q_off: int, k_off: int, v_off: int,
                    q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
-                   cos_sin: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None) -> None:
+                   cos_sin: Optional[torch.Tensor] = None, status: Optional[torch.Tensor] = None, early_start: int = EARLY_FIRST) -> None:
     """:func:`nanoflow_b200.ops.rope_append` into the 8-bit cache: rotate q and k, write q to ``q_out`` (bf16) and k and v, each
     vector with its own scale (largest magnitude / 448 or / 127), into their page slots.
 
@@ -81,16 +85,16 @@ def rope_append_q8(qkv: torch.Tensor, q_out: torch.Tensor, kv_pool: torch.Tensor
     Two tokens of a call must not have the same request and position. A vector with an infinity or NaN is cached as NaN, one
     whose largest magnitude is below 2^-80 as zeros. A token whose page does not exist is not cached and reported in ``status``."""
     _calls().rope_append(qkv, q_out, kv_pool, kv_scale, inv_freq, positions, token_req, kv_indptr, kv_indices, q_heads, kv_heads, head_dim,
-                         q_off, k_off, v_off, q_norm, k_norm, eps, cos_sin, status)
+                         q_off, k_off, v_off, q_norm, k_norm, eps, cos_sin, status, early_start)
 
 
 def kv_read_q8(kv_pool: torch.Tensor, kv_scale: torch.Tensor, page_ids: torch.Tensor, *, out: Optional[torch.Tensor] = None,
-               status: Optional[torch.Tensor] = None) -> torch.Tensor:
+               status: Optional[torch.Tensor] = None, early_start: int = EARLY_FIRST) -> torch.Tensor:
     """``out[i]`` = the bf16 values of page ``page_ids[i]``: a pool that ``attn_prefill`` reads with the page list 0, 1, 2, ...
     Pages that do not exist are reported in ``status`` and leave their place in ``out`` as it was."""
     if out is None:
         out = torch.empty((page_ids.numel(), *kv_pool.shape[1:]), dtype=torch.bfloat16, device=kv_pool.device)
-    _calls().read(kv_pool, kv_scale, page_ids, out, status)
+    _calls().read(kv_pool, kv_scale, page_ids, out, status, early_start)
     return out
 
 
@@ -115,22 +119,22 @@ def decode_workspace_q8(*, requests: int, q_heads: int, kv_heads: int, head_dim:
 
 def attn_decode_q8(q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, *, q_heads: int, req_begin: int,
                    req_count: int, workspace: torch.Tensor, sm_scale: Optional[float] = None, num_ctas: int = 0,
-                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                   status: Optional[torch.Tensor] = None, early_start: int = EARLY_FIRST | EARLY_FURTHER) -> torch.Tensor:
     """:func:`nanoflow_b200.ops.attn_decode` over the 8-bit cache: single-query attention for requests [req_begin, req_begin +
     req_count), each with a row of ``q`` of its own. Contexts are cut over the CTAs by their pages, whatever their lengths. Requests
     without pages get zeros; rows of other requests are left as they were. Page numbers, rows and page lists that are none are
     reported in ``status``. ``workspace``: :func:`decode_workspace_q8`. ``num_ctas``: CTA budget, 0 = all that fit."""
     _calls().decode("attn_decode_q8", q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, None, 0, q_heads,
-                    req_begin, req_count, sm_scale, num_ctas, workspace, status)
+                    req_begin, req_count, sm_scale, num_ctas, workspace, status, early_start)
     return out
 
 
 def attn_decode_shared_q8(q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, prefix_pages: torch.Tensor,
                           prefix_len: int, *, q_heads: int, req_begin: int, req_count: int, workspace: torch.Tensor,
                           sm_scale: Optional[float] = None, num_ctas: int = 0,
-                          status: Optional[torch.Tensor] = None) -> torch.Tensor:
+                          status: Optional[torch.Tensor] = None, early_start: int = EARLY_FIRST | EARLY_FURTHER) -> torch.Tensor:
     """:func:`attn_decode_q8` for requests that all see the same first ``prefix_len`` tokens, those of ``prefix_pages``; their own
     page lists hold what comes after (or nothing). The prefix is read once for all of them."""
     _calls().decode("attn_decode_shared_q8", q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, prefix_pages,
-                    prefix_len, q_heads, req_begin, req_count, sm_scale, num_ctas, workspace, status)
+                    prefix_len, q_heads, req_begin, req_count, sm_scale, num_ctas, workspace, status, early_start)
     return out

@@ -377,6 +377,47 @@ def test_workspace_may_hold_anything(prefix, lengths):
     assert bool(outs[0].isfinite().all()) and torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("lengths", [([30, 5], [17, 18]), ([900, 33, 250, 1000], [3, 1500, 1, 600])])
+def test_kernels_that_start_early_see_what_the_ones_before_wrote(lengths):
+    """Lists, queries and the cache change in front of every call, on one stream without a wait: the rows of calls one by one."""
+    heads, kv_heads, dim, n = 8, 2, 128, len(lengths[0])
+    pool, scale = _cache(300, kv_heads, dim, E4M3)
+    keep = pool.clone(), scale.clone()
+    sets = [_lists(x, 250, 5 + i) for i, x in enumerate(lengths)]
+    size = max(idx.numel() for _, idx, _ in sets)
+    sets = [(ptr, torch.nn.functional.pad(idx, (0, size - idx.numel())), last) for ptr, idx, last in sets]
+    qkv = [torch.randn(n, (heads + 2 * kv_heads) * dim, device="cuda").to(torch.bfloat16) for _ in sets]
+    lists, row, q = [torch.empty_like(t) for t in sets[0]], torch.empty_like(qkv[0]), torch.empty(n, heads * dim, dtype=torch.bfloat16, device="cuda")
+    front, qo = torch.arange(250, 290, dtype=torch.int32, device="cuda"), torch.arange(n + 1, dtype=torch.int32, device="cuda")
+    ws = ops.decode_workspace_q8(requests=n, q_heads=heads, kv_heads=kv_heads, head_dim=dim, prefix_len=630)
+    freq = torch.rand(dim // 2, device="cuda")
+
+    def run(early, wait):
+        pool.view(torch.uint8).copy_(keep[0].view(torch.uint8))
+        scale.copy_(keep[1])
+        outs = []
+        for i in range(12):
+            for to, new in zip(lists, sets[i & 1]):
+                to.copy_(new)
+            row.copy_(qkv[i & 1])
+            position = (lists[0][1:] - lists[0][:-1]) * 16 - 16 + lists[2] - 1
+            ops.rope_append_q8(row, q, pool, scale, freq, position.int(), qo[:n], lists[0], lists[1], q_heads=heads, kv_heads=kv_heads, head_dim=dim,
+                               q_off=0, k_off=heads * dim, v_off=(heads + kv_heads) * dim, early_start=early & 1)
+            a = ops.attn_decode_q8(q, torch.zeros_like(q), pool, scale, qo, *lists, q_heads=heads, req_begin=0, req_count=n, workspace=ws,
+                                   early_start=early)
+            b = ops.attn_decode_shared_q8(q, torch.zeros_like(q), pool, scale, qo, *lists, front, 630, q_heads=heads, req_begin=0, req_count=n,
+                                          workspace=ws, early_start=early)
+            outs += [a, b, ops.kv_read_q8(pool, scale, lists[1], early_start=early & 1)]
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return outs
+
+    want = run(0, True)
+    for early in (0, 1, 2, 3, 3):
+        assert all(torch.equal(x, y) for x, y in zip(run(early, False), want))
+
+
 def test_lists_that_are_none_are_reported():
     """Page numbers, rows and page lists out of range: a status, finite rows, and a workspace that still serves."""
     pool, scale = _cache(40, 2, 128, E4M3)
