@@ -35,9 +35,9 @@ __device__ __forceinline__ float2 turn(int pos, float f) {
 
 // A CTA per token; HD / 16 threads per head, each with eight elements of either half, so that a thread holds both elements of its
 // eight pairs, and the same pairs for every head that it takes: its cosines and sines stay in registers. What bounds it is the issue
-// of instructions, and latency: arithmetic is two elements at a time, and a thread requests its elements of BATCH heads before the
+// of instructions, and latency (2048 tokens, 32 / 8 heads, norms: 13 us for 46 MB; 683 tokens 8): arithmetic is two elements at a time, and a thread requests its elements of BATCH heads before the
 // CTA works out the token's angles and page. It does not let the next kernel start: CTAs that wait beside its last ones cost more
-// than their launch (2048 tokens and a kv_read_q8 behind them 17.7 us, so 15.9).
+// than their launch (2048 tokens and a kv_read_q8 behind them 17.7 us, without 15.9).
 template <int HD, int KIND>
 __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_rope_append_q8_params p) {
   constexpr int HALF = HD / 2, LPH = HD / 16, AT_ONCE = kAppendThreads / LPH, BATCH = 3;
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_r
 }
 
 // A thread has eight numbers per step: an 8-byte load, their vector's scale, a 16-byte store, so that a warp's loads and its stores
-// are of whole rows (16 numbers and two stores 32 bytes apart: 4096 pages 77 us instead of 69). All loads of a CTA's STEPS steps are
-// on their way before the first store.
+// are of whole rows (16 numbers and two stores 32 bytes apart: 4096 pages 77 us instead of 69). All loads of a CTA's steps are on
+// their way before the first store: 4096 pages of 8 heads 66 us, 6.2 TB/s, 0.94 of a copy's rate.
 constexpr int kReadSteps = 8;
 template <int HD, int KIND>
 __global__ void __launch_bounds__(256) kv_read_q8_kernel(nfk_kv_read_q8_params p, int parts) {
