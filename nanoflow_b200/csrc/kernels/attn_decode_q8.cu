@@ -3,7 +3,7 @@
 //   o_h = sum_j e^(s_hj) v_j / sum_j e^(s_hj),   s_hj = sm_scale (q_h . k_j),   k_j = number_j * kscale_j, v_j likewise
 //
 // Bound by the cache's bytes: 683 requests of 1024 to 1536 tokens, 32 / 8 heads, 316 us, 5.8 TB/s, 0.89 of a copy's rate; 256
-// requests of 200 to 2000, 64 / 8 heads, 94 us, 0.73 (82 without the join). A warp reads pages straight into the layout that the tensor cores take: with S^T = K Q^T the keys
+// requests of 200 to 2000, 64 / 8 heads, 93 us, 0.74 (83 without the join). A warp reads pages straight into the layout that the tensor cores take: with S^T = K Q^T the keys
 // are the 16-row operand (a page's 16 tokens) and the up to 8 query heads of a KV head the 8 columns (16 heads: two such
 // products), and which elements of head_dim form a step of the product is free, so a lane's bytes of a key are 16 neighbours, its
 // f16 pairs the operand's registers, and no lane needs what another one loaded. O^T = V^T P^T works the same way: V^T is the
@@ -112,54 +112,64 @@ __device__ __forceinline__ State state_at(const void* workspace, const float* ml
   return State{__ldcg(reinterpret_cast<const float2*>(ml) + i),
                static_cast<unsigned int>((reinterpret_cast<const char*>(o) - static_cast<const char*>(workspace)) >> 4) + i * (HD / 4)};
 }
-// Sum of n states, the i-th being at(i), in their order. Lanes fetch 32 references and sums at a time and AHEAD rows are requested
-// without waiting for one another.
-template <int HD, int AHEAD, class At>
-__device__ __forceinline__ Row<HD> sum_states(const void* workspace, int n, At at) {
+// Sums of n states for H neighbouring heads, the i-th of head k being at(i, k), in their order. Lanes fetch 32 references and sums at
+// a time and AHEAD rows of each head are requested without waiting for one another.
+template <int HD, int AHEAD, int H, class At>
+__device__ __forceinline__ void sum_states(const void* workspace, int n, At at, Row<HD> (&all)[H]) {
   constexpr int N = Row<HD>::N;
   const int lane = threadIdx.x & 31;
   const char* base = static_cast<const char*>(workspace) + lane * (N * 4);
-  Row<HD> all;
   for (int i0 = 0; i0 < n; i0 += 32) {
     const int here = min(32, n - i0);
-    const State mine = at(i0 + min(lane, here - 1));
-    Row<HD> part;
-    float w = 0.f;
-    for (int i = 0; i < here; i += AHEAD) {
-      float x[AHEAD][N];
+    State mine[H];
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        if (i + k >= here) break;
-        const char* row = base + (static_cast<unsigned long long>(__shfl_sync(0xffffffffu, mine.row, i + k)) << 4);
-        if constexpr (HD == 128) {
-          const float4 v = __ldcg(reinterpret_cast<const float4*>(row));
-          x[k][0] = v.x; x[k][1] = v.y; x[k][2] = v.z; x[k][3] = v.w;
-        } else {
-          const float2 v = __ldcg(reinterpret_cast<const float2*>(row));
-          x[k][0] = v.x; x[k][1] = v.y;
+    for (int k = 0; k < H; ++k) mine[k] = at(i0 + min(lane, here - 1), k);
+    Row<HD> part[H];
+    float w[H] = {};
+    for (int i = 0; i < here; i += AHEAD) {
+      float x[AHEAD][H][N];
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (i + j >= here) break;
+        const char* row = base + (static_cast<unsigned long long>(__shfl_sync(0xffffffffu, mine[0].row, i + j)) << 4);
+#pragma unroll
+        for (int k = 0; k < H; ++k)
+          if constexpr (HD == 128) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(row + k * (HD * 4)));
+            x[j][k][0] = v.x; x[j][k][1] = v.y; x[j][k][2] = v.z; x[j][k][3] = v.w;
+          } else {
+            const float2 v = __ldcg(reinterpret_cast<const float2*>(row + k * (HD * 4)));
+            x[j][k][0] = v.x; x[j][k][1] = v.y;
+          }
+      }
+      if (i == 0)                                              // (while the first rows are on their way)
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          part[k].m = mine[k].ml.x;
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) part[k].m = fmaxf(part[k].m, __shfl_xor_sync(0xffffffffu, part[k].m, off));
+          w[k] = lane < here ? q8_exp2(mine[k].ml.x - (part[k].m == -INFINITY ? 0.f : part[k].m)) : 0.f;
+          part[k].l = mine[k].ml.y * w[k];
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) part[k].l += __shfl_xor_sync(0xffffffffu, part[k].l, off);
+        }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) {
+        if (i + j >= here) break;
+#pragma unroll
+        for (int k = 0; k < H; ++k) {
+          const float by = __shfl_sync(0xffffffffu, w[k], i + j);
+#pragma unroll
+          for (int e = 0; e < N; ++e) part[k].o[e] += by * x[j][k][e];
         }
       }
-      if (i == 0) {                                            // (while the first rows are on their way)
-        part.m = mine.ml.x;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) part.m = fmaxf(part.m, __shfl_xor_sync(0xffffffffu, part.m, off));
-        w = lane < here ? q8_exp2(mine.ml.x - (part.m == -INFINITY ? 0.f : part.m)) : 0.f;
-        part.l = mine.ml.y * w;
-#pragma unroll
-        for (int off = 16; off > 0; off >>= 1) part.l += __shfl_xor_sync(0xffffffffu, part.l, off);
-      }
-#pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        if (i + k >= here) break;
-        const float by = __shfl_sync(0xffffffffu, w, i + k);
-#pragma unroll
-        for (int e = 0; e < N; ++e) part.o[e] += by * x[k][e];
-      }
     }
-    if (i0 == 0) all = part;
-    else all.add(part);
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      if (i0 == 0) all[k] = part[k];
+      else all[k].add(part[k]);
+    }
   }
-  return all;
 }
 
 __device__ __forceinline__ float2 ld_cluster_f32x2(uint32_t a) {
@@ -562,22 +572,25 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   }
 }
 
-// Joins the states of requests that lie in more than one range, a warp to each (range that one begins in, head). Bound by latency:
-// record, then states, in some waves; 10 us for 256 requests of 64 heads. Fewer CTAs that walk over the records were slower by 2 to 4
-// us, and so were more of them to an SM with two or four rows ahead instead of eight (sixteen: 1 to 5 us slower).
-template <int HD>
+// Joins the states of requests that lie in more than one range, a warp to each (range that one begins in, H heads). Bound by latency:
+// record, then states, in some waves; 8 us for 256 requests of 64 heads. Fewer CTAs that walk over the records were slower by 2 to 4 us.
+template <int HD, int H>
 __global__ void __launch_bounds__(128)
 attn_join_parts_q8_kernel(nfk_attn_q8_params p, const DecodeRecord* records, States parts, unsigned int group, unsigned int n_ranges) {
-  const unsigned int e = blockIdx.x * 4 + (threadIdx.x >> 5), range = e / group, h = e - range * group;
+  const unsigned int e = blockIdx.x * 4 + (threadIdx.x >> 5), range = e / (group / H), h = (e - range * (group / H)) * H;
   await_previous();
   if (range >= n_ranges) return;
   const int4 raw = __ldcg(reinterpret_cast<const int4*>(records) + range);
   const DecodeRecord rec = {raw.x, raw.y, raw.z, raw.w};
   if (rec.n == 0) return;
-  const Row<HD> row = sum_states<HD, 8>(p.workspace, rec.n, [&](int i) {
-    return state_at<HD>(p.workspace, parts.ml, parts.o, ((range + i) * 2 + (i == 0 ? 1 : 0)) * group + h);
-  });
-  if (rec.tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(rec.tok) * p.q_heads + rec.kvh * group + h) * HD);
+  Row<HD> rows[H];
+  sum_states<HD, H == 2 ? 2 : 6>(p.workspace, rec.n, [&](int i, int k) {
+    return state_at<HD>(p.workspace, parts.ml, parts.o, ((range + i) * 2 + (i == 0 ? 1 : 0)) * group + h + k);
+  }, rows);
+  if (rec.tok >= 0)
+#pragma unroll
+    for (int k = 0; k < H; ++k)
+      rows[k].finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(rec.tok) * p.q_heads + rec.kvh * group + h + k) * HD);
 }
 
 // The same row by row, with the shared prefix's states where there is one, and WARPS warps to a row: a context of 900 tokens is 29
@@ -590,7 +603,7 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = warp % WARPS;
   const int* indptr = p.kv_indptr + p.req_begin;
   // lists and their cut while the kernels before this one still run: they do not write them
-  const unsigned int e = blockIdx.x * (4 / WARPS) + warp / WARPS, q_heads = p.q_heads;
+  const unsigned int q_heads = p.q_heads, e = blockIdx.x * (4 / WARPS) + warp / WARPS;             // the row, r * q_heads + head
   const bool on = e < p.req_count * q_heads;
   const unsigned int r = on ? e / q_heads : 0, head = on ? e - r * q_heads : 0, kvh = head / group, h = head - kvh * group;
   const int base = indptr[0], pages_all = indptr[p.req_count] - base, begin = indptr[r] - base, end = indptr[r + 1] - base;
@@ -617,12 +630,14 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   if (p.prefix_len == 0 && n_own <= 1) tok = -1, n_all = 0;    // the row has been written
   // all states of the row, WARPS shares of them one after the other
   const int a = n_all * which / WARPS, b = n_all * (which + 1) / WARPS;
-  Row<HD> row = sum_states<HD, WARPS == 1 ? 8 : 16>(p.workspace, b - a, [&](int i) {
+  Row<HD> rows[1];
+  Row<HD>& row = rows[0];
+  sum_states<HD, WARPS == 1 ? 6 : 16>(p.workspace, b - a, [&](int i, int) {
     const int k = a + i;
     const bool is_front = k >= n_own, whole = n_own == 1;
     const unsigned int at = is_front ? front + (k - n_own) * f.rows : whole ? e : ((k0 + k) * 2 + (k == 0 ? 1 : 0)) * group + h;
     return state_at<HD>(p.workspace, is_front ? f.ml : whole ? wholes.ml : parts.ml, is_front ? f.o : whole ? wholes.o : parts.o, at);
-  });
+  }, rows);
   if (WARPS > 1) {
 #pragma unroll
     for (int i = 0; i < Row<HD>::N; ++i) shared_o[warp][lane * Row<HD>::N + i] = row.o[i];
@@ -696,16 +711,15 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, int* bad_lists, Dec
   // Few rows: four warps to each, since there are many pieces to a row then. With a prefix every row has states to join. Else the
   // pieces lead to the rows, of which most lie in one range.
   const int rows = p.req_count * p.q_heads, group = p.q_heads / p.kv_heads;
-  if (rows <= 8 * sms) {
-    if (!done(launch_kernel(early_further(p.early_start), attn_join_rows_q8_kernel<HD, 4>, rows, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, group, ctas))) return NF_ERR_CUDA;
-  } else if (SHARED) {
-    if (!done(launch_kernel(early_further(p.early_start), attn_join_rows_q8_kernel<HD, 1>, (rows + 3) / 4, 128, 0, stream, 1, p, f, bad_lists, parts, wholes, group, ctas)))
-      return NF_ERR_CUDA;
-  } else {
-    if (!done(launch_kernel(early_further(p.early_start), attn_join_parts_q8_kernel<HD>, ctas * group, 128, 0, stream, 1, p, records, parts, group, ctas * kWarps)))
-      return NF_ERR_CUDA;
-  }
-  return NF_OK;
+  const auto join = [&](auto kernel, int grid, auto... args) {
+    return done(launch_kernel(early_further(p.early_start), kernel, grid, 128, 0, stream, 1, args...)) ? NF_OK : NF_ERR_CUDA;
+  };
+  if (rows <= 8 * sms) return join(attn_join_rows_q8_kernel<HD, 4>, rows, p, f, bad_lists, parts, wholes, group, ctas);
+  if (SHARED) return join(attn_join_rows_q8_kernel<HD, 1>, (rows + 3) / 4, p, f, bad_lists, parts, wholes, group, ctas);
+  // Two heads to a warp where a KV head has many (groups of 8: 256 requests 94.1 us instead of 95.5; of 16: 31.8 instead of 32.5; of 4:
+  // 88 instead of 87.4).
+  if (group >= 8 && group % 2 == 0) return join(attn_join_parts_q8_kernel<HD, 2>, ctas * (group / 2), p, records, parts, group, ctas * kWarps);
+  return join(attn_join_parts_q8_kernel<HD, 1>, ctas * group, p, records, parts, group, ctas * kWarps);
 }
 
 template <int HD, int NT, int KIND, class... A>
