@@ -619,8 +619,8 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   }
   if (on && p.prefix_len > 0) {
     const unsigned int in = r / static_cast<unsigned int>(f.reqs_per_block), item = kvh * f.blocks + in;
-    const int c0 = f.cut.of(item * f.tiles);
-    n_prefix = f.cut.of((item + 1) * f.tiles - 1) - c0 + 1;
+    const int span = f.lead + f.tiles, c0 = f.cut.of(item * span + f.lead);
+    n_prefix = f.cut.of((item + 1) * span - 1) - c0 + 1;
     front = (item + c0) * f.rows + (r - in * f.reqs_per_block) * group + h;
   }
   await_previous();
@@ -742,7 +742,7 @@ bool sizes_built(const nfk_attn_q8_params& p) {
 bool counts_fit(const nfk_attn_q8_params& p, const PrefixPlan& f) {
   const long long most = 0x7ffffff0ll;
   return static_cast<long long>(p.num_indices) * p.kv_heads <= most && static_cast<long long>(p.req_count) * p.q_heads <= most &&
-         static_cast<long long>(p.kv_heads) * f.blocks <= most / (f.tiles > 0 ? f.tiles : 1) &&
+         static_cast<long long>(p.kv_heads) * f.blocks <= most / (f.tiles > 0 ? f.lead + f.tiles : 1) &&
          static_cast<long long>(p.req_begin) + p.req_count <= most;
 }
 bool aligned16(const void* a) { return (reinterpret_cast<uintptr_t>(a) & 15) == 0; }

@@ -25,11 +25,11 @@ struct Ranges {
 };
 
 // The shared prefix: the query rows of a KV head (requests x group) are cut into blocks of at most `rows` (128 or 256) rows, whole
-// requests each. An item is (KV head, block), its units the prefix's tiles of 64 tokens. The piece of item i by CTA c has number
+// requests each. An item is (KV head, block), its units `lead` units for its beginning and then the prefix's tiles of 64 tokens. The piece of item i by CTA c has number
 // i + c: along the row of units every new piece raises one of the two.
 constexpr int kPrefixTile = 64;
 struct PrefixPlan {
-  int rows, reqs_per_block, blocks, tiles, ctas;
+  int rows, reqs_per_block, blocks, tiles, lead, ctas;
   int most_ctas;             // that this prefix or a part of it is cut over
   Ranges cut;                // of the units
   float* ml;                 // states, [pieces][rows]: reference (of exponents to base 2) and sum,

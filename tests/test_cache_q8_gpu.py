@@ -347,6 +347,23 @@ def test_more_requests_than_a_block_lists(prefix):
     _check_rows(out, ref.attn_decode_q8(q, *args, q_heads=2, req_begin=0, req_count=1100, prefix_pages=front, prefix_len=prefix), 64)
 
 
+@pytest.mark.parametrize("heads,kv_heads,requests,prefix,ctas", [(8, 2, 5, 5000, 3), (16, 4, 70, 3333, 7), (16, 4, 70, 3333, 0), (3, 1, 2, 9001, 40), (32, 8, 9, 700, 5)])
+def test_shared_prefix_over_few_ctas(heads, kv_heads, requests, prefix, ctas):
+    """Shares with the ends of several items, shares that end where an item begins."""
+    pages = -(-prefix // 16)
+    pool, scale = _cache(pages + 60, kv_heads, 64, E4M3, seed=4)
+    ptr, idx, last = _lists([(7 * i) % 12 for i in range(requests)], pages + 60, 6)
+    front = torch.arange(pages, dtype=torch.int32, device="cuda").flip(0).contiguous()
+    q = torch.randn(requests, heads * 64, device="cuda").to(torch.bfloat16)
+    args = (pool, scale, torch.arange(requests + 1, dtype=torch.int32, device="cuda"), ptr, idx, last)
+    ws = ops.decode_workspace_q8(requests=requests, q_heads=heads, kv_heads=kv_heads, head_dim=64, prefix_len=prefix)
+    ws.fill_(255)
+    out, st = torch.zeros_like(q), ops.new_status()
+    ops.attn_decode_shared_q8(q, out, *args, front, prefix, q_heads=heads, req_begin=0, req_count=requests, workspace=ws, num_ctas=ctas, status=st)
+    ops.check_status(st)
+    _check_rows(out, ref.attn_decode_q8(q, *args, q_heads=heads, req_begin=0, req_count=requests, prefix_pages=front, prefix_len=prefix), 64)
+
+
 def test_no_prefix_is_plain_decode():
     pool, scale = _cache(40, 2, 128, E4M3)
     ptr, idx, last = _lists([100, 7, 333], 40, 3)
