@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_r
       for (int o = LPH / 2; o > 0; o >>= 1) most = max3_magnitude(most, __shfl_xor_sync(0xffffffffu, most, o), 0.f);
       if (on && !is_q) {
         const int hh = is_k ? h - p.q_heads : h - p.q_heads - p.kv_heads;
-        float scale = most * (1.f / q8_largest<KIND>()), inv = __fdividef(q8_largest<KIND>(), most);
+        // (a quarter of both: __fdividef gives 0 for a divisor above 2^126)
+        float scale = most * (1.f / q8_largest<KIND>()), inv = __fdividef(0.25f * q8_largest<KIND>(), 0.25f * most);
         if (!(most >= kQ8Smallest && most <= 3.402823466e38f)) {       // nothing to speak of, or not finite
           scale = most < kQ8Smallest ? 0.f : __uint_as_float(0x7fc00000u);
           inv = 0.f;
