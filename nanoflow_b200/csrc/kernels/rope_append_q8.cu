@@ -33,6 +33,9 @@ __device__ __forceinline__ float2 turn(int pos, float f) {
   return make_float2(c, s);
 }
 
+// Mean squares (and eps) that a norm takes as fp32 sums them: nothing that counts is lost below, and the sum of 128 squares is finite.
+constexpr float kLeastSquare = 7.8886091e-31f, kMostSquare = 1.329228e36f;      // 2^-100, 2^120
+
 // A CTA per token; HD / 16 threads per head, each with eight elements of either half, so that a thread holds both elements of its
 // eight pairs, and the same pairs for every head that it takes: its cosines and sines stay in registers. What bounds it is the issue
 // of instructions, and latency (2048 tokens, 32 / 8 heads, norms: 13 us for 46 MB; 683 tokens 8): arithmetic is two elements at a time, and a thread requests its elements of BATCH heads before the
@@ -84,6 +87,18 @@ __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_r
     si[j] = reinterpret_cast<const f32x2*>(sines + 8 * l)[j];
     minus_si[j] = si[j] ^ 0x8000000080000000ull;
   }
+  // the head's largest magnitude, NaN where there is one
+  const auto largest = [](const f32x2 (&x)[4], const f32x2 (&y)[4]) {
+    float most = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      most = max3_magnitude(most, halves(x[j]).x, halves(x[j]).y);
+      most = max3_magnitude(most, halves(y[j]).x, halves(y[j]).y);
+    }
+#pragma unroll
+    for (int o = LPH / 2; o > 0; o >>= 1) most = max3_magnitude(most, __shfl_xor_sync(0xffffffffu, most, o), 0.f);
+    return most;
+  };
   for (int first = 0; first < heads; first += BATCH * AT_ONCE) {
     if (first > 0) load(first);
 #pragma unroll
@@ -96,16 +111,32 @@ __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_r
       unpack8(on ? hi[i] : make_uint4(0, 0, 0, 0), b);
       const bool norm = is_q ? p.q_norm != nullptr : is_k && p.k_norm != nullptr;
       if (__any_sync(0xffffffffu, norm)) {
-        f32x2 ss = mul2(a[0], a[0]);
+        const auto mean = [&]() {
+          f32x2 ss = mul2(a[0], a[0]);
 #pragma unroll
-        for (int j = 1; j < 4; ++j) ss = fma2(a[j], a[j], ss);
+          for (int j = 1; j < 4; ++j) ss = fma2(a[j], a[j], ss);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) ss = fma2(b[j], b[j], ss);
-        float sum = halves(ss).x + halves(ss).y;
+          for (int j = 0; j < 4; ++j) ss = fma2(b[j], b[j], ss);
+          float sum = halves(ss).x + halves(ss).y;
 #pragma unroll
-        for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          for (int o = LPH / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          return sum * (1.f / HD);
+        };
+        float square = mean() + p.eps;
+        const bool far = norm && !(square >= kLeastSquare && square <= kMostSquare);
+        if (__any_sync(0xffffffffu, far)) {                    // such a head once more, brought to [1, 2) by a power of two
+          const float top = largest(a, b);
+          const float by = far ? __uint_as_float((254u - min(max(__float_as_uint(top) >> 23 & 255u, 47u), 253u)) << 23) : 1.f;      // (up to 2^80)
+          const f32x2 by2 = pair(by, by);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            a[j] = mul2(a[j], by2);
+            b[j] = mul2(b[j], by2);
+          }
+          square = mean() + p.eps * by * by;
+        }
         if (norm) {
-          const float inv = rsqrtf(sum * (1.f / HD) + p.eps);
+          const float inv = rsqrtf(square);
           const f32x2 inv2 = pair(inv, inv);
           const f32x2* w = reinterpret_cast<const f32x2*>(weights[is_q ? 0 : 1] + 8 * l);
 #pragma unroll
@@ -129,14 +160,7 @@ __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_r
         *reinterpret_cast<uint4*>(dst + HALF) = pack8(b);
       }
       if (__all_sync(0xffffffffu, is_q)) continue;
-      float most = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        most = max3_magnitude(most, halves(a[j]).x, halves(a[j]).y);
-        most = max3_magnitude(most, halves(b[j]).x, halves(b[j]).y);
-      }
-#pragma unroll
-      for (int o = LPH / 2; o > 0; o >>= 1) most = max3_magnitude(most, __shfl_xor_sync(0xffffffffu, most, o), 0.f);
+      const float most = largest(a, b);
       if (on && !is_q) {
         const int hh = is_k ? h - p.q_heads : h - p.q_heads - p.kv_heads;
         // (a quarter of both: __fdividef gives 0 for a divisor above 2^126)

@@ -73,3 +73,30 @@ def test_append_of_the_largest_finite_vectors(kind):
         assert 2.0 ** 126 < float(rk.abs().max()) < 2.0 ** 128
         _, numbers, scale, _ = _append(normal, kind, k_norm=w)
         _check_vectors(rk[:, 0], numbers[0], scale[0], kind)
+
+
+@KINDS
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -120, 1e-6, 3.0])
+def test_norms_of_heads_whose_squares_leave_fp32(kind, eps):
+    """Entries from 2^-120 to the largest of bf16 in front of the norms of queries and keys, one size to a token, normal ones between
+    them (which keep the bits that they have alone)."""
+    g = torch.Generator().manual_seed(2)
+    sizes = [2.0 ** 60, 2.0 ** 63, 1.0, 2.0 ** 64, 2.0 ** 90, 2.0 ** 120, 2.0 ** 125, 1.0, 2.0 ** -50, 2.0 ** -70, 2.0 ** -75, 2.0 ** -120]
+    x = torch.randn(len(sizes), 3 * DIM, generator=g).clamp(-3.9, 3.9)
+    x = (x.double() * torch.tensor(sizes, dtype=torch.double)[:, None]).to(torch.bfloat16)
+    x[6, DIM] = x[6, 5] = LARGEST_BF16
+    assert bool(x.isfinite().all())
+    w = [(1 + 0.1 * torch.randn(DIM, generator=g)).to(torch.bfloat16) for _ in range(2)]
+    positions = [3 * t for t in range(len(sizes))]
+    q, numbers, scale, _ = _append(x.cuda(), kind, positions, q_norm=w[0].cuda(), k_norm=w[1].cuda(), eps=eps)
+    rq, rk, rv = ref.rope_append_q8(x, torch.ones(DIM // 2), torch.tensor(positions), q_heads=1, kv_heads=1, head_dim=DIM, q_off=0, k_off=DIM,
+                                    v_off=2 * DIM, q_norm=w[0], k_norm=w[1], eps=eps)
+    # angles, norms' sums and the rotation in fp32: 2^-20 of the largest entry (and bf16's smallest step, 2^-133)
+    err = (q.cpu().double() - rq[:, 0]).abs()
+    assert bool((err <= 2.0 ** -8 * rq[:, 0].abs() + 2.0 ** -20 * rq[:, 0].abs().amax(-1, keepdim=True) + 2.0 ** -133).all()), float(err.max())
+    seen = rk[:, 0].abs().amax(-1) >= 2.0 ** -79              # (below 2^-80 vectors are zeros)
+    _check_vectors(rk[seen, 0], numbers[0][seen], scale[0][seen], kind)
+    assert not numbers[0][~seen].any() and not scale[0][~seen].any()
+    normal = [2, 7]
+    alone = _append(x[normal].cuda(), kind, [positions[t] for t in normal], q_norm=w[0].cuda(), k_norm=w[1].cuda(), eps=eps)
+    assert torch.equal(alone[0], q[normal]) and torch.equal(alone[1][0], numbers[0][normal]) and torch.equal(alone[2][0], scale[0][normal])
