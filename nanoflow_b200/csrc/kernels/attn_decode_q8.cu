@@ -190,11 +190,12 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   __shared__ int starts[kListed + 1];                          // places of the requests' first pages in the row, for up to kListed requests
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int group = p.q_heads / p.kv_heads;
-  const int* indptr = p.kv_indptr + p.req_begin;
-  // The lists are complete before the kernel that joins states may start, which looks at them at once. (With a prefix, its kernel
-  // starts this one behind them.)
+  // (A prefix's kernel lets this one read without a wait, see let_next_read.)
+  const Early<int, SHARED> indptr{p.kv_indptr + p.req_begin}, indices{p.kv_indices}, rows{p.qo_indptr + p.req_begin},
+      last_lens{p.kv_last_page_len + p.req_begin};
   if (!SHARED) await_previous();
-  let_next_start();
+  if (MODE != PLAIN) let_next_start();
+  else if (warp == kWarps - 1) let_next_read();                // for the kernel that joins states
   const int base = indptr[0];
   const bool in_shared = p.req_count <= kListed;
   auto start_of = [&](int r) { return in_shared ? starts[r] : indptr[r] - base; };
@@ -236,7 +237,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
     if (i_left > 0) {
       if (ids_left == 0) {
         ids_left = min(32, pages_all - i_page);
-        ids = lane < ids_left ? p.kv_indices[base + i_page + lane] : 0;
+        ids = lane < ids_left ? indices[base + i_page + lane] : 0;
         if (ids < 0 || ids >= p.num_pages) {
           report_status(p.status, NF_ST_BAD_INDEX);
           ids = 0;
@@ -281,7 +282,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   };
 
   auto row_of = [&](int r) {                                   // the request's row of q and out
-    const int tok = p.qo_indptr[p.req_begin + r];
+    const int tok = rows[r];
     if (tok >= 0 && tok < p.num_tokens) return tok;
     if (lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
     return -1;
@@ -316,7 +317,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
     if (MODE != FEW) r = find(at);
     for (int i = 0; i < n;) {
       // ---- a request's run of pages in this range ----
-      const int last_len = p.kv_last_page_len[p.req_begin + r];
+      const int last_len = last_lens[r];
       const int tok = row_of(r);
       const int r_begin = start_of(r), r_end = start_of(r + 1);
       const int count = min(n - i, r_end - at);
@@ -327,8 +328,8 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
       for (int nt = 0; nt < NT; ++nt) {
         const int h = nt * 8 + g;
         const bool on = tok >= 0 && h < group;
-        const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) +
-                                                          (static_cast<long long>(on ? tok : 0) * p.q_heads + kvh * group + (on ? h : 0)) * HD) + t * 2;
+        const Early<uint4, SHARED> src{reinterpret_cast<const uint4*>(reinterpret_cast<const __nv_bfloat16*>(p.q) +
+                                                                      (static_cast<long long>(on ? tok : 0) * p.q_heads + kvh * group + (on ? h : 0)) * HD) + t * 2};
         uint4 raw[KS / 2];
         uint32_t most = 0;
 #pragma unroll
@@ -566,8 +567,9 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
   } else {
     if (lane == 0) records[range] = record;
     cp_async_wait<0>();
-    // One CTA stays until the prefix's kernel is complete, so that this one is not complete before it. (With all of them 64 requests
-    // behind 32768 tokens took 115 us instead of 110: SMs that have ended their share of the prefix would hold this kernel's first CTAs.)
+    // One CTA stays until the prefix's kernel is complete, so that this one is not complete before it. With all of them
+    // 64 requests behind 32768 tokens took 115 us instead of 110: SMs that have ended their share of the prefix would hold this kernel's
+    // first CTAs.
     if (SHARED && blockIdx.x == gridDim.x - 1) await_previous();
   }
 }
@@ -601,13 +603,13 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   __shared__ float shared_ml[4][2];
   __shared__ float shared_o[4][HD];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = warp % WARPS;
-  const int* indptr = p.kv_indptr + p.req_begin;
-  // lists and their cut while the kernels before this one still run: they do not write them
+  // lists and their cut while the kernels before this one still run (let_next_read)
+  const Early<int> indptr{p.kv_indptr + p.req_begin}, toks{p.qo_indptr + p.req_begin};
   const unsigned int q_heads = p.q_heads, e = blockIdx.x * (4 / WARPS) + warp / WARPS;             // the row, r * q_heads + head
   const bool on = e < p.req_count * q_heads;
   const unsigned int r = on ? e / q_heads : 0, head = on ? e - r * q_heads : 0, kvh = head / group, h = head - kvh * group;
   const int base = indptr[0], pages_all = indptr[p.req_count] - base, begin = indptr[r] - base, end = indptr[r + 1] - base;
-  int tok = p.qo_indptr[p.req_begin + r];
+  int tok = toks[r];
   const bool tok_ok = tok >= 0 && tok < p.num_tokens;
   if (!tok_ok) tok = -1;
   const Ranges ranges(pages_all * p.kv_heads, decode_ranges(pages_all * p.kv_heads, decode_ctas));

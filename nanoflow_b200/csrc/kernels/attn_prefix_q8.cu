@@ -245,7 +245,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
   const uint32_t tmem = *tmem_slot;
   // The requests' own tokens begin where SMs are done with the prefix. (Beside it, with three stages and 96 registers so that a CTA of
   // either fits an SM, both were slower: 256 requests behind 8192 tokens 104 us instead of 81.)
-  let_next_start();
+  if (warp == MMA_WARP) let_next_read();         // (the warp that has time for it)
   const int group = p.q_heads / p.kv_heads;
   auto fail = [&](unsigned int code) {
     if (lane == 0) report_status(p.status, code);
