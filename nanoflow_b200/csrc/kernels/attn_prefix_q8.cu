@@ -70,29 +70,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
       : "memory");
 }
 
-// A CTA's share of the units, one item after the other.
-struct Share {
-  int u, end, lead, tiles, blocks;
-  int item, kvh, block, t0, n;         // the current part: tiles t0 .. t0 + n - 1 of item (kvh, block)
-  __device__ __forceinline__ explicit Share(const PrefixPlan& f) : lead(f.lead), tiles(f.tiles), blocks(f.blocks) {
-    u = f.cut.begin(blockIdx.x);
-    end = f.cut.begin(blockIdx.x + 1);
-  }
-  __device__ __forceinline__ bool next() {
-    while (u < end) {
-      const int span = lead + tiles, from = (item = u / span) * span, to = min(end - from, span);
-      t0 = max(u - from - lead, 0);
-      n = to - lead - t0;
-      u = from + to;
-      if (n <= 0) continue;                                      // no more than the item's beginning
-      kvh = item / blocks;
-      block = item - kvh * blocks;
-      return true;
-    }
-    return false;
-  }
-};
-
 // Keys (PART 0) or values (PART 1) of the CTA's tiles: tokens 32 half .. 32 half + 31 of each, by one warp.
 template <int HD, int SLOTS, int KIND, int PART>
 __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const PrefixPlan& f, int half, uint32_t sb, float* scales, float* v_refs,
@@ -139,7 +116,7 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
       sc[k] = page < 0 ? 0.f : p.kv_scale[((static_cast<long long>(page) * 2 + PART) * p.kv_heads + kvh) * kQ8Page + lane % kQ8Page];
     }
   };
-  Share now(f), ahead = now;
+  Share now(f, blockIdx.x), ahead = now;
   int left = 0, tile_ahead = 0;                                  // the tile that is loaded next
   auto advance = [&]() {                                         // false: none
     if (left == 0) {
@@ -223,8 +200,15 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   await_previous();                              // (before tensor memory is taken, which the kernel before may need)
+  // a piece that will not be computed: its rows come out as NaN, and not as what an earlier call left in the workspace
+  auto spoil = [&](int item) {
+    if (threadIdx.x < 128 * SLOTS)
+      __stcg(reinterpret_cast<float2*>(f.ml) + static_cast<long long>(item + blockIdx.x) * (128 * SLOTS) + threadIdx.x, make_float2(0.f, __uint_as_float(0x7fc00000u)));
+  };
   if ((sb & 1023u) != 0u) {                      // the operands' layouts need it; report instead of computing garbage
     if (threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
+    Share all(f, blockIdx.x);
+    if (all.next()) all.rest(spoil);
     return;
   }
   if (threadIdx.x == 0) {
@@ -288,7 +272,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       return true;
     };
     bool ok = true;
-    Share now(f);
+    Share now(f, blockIdx.x);
     while (ok && now.next()) {
       if (!passed(C::Q_FULL, parts & 1) || !issue_s(g, g)) { fail(NF_ST_TIMEOUT_SMEM_FULL); break; }
       for (int t = 0; ok && t < now.n; ++t) {
@@ -325,7 +309,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     const int in_block = row / group, hh = row - in_block * group;
     uint32_t g = 0;
     bool ok = true;
-    Share now(f);
+    Share now(f, blockIdx.x);
     while (ok && now.next()) {
       // ---- this thread's row of Q. The products of the item before have all been formed: its last scores have been read. ----
       const int r = now.block * f.reqs_per_block + in_block;
@@ -454,7 +438,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       }
       if (!ok) break;
       g += now.n;
-      if (!passed(C::PV_DONE + slot * 2 + ((g - 1) & 1), ((g - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
+      if (!passed(C::PV_DONE + slot * 2 + ((g - 1) & 1), ((g - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); ok = false; break; }
       tc_fence_after();
       const long long at = static_cast<long long>(now.item + blockIdx.x) * (128 * SLOTS) + row;
       const float back = v_ref / kHeadroom;
@@ -488,6 +472,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[C::O_FREE]);
     }
+    if (!ok) now.rest(spoil);                    // (the current one, whose state is written last, among them)
   }
 
   tc_fence_before();

@@ -36,6 +36,35 @@ struct PrefixPlan {
   float* o;                  // [pieces][rows][head_dim], not divided by the sum
 };
 
+// A CTA's share of the units, one item after the other.
+struct Share {
+  int u, end, lead, tiles, blocks;
+  int item, kvh, block, t0, n;         // the current part: tiles t0 .. t0 + n - 1 of item (kvh, block)
+  __host__ __device__ __forceinline__ Share(const PrefixPlan& f, int cta) : lead(f.lead), tiles(f.tiles), blocks(f.blocks) {
+    u = f.cut.begin(cta);
+    end = f.cut.begin(cta + 1);
+  }
+  __host__ __device__ __forceinline__ bool next() {
+    while (u < end) {
+      const int span = lead + tiles, from = (item = u / span) * span, to = end - from < span ? end - from : span;
+      t0 = u - from > lead ? u - from - lead : 0;
+      n = to - lead - t0;
+      u = from + to;
+      if (n <= 0) continue;                                      // no more than the item's beginning
+      kvh = item / blocks;
+      block = item - kvh * blocks;
+      return true;
+    }
+    return false;
+  }
+  // f(item) for the current part and those that would follow
+  template <class F>
+  __host__ __device__ __forceinline__ void rest(F f) {
+    do f(item);
+    while (next());
+  }
+};
+
 // The row of pages of the decode kernel is cut into a range for each of its warps, of two pages at least.
 constexpr int kDecodeCtasPerSm = 4, kDecodeWarps = 4;      // at most, of so many warps
 __host__ __device__ __forceinline__ int decode_ranges(int units, int ctas) {
