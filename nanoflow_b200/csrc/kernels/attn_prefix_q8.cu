@@ -40,7 +40,7 @@ struct Pre {
   static constexpr int kBytes = kBars + 256;
   // barriers
   static constexpr int Q_FULL = 0, O_FREE = 1, K_FULL = 2, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages, V_EMPTY = V_FULL + kStages,
-                       S_FULL = V_EMPTY + kStages, P_FULL = S_FULL + 2 * SLOTS, PV_DONE = P_FULL + 2 * SLOTS, kNumBars = PV_DONE + 2 * SLOTS;
+                       S_FULL = V_EMPTY + kStages, P_FULL = S_FULL + 2 * SLOTS, PV_DONE = P_FULL + 2 * SLOTS, LAST = PV_DONE + 2 * SLOTS, kNumBars = LAST + 1;
   static_assert(kBars % 8 == 0 && kNumBars * 8 + 8 <= 256, "room for the barriers");
 };
 
@@ -274,7 +274,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     bool ok = true;
     Share now(f, blockIdx.x);
     while (ok && now.next()) {
-      if (!passed(C::Q_FULL, parts & 1) || !issue_s(g, g)) { fail(NF_ST_TIMEOUT_SMEM_FULL); break; }
+      if (!passed(C::Q_FULL, parts & 1) || !issue_s(g, g)) { fail(NF_ST_TIMEOUT_SMEM_FULL); ok = false; break; }
       for (int t = 0; ok && t < now.n; ++t) {
         const uint32_t gt = g + t;
         if (t + 1 < now.n && !issue_s(gt + 1, gt)) { fail(NF_ST_TIMEOUT_SMEM_FULL); ok = false; break; }
@@ -299,6 +299,11 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       }
       g += now.n;
       ++parts;
+    }
+    if (!ok) {                                   // products in flight get a bounded chance to end before their memory is given back
+      if (elect_one()) umma_commit(&bars[C::LAST]);
+      __syncwarp();
+      (void)mbar_wait(&bars[C::LAST], 0);
     }
   } else {
     // ------------------------------------------------------------------ softmax (a thread per query row)

@@ -30,3 +30,12 @@ def test_the_kernel_spoils_what_it_does_not_compute():
     softmax = text[text.index("softmax (a thread per query row)"):]
     assert "if (!ok) now.rest(spoil);" in softmax and softmax.count("ok = false; break;") == softmax.count("fail(NF_ST_")
     assert "all.rest(spoil);" in text[:text.index("mbar_init")]
+
+
+def test_products_in_flight_end_before_their_memory_is_given_back():
+    text = (build.KERNEL_DIR / "attn_prefix_q8.cu").read_text()
+    products = text[text.index("products (the warp walks"):text.index("softmax (a thread per query row)")]
+    assert products.count("ok = false; break;") == products.count("fail(NF_ST_")
+    end = products[products.rindex("if (!ok) {"):]
+    assert end.index("umma_commit(&bars[C::LAST])") < end.index("mbar_wait(&bars[C::LAST], 0)")
+    assert text.index("mbar_wait(&bars[C::LAST], 0)") < text.index("tmem_dealloc(")
