@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -75,11 +76,12 @@ int count(const char* what, const Tensor& t, const char* name) {
   if (t.numel() > INT32_MAX) refuse(what, std::string(name) + " has too many entries");
   return static_cast<int>(t.numel());
 }
-unsigned int* status_word(const char* what, PyObject* o, c10::Device device) {
+const Tensor* status_word(const char* what, PyObject* o, c10::Device device) {
   const Tensor* t = optional(what, "status", o, at::kInt, device);
   if (t != nullptr && t->numel() < 1) refuse(what, "status must have a word");
-  return t == nullptr ? nullptr : static_cast<unsigned int*>(t->data_ptr());
+  return t;
 }
+unsigned int* word(const Tensor* t) { return t == nullptr ? nullptr : static_cast<unsigned int*>(t->data_ptr()); }
 
 struct Cache {
   const Tensor& pool;
@@ -103,15 +105,26 @@ Cache cache(const char* what, PyObject* pool_arg, PyObject* scale_arg) {
                e4m3 ? NFK_Q8_E4M3 : NFK_Q8_INT8, pool.device()};
 }
 
-// What a kernel writes must not lie over what other threads of it still read.
-void apart(const char* what, const Tensor& in, const Tensor& out) {
-  if (in.numel() == 0 || out.numel() == 0) return;
-  const auto end = [](const Tensor& t) {
+// What a kernel writes must not lie over anything else that it reads or writes. (Null: a tensor that the call goes without.)
+void apart(const char* what, std::initializer_list<const Tensor*> written, std::initializer_list<const Tensor*> read) {
+  struct Span {
+    const char *begin, *end;
+  } spans[16];
+  int n = 0, n_written = 0;
+  const auto add = [&](const Tensor* t) {
+    if (t == nullptr || t->numel() == 0) return;
     int64_t last = 0;
-    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
-    return static_cast<const char*>(t.data_ptr()) + (last + 1) * t.element_size();
+    for (int64_t d = 0; d < t->dim(); ++d) last += (t->size(d) - 1) * t->stride(d);
+    const char* begin = static_cast<const char*>(t->data_ptr());
+    spans[n++] = Span{begin, begin + (last + 1) * t->element_size()};
   };
-  if (static_cast<const char*>(in.data_ptr()) < end(out) && static_cast<const char*>(out.data_ptr()) < end(in)) refuse(what, "input and output overlap");
+  if (written.size() + read.size() > 16) refuse(what, "too many tensors");
+  for (const Tensor* t : written) add(t);
+  n_written = n;
+  for (const Tensor* t : read) add(t);
+  for (int i = 0; i < n_written; ++i)
+    for (int j = i + 1; j < n; ++j)
+      if (spans[i].begin < spans[j].end && spans[j].begin < spans[i].end) refuse(what, "tensors overlap, and one of them is written");
 }
 
 template <class P>
@@ -181,7 +194,8 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if ((q_norm != nullptr && q_norm->numel() != hd) || (k_norm != nullptr && k_norm->numel() != hd)) refuse(what, "norms must be [head_dim]");
     const Tensor* cos_sin = optional(what, "cos_sin", a[18], at::kFloat, c.device);
     if (cos_sin != nullptr && cos_sin->numel() < T * hd) refuse(what, "cos_sin must be [T, head_dim/2, 2]");
-    apart(what, qkv, q_out);
+    const Tensor* status = status_word(what, a[19], c.device);
+    apart(what, {&q_out, &c.pool, &c.scale, status}, {&qkv, &inv_freq, &positions, &token_req, &kv_indptr, &kv_indices, q_norm, k_norm, cos_sin});
     p.qkv = qkv.data_ptr();
     p.ld_qkv = T > 1 ? qkv.stride(0) : (columns + 7) / 8 * 8;
     p.q_out = q_out.data_ptr();
@@ -200,7 +214,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.num_reqs = count(what, kv_indptr, "kv_indptr") - 1;
     p.num_indices = count(what, kv_indices, "kv_indices");
     p.kind = c.kind;
-    p.status = status_word(what, a[19], c.device);
+    p.status = word(status);
     p.early_start = whole(a[20], what, "early_start");
     if (T > 0) launch("nfk_rope_append_q8", entries.append, p, c.device);
   });
@@ -215,8 +229,8 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const Tensor& out = checked(what, "out", a[3], at::kBFloat16, c.device);
     if (out.dim() != 5 || out.size(0) != page_ids.numel() || out.sizes().slice(1) != c.pool.sizes().slice(1))
       refuse(what, "out must be [pages, 2, kv_heads, 16, head_dim]");
-    apart(what, c.pool, out);
-    apart(what, c.scale, out);
+    const Tensor* status = status_word(what, a[4], c.device);
+    apart(what, {&out, status}, {&c.pool, &c.scale, &page_ids});
     nfk_kv_read_q8_params p = {};
     p.kv_pool = c.pool.data_ptr();
     p.kv_scale = static_cast<const float*>(c.scale.data_ptr());
@@ -227,7 +241,7 @@ PyObject* read(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.head_dim = c.head_dim;
     p.num_pages = c.pages;
     p.kind = c.kind;
-    p.status = status_word(what, a[4], c.device);
+    p.status = word(status);
     p.early_start = whole(a[5], what, "early_start");
     if (p.n_pages > 0) launch("nfk_kv_read_q8", entries.read, p, c.device);
   });
@@ -268,14 +282,16 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const int64_t end = static_cast<int64_t>(p.req_begin) + p.req_count;
     if (p.req_begin < 0 || p.req_count < 0 || qo_indptr.numel() < end || kv_indptr.numel() < end + 1 || last.numel() < end)
       refuse(what, "requests " + std::to_string(p.req_begin) + " to " + std::to_string(end) + " are not all listed");
+    const Tensor* pages = nullptr;
     if (p.prefix_len > 0) {
-      const Tensor& pages = checked(what, "prefix_pages", a[9], at::kInt, c.device);
-      if (pages.numel() < (static_cast<int64_t>(p.prefix_len) + kPage - 1) / kPage) refuse(what, "prefix_pages lists fewer pages than prefix_len needs");
-      p.prefix_pages = static_cast<const int*>(pages.data_ptr());
+      pages = &checked(what, "prefix_pages", a[9], at::kInt, c.device);
+      if (pages->numel() < (static_cast<int64_t>(p.prefix_len) + kPage - 1) / kPage) refuse(what, "prefix_pages lists fewer pages than prefix_len needs");
+      p.prefix_pages = static_cast<const int*>(pages->data_ptr());
     }
     if (a[16] == Py_None) refuse(what, "needs a workspace (decode_workspace_q8)");
     const Tensor& workspace = checked(what, "workspace", a[16], at::kByte, c.device);
-    apart(what, q, out);
+    const Tensor* status = status_word(what, a[17], c.device);
+    apart(what, {&out, &workspace, status}, {&q, &c.pool, &c.scale, &qo_indptr, &kv_indptr, &kv_indices, &last, pages});
     p.q = q.data_ptr();
     p.out = out.data_ptr();
     p.kv_pool = c.pool.data_ptr();
@@ -288,7 +304,7 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.num_indices = count(what, kv_indices, "kv_indices");
     p.workspace = workspace.data_ptr();
     p.workspace_bytes = workspace.numel();
-    p.status = status_word(what, a[17], c.device);
+    p.status = word(status);
     p.early_start = whole(a[18], what, "early_start");
     if (p.req_count > 0) launch(what, entries.decode, p, c.device);
   });
