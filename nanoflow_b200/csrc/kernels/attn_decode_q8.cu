@@ -579,20 +579,21 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
 template <int HD, int H>
 __global__ void __launch_bounds__(128)
 attn_join_parts_q8_kernel(nfk_attn_q8_params p, const DecodeRecord* records, States parts, unsigned int group, unsigned int n_ranges) {
-  const unsigned int e = blockIdx.x * 4 + (threadIdx.x >> 5), range = e / (group / H), h = (e - range * (group / H)) * H;
   await_previous();
-  if (range >= n_ranges) return;
-  const int4 raw = __ldcg(reinterpret_cast<const int4*>(records) + range);
-  const DecodeRecord rec = {raw.x, raw.y, raw.z, raw.w};
-  if (rec.n == 0) return;
-  Row<HD> rows[H];
-  sum_states<HD, H == 2 ? 2 : 6>(p.workspace, rec.n, [&](int i, int k) {
-    return state_at<HD>(p.workspace, parts.ml, parts.o, ((range + i) * 2 + (i == 0 ? 1 : 0)) * group + h + k);
-  }, rows);
-  if (rec.tok >= 0)
+  for (unsigned int e = blockIdx.x * 4 + (threadIdx.x >> 5); e < n_ranges * (group / H); e += gridDim.x * 4) {
+    const unsigned int range = e / (group / H), h = (e - range * (group / H)) * H;
+    const int4 raw = __ldcg(reinterpret_cast<const int4*>(records) + range);
+    const DecodeRecord rec = {raw.x, raw.y, raw.z, raw.w};
+    if (rec.n == 0) continue;
+    Row<HD> rows[H];
+    sum_states<HD, H == 2 ? 2 : 6>(p.workspace, rec.n, [&](int i, int k) {
+      return state_at<HD>(p.workspace, parts.ml, parts.o, ((range + i) * 2 + (i == 0 ? 1 : 0)) * group + h + k);
+    }, rows);
+    if (rec.tok < 0) continue;
 #pragma unroll
     for (int k = 0; k < H; ++k)
       rows[k].finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(rec.tok) * p.q_heads + rec.kvh * group + h + k) * HD);
+  }
 }
 
 // The same row by row, with the shared prefix's states where there is one, and WARPS warps to a row: a context of 900 tokens is 29
@@ -605,60 +606,65 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, which = warp % WARPS;
   // lists and their cut while the kernels before this one still run (let_next_read)
   const Early<int> indptr{p.kv_indptr + p.req_begin}, toks{p.qo_indptr + p.req_begin};
-  const unsigned int q_heads = p.q_heads, e = blockIdx.x * (4 / WARPS) + warp / WARPS;             // the row, r * q_heads + head
-  const bool on = e < p.req_count * q_heads;
-  const unsigned int r = on ? e / q_heads : 0, head = on ? e - r * q_heads : 0, kvh = head / group, h = head - kvh * group;
-  const int base = indptr[0], pages_all = indptr[p.req_count] - base, begin = indptr[r] - base, end = indptr[r + 1] - base;
-  int tok = toks[r];
-  const bool tok_ok = tok >= 0 && tok < p.num_tokens;
-  if (!tok_ok) tok = -1;
+  const unsigned int q_heads = p.q_heads, n_rows = p.req_count * q_heads;
+  const int base = indptr[0], pages_all = indptr[p.req_count] - base;
   const Ranges ranges(pages_all * p.kv_heads, decode_ranges(pages_all * p.kv_heads, decode_ctas));
-  int k0 = 0, n_own = 0, n_prefix = 0;
-  unsigned int front = 0;                                      // the prefix's first state of this row
-  if (on && end > begin) {
-    k0 = ranges.of(kvh * pages_all + begin);
-    n_own = ranges.of(kvh * pages_all + end - 1) - k0 + 1;
-  }
-  if (on && p.prefix_len > 0) {
-    const unsigned int in = r / static_cast<unsigned int>(f.reqs_per_block), item = kvh * f.blocks + in;
-    const int span = f.lead + f.tiles, c0 = f.cut.of(item * span + f.lead);
-    n_prefix = f.cut.of((item + 1) * span - 1) - c0 + 1;
-    front = (item + c0) * f.rows + (r - in * f.reqs_per_block) * group + h;
-  }
-  await_previous();
-  if (on && !tok_ok && lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
-  if (*bad_lists != 0) n_own = 0;
-  int n_all = n_own + n_prefix;
-  if (p.prefix_len == 0 && n_own <= 1) tok = -1, n_all = 0;    // the row has been written
-  // all states of the row, WARPS shares of them one after the other
-  const int a = n_all * which / WARPS, b = n_all * (which + 1) / WARPS;
-  Row<HD> rows[1];
-  Row<HD>& row = rows[0];
-  sum_states<HD, WARPS == 1 ? 6 : 16>(p.workspace, b - a, [&](int i, int) {
-    const int k = a + i;
-    const bool is_front = k >= n_own, whole = n_own == 1;
-    const unsigned int at = is_front ? front + (k - n_own) * f.rows : whole ? e : ((k0 + k) * 2 + (k == 0 ? 1 : 0)) * group + h;
-    return state_at<HD>(p.workspace, is_front ? f.ml : whole ? wholes.ml : parts.ml, is_front ? f.o : whole ? wholes.o : parts.o, at);
-  }, rows);
-  if (WARPS > 1) {
-#pragma unroll
-    for (int i = 0; i < Row<HD>::N; ++i) shared_o[warp][lane * Row<HD>::N + i] = row.o[i];
-    if (lane == 0) {
-      shared_ml[warp][0] = row.m;
-      shared_ml[warp][1] = row.l;
+  for (unsigned int first = blockIdx.x * (4 / WARPS); first < n_rows; first += gridDim.x * (4 / WARPS)) {
+    const unsigned int e = first + warp / WARPS;                 // the row, r * q_heads + head
+    const bool on = e < n_rows;
+    const unsigned int r = on ? e / q_heads : 0, head = on ? e - r * q_heads : 0, kvh = head / group, h = head - kvh * group;
+    const int begin = indptr[r] - base, end = indptr[r + 1] - base;
+    int tok = toks[r];
+    const bool tok_ok = tok >= 0 && tok < p.num_tokens;
+    if (!tok_ok) tok = -1;
+    int k0 = 0, n_own = 0, n_prefix = 0;
+    unsigned int front = 0;                                      // the prefix's first state of this row
+    if (on && end > begin) {
+      k0 = ranges.of(kvh * pages_all + begin);
+      n_own = ranges.of(kvh * pages_all + end - 1) - k0 + 1;
     }
-    __syncthreads();
-    if (which == 0)
-      for (int k = 1; k < WARPS; ++k) {
-        Row<HD> other;
-        other.m = shared_ml[warp + k][0];
-        other.l = shared_ml[warp + k][1];
+    if (on && p.prefix_len > 0) {
+      const unsigned int in = r / static_cast<unsigned int>(f.reqs_per_block), item = kvh * f.blocks + in;
+      const int span = f.lead + f.tiles, c0 = f.cut.of(item * span + f.lead);
+      n_prefix = f.cut.of((item + 1) * span - 1) - c0 + 1;
+      front = (item + c0) * f.rows + (r - in * f.reqs_per_block) * group + h;
+    }
+    await_previous();
+    if (on && !tok_ok && lane == 0) report_status(p.status, NF_ST_BAD_INDEX);
+    if (*bad_lists != 0) n_own = 0;
+    int n_all = n_own + n_prefix;
+    if (p.prefix_len == 0 && n_own <= 1) tok = -1, n_all = 0;    // the row has been written
+    // all states of the row, WARPS shares of them one after the other
+    const int a = n_all * which / WARPS, b = n_all * (which + 1) / WARPS;
+    Row<HD> rows[1];
+    Row<HD>& row = rows[0];
+    sum_states<HD, WARPS == 1 ? 6 : 16>(p.workspace, b - a, [&](int i, int) {
+      const int k = a + i;
+      const bool is_front = k >= n_own, whole = n_own == 1;
+      const unsigned int at = is_front ? front + (k - n_own) * f.rows : whole ? e : ((k0 + k) * 2 + (k == 0 ? 1 : 0)) * group + h;
+      return state_at<HD>(p.workspace, is_front ? f.ml : whole ? wholes.ml : parts.ml, is_front ? f.o : whole ? wholes.o : parts.o, at);
+    }, rows);
+    if (WARPS > 1) {
 #pragma unroll
-        for (int i = 0; i < Row<HD>::N; ++i) other.o[i] = shared_o[warp + k][lane * Row<HD>::N + i];
-        row.add(other);
+      for (int i = 0; i < Row<HD>::N; ++i) shared_o[warp][lane * Row<HD>::N + i] = row.o[i];
+      if (lane == 0) {
+        shared_ml[warp][0] = row.m;
+        shared_ml[warp][1] = row.l;
       }
+      __syncthreads();
+      if (which == 0)
+        for (int k = 1; k < WARPS; ++k) {
+          Row<HD> other;
+          other.m = shared_ml[warp + k][0];
+          other.l = shared_ml[warp + k][1];
+#pragma unroll
+          for (int i = 0; i < Row<HD>::N; ++i) other.o[i] = shared_o[warp + k][lane * Row<HD>::N + i];
+          row.add(other);
+        }
+    }
+    if (which == 0 && tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(tok) * q_heads + head) * HD);
+    if (WARPS > 1) __syncthreads();                            // (before the next rows' states go there)
   }
-  if (which == 0 && tok >= 0) row.finish(reinterpret_cast<__nv_bfloat16*>(p.out) + (static_cast<long long>(tok) * q_heads + head) * HD);
 }
 
 // CTAs that share a request's pages for one KV head in a small batch, 0 where the general form is at least as fast: one launch instead
@@ -714,6 +720,7 @@ int launch(const nfk_attn_q8_params& p, const PrefixPlan& f, int* bad_lists, Dec
   // pieces lead to the rows, of which most lie in one range.
   const int rows = p.req_count * p.q_heads, group = p.q_heads / p.kv_heads;
   const auto join = [&](auto kernel, int grid, auto... args) {
+    if (p.num_ctas > 0 && p.num_ctas < grid) grid = p.num_ctas;
     return done(launch_kernel(early_further(p.early_start), kernel, grid, 128, 0, stream, 1, args...)) ? NF_OK : NF_ERR_CUDA;
   };
   if (rows <= 8 * sms) return join(attn_join_rows_q8_kernel<HD, 4>, rows, p, f, bad_lists, parts, wholes, group, ctas);
