@@ -747,9 +747,9 @@ bool sizes_built(const nfk_attn_q8_params& p) {
   return (p.head_dim == 64 || p.head_dim == 128) && p.kv_heads > 0 && p.q_heads > 0 && p.q_heads % p.kv_heads == 0 &&
          p.q_heads / p.kv_heads <= 16;
 }
-// All units, and all places in their rows, are counted in 32 bits.
+// All units, and all places in their rows, are counted in 32 bits, with room for a step of all warps behind the last one.
 bool counts_fit(const nfk_attn_q8_params& p, const PrefixPlan& f) {
-  const long long most = 0x7ffffff0ll;
+  const long long most = 0x7fff0000ll;
   return static_cast<long long>(p.num_indices) * p.kv_heads <= most && static_cast<long long>(p.req_count) * p.q_heads <= most &&
          static_cast<long long>(p.kv_heads) * f.blocks <= most / (f.tiles > 0 ? f.lead + f.tiles : 1) &&
          static_cast<long long>(p.req_begin) + p.req_count <= most;
