@@ -74,7 +74,7 @@ struct Dec {
   }
 };
 
-// A softmax state for one head, spread over the lanes of a warp: HD / 32 elements each.
+// A softmax state for one head, spread over the lanes of a warp: HD / 32 elements each (see kStateUnit).
 template <int HD>
 struct Row {
   static constexpr int N = HD / 32;
@@ -89,7 +89,7 @@ struct Row {
   }
   __device__ __forceinline__ void finish(__nv_bfloat16* out) const {
     const int lane = threadIdx.x & 31;
-    const float inv = l == 0.f ? 0.f : 1.f / l;                // (a sum that is NaN stays visible)
+    const float inv = l == 0.f ? 0.f : 1.f / (kStateUnit * l);                // (a sum that is NaN stays visible)
     if constexpr (HD == 128)
       reinterpret_cast<uint2*>(out)[lane] = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
     else
@@ -479,7 +479,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
       }
 
       // ---- the run's end: the final row where it is the whole request and no prefix joins it, else its state ----
-      const float v_back = v_ref / kHeadroom;
+      const float v_back = v_ref / kHeadroom, s_back = v_back * kStateUnit;
       const bool final = begins && ends && MODE == PLAIN;
       // states of this run's heads: of a whole request by its number; of a piece by the range's, those of a request that began before
       // it first; in a cluster over the warp's own pipeline, which is done
@@ -512,7 +512,7 @@ attn_decode_q8_kernel(nfk_attn_q8_params p, int* bad_lists, DecodeRecord* record
             float4* dst = reinterpret_cast<float4*>(states.o + (first + h) * HD + g * VB);
 #pragma unroll
             for (int j = 0; j < MT; j += 2)
-              dst[j / 2] = make_float4(o[nt][j][e] * v_back, o[nt][j][2 + e] * v_back, o[nt][j + 1][e] * v_back, o[nt][j + 1][2 + e] * v_back);
+              dst[j / 2] = make_float4(o[nt][j][e] * s_back, o[nt][j][2 + e] * s_back, o[nt][j + 1][e] * s_back, o[nt][j + 1][2 + e] * s_back);
           }
         }
 

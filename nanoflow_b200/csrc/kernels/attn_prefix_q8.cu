@@ -446,7 +446,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
       if (!passed(C::PV_DONE + slot * 2 + ((g - 1) & 1), ((g - 1) >> 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); ok = false; break; }
       tc_fence_after();
       const long long at = static_cast<long long>(now.item + blockIdx.x) * (128 * SLOTS) + row;
-      const float back = v_ref / kHeadroom;
+      const float back = v_ref / kHeadroom * kStateUnit;
       // by way of the warp's own rows of Q, which no product reads any more, so that stores are of whole rows (a thread's own row by
       // itself took 5300 cycles, as long as two tiles; now 4000)
       float* const rows_o = f.o + (at - lane) * HD;

@@ -10,6 +10,9 @@ namespace nf {
 
 constexpr int kQ8Page = 16;
 constexpr float kQ8Log2e = 1.4426950408889634f;
+// States hold their sums of values times this, 2^-32: up to 2^32 weights of 1 on the largest values of bf16 stay finite, and values from
+// 2^-80 on (smaller ones are not cached) keep their bits.
+constexpr float kStateUnit = 2.3283064365386963e-10f;
 
 // A row of n units in w ranges (w <= n): the first n % w ranges have one more than the others.
 struct Ranges {
@@ -33,7 +36,7 @@ struct PrefixPlan {
   int most_ctas;             // that this prefix or a part of it is cut over
   Ranges cut;                // of the units
   float* ml;                 // states, [pieces][rows]: reference (of exponents to base 2) and sum,
-  float* o;                  // [pieces][rows][head_dim], not divided by the sum
+  float* o;                  // [pieces][rows][head_dim], times kStateUnit, not divided by the sum
 };
 
 // A CTA's share of the units, one item after the other.

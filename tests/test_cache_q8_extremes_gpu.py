@@ -100,3 +100,27 @@ def test_norms_of_heads_whose_squares_leave_fp32(kind, eps):
     normal = [2, 7]
     alone = _append(x[normal].cuda(), kind, [positions[t] for t in normal], q_norm=w[0].cuda(), k_norm=w[1].cuda(), eps=eps)
     assert torch.equal(alone[0], q[normal]) and torch.equal(alone[1][0], numbers[0][normal]) and torch.equal(alone[2][0], scale[0][normal])
+
+
+@KINDS
+@pytest.mark.parametrize("size", [2.0 ** 126, 2.0 ** -70])
+@pytest.mark.parametrize("lengths,prefix", [([100, 7, 40], 0), ([4000, 7, 333, 50], 0), ([37 * i % 301 for i in range(1, 200)], 0), ([100, 0, 700], 900)])
+def test_attention_over_values_at_the_ends_of_the_range(kind, size, lengths, prefix):
+    """Values next to the largest of bf16, and next to those that are stored as zeros: sums over tokens leave fp32, results do not."""
+    import test_cache_q8_gpu as base
+
+    n, heads, kv_heads = len(lengths), 8, 2
+    pages = sum(-(-x // 16) for x in lengths) + -(-prefix // 16) + 1
+    pool, scale = base._cache(pages, kv_heads, DIM, kind, spread=0.0)
+    scale[:, 1] = scale[:, 1] * (size / (scale[:, 1].max() * ref.Q8_LARGEST[kind] / 3.9))       # the largest value: 3.9 sizes
+    pool.view(torch.int8)[:, 1] &= 0x7f          # all of one sign, so that sums grow
+    assert float(ref.kv_values_q8(pool, scale, torch.arange(pages)).abs().max()) < 2.0 ** 128
+    ptr, idx, last = base._lists(lengths, pages, 3)
+    front = torch.arange(-(-prefix // 16), dtype=torch.int32, device="cuda")
+    q = torch.randn(n, heads * DIM, device="cuda").to(torch.bfloat16)
+    args = (pool, scale, torch.arange(n + 1, dtype=torch.int32, device="cuda"), ptr, idx, last)
+    ws = ops.decode_workspace_q8(requests=n, q_heads=heads, kv_heads=kv_heads, head_dim=DIM, prefix_len=prefix)
+    out = torch.full_like(q, 3.0)
+    ops.attn_decode_shared_q8(q, out, *args, front, prefix, q_heads=heads, req_begin=0, req_count=n, workspace=ws)
+    base._check_rows(out, ref.attn_decode_q8(q, *args, q_heads=heads, req_begin=0, req_count=n, prefix_pages=front if prefix else None,
+                                             prefix_len=prefix), DIM)
