@@ -75,20 +75,6 @@ __device__ __forceinline__ float fast_exp2(float x) {
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-// Shared-memory descriptor of an MN-major operand in the 128-byte swizzle: 64 elements along M/N are
-// contiguous (one 128-byte row per k index), `lbo` bytes lead to the next 64 elements along M/N, `sbo`
-// bytes to the next group of eight k indices.
-__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
-  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
-  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-constexpr uint32_t kIdescBMnMajor = 1u << 16;
-
 struct Item {
   int req, tok0, ntok, kvh, pg0, np, kv_len, q_end, n_tiles;
   int t_first;      // first key tile (EXT: the one the first row's window or chunk starts in)

@@ -3,14 +3,14 @@
 //   o_h = sum_j e^(s_hj) v_j / sum_j e^(s_hj),   s_hj = sm_scale (q_h . k_j),   k_j = number_j * kscale_j, v_j likewise
 //
 // Bound by the cache's bytes: 683 requests of 1024 to 1536 tokens, 32 / 8 heads, 316 us, 5.8 TB/s, 0.89 of a copy's rate; 256
-// requests of 200 to 2000, 64 / 8 heads, 93 us, 0.74 (83 without the join). A warp reads pages straight into the layout that the tensor cores take: with S^T = K Q^T the keys
-// are the 16-row operand (a page's 16 tokens) and the up to 8 query heads of a KV head the 8 columns (16 heads: two such
-// products), and which elements of head_dim form a step of the product is free, so a lane's bytes of a key are 16 neighbours, its
-// f16 pairs the operand's registers, and no lane needs what another one loaded. O^T = V^T P^T works the same way: V^T is the
-// 16-row operand, two of its rows are two neighbouring elements, and a lane reads 16 neighbours of the four tokens whose weights
-// it multiplies. P^T gets into its layout by one transposing move per 8 tokens.
+// requests of 200 to 2000, 64 / 8 heads, 93 us, 0.74 (83 without the join). A warp reads pages straight into the layout that the
+// tensor cores take: with S^T = K Q^T the keys are the 16-row operand (a page's 16 tokens) and the up to 8 query heads of a KV head
+// the 8 columns (16 heads: two such products), and which elements of head_dim form a step of the product is free, so a lane's bytes
+// of a key are 16 neighbours, its f16 pairs the operand's registers, and no lane needs what another one loaded. O^T = V^T P^T works
+// the same way: V^T is the 16-row operand, two of its rows are two neighbouring elements, and a lane reads 16 neighbours of the
+// four tokens whose weights it multiplies. P^T gets into its layout by one transposing move per 8 tokens.
 // Numbers are exact in f16. Queries are, too, up to a power of two per head (their small elements may be rounded at 2^-25 of the
-// largest). The keys' scales join the scores in fp32; the values' scales join the weights, which are rounded to f16 (2^-12)
+// largest). The keys' scales join the scores in fp32; the values' scales join the weights, which are rounded to f16 (2^-11)
 // relative to the largest value scale so far, `v_ref`, with 2^7 of headroom: values up to 2^20 smaller keep full precision.
 //
 // A warp keeps a reference per head instead of a running maximum: it moves only where a score exceeds it by 8 (in exponents to

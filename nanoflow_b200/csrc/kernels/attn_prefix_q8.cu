@@ -1,12 +1,12 @@
 // Attention of a batch's query tokens over a prefix that all of them see, in the 8-bit paged cache, on the 5th-generation tensor
 // cores: partial softmax states for attn_decode_q8.cu to join with each request's own tokens.
 //
-// The query rows of a KV head (requests x group, 128 to a block) are one operand for every key, so the prefix is read once per
+// The query rows of a KV head (requests x group, 128 or 256 to a block) are one operand for every key, so the prefix is read once per
 // block instead of once per request, and the work is bound by the products (4 rows tokens head_dim operations) as soon as there
 // are some ten requests: 256 requests behind 8192 tokens, 32 / 8 heads, 52 us, 660 TFLOP/s, 0.40 of the measured rate; 64 of 64 / 8
 // heads behind 32768 91 us, 0.45. A tile of two slots takes 2200 cycles: 1024 of 2^x, 1280 of products (scores read Q from shared
-// memory for 64 columns at a time), 900 of instruction issue, which overlap in part. Items (KV head, block) times tiles of 64 tokens are a row of units that is cut evenly over the CTAs (two
-// to an SM); each leaves a piece per item.
+// memory for 64 columns at a time), 900 of instruction issue, which overlap in part. Items (KV head, block) times tiles of 64 tokens
+// are a row of units that is cut evenly over the CTAs (two to an SM, or one); each leaves a piece per item.
 //
 // A block has one or two slots of 128 rows: with two, which share the tiles, a CTA has the SM, with one there are two CTAs.
 //
@@ -44,13 +44,6 @@ struct Pre {
   static_assert(kBars % 8 == 0 && kNumBars * 8 + 8 <= 256, "room for the barriers");
 };
 
-// MN-major operand in the 128-byte swizzle: 64 elements along N are one 128-byte row per k index, `lbo` bytes lead to the next 64,
-// `sbo` bytes to the next eight k indices.
-__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
-  return static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4) | static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16 |
-         static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32 | static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
-}
-constexpr uint32_t kIdescBMnMajor = 1u << 16;
 // f16 x f16 -> fp32
 constexpr uint32_t idesc_f16(int m, int n) { return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24); }
 
@@ -87,7 +80,7 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
   uint4 raw[NI];
   float sc[2];
   // lane j < 4: the vectors of page j of the tile, -1 where there is none
-  auto page_of = [&](int kvh, int tile) {
+  auto page_of = [&](int tile) {
     int at = -1;
     const int slot = tile * (kTile / kQ8Page) + lane;
     if (lane < kTile / kQ8Page && slot < n_pages) {
@@ -130,9 +123,9 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
     return true;
   };
   // numbers are requested a tile ahead, page numbers two
-  if (advance()) load(page_of(ahead.kvh, tile_ahead), ahead.kvh);
+  if (advance()) load(page_of(tile_ahead), ahead.kvh);
   bool more = advance();
-  int at = more ? page_of(ahead.kvh, tile_ahead) : -1, kvh = ahead.kvh;
+  int at = more ? page_of(tile_ahead) : -1, kvh = ahead.kvh;
   uint32_t g = 0;
   while (now.next()) {
     float v_ref = 7.8886091e-31f;                                // 2^-100
@@ -140,7 +133,7 @@ __device__ __forceinline__ void bring_tiles(const nfk_attn_q8_params& p, const P
       const int s = g % C::kStages, ring = g % C::kRing;
       const int valid = p.prefix_len - (now.t0 + t) * kTile;     // tokens of the tile
       const bool more_then = more && advance();
-      const int kvh_then = ahead.kvh, at_then = more_then ? page_of(kvh_then, tile_ahead) : -1;
+      const int kvh_then = ahead.kvh, at_then = more_then ? page_of(tile_ahead) : -1;
       if (!__all_sync(0xffffffffu, wait_or_abort(&empty[s], (g / C::kStages & 1) ^ 1, abort_flag))) {
         if (lane == 0) report_status(p.status, NF_ST_TIMEOUT_SMEM_EMPTY);
         *abort_flag = 1;
@@ -247,7 +240,7 @@ attn_prefix_q8_kernel(nfk_attn_q8_params p, PrefixPlan f) {
     // ------------------------------------------------------------------ products (the warp walks, an elected lane issues)
     const uint32_t idesc_s = idesc_f16(128, kTile), idesc_o = idesc_f16(128, HD) | kIdescBMnMajor;
     const uint64_t q_desc = umma_desc_k_sw128(sb + C::kQ), k_desc = umma_desc_k_sw128(sb + C::kK);
-    const uint64_t v_desc = desc_mn_sw128(sb + C::kV, kHalfBytes, 1024);
+    const uint64_t v_desc = umma_desc_mn_sw128(sb + C::kV, kHalfBytes, 1024);
     uint32_t g = 0, parts = 0;
     // S(gt) goes over P(gt - 2), which PV(gt - 2) reads: the latest PV issued must have completed
     auto issue_s = [&](uint32_t gt, uint32_t pv_issued) {

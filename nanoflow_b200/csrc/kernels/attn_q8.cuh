@@ -1,8 +1,8 @@
 // What the two kernels of attention over the 8-bit cache share: how work is cut, and where partial results lie.
 //
-// Both walk a row of equal units (pages, or tiles of the shared prefix) that is cut into equal ranges without regard to where a
-// request ends: worker w of W takes units [w U / W, (w + 1) U / W). What a range holds of a request (or of a block of query rows)
-// is a piece, and pieces are joined by their softmax states.
+// Both walk a row of equal units (pages, or tiles of the shared prefix) that is cut into ranges of equal length, give or take a unit
+// (Ranges), without regard to where a request ends. What a range holds of a request (or of a block of query rows) is a piece, and
+// pieces are joined by their softmax states.
 #pragma once
 #include "cache_q8.cuh"
 
@@ -28,8 +28,8 @@ struct Ranges {
 };
 
 // The shared prefix: the query rows of a KV head (requests x group) are cut into blocks of at most `rows` (128 or 256) rows, whole
-// requests each. An item is (KV head, block), its units `lead` units for its beginning and then the prefix's tiles of 64 tokens. The piece of item i by CTA c has number
-// i + c: along the row of units every new piece raises one of the two.
+// requests each. An item is (KV head, block), its units `lead` units for its beginning and then the prefix's tiles of 64 tokens. The
+// piece of item i by CTA c has number i + c: along the row of units every new piece raises one of the two.
 constexpr int kPrefixTile = 64;
 struct PrefixPlan {
   int rows, reqs_per_block, blocks, tiles, lead, ctas;

@@ -329,11 +329,24 @@ NF_DEVICE uint64_t umma_desc_k_sw128(uint32_t smem_addr) {
   d |= static_cast<uint64_t>(2) << 61;                            // SWIZZLE_128B
   return d;
 }
+// Shared-memory descriptor of an MN-major operand in the 128-byte swizzle: 64 elements along M/N are
+// contiguous (one 128-byte row per k index), `lbo` bytes lead to the next 64 elements along M/N, `sbo`
+// bytes to the next group of eight k indices.
+NF_DEVICE uint64_t umma_desc_mn_sw128(uint32_t smem_addr, uint32_t lbo, uint32_t sbo) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>((lbo >> 4) & 0x3FFF) << 16;
+  d |= static_cast<uint64_t>((sbo >> 4) & 0x3FFF) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
 // Instruction descriptor: bf16 x bf16 -> fp32, both operands K-major.
 __host__ __device__ constexpr uint32_t umma_idesc_bf16(int m, int n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
          (static_cast<uint32_t>(m >> 4) << 24);
 }
+constexpr uint32_t kIdescBMnMajor = 1u << 16;         // (or'ed to it: the second operand is MN-major)
 
 // ---- launches that overlap the end of the kernel before them ------------------------------------------
 // A kernel launched early (launch_kernel) may start while the kernel before it on the stream still runs, as soon as every

@@ -38,9 +38,10 @@ constexpr float kLeastSquare = 7.8886091e-31f, kMostSquare = 1.329228e36f;      
 
 // A CTA per token; HD / 16 threads per head, each with eight elements of either half, so that a thread holds both elements of its
 // eight pairs, and the same pairs for every head that it takes: its cosines and sines stay in registers. What bounds it is the issue
-// of instructions, and latency (2048 tokens, 32 / 8 heads, norms: 13 us for 46 MB; 683 tokens 8): arithmetic is two elements at a time, and a thread requests its elements of BATCH heads before the
-// CTA works out the token's angles and page. It does not let the next kernel start: CTAs that wait beside its last ones cost more
-// than their launch (2048 tokens and a kv_read_q8 behind them 17.7 us, without 15.9).
+// of instructions, and latency (2048 tokens, 32 / 8 heads, norms: 13 us for 46 MB; 683 tokens 8): arithmetic is two elements at a time,
+// and a thread requests its elements of BATCH heads before the CTA works out the token's angles and page. It does not let the next
+// kernel start: CTAs that wait beside its last ones cost more than their launch (2048 tokens and a kv_read_q8 behind them 17.7 us,
+// without 15.9).
 template <int HD, int KIND>
 __global__ void __launch_bounds__(kAppendThreads, 5) rope_append_q8_kernel(nfk_rope_append_q8_params p) {
   constexpr int HALF = HD / 2, LPH = HD / 16, AT_ONCE = kAppendThreads / LPH, BATCH = 3;
