@@ -616,7 +616,7 @@ attn_join_rows_q8_kernel(nfk_attn_q8_params p, PrefixPlan f, const int* bad_list
     const int begin = indptr[r] - base, end = indptr[r + 1] - base;
     int tok = toks[r];
     const bool tok_ok = tok >= 0 && tok < p.num_tokens;
-    if (!tok_ok) tok = -1;
+    if (!on || !tok_ok) tok = -1;                              // (a warp behind the last row has looked at row 0)
     int k0 = 0, n_own = 0, n_prefix = 0;
     unsigned int front = 0;                                      // the prefix's first state of this row
     if (on && end > begin) {
