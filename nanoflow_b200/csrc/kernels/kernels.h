@@ -265,7 +265,7 @@ int nfk_attn_prefill_ws(const nfk_attn_params* p, cudaStream_t stream);
 enum { NFK_Q8_E4M3 = 0, NFK_Q8_INT8 = 1 };
 // Counterpart of nfk_rope_append for that pool. q_norm / k_norm: RMS norm of every query / key head before the rotation.
 // A vector's scale is its largest magnitude / 448 (e4m3) or / 127 (whole numbers); vectors below 2^-80 are stored as zeros, a
-// vector that is not finite gets the scale NaN.
+// vector that is not finite, or that rotation takes beyond fp32, gets the scale NaN. Two tokens must not have the same place.
 typedef struct nfk_rope_append_q8_params {
   const void* qkv;           // [T][ld_qkv] bf16
   long long ld_qkv;
@@ -301,7 +301,8 @@ typedef struct nfk_kv_read_q8_params {
 int nfk_kv_read_q8(const nfk_kv_read_q8_params* p, cudaStream_t stream);
 
 // One query token per request (row qo_indptr[b] of q) over its cached tokens; with prefix_len > 0 all requests also see the
-// prefix_len tokens of prefix_pages, in front of their own. Requests that see nothing get zeros.
+// prefix_len tokens of prefix_pages, in front of their own. Requests that see nothing get zeros. A prefix's kernel that gives up (a
+// status of a wait that ran out) leaves NaN in the rows that it has part in. No other thread launches on the stream during a call.
 typedef struct nfk_attn_q8_params {
   const void* q;             // [num_tokens][q_heads * head_dim] bf16
   void* out;                 // [num_tokens][q_heads * head_dim] bf16
@@ -315,7 +316,7 @@ typedef struct nfk_attn_q8_params {
   int q_heads, kv_heads, head_dim, num_pages, num_tokens, num_indices;
   int req_begin, req_count, prefix_len, kind;
   float sm_scale;
-  int num_ctas;              // CTA budget; 0 = as many as fit
+  int num_ctas;              // CTA budget of each of the call's kernels; 0 = as many as fit
   int early_start;           // see nfk_gemm_params
   void* workspace;           // nfk_attn_q8_workspace bytes at 256, whatever they hold; calls that may run at the same time each
   long long workspace_bytes; // need their own

@@ -38,7 +38,7 @@ constexpr float kLeastSquare = 7.8886091e-31f, kMostSquare = 1.329228e36f;      
 
 // A CTA per token; HD / 16 threads per head, each with eight elements of either half, so that a thread holds both elements of its
 // eight pairs, and the same pairs for every head that it takes: its cosines and sines stay in registers. What bounds it is the issue
-// of instructions, and latency (2048 tokens, 32 / 8 heads, norms: 13 us for 46 MB; 683 tokens 8): arithmetic is two elements at a time,
+// of instructions, and latency (2048 tokens, 32 / 8 heads, norms: 13 us for 46 MB; 683 tokens of 64 / 8 heads 6.4): arithmetic is two elements at a time,
 // and a thread requests its elements of BATCH heads before the CTA works out the token's angles and page. It does not let the next
 // kernel start: CTAs that wait beside its last ones cost more than their launch (2048 tokens and a kv_read_q8 behind them 17.7 us,
 // without 15.9).

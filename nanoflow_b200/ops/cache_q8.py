@@ -4,6 +4,8 @@ The cache of a layer is a pool ``[num_pages, 2, kv_heads, 16, head_dim]`` of ``f
 for every vector, ``[num_pages, 2, kv_heads, 16]`` in fp32; a cached value is number * scale. Pages, page lists and the calls
 have the form of the bf16 cache (:func:`nanoflow_b200.ops.rope_append`, :func:`nanoflow_b200.ops.attn_decode`), at half the bytes.
 
+No tensor that a call writes (outputs, the workspace, the cache in the write, ``status``) may overlap another one of its tensors.
+
 ``early_start`` (EARLY_*) of the calls: their kernels may be launched while the one before them on the stream still runs, and wait
 for it there; 0 keeps the SMs free until then, for another stream's kernels beside it.
 """
@@ -82,8 +84,9 @@ def rope_append_q8(qkv: torch.Tensor, q_out: torch.Tensor, kv_pool: torch.Tensor
 
     ``q_norm`` / ``k_norm`` (bf16 ``[head_dim]``): RMS norm of every query / key head in front of the rotation, with ``eps``.
     ``cos_sin``: the iteration's table from ``rope_table``; without it angles are computed here, in 64 bits.
-    Two tokens of a call must not have the same request and position. A vector with an infinity or NaN is cached as NaN, one
-    whose largest magnitude is below 2^-80 as zeros. A token whose page does not exist is not cached and reported in ``status``."""
+    Two tokens of a call must not have the same place (request and position, or pages that two requests share). A vector with an
+    infinity or NaN, or a key that rotation takes beyond fp32, is cached as NaN, one whose largest magnitude is below 2^-80 as zeros. A
+    token whose page does not exist is not cached and reported in ``status``."""
     _calls().rope_append(qkv, q_out, kv_pool, kv_scale, inv_freq, positions, token_req, kv_indptr, kv_indices, q_heads, kv_heads, head_dim,
                          q_off, k_off, v_off, q_norm, k_norm, eps, cos_sin, status, early_start)
 
@@ -122,8 +125,13 @@ def attn_decode_q8(q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, 
                    status: Optional[torch.Tensor] = None, early_start: int = EARLY_FIRST | EARLY_FURTHER) -> torch.Tensor:
     """:func:`nanoflow_b200.ops.attn_decode` over the 8-bit cache: single-query attention for requests [req_begin, req_begin +
     req_count), each with a row of ``q`` of its own. Contexts are cut over the CTAs by their pages, whatever their lengths. Requests
-    without pages get zeros; rows of other requests are left as they were. Page numbers, rows and page lists that are none are
-    reported in ``status``. ``workspace``: :func:`decode_workspace_q8`. ``num_ctas``: CTA budget, 0 = all that fit."""
+    without pages get zeros; rows of other requests are left as they were. ``workspace``: :func:`decode_workspace_q8`. ``num_ctas``: CTA
+    budget of each kernel, 0 = all that fit.
+
+    Reported in ``status``: page numbers that are none (page 0 is read instead), rows that are none (left out), page lists that fall or
+    leave ``kv_indices`` (as if there were no pages). Small batches, by ``kv_indices.numel()``, take one launch instead of two; with a list
+    that is longer than its pages sums may differ in their last bits. Values whose scale is more than 2^20 below the request's largest
+    lose bits of their weights; scores that fp32 does not hold give NaN."""
     _calls().decode("attn_decode_q8", q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, None, 0, q_heads,
                     req_begin, req_count, sm_scale, num_ctas, workspace, status, early_start)
     return out
@@ -134,7 +142,8 @@ def attn_decode_shared_q8(q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_in
                           sm_scale: Optional[float] = None, num_ctas: int = 0,
                           status: Optional[torch.Tensor] = None, early_start: int = EARLY_FIRST | EARLY_FURTHER) -> torch.Tensor:
     """:func:`attn_decode_q8` for requests that all see the same first ``prefix_len`` tokens, those of ``prefix_pages``; their own
-    page lists hold what comes after (or nothing). The prefix is read once for all of them."""
+    page lists hold what comes after (or nothing). The prefix is read once for all of them. If a wait in its kernel runs out
+    (``status``), the rows that it has part in are NaN."""
     _calls().decode("attn_decode_shared_q8", q, out, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, prefix_pages,
                     prefix_len, q_heads, req_begin, req_count, sm_scale, num_ctas, workspace, status, early_start)
     return out
