@@ -328,6 +328,92 @@ long long nfk_attn_q8_workspace(const nfk_attn_q8_params* p);
 int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream);
 
 // ------------------------------------------------------------------------------------------------
+// Drafted tokens (page_tables.cu, rope_slots.cu, attn_tree.cu, tree.cu): a step in which each request brings a tree or a chain of
+// tokens that the model is to check. bf16 cache pools [num_pages][2][kv_heads][16][head_dim]; a token's place in a pool is
+// its slot, page * 16 + place in the page.
+// ------------------------------------------------------------------------------------------------
+// Page tables: row r holds the pages of one request, table[r * max_pages + i] those of its tokens 16 i .. 16 i + 15. Free pages are a
+// stack; `ticket` is a word of the tables' own, zero between calls.
+//
+// nfk_tables_grow: lengths[rows[r]] += tokens[r]; the k-th page that the call takes, requests in their order, is
+// free_pages[free_count - 1 - k]. Lists of the requests as they are afterwards; of the new tokens their positions, requests and slots
+// (entries behind the last token: 0, -1, -1).
+// nfk_tables_trim: lengths[rows[r]] -= min(tokens[r], lengths[rows[r]]); the k-th of the n pages that come free goes to
+// free_pages[free_count + n - 1 - k]: a trim takes back the grow before it. The lists are not looked at.
+// A row that is none or comes twice, a negative count, or a size that does not fit (pages of a row, free pages, lists): nothing
+// changes, all lists are empty, and `status` says so.
+enum { NFK_TABLES_REQUESTS = 4096, NFK_TABLES_ROWS = 65536 };
+typedef struct nfk_tables_params {
+  int* table; int* lengths; int* free_pages; int* free_count; unsigned int* ticket;
+  const int* rows; const int* tokens;
+  int* qo_indptr; int* kv_indptr; int* kv_indices; int* kv_last_page_len; int* positions; int* token_req; int* slots;
+  int requests, max_requests, max_pages, num_pages, num_indices, num_tokens;   // entries of kv_indices; of positions, token_req, slots
+  int early_start;
+  unsigned int* status;
+} nfk_tables_params;
+int nfk_tables_grow(const nfk_tables_params* p, cudaStream_t stream);
+int nfk_tables_trim(const nfk_tables_params* p, cudaStream_t stream);
+
+// Rotation of queries and keys, q to q_out and k, v to their slots. Of the first 2 * pairs elements of a head, i and i + pairs are a pair,
+// or with `interleaved` 2 i and 2 i + 1; (x, y) becomes factor * (x cos - y sin, y cos + x sin) at the angle positions[t] * inv_freq[i],
+// formed in 64 bits. Tokens whose slot is negative are not cached (padding); slots that do not exist are reported.
+typedef struct nfk_rope_slots_params {
+  const void* qkv; long long ld_qkv; int q_off, k_off, v_off;   // columns of qkv
+  void* q_out; void* kv_pool; const float* inv_freq; const int* positions; const int* slots;
+  float factor;
+  int T, q_heads, kv_heads, head_dim, pairs, interleaved, num_pages;
+  int early_start;
+  unsigned int* status;
+} nfk_rope_slots_params;
+int nfk_rope_slots(const nfk_rope_slots_params* p, cudaStream_t stream);
+
+// Attention of the n query tokens of each request over its cached tokens, the last n of which are themselves: all see the ones in front
+// of those, and token i drafted token j where bit j of its row of `tree` is set ([num_tokens][words] of 64 bits; null: j <= i).
+typedef struct nfk_attn_tree_params {
+  const void* q; long long ld_q; void* out; long long ld_out; const void* kv_pool;
+  const int* qo_indptr; const int* kv_indptr; const int* kv_indices; const int* kv_last_page_len; const unsigned long long* tree;
+  int q_heads, kv_heads, head_dim, num_pages, num_tokens, num_indices, req_begin, req_count, words;
+  float sm_scale;
+  int num_ctas;              // CTA budget of each kernel, 0 = all that fit
+  int early_start;
+  void* workspace;           // nfk_attn_tree_workspace bytes at 256, whatever they hold; calls that may run at the same time each
+  long long workspace_bytes; // need their own
+  unsigned int* status;
+} nfk_attn_tree_params;
+long long nfk_attn_tree_workspace(const nfk_attn_tree_params* p);   // by head_dim; 0: unsupported
+int nfk_attn_tree(const nfk_attn_tree_params* p, cudaStream_t stream);
+
+// Trees: parents[t] is the place of token t's parent among its request's tokens, in front of it; -1: none.
+enum { NFK_TREE_NODES = 512 };
+typedef struct nfk_tree_masks_params {    // mask[t]: bits of t and of what it descends from; positions[t] = the request's first one + depth
+  const int* parents; const int* qo_indptr; unsigned long long* mask; int* positions;   // (positions: may be null)
+  int requests, num_tokens, words;
+  int early_start;
+  unsigned int* status;
+} nfk_tree_masks_params;
+int nfk_tree_masks(const nfk_tree_masks_params* p, cudaStream_t stream);
+// From each request's token 0 on to the first child that holds what `targets` says behind its parent: path[r] the places of the tokens
+// that this comes by (-1 behind the last), counts[r] how many, next_tokens[r] the target behind the last, dropped[r] (may be null) the others' number.
+typedef struct nfk_tree_accept_params {
+  const int* tokens; const int* parents; const int* targets; const int* qo_indptr;
+  int* path; int* counts; int* next_tokens; int* dropped;
+  int requests, num_tokens, max_path;
+  int early_start;
+  unsigned int* status;
+} nfk_tree_accept_params;
+int nfk_tree_accept(const nfk_tree_accept_params* p, cudaStream_t stream);
+// In every pool: the vectors of token path[r][k] of request r to the slot of its token k, k < counts[r].
+enum { NFK_KEEP_POOLS = 64 };
+typedef struct nfk_kv_keep_params {
+  void* pools[NFK_KEEP_POOLS]; int num_pools;
+  const int* slots; const int* path; const int* counts; const int* qo_indptr;
+  int requests, num_tokens, max_path, num_pages, kv_heads, head_dim;
+  int early_start;
+  unsigned int* status;
+} nfk_kv_keep_params;
+int nfk_kv_keep(const nfk_kv_keep_params* p, cudaStream_t stream);
+
+// ------------------------------------------------------------------------------------------------
 // Layer-list models: residual step, latent attention, mLSTM (residual_norm.cu, latent.cu, mlstm.cu)
 // ------------------------------------------------------------------------------------------------
 enum { NFK_NORM_NONE = 0, NFK_NORM_RMS = 1, NFK_NORM_LAYER = 2, NFK_NORM_SCALE = 3 };   // SCALE: only times the weights

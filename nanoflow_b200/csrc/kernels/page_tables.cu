@@ -1,0 +1,282 @@
+// Page tables on the GPU: growth by a step's tokens, with the lists that the step's kernels read, and the way back.
+//
+//   nfk_tables_grow  pages(r) = ceil((lengths + tokens) / 16), places of requests in the lists by sums over the requests in front
+//   nfk_tables_trim  pages of dropped tokens back onto the stack of free ones
+//
+// One launch each, bound by latency (a chain of three loads, a scan) for all but the largest batches: every CTA works out all sums by
+// itself, in shared memory, and then writes its share of the lists, an entry's request found by bisection. What the call changes
+// is written by the CTA that is the last to have read it, known by a ticket.
+#include "common.cuh"
+#include "kernels.h"
+
+namespace nf {
+namespace {
+
+constexpr int kPage = 16;
+constexpr int kThreads = 512;
+// entries of the lists that a thread writes before there are further CTAs
+constexpr int kPerThread = 4;
+
+__device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPage - 1) / kPage; }
+
+// Sums over the requests in front of each, of up to three things.
+struct Sums {
+  int* row;         // [requests] row of the tables
+  int* old;         // [requests] length before the call
+  int* at[3];       // [requests + 1]
+  unsigned int* taken;   // rows, a bit each
+};
+__device__ __forceinline__ Sums sums_in(uint8_t* smem, int requests) {
+  Sums s;
+  int* a = reinterpret_cast<int*>(smem);
+  s.row = a;
+  s.old = a + requests;
+  for (int k = 0; k < 3; ++k) s.at[k] = a + 2 * requests + k * (requests + 1);
+  s.taken = reinterpret_cast<unsigned int*>(s.at[2] + requests + 1);
+  return s;
+}
+int smem_bytes(int requests, int max_requests) { return (5 * requests + 3 + (max_requests + 31) / 32) * 4; }
+
+// at[k][r] = sum of what[k] of the requests in front of r; false where one does not fit 32 bits. Entries hold `what` before.
+__device__ __forceinline__ bool scan(const Sums& s, int requests, long long (&total)[3]) {
+  __shared__ long long warp_sum[3][kThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (requests + kThreads - 1) / kThreads, r0 = min(requests, static_cast<int>(threadIdx.x) * per), r1 = min(requests, r0 + per);
+  long long mine[3] = {0, 0, 0}, sum[3];
+  for (int r = r0; r < r1; ++r)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) mine[k] += s.at[k][r];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    sum[k] = mine[k];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long v = __shfl_up_sync(0xffffffffu, sum[k], o);
+      if (lane >= o) sum[k] += v;
+    }
+    if (lane == 31) warp_sum[k][warp] = sum[k];
+  }
+  __syncthreads();
+  bool fits = true;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    long long before = sum[k] - mine[k];
+    total[k] = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+      const long long v = warp_sum[k][w];
+      if (w < warp) before += v;
+      total[k] += v;
+    }
+    fits = fits && total[k] <= 0x7fffffff;
+    if (total[k] <= 0x7fffffff) {
+      int a = static_cast<int>(before);
+      for (int r = r0; r < r1; ++r) {
+        const int n = s.at[k][r];
+        s.at[k][r] = a;
+        a += n;
+      }
+      if (threadIdx.x == 0) s.at[k][requests] = static_cast<int>(total[k]);
+    }
+  }
+  __syncthreads();
+  return fits;
+}
+// The request that entry e belongs to: the last one with at[r] <= e.
+__device__ __forceinline__ int holder(const int* at, int requests, int e) {
+  int r = 0, n = requests;
+  while (n > 1) {
+    const int half = n >> 1;
+    if (at[r + half] <= e) {
+      r += half;
+      n -= half;
+    } else {
+      n = half;
+    }
+  }
+  return r;
+}
+// Requests as they come, into row, old and at[0] (tokens); false, for all threads, where one is none.
+__device__ __forceinline__ bool read_requests(const nfk_tables_params& p, const Sums& s) {
+  const int words = (p.max_requests + 31) / 32;
+  for (int w = threadIdx.x; w < words; w += kThreads) s.taken[w] = 0;
+  __syncthreads();
+  bool bad = false;
+  for (int r = threadIdx.x; r < p.requests; r += kThreads) {
+    const int row = p.rows[r], n = p.tokens[r];
+    bool ok = row >= 0 && row < p.max_requests && n >= 0;
+    if (ok) ok = (atomicOr(&s.taken[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u) == 0u;
+    const int old = ok ? p.lengths[row] : 0;
+    ok = ok && old >= 0 && old <= p.max_pages * kPage;
+    s.row[r] = row;
+    s.old[r] = old;
+    s.at[0][r] = n;
+    bad = bad || !ok;
+  }
+  return __syncthreads_or(bad) == 0;
+}
+// Whether this CTA is the last one to have read what the call changes; all threads.
+__device__ __forceinline__ bool last_reader(unsigned int* ticket) {
+  if (gridDim.x == 1) return true;               // (behind a barrier of the block)
+  __shared__ int last;
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(ticket, 1u) == gridDim.x - 1;
+    if (last) {
+      *ticket = 0;
+      __threadfence();
+    }
+  }
+  __syncthreads();
+  return last != 0;
+}
+
+__global__ void __launch_bounds__(kThreads) tables_grow_kernel(nfk_tables_params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const Sums s = sums_in(smem, p.requests);
+  const int R = p.requests;
+  let_next_start();
+  await_previous();
+  const int free_count = *p.free_count;
+  bool ok = read_requests(p, s) && free_count >= 0 && free_count <= p.num_pages;
+  long long total[3] = {0, 0, 0};                // tokens, pages, pages taken
+  if (ok) {
+    bool bad = false;
+    for (int r = threadIdx.x; r < R; r += kThreads) {
+      const int old = s.old[r], n = s.at[0][r];
+      if (n > p.max_pages * kPage - old) {
+        bad = true;
+        continue;
+      }
+      s.at[1][r] = pages_of(old + n);
+      s.at[2][r] = pages_of(old + n) - pages_of(old);
+    }
+    ok = __syncthreads_or(bad) == 0;
+  }
+  if (ok) ok = scan(s, R, total) && total[0] <= p.num_tokens && total[1] <= p.num_indices && total[2] <= free_count;
+  const bool last = last_reader(p.ticket);
+  if (!ok) {
+    total[0] = total[1] = 0;
+    if (last && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
+  }
+  const int at = blockIdx.x * kThreads + threadIdx.x, step = gridDim.x * kThreads;
+  for (int r = at; r <= R; r += step) {
+    p.qo_indptr[r] = ok ? s.at[0][r] : 0;
+    p.kv_indptr[r] = ok ? s.at[1][r] : 0;
+    if (r < R) {
+      const int length = ok ? s.old[r] + s.at[0][r + 1] - s.at[0][r] : 0;
+      p.kv_last_page_len[r] = length - max(pages_of(length) - 1, 0) * kPage;
+    }
+  }
+  // page i of request r: the table's, or a new one
+  auto page = [&](int r, int i) {
+    const int had = pages_of(s.old[r]);
+    return i < had ? p.table[static_cast<long long>(s.row[r]) * p.max_pages + i] : p.free_pages[free_count - 1 - (s.at[2][r] + i - had)];
+  };
+  for (int e = at; e < static_cast<int>(total[1]); e += step) {
+    const int r = holder(s.at[1], R, e), i = e - s.at[1][r], id = page(r, i);
+    p.kv_indices[e] = id;
+    if (i >= pages_of(s.old[r])) p.table[static_cast<long long>(s.row[r]) * p.max_pages + i] = id;
+  }
+  for (int t = at; t < p.num_tokens; t += step) {
+    int pos = 0, req = -1, slot = -1;
+    if (t < static_cast<int>(total[0])) {
+      req = holder(s.at[0], R, t);
+      pos = s.old[req] + t - s.at[0][req];
+      slot = page(req, pos / kPage) * kPage + pos % kPage;
+    }
+    p.positions[t] = pos;
+    p.token_req[t] = req;
+    p.slots[t] = slot;
+  }
+  if (last && ok) {
+    for (int r = threadIdx.x; r < R; r += kThreads) p.lengths[s.row[r]] = s.old[r] + s.at[0][r + 1] - s.at[0][r];
+    if (threadIdx.x == 0) *p.free_count = free_count - static_cast<int>(total[2]);
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) tables_trim_kernel(nfk_tables_params p) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  const Sums s = sums_in(smem, p.requests);
+  const int R = p.requests;
+  let_next_start();
+  await_previous();
+  const int free_count = *p.free_count;
+  bool ok = read_requests(p, s) && free_count >= 0 && free_count <= p.num_pages;
+  long long total[3] = {0, 0, 0};                // new lengths (their sums are not looked at), unused, pages that come free
+  if (ok) {
+    for (int r = threadIdx.x; r < R; r += kThreads) {
+      const int old = s.old[r], length = old - min(s.at[0][r], old);
+      s.at[0][r] = length;
+      s.at[1][r] = 0;
+      s.at[2][r] = pages_of(old) - pages_of(length);
+      s.old[r] = length;
+    }
+    __syncthreads();
+    (void)scan(s, R, total);
+    ok = total[2] <= p.num_pages - free_count;
+  }
+  const bool last = last_reader(p.ticket);
+  if (!ok) {
+    if (last && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
+    return;
+  }
+  const int n = static_cast<int>(total[2]);
+  for (int e = blockIdx.x * kThreads + threadIdx.x; e < n; e += gridDim.x * kThreads) {
+    const int r = holder(s.at[2], R, e);
+    p.free_pages[free_count + n - 1 - e] = p.table[static_cast<long long>(s.row[r]) * p.max_pages + pages_of(s.old[r]) + e - s.at[2][r]];
+  }
+  if (last) {
+    for (int r = threadIdx.x; r < R; r += kThreads) p.lengths[s.row[r]] = s.old[r];
+    if (threadIdx.x == 0) *p.free_count = free_count + n;
+  }
+}
+
+template <bool GROW>
+int launch(const nfk_tables_params& p, long long entries, cudaStream_t stream) {
+  const auto kernel = GROW ? tables_grow_kernel : tables_trim_kernel;
+  const int bytes = smem_bytes(p.requests, p.max_requests);
+  static bool attr_dev[kMaxDevices] = {false};   // the attribute is per device
+  bool& attr = attr_dev[device_slot()];
+  if (!attr) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(NFK_TABLES_REQUESTS, NFK_TABLES_ROWS)) != cudaSuccess) {
+      (void)cudaGetLastError();
+      return NF_ERR_CUDA;
+    }
+    attr = true;
+  }
+  long long ctas = (entries + kThreads * kPerThread - 1) / (kThreads * kPerThread);
+  if (ctas > device_sm_count()) ctas = device_sm_count();
+  if (ctas < 1) ctas = 1;
+  if (launch_kernel(early_first(p.early_start), kernel, static_cast<int>(ctas), kThreads, bytes, stream, 1, p) == cudaSuccess) return NF_OK;
+  (void)cudaGetLastError();
+  return NF_ERR_CUDA;
+}
+int check(const nfk_tables_params* p) {
+  if (p == nullptr || p->requests < 0 || p->requests > NFK_TABLES_REQUESTS || p->max_requests < 1 || p->max_requests > NFK_TABLES_ROWS ||
+      p->max_pages < 1 || p->max_pages > 0x7fffffff / kPage || p->num_pages < 1 || p->num_pages > 0x7fffffff / kPage)
+    return NF_ERR_BAD_ARG;
+  return p->table && p->lengths && p->free_pages && p->free_count && p->ticket && p->rows && p->tokens ? NF_OK : NF_ERR_BAD_ARG;
+}
+
+}  // namespace
+}  // namespace nf
+
+extern "C" int nfk_tables_grow(const nfk_tables_params* p, cudaStream_t stream) {
+  using namespace nf;
+  const int rc = check(p);
+  if (rc != NF_OK) return rc;
+  if (!p->qo_indptr || !p->kv_indptr || !p->kv_indices || !p->kv_last_page_len || !p->positions || !p->token_req || !p->slots ||
+      p->num_indices < 0 || p->num_tokens < 0)
+    return NF_ERR_BAD_ARG;
+  // (lists of a captured graph may be far longer than what a step fills, so that both count)
+  return launch<true>(*p, static_cast<long long>(p->num_indices) + p->num_tokens, stream);
+}
+
+extern "C" int nfk_tables_trim(const nfk_tables_params* p, cudaStream_t stream) {
+  using namespace nf;
+  const int rc = check(p);
+  if (rc != NF_OK) return rc;
+  if (p->requests == 0) return NF_OK;
+  return launch<false>(*p, static_cast<long long>(p->requests) * 64, stream);
+}

@@ -730,3 +730,5 @@ def kv_move_pages(pool: torch.Tensor, staging: torch.Tensor, page_ids: torch.Ten
 
 from .cache_q8 import (attn_decode_q8, attn_decode_shared_q8, decode_workspace_q8, kv_pool_q8, kv_read_q8,  # noqa: E402
                        rope_append_q8)
+from .draft import (BatchLists, PageTables, attn_tree, batch_lists, kv_keep, page_tables, rope_append_slots, rope_frequencies,  # noqa: E402
+                    tables_grow, tables_trim, tree_accept, tree_masks, tree_workspace)

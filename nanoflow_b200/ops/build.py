@@ -136,7 +136,7 @@ def build_calls(verbose: bool = False) -> None:
     suffix = sysconfig.get_config_var("EXT_SUFFIX") or ".so"
     for src in sorted(CALLS_DIR.glob("*.cpp")):
         out = PKG / "ops" / f"_{src.stem}{suffix}"
-        if _newer(out, [src, KERNEL_DIR / "kernels.h"]):
+        if _newer(out, [src, KERNEL_DIR / "kernels.h", *CALLS_DIR.glob("*.h")]):
             _run(["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
                   f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I", sysconfig.get_paths()["include"],
                   "-I", home / "include", "-I", home / "include" / "torch" / "csrc" / "api" / "include",
