@@ -525,35 +525,37 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             const int left = end - (at + k * 32);
             bits[k] = on ? seen_bits(tree, 2 * p.words, node, f.all, at + k * 32 - ctx) & (left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u) : 0u;
           }
-          if (!f.two || slot == 0) {
-            // ---- values of the tile: a thread per token ----
-            const uint32_t v = ring + v_at(tile, tiles);
-            if (!passed(C::FULL + v % NST, v / NST & 1)) { ok = false; break; }
-            const int token = at + row;
-            if (token >= ctx) {
-              const uint32_t v_row = sb + C::kRing + v % NST * C::kStage + row * 128;
-              bool odd = false;
-#pragma unroll
-              for (int c = 0; c < HD / 8; ++c) {
-                const uint32_t a = v_row + (c >> 3) * C::kHalf + (((c & 7) ^ (row & 7)) << 4);
-                if (token >= end) {
-                  st_shared_v4(a, make_uint4(0u, 0u, 0u, 0u));
-                } else {
-                  uint4 w = ld_shared_v4(a);
-                  if (odd_pair(w.x) || odd_pair(w.y) || odd_pair(w.z) || odd_pair(w.w)) {
-                    odd = true;
-                    w = make_uint4(without_odd(w.x), without_odd(w.y), without_odd(w.z), without_odd(w.w));
-                    st_shared_v4(a, w);
-                  }
-                }
-              }
-              if (odd) odd_item[n_item & 1] = static_cast<int>(n_item);
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
-          }
         }
         if (!passed(C::S_FULL + slot, n_done & 1)) { ok = false; break; }
+        if (care && (!f.two || slot == 0)) {
+          // ---- values of the tile: a thread per token ----
+          // (Behind the wait for the scores: a parity tells only neighbouring phases apart, and where the scores have been issued, what
+          // was in the ring's place before these values has come and been used.)
+          const uint32_t v = ring + v_at(tile, tiles);
+          if (!passed(C::FULL + v % NST, v / NST & 1)) { ok = false; break; }
+          const int token = at + row;
+          if (token >= ctx) {
+            const uint32_t v_row = sb + C::kRing + v % NST * C::kStage + row * 128;
+            bool odd = false;
+#pragma unroll
+            for (int c = 0; c < HD / 8; ++c) {
+              const uint32_t a = v_row + (c >> 3) * C::kHalf + (((c & 7) ^ (row & 7)) << 4);
+              if (token >= end) {
+                st_shared_v4(a, make_uint4(0u, 0u, 0u, 0u));
+              } else {
+                uint4 w = ld_shared_v4(a);
+                if (odd_pair(w.x) || odd_pair(w.y) || odd_pair(w.z) || odd_pair(w.w)) {
+                  odd = true;
+                  w = make_uint4(without_odd(w.x), without_odd(w.y), without_odd(w.z), without_odd(w.w));
+                  st_shared_v4(a, w);
+                }
+              }
+            }
+            if (odd) odd_item[n_item & 1] = static_cast<int>(n_item);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
         if (warp_on) {
           tc_fence_after();
           uint32_t x[4][32];

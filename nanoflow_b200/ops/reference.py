@@ -462,3 +462,118 @@ def attn_decode_q8(q, kv_pool, kv_scale, qo_indptr, kv_indptr, kv_indices, kv_la
         most = k.shape[1] * v.abs().amax((1, 2))[:, None, None].expand_as(size)
         out[int(qo_indptr[b])] = tuple(t.reshape(q_heads, -1) for t in (p @ v, p @ v.abs(), size, most))
     return out
+
+
+# ---- drafted tokens (ops/draft.py), in Python and 64 bits -----------------------------------------------------------------
+def tables_grow(table, lengths, free_pages, free_count, rows, new_tokens):
+    """In place on ``table``, ``lengths`` and ``free_count`` (CPU tensors); returns the lists as a dict of Python lists."""
+    li = {k: [] for k in ("kv_indices", "kv_last_page_len", "positions", "token_req", "slots")}
+    li["qo_indptr"], li["kv_indptr"] = [0], [0]
+    top = int(free_count[0])
+    for r, (row, new) in enumerate(zip(rows.tolist(), new_tokens.tolist())):
+        old = int(lengths[row])
+        had, pages = (old + 15) // 16, (old + new + 15) // 16
+        for i in range(had, pages):
+            top -= 1
+            table[row, i] = free_pages[top]
+        lengths[row] = old + new
+        own = table[row, :pages].tolist()
+        li["kv_indices"] += own
+        li["kv_indptr"].append(len(li["kv_indices"]))
+        li["kv_last_page_len"].append(old + new - (pages - 1) * 16 if pages else 0)
+        for pos in range(old, old + new):
+            li["positions"].append(pos)
+            li["token_req"].append(r)
+            li["slots"].append(own[pos // 16] * 16 + pos % 16)
+        li["qo_indptr"].append(len(li["slots"]))
+    free_count[0] = top
+    return li
+
+
+def tables_trim(table, lengths, free_pages, free_count, rows, dropped):
+    """In place on ``lengths``, ``free_pages`` and ``free_count``."""
+    free = []
+    for row, n in zip(rows.tolist(), dropped.tolist()):
+        old = int(lengths[row])
+        lengths[row] = old - min(n, old)
+        free += table[row, (int(lengths[row]) + 15) // 16:(old + 15) // 16].tolist()
+    top = int(free_count[0])
+    for k, page in enumerate(free):
+        free_pages[top + len(free) - 1 - k] = page
+    free_count[0] = top + len(free)
+
+
+def rope_layout(x, positions, inv_freq, interleaved=False, factor=1.0):
+    """x: [T, heads, head_dim] with its first 2 len(inv_freq) elements turned; in 64 bits."""
+    x, n = x.double().clone(), inv_freq.numel()
+    ang = positions.double()[:, None] * inv_freq.double()[None, :]
+    cos, sin = (ang.cos() * factor)[:, None], (ang.sin() * factor)[:, None]
+    a, b = (slice(0, 2 * n, 2), slice(1, 2 * n, 2)) if interleaved else (slice(0, n), slice(n, 2 * n))
+    u, v = x[..., a].clone(), x[..., b].clone()
+    x[..., a], x[..., b] = u * cos - v * sin, v * cos + u * sin
+    return x
+
+
+def attn_tree(q, kv_pool, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tree, *, q_heads, sm_scale=None):
+    """(attention, attention of the values' magnitudes), [T, q_heads, head_dim] in 64 bits; ``tree``: words as the operator's, or None."""
+    _, _, kv_heads, _, hd = kv_pool.shape
+    scale, group = sm_scale or hd ** -0.5, q_heads // kv_heads
+    q = q.double().view(-1, q_heads, hd)
+    out, size = torch.zeros_like(q), torch.zeros_like(q)
+    for r in range(kv_last_page_len.numel()):
+        a, b = int(qo_indptr[r]), int(qo_indptr[r + 1])
+        pages = kv_indices[int(kv_indptr[r]):int(kv_indptr[r + 1])].long()
+        n, length = b - a, (len(pages) - 1) * 16 + int(kv_last_page_len[r]) if len(pages) else 0
+        if n == 0 or length < n:
+            continue
+        sees = torch.ones(n, length, dtype=torch.bool)
+        for i in range(n):
+            for j in range(n):
+                sees[i, length - n + j] = j <= i if tree is None else j < 64 * tree.shape[1] and bool(int(tree[a + i, j // 64]) >> (j % 64) & 1)
+        for h in range(kv_heads):
+            k, v = (kv_pool[pages, s, h].double().reshape(-1, hd)[:length] for s in (0, 1))
+            for i in range(n):
+                if not sees[i].any():
+                    continue
+                p = torch.softmax(q[a + i, h * group:(h + 1) * group] @ k[sees[i]].T * scale, -1)
+                out[a + i, h * group:(h + 1) * group] = p @ v[sees[i]]
+                size[a + i, h * group:(h + 1) * group] = p @ v[sees[i]].abs()
+    return out, size
+
+
+def tree_masks(parents, qo_indptr, words):
+    """(mask words, depths)."""
+    mask, depth = torch.zeros(parents.numel(), words, dtype=torch.int64), torch.zeros(parents.numel(), dtype=torch.int32)
+    for a, b in zip(qo_indptr.tolist(), qo_indptr.tolist()[1:]):
+        for i in range(b - a):
+            j, bits, steps = i, 0, -1
+            while j >= 0:
+                bits, steps, j = bits | 1 << j, steps + 1, int(parents[a + j])
+            depth[a + i] = steps
+            for w in range(words):
+                v = bits >> (64 * w) & (1 << 64) - 1
+                mask[a + i, w] = v - (1 << 64) if v >> 63 else v
+    return mask, depth
+
+
+def tree_accept(tokens, parents, targets, qo_indptr, places):
+    """Paths (lists), next tokens, numbers of dropped tokens."""
+    paths, following, dropped = [], [], []
+    for a, b in zip(qo_indptr.tolist(), qo_indptr.tolist()[1:]):
+        path, at = [], 0 if b > a and places > 0 else -1
+        while at >= 0:
+            path.append(at)
+            fits = [i for i in range(at + 1, b - a) if int(parents[a + i]) == at and int(tokens[a + i]) == int(targets[a + at])]
+            at = fits[0] if fits and len(path) < places else -1
+        paths.append(path)
+        following.append(int(targets[a + path[-1]]) if path else -1)
+        dropped.append(b - a - len(path))
+    return paths, following, dropped
+
+
+def kv_keep(kv_pool, slots, paths, qo_indptr):
+    """In place on one pool; ``paths`` as lists."""
+    for path, a in zip(paths, qo_indptr.tolist()):
+        for k, i in enumerate(path):
+            to, source = int(slots[a + k]), int(slots[a + i])
+            kv_pool[to // 16, :, :, to % 16] = kv_pool[source // 16, :, :, source % 16].clone()
