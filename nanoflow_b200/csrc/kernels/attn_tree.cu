@@ -32,32 +32,15 @@
 namespace nf {
 namespace {
 
-constexpr int kTile = 128;            // cached tokens per tile
+constexpr int kTile = 64;             // cached tokens per tile
 constexpr int kTilePages = kTile / kPage;
-constexpr int kThreads = 320;         // warps 0-3 slot 0, 4-7 slot 1, 8 copies, 9 products
+constexpr int kThreads = 352;         // warps 0-3 slot 0, 4-7 slot 1, 8 copies, 9 and 10 products of either slot
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
 constexpr float kGap = 8.f;           // log2 of how far a row's maximum may outgrow its reference
 // What an item's beginning and end cost, in pages: where the work is cut, the ends count too.
 constexpr int kLead = 8;
 // Pages that a CTA takes at least, so that the states of short requests do not outweigh their pages.
 constexpr int kLeast = 8;
-
-template <int HD>
-struct Cfg {
-  static constexpr int NH = HD / 64;
-  static constexpr int kHalf = kTile * 128;                    // [128 tokens or rows][64 elements]
-  static constexpr int kStage = NH * kHalf;                    // a tile of keys or of values; a slot's queries
-  static constexpr int kStages = HD == 128 ? 5 : 10;
-  static constexpr int kRing = 2 * kStage;                     // (queries of both slots in front)
-  static constexpr int kMl = kRing + kStages * kStage;         // [2 slots][128] float2
-  static constexpr int kBars = kMl + 2 * 128 * 8;
-  static constexpr int kBytes = kBars + 512;
-  enum Bar : int {
-    FULL = 0, EMPTY = FULL + kStages, Q_FULL = EMPTY + kStages, Q_EMPTY, READ, O_FREE, LAST, S_FULL, P_FULL = S_FULL + 2, PV_DONE = P_FULL + 2,
-    MERGE = PV_DONE + 2, kNum = MERGE + 4
-  };
-  static_assert(kNum * 8 + 8 + 64 + 16 + 64 <= 512 && kBytes <= 227 * 1024, "shared memory");
-};
 
 // What the roles need to know of a piece.
 struct Piece {
@@ -72,6 +55,23 @@ struct Piece {
   int to;            // piece number, -1: the whole item
   int two;           // blocks of more than 128 rows: each slot its own
 };
+template <int HD>
+struct Cfg {
+  static constexpr int NH = HD / 64;
+  static constexpr int kQHalf = 128 * 128, kHalf = kTile * 128;        // [128 rows or 64 tokens][64 elements]
+  static constexpr int kQ = NH * kQHalf, kStage = NH * kHalf;  // a slot's queries; a tile of keys or of values
+  static constexpr int kStages = HD == 128 ? 8 : 16;           // (a power of two)
+  static constexpr int kRing = 2 * kQ;                         // (queries of both slots in front)
+  static constexpr int kMl = kRing + kStages * kStage;         // [2 slots][128] float2
+  static constexpr int kBars = kMl + 2 * 128 * 8;
+  static constexpr int kBytes = kBars + 640;
+  enum Bar : int {
+    FULL = 0, EMPTY = FULL + kStages, Q_FULL = EMPTY + kStages, Q_EMPTY, READ, O_FREE, LAST, CARE = LAST + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 4,
+    PV_DONE = P_FULL + 4, MERGE = PV_DONE + 4, kNum = MERGE + 4   // (S_FULL to PV_DONE: two to a slot, which its tiles use in turn)
+  };
+  static_assert(kNum * 8 + 20 + sizeof(Piece) <= 640 && kBytes <= 227 * 1024, "shared memory");
+};
+
 // What a CTA leaves for the kernel that joins states: the item that begins with it and goes on behind it, if there is one.
 struct Record {
   int pieces, tok, nodes, kvh;
@@ -164,6 +164,15 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* t
       "l"(reinterpret_cast<uint64_t>(tm)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
       : "memory");
 }
+__device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
 // bf16 pairs with an infinity or NaN in them
 __device__ __forceinline__ bool odd_pair(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
@@ -172,18 +181,51 @@ __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
   return w;
 }
 
-// Infinities and NaN of the drafted tokens [from, end) that the row sees, in 16 columns: as terms of its sums they are what they are,
+// Of N x N pieces, N lanes with a row of them each: lane j gets piece j of all N rows.
+template <int N>
+__device__ __forceinline__ void exchange(uint4* v) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = N / 2; s > 0; s >>= 1)
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if ((k & s) != 0) continue;
+      const bool up = (lane & s) != 0;
+      const uint4 give = up ? v[k] : v[k | s];
+      uint4 get;
+      get.x = __shfl_xor_sync(0xffffffffu, give.x, s);
+      get.y = __shfl_xor_sync(0xffffffffu, give.y, s);
+      get.z = __shfl_xor_sync(0xffffffffu, give.z, s);
+      get.w = __shfl_xor_sync(0xffffffffu, give.w, s);
+      if (up) v[k] = get;
+      else v[k | s] = get;
+    }
+}
+// Waits, for a while, until *count is `goal`; for a whole warp.
+__device__ __forceinline__ bool reached(volatile int* count, int goal, volatile int* abort_flag) {
+  bool ok = false;
+  for (int it = 0; it < (1 << 22) && !ok && *abort_flag == 0; ++it) ok = *count >= goal;
+  __threadfence_block();
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+// Quotients of what fits 32 bits without the long way of 64.
+__device__ __forceinline__ long long divide(long long a, long long b) {
+  if (((a | b) >> 32) == 0) return static_cast<unsigned int>(a) / static_cast<unsigned int>(b);
+  return a / b;
+}
+
+// Infinities and NaN of the drafted tokens [from, end) that the row sees, in 32 columns: as terms of its sums they are what they are,
 // whatever their weights. (Only where there are some.)
 template <int HD>
 __device__ __forceinline__ void restore_odd(const nfk_attn_tree_params& p, const Piece& f, const uint32_t* tree, int node, int from, int end, int c,
-                                         float (&o)[16]) {
+                                         float (&o)[32]) {
   for (int t = from; t < end; ++t) {
     if ((seen_bits(tree, 2 * p.words, node, f.all, t - (f.len - f.all)) & 1u) == 0u) continue;
     int page = p.kv_indices[f.list + t / kPage];
     if (page < 0 || page >= p.num_pages) page = 0;               // (as it was read)
     const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.kv_pool) + (((static_cast<long long>(page) * 2 + 1) * p.kv_heads + f.kvh) * kPage + t % kPage) * HD + c;
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
+    for (int j = 0; j < 32; ++j) {
       const float x = __bfloat162float(v[j]);
       if (!isfinite(x)) o[j] += x;
     }
@@ -202,7 +244,8 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::kNum);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   volatile int* odd_item = reinterpret_cast<volatile int*>(tmem_slot + 2);         // [2]: numbers of items with odd values
-  Piece* piece_s = reinterpret_cast<Piece*>(tmem_slot + 4);
+  int* cleared = reinterpret_cast<int*>(tmem_slot + 4);                            // warps of slot 0 that have been through a tile's values
+  Piece* piece_s = reinterpret_cast<Piece*>(tmem_slot + 5);
   // (before the roles begin) sums of the warps' units, units in front of the CTA's first request, its number
   long long* scan_s = reinterpret_cast<long long*>(smem + C::kMl);
   long long* start_off_s = scan_s + kThreads / 32;
@@ -219,18 +262,20 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   if (threadIdx.x == 0) {
     for (int b = 0; b < C::kNum; ++b) {
-      const int n = b == C::READ ? 9 : b == C::O_FREE ? 8 : (b >= C::P_FULL && b < C::PV_DONE) ? 4 : b >= C::MERGE ? 2 : 1;
+      const int n = b == C::READ ? 10 : b == C::O_FREE ? 8 : (b >= C::P_FULL && b < C::PV_DONE) ? 4
+                    : b >= C::MERGE || b == C::Q_EMPTY || (b >= C::EMPTY && b < C::Q_FULL) ? 2 : 1;
       mbar_init(&bars[b], n);
     }
     *abort_flag = 0;
     odd_item[0] = odd_item[1] = -1;
+    *cleared = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmKV);
   }
   await_previous();                              // (before tensor memory is taken, which the kernel before may need)
   if (warp == kMmaWarp) {
-    tmem_alloc(tmem_slot, 512);                  // of each slot (256 columns): scores in [0, 128), sums in [128, 128 + HD)
+    tmem_alloc(tmem_slot, 512);                  // of each slot (256 columns): scores in [0, 64) and [64, 128), sums in [128, 128 + HD)
     tmem_relinquish();
   }
   // ---- where this CTA's share of the units begins: units of every thread's requests, scanned ----
@@ -282,10 +327,15 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     if (lane == 0) report_status(p.status, code);
     *abort_flag = 1;
   };
-  auto passed = [&](int bar, uint32_t parity) { return __all_sync(0xffffffffu, wait_or_abort(&bars[bar], parity, abort_flag)) != 0; };
-  // ring positions of an item's tiles, in the order of their use: K0, K1, V0, K2, V1, ... , V(n-1)
-  auto k_at = [](int t) { return t == 0 ? 0 : 2 * t - 1; };
-  auto v_at = [](int t, int n) { return t == n - 1 ? 2 * n - 1 : 2 * t + 2; };
+  const uint32_t bars_at = smem_u32(bars);
+  // for a whole warp; most barriers have been passed long before
+  auto passed = [&](int bar, uint32_t parity) {
+    return __all_sync(0xffffffffu, mbar_test(bars_at + bar * 8, parity)) != 0 || __all_sync(0xffffffffu, wait_or_abort(&bars[bar], parity, abort_flag)) != 0;
+  };
+  // Places of an item's tiles in the ring, in the order K0 K1 K2 K3 V0 K4 V1 K5 ... : keys are four tiles ahead, as far as both slots' scores
+  // are issued ahead of the second products.
+  auto k_at = [](int t) { return t + max(0, t - 3); };
+  auto v_at = [](int t, int n) { return t + min(n, t + 4); };
 
   if (!works || start_req < 0) {
     if (threadIdx.x == 0) ws.records[blockIdx.x] = Record{0, 0, 0, 0};
@@ -299,12 +349,12 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     for (int r = start_req; ok && r < p.req_count && at < u1; ++r) {
       const Request q = read_request(p, r, 2 * per_slot, false);
       const long long span = kLead + q.pages, n_items = q.blocks * p.kv_heads;
-      for (long long i = max(0ll, (u0 - at) / (span > 0 ? span : 1)); ok && i < n_items; ++i) {
+      for (long long i = u0 > at ? divide(u0 - at, span) : 0; ok && i < n_items; ++i) {
         const long long s = at + i * span;       // the item's first unit
         if (s >= u1) break;
         if (s + span <= u0) continue;
         Piece f;
-        f.kvh = static_cast<int>(i / q.blocks);
+        f.kvh = static_cast<int>(divide(i, q.blocks));
         f.node = static_cast<int>(i - f.kvh * q.blocks) * 2 * per_slot;
         f.tok = q.tok + f.node;
         f.nodes = min(2 * per_slot, q.n - f.node);
@@ -320,16 +370,13 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if (s < u0) continue;                  // rows of zeros: by the CTA that the item begins with
         } else {
           if (f.pages == 0) continue;
-          const int c0 = cut.of(first), c1 = cut.of(s + span - 1);
-          if (c0 != c1) {
-            f.to = 2 * blockIdx.x + (c0 == static_cast<int>(blockIdx.x) ? 1 : 0);
-            if (c0 == static_cast<int>(blockIdx.x)) record = Record{c1 - c0 + 1, f.tok, f.nodes, f.kvh};
-          }
+          const bool begins = first >= u0, ends = s + span <= u1;
+          if (!begins || !ends) f.to = 2 * blockIdx.x + (begins ? 1 : 0);
+          if (begins && !ends) record = Record{cut.of(s + span - 1) - static_cast<int>(blockIdx.x) + 1, f.tok, f.nodes, f.kvh};
         }
         const int tiles = (f.pages + kTilePages - 1) / kTilePages;
         const int* list = p.kv_indices + q.list + f.page0;
-        // Page numbers of 32 pages (four tiles) at a time, a lane each; keys are a tile ahead of values, so that of the next 32 come first
-        // when there is one tile of the others left.
+        // Page numbers of 32 pages (eight tiles) at a time, a lane each; keys are four tiles ahead of values, so that two such groups are held.
         auto fetch = [&](int group_of_32) {
           const int j = group_of_32 * 32 + lane;
           int page = -1;
@@ -344,18 +391,19 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         };
         int held[2] = {-1, -1};
         auto issue = [&](int pos, int tile, int part) {
-          if (part == 0 && (tile & 3) == 0) {
-            if ((tile >> 2 & 1) != 0) held[1] = fetch(tile >> 2);
-            else held[0] = fetch(tile >> 2);
+          const bool second = (tile >> 3 & 1) != 0;
+          if (part == 0 && (tile & 7) == 0) {
+            if (second) held[1] = fetch(tile >> 3);
+            else held[0] = fetch(tile >> 3);
           }
-          const int pages = (tile >> 2 & 1) != 0 ? held[1] : held[0];
+          const int pages = second ? held[1] : held[0];
           const uint32_t at_ring = ring + pos, stage = at_ring % NST;
           if (!passed(C::EMPTY + stage, (at_ring / NST & 1) ^ 1)) return false;
           uint8_t* to = smem + C::kRing + stage * C::kStage;
           int rows[kTilePages];
 #pragma unroll
           for (int j = 0; j < kTilePages; ++j) {
-            const int page = __shfl_sync(0xffffffffu, pages, (tile & 3) * kTilePages + j);
+            const int page = __shfl_sync(0xffffffffu, pages, (tile & 7) * kTilePages + j);
             rows[j] = page < 0 ? no_row : ((page * 2 + part) * p.kv_heads + f.kvh) * kPage;
           }
           if (elect_one()) {
@@ -370,13 +418,14 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           return true;
         };
         // the first tiles are on their way before the queries, which wait for the item before
-        const int ahead = min(2 * tiles, 3);
         auto issue_at = [&](int pos) {           // the inverse of k_at, v_at
-          const bool key = pos == 0 || ((pos & 1) != 0 && pos != 2 * tiles - 1);
-          return issue(pos, key ? (pos + 1) / 2 : pos == 2 * tiles - 1 ? tiles - 1 : pos / 2 - 1, key ? 0 : 1);
+          if (pos < min(tiles, 4)) return issue(pos, pos, 0);
+          if (pos >= 2 * tiles - 4) return issue(pos, pos - tiles, 1);
+          return (pos & 1) != 0 ? issue(pos, (pos + 3) / 2, 0) : issue(pos, pos / 2 - 2, 1);
         };
         int pos = 0;
-        for (; ok && pos < ahead; ++pos) ok = issue_at(pos);
+        if (n_item > 0)
+          for (; ok && pos < min(tiles, 4); ++pos) ok = issue_at(pos);
         if (!ok || !passed(C::READ, (n_item & 1) ^ 1) || !passed(C::Q_EMPTY, (n_item & 1) ^ 1)) {
           ring += pos;
           ok = false;
@@ -389,7 +438,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int slot = 0; slot < slots; ++slot)
 #pragma unroll
             for (int h = 0; h < NH; ++h)
-              tma_load_3d(smem + slot * C::kStage + h * C::kHalf, &tmQ, &bars[C::Q_FULL], h * 64, f.kvh * group, f.tok + slot * per_slot);
+              tma_load_3d(smem + slot * C::kQ + h * C::kQHalf, &tmQ, &bars[C::Q_FULL], h * 64, f.kvh * group, f.tok + slot * per_slot);
         }
         __syncwarp();
         ++n_item;
@@ -411,90 +460,116 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
     // copies still in flight must have landed before the CTA gives its shared memory back
     for (uint32_t k = ring > NST ? ring - NST : 0; k < ring; ++k) (void)mbar_wait(&bars[C::FULL + k % NST], k / NST & 1);
-  } else if (warp == kMmaWarp) {
+  } else if (warp >= kMmaWarp) {
     // ------------------------------------------------------------------ products (the warp walks, an elected lane issues)
     const uint32_t idesc_s = umma_idesc_bf16(128, kTile), idesc_o = umma_idesc_bf16(128, HD) | kIdescBMnMajor;
     const uint64_t q_desc = umma_desc_k_sw128(sb), k_desc = umma_desc_k_sw128(sb + C::kRing);
     const uint64_t v_desc = umma_desc_mn_sw128(sb + C::kRing, C::kHalf, 1024);
-    uint32_t ring = 0, n_item = 0, done[2] = {0, 0};           // second products issued, of each slot
+    // A warp per slot: what it spends is not the products but the waits in front of them (some 100 cycles each, also where the barrier has
+    // long been passed), and one warp for both took 2600 cycles for a tile of both.
+    const int slot = warp - kMmaWarp;
+    const uint32_t t_s = tmem + slot * 256, t_o = t_s + 2 * kTile;
+    uint32_t ring = 0, n_item = 0, n_tile = 0;   // (tiles of this slot in front of this item)
+    int n_cleared = 0;
     bool ok = true;
     for (;;) {
       if (!passed(C::Q_FULL, n_item & 1)) { ok = false; break; }
-      const int nodes = piece_s->nodes, pages = piece_s->pages, two = piece_s->two;
+      const int nodes = piece_s->nodes, pages = piece_s->pages, two = piece_s->two, page0 = piece_s->page0;
+      const int care_from = min(piece_s->len - piece_s->all, min(piece_s->len, (page0 + pages) * kPage));
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[C::READ]);
       if (nodes == 0) break;
       const int tiles = (pages + kTilePages - 1) / kTilePages;
-      const int n0 = two ? tiles : (tiles + 1) / 2, n1 = two ? tiles : tiles / 2;
-      int left = n0 + n1;                        // scores to issue
-      // S(slot) of its i-th tile goes over the weights of the one before, which that one's second product reads: it must have ended
-      auto scores = [&](int slot, int i) {
-        const int tile = two ? i : 2 * i + slot;
-        const uint32_t k = ring + k_at(tile);
-        if (done[slot] > 0 && !passed(C::PV_DONE + slot, (done[slot] - 1) & 1)) return false;
+      const int n = two ? tiles : (tiles + 1 - slot) / 2;
+      const uint64_t qd = q_desc + static_cast<uint64_t>((two ? slot : 0) * (C::kQ >> 4));
+      // The other slot's tiles pass by: both warps wait for all of the ring's places in their order, since a parity tells only neighbouring
+      // phases apart.
+      auto pass_by = [&](uint32_t place) {
+        if (!passed(C::FULL + place % NST, place / NST & 1)) return false;
+        if (lane == 0) mbar_arrive(&bars[C::EMPTY + place % NST]);
+        return true;
+      };
+      auto other_keys = [&](int i) {
+        const int tile = 2 * i + (slot ^ 1);
+        return two || tile >= tiles || pass_by(ring + k_at(tile));
+      };
+      auto other_values = [&](int i) {
+        const int tile = 2 * i + (slot ^ 1);
+        return two || tile >= tiles || pass_by(ring + v_at(tile, tiles));
+      };
+      // S(i) goes over the weights of the slot's tile before the last one, which that one's second product reads: it must have ended
+      auto scores = [&](int i) {
+        const uint32_t k = ring + k_at(two ? i : 2 * i + slot), g = n_tile + i, at = slot * 2 + (g & 1);
+        if (g >= 2 && !passed(C::PV_DONE + at, ((g >> 1) - 1) & 1)) return false;
         if (!passed(C::FULL + k % NST, k / NST & 1)) return false;
         tc_fence_after();
         if (elect_one()) {
-          const uint64_t qd = q_desc + static_cast<uint64_t>((two ? slot : 0) * (C::kStage >> 4)), kd = k_desc + static_cast<uint64_t>(k % NST * (C::kStage >> 4));
+          const uint64_t kd = k_desc + static_cast<uint64_t>(k % NST * (C::kStage >> 4));
 #pragma unroll
           for (int h = 0; h < NH; ++h)
 #pragma unroll
             for (int s = 0; s < 4; ++s)
-              umma_bf16_ss(tmem + slot * 256, qd + ((h * C::kHalf + s * 32) >> 4), kd + ((h * C::kHalf + s * 32) >> 4), idesc_s, (h | s) ? 1u : 0u);
-          umma_commit(&bars[C::S_FULL + slot]);
-          if (!two || slot == 1) umma_commit(&bars[C::EMPTY + k % NST]);
-          if (left == 1) umma_commit(&bars[C::Q_EMPTY]);
+              umma_bf16_ss(t_s + (g & 1) * kTile, qd + ((h * C::kQHalf + s * 32) >> 4), kd + ((h * C::kHalf + s * 32) >> 4), idesc_s, (h | s) ? 1u : 0u);
+          umma_commit(&bars[C::S_FULL + at]);
+          umma_commit(&bars[C::EMPTY + k % NST]);
+          if (i == n - 1) umma_commit(&bars[C::Q_EMPTY]);
         }
         __syncwarp();
-        --left;
         return true;
       };
-      auto sums = [&](int slot, int i) {
+      auto sums = [&](int i) {
         const int tile = two ? i : 2 * i + slot;
-        const uint32_t v = ring + v_at(tile, tiles);
+        const uint32_t v = ring + v_at(tile, tiles), g = n_tile + i, at = slot * 2 + (g & 1);
         // the item before must have been read out of both slots' sums
         if (i == 0 && !passed(C::O_FREE, (n_item & 1) ^ 1)) return false;
-        if (!passed(C::FULL + v % NST, v / NST & 1) || !passed(C::P_FULL + slot, done[slot] & 1)) return false;
+        if (!passed(C::FULL + v % NST, v / NST & 1)) return false;
+        if (page0 * kPage + (tile + 1) * kTile > care_from) {    // the values are gone through first, by slot 0 for both if both have them
+          if (!two || slot == 0) {
+            if (lane == 0) mbar_arrive(&bars[C::CARE + slot]);
+          } else if (!reached(cleared, n_cleared += 4, abort_flag)) {
+            return false;
+          }
+        }
+        if (!passed(C::P_FULL + at, g >> 1 & 1)) return false;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t vd = v_desc + static_cast<uint64_t>(v % NST * (C::kStage >> 4));
 #pragma unroll
           for (int s = 0; s < kTile / 16; ++s)
-            umma_bf16_ts(tmem + slot * 256 + kTile, tmem + slot * 256 + s * 8, vd + ((s * 2048) >> 4), idesc_o, (i | s) ? 1u : 0u);
-          umma_commit(&bars[C::PV_DONE + slot]);
-          if (!two || slot == 1) umma_commit(&bars[C::EMPTY + v % NST]);
+            umma_bf16_ts(t_o, t_s + (g & 1) * kTile + s * 8, vd + ((s * 2048) >> 4), idesc_o, (i | s) ? 1u : 0u);
+          umma_commit(&bars[C::PV_DONE + at]);
+          umma_commit(&bars[C::EMPTY + v % NST]);
         }
         __syncwarp();
-        ++done[slot];
         return true;
       };
-      if (tiles == 0) {                          // (phases are not skipped: a parity stands for every other one)
+      if (n == 0) {                              // (phases are not skipped: a parity stands for every other one)
+        if (lane == 0) mbar_arrive(&bars[C::Q_EMPTY]);
         ok = passed(C::O_FREE, (n_item & 1) ^ 1);
-        if (elect_one()) mbar_arrive(&bars[C::Q_EMPTY]);
-        __syncwarp();
+      } else {
+        ok = scores(0);
       }
-      ok = ok && (n0 == 0 || scores(0, 0)) && (n1 == 0 || scores(1, 0));
-      for (int i = 0; ok && i < n0; ++i) {
-        // (with two row blocks slot 0 has made the tile's values fit to be multiplied before slot 1 comes to them)
-        ok = sums(0, i) && (i + 1 >= n0 || scores(0, i + 1)) && (i >= n1 || sums(1, i)) && (i + 1 >= n1 || scores(1, i + 1));
-      }
+      ok = ok && other_keys(0);
+      for (int i = 0; ok && i < (two ? tiles : (tiles + 1) / 2); ++i)
+        ok = (i + 1 >= n || scores(i + 1)) && other_keys(i + 1) && (i >= n || sums(i)) && other_values(i);
       if (!ok) break;
       ring += 2 * tiles;
+      n_tile += n;
       ++n_item;
     }
     if (!ok) {                                   // products in flight get a bounded chance to end before their memory is given back
       fail(NF_ST_TIMEOUT_SMEM_FULL);
-      if (elect_one()) umma_commit(&bars[C::LAST]);
+      if (elect_one()) umma_commit(&bars[C::LAST + slot]);
       __syncwarp();
-      (void)mbar_wait(&bars[C::LAST], 0);
+      (void)mbar_wait(&bars[C::LAST + slot], 0);
     }
   } else {
     // ------------------------------------------------------------------ softmax (a thread per query row)
     const int slot = warp >> 2, row = (warp & 3) * 32 + lane;
-    const uint32_t t_s = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + slot * 256, t_o = t_s + kTile;
+    const uint32_t t_slot = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + slot * 256, t_o = t_slot + 2 * kTile;
     const int in_slot = row / group, hh = row - in_slot * group;
     const float scale = p.sm_scale * kLog2e;
-    uint32_t ring = 0, n_item = 0, n_done = 0, n_merge = 0;
+    uint32_t ring = 0, n_item = 0, n_done = 0, n_merge = 0, n_care = 0;
     // States that will not be formed are NaN, and not what an earlier call left in the workspace.
 #pragma unroll
     for (int k = 0; k < 2; ++k) __stcg(ws.ml + (2 * blockIdx.x + k) * 256 + slot * 128 + row, make_float2(0.f, __uint_as_float(0x7fc00000u)));
@@ -518,28 +593,31 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int tile = f.two ? i : 2 * i + slot;
         const int at = f.page0 * kPage + tile * kTile;                   // the tile's first token
         const bool care = at + kTile > min(ctx, end);
-        uint32_t bits[4] = {~0u, ~0u, ~0u, ~0u};
+        uint32_t bits[2] = {~0u, ~0u};
         if (care) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          for (int k = 0; k < 2; ++k) {
             const int left = end - (at + k * 32);
             bits[k] = on ? seen_bits(tree, 2 * p.words, node, f.all, at + k * 32 - ctx) & (left >= 32 ? ~0u : left > 0 ? (1u << left) - 1u : 0u) : 0u;
           }
         }
-        if (!passed(C::S_FULL + slot, n_done & 1)) { ok = false; break; }
+        const int b = slot * 2 + (n_done & 1);
+        const uint32_t t_s = t_slot + (n_done & 1) * kTile;
+        if (!passed(C::S_FULL + b, n_done >> 1 & 1)) { ok = false; break; }
         if (care && (!f.two || slot == 0)) {
-          // ---- values of the tile: a thread per token ----
-          // (Behind the wait for the scores: a parity tells only neighbouring phases apart, and where the scores have been issued, what
-          // was in the ring's place before these values has come and been used.)
+          // ---- values of the tile: two threads per token ----
+          // (by way of the warp that waits for all of the ring's places in their order)
           const uint32_t v = ring + v_at(tile, tiles);
-          if (!passed(C::FULL + v % NST, v / NST & 1)) { ok = false; break; }
-          const int token = at + row;
+          if (!passed(C::CARE + slot, n_care & 1) || !passed(C::FULL + v % NST, v / NST & 1)) { ok = false; break; }
+          ++n_care;
+          const int in_tile = row & (kTile - 1), token = at + in_tile;
           if (token >= ctx) {
-            const uint32_t v_row = sb + C::kRing + v % NST * C::kStage + row * 128;
+            const uint32_t v_row = sb + C::kRing + v % NST * C::kStage + in_tile * 128;
             bool odd = false;
 #pragma unroll
-            for (int c = 0; c < HD / 8; ++c) {
-              const uint32_t a = v_row + (c >> 3) * C::kHalf + (((c & 7) ^ (row & 7)) << 4);
+            for (int k = 0; k < HD / 16; ++k) {
+              const int c = (row / kTile) * (HD / 16) + k;
+              const uint32_t a = v_row + (c >> 3) * C::kHalf + (((c & 7) ^ (in_tile & 7)) << 4);
               if (token >= end) {
                 st_shared_v4(a, make_uint4(0u, 0u, 0u, 0u));
               } else {
@@ -555,16 +633,20 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
           fence_proxy_async_smem();
           __syncwarp();
+          if (f.two && lane == 0) {
+            __threadfence_block();
+            atomicAdd(cleared, 1);
+          }
         }
         if (warp_on) {
           tc_fence_after();
-          uint32_t x[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(t_s + c * 32, x[c]);
+          uint32_t x[2][32];
+          tmem_ld_32x32b_x32(t_s, x[0]);
+          tmem_ld_32x32b_x32(t_s + 32, x[1]);
           tmem_ld_wait();
           if (care) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 2; ++c) {
               sees = sees || bits[c] != 0u;
 #pragma unroll
               for (int j = 0; j < 32; ++j)
@@ -575,16 +657,16 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
           float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) mq[c] = max3(mq[c], __uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1]));
+            for (int j = 0; j < 32; j += 2) mq[2 * c + (j >> 1 & 1)] = max3(mq[2 * c + (j >> 1 & 1)], __uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1]));
           const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * scale;
           const bool grow = mx > ref + kGap || (ref == -INFINITY && mx > -INFINITY);
           if (i == 0) {
             ref = mx;
           } else if (__any_sync(0xffffffffu, grow)) {
-            // The second product before this tile's is the last one issued, and it has ended: the tile's scores were issued after that.
-            if (!passed(C::PV_DONE + slot, (n_done - 1) & 1)) { ok = false; break; }
+            // Sums may be touched between two products only: that of the tile before is the last one issued (this tile's needs its weights)
+            if (!passed(C::PV_DONE + slot * 2 + ((n_done - 1) & 1), (n_done - 1) >> 1 & 1)) { ok = false; break; }
             tc_fence_after();
             const float alpha = grow ? (ref == -INFINITY ? 0.f : fast_exp2(ref - mx)) : 1.f;
 #pragma unroll 1
@@ -607,30 +689,27 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           const float ms = ref == -INFINITY ? 0.f : ref;
           const f32x2 scale2 = pair(scale, scale), ms2 = pair(-ms, -ms);
           f32x2 rs[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+          uint32_t pk[32];                       // column j: tokens 2j, 2j + 1
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t pk[32];                     // column j: tokens 2j, 2j + 1
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              const float2 y = halves(fma2(pair(__uint_as_float(x[2 * c + (j >> 4)][2 * (j & 15)]), __uint_as_float(x[2 * c + (j >> 4)][2 * (j & 15) + 1])), scale2, ms2));
-              const float e0 = fast_exp2(y.x), e1 = fast_exp2(y.y);
-              rs[j & 1] = add2(rs[j & 1], pair(e0, e1));
-              pk[j] = pack_bf16x2(e0, e1);
-            }
-            tmem_st_32x32b_x32(t_s + c * 32, pk);
+          for (int j = 0; j < 32; ++j) {
+            const float2 y = halves(fma2(pair(__uint_as_float(x[j >> 4][2 * (j & 15)]), __uint_as_float(x[j >> 4][2 * (j & 15) + 1])), scale2, ms2));
+            const float e0 = fast_exp2(y.x), e1 = fast_exp2(y.y);
+            rs[j & 1] = add2(rs[j & 1], pair(e0, e1));
+            pk[j] = pack_bf16x2(e0, e1);
           }
+          tmem_st_32x32b_x32(t_s, pk);
           const float2 t = halves(add2(rs[0], rs[1]));
           l += t.x + t.y;
           tmem_st_wait();
           tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars[C::P_FULL + slot]);
+        if (lane == 0) mbar_arrive(&bars[C::P_FULL + b]);
         ++n_done;
       }
       if (!ok) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
       ring += 2 * tiles;
-      if (n_mine > 0 && !passed(C::PV_DONE + slot, (n_done - 1) & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
+      if (n_mine > 0 && !passed(C::PV_DONE + slot * 2 + ((n_done - 1) & 1), (n_done - 1) >> 1 & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
       tc_fence_after();
       if (sees && l == 0.f) l = __uint_as_float(0x7fc00000u);            // all that it sees has a score of minus infinity
       // ---- sums of the row: columns [from, to), a0 times those of slot 0 and a1 times those of slot 1 ----
@@ -665,35 +744,72 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const bool odd = odd_item[n_item & 1] == static_cast<int>(n_item);
       // a row without weights: zeros, or NaN (l) where it sees something
       const float by = f.to < 0 ? (l > 0.f ? 1.f / l : l) : 1.f;
-      const long long out_row = static_cast<long long>(f.tok + node_in) * p.ld_out + (f.kvh * group + hh) * HD;
-      const long long o_row = (static_cast<long long>(f.to) * 256 + (f.two ? slot * 128 : 0) + row) * HD;
+      // (in steps of eight elements: row strides are multiples of that)
+      const int out_row = static_cast<int>((static_cast<long long>(f.tok + node_in) * p.ld_out + (f.kvh * group + hh) * HD) >> 3);
       if (warp_on) {
         const bool use_mine = a_mine != 0.f, use_other = a_other != 0.f;
+        const int rows_on = min(per_slot, f.nodes - (f.two ? slot * per_slot : 0)) * group - (warp & 3) * 32;   // of this warp
+        float* o_rows = ws.o + ((static_cast<long long>(f.to) * 256 + (f.two ? slot * 128 : 0) + (warp & 3) * 32) * HD);
+        auto columns = [&](int c, float (&o)[32]) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            uint32_t a[16], other[16];
+            tmem_ld_32x32b_x16n(t_o + c + 16 * k, a);
+            if (!f.two) tmem_ld_32x32b_x16n((t_o ^ 256u) + c + 16 * k, other);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              o[16 * k + j] = (use_mine ? a_mine * __uint_as_float(a[j]) : 0.f) + (use_other ? a_other * __uint_as_float(other[j]) : 0.f);
+          }
+          if (odd && on) restore_odd<HD>(p, f, tree, node, max(f.page0 * kPage, ctx), end, c, o);
+        };
+        // A thread has its own row; eight lanes exchange theirs, so that a store is of 128 bytes of four rows (each thread its own: 2.2 us
+        // longer, the stores' 32 lines at a time).
+        if (f.to < 0) {
+          auto packed = [&](const float (&o)[32], uint4* v) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              v[k] = make_uint4(pack_bf16x2(o[8 * k] * by, o[8 * k + 1] * by), pack_bf16x2(o[8 * k + 2] * by, o[8 * k + 3] * by),
+                                pack_bf16x2(o[8 * k + 4] * by, o[8 * k + 5] * by), pack_bf16x2(o[8 * k + 6] * by, o[8 * k + 7] * by));
+          };
+          uint4* out = static_cast<uint4*>(p.out);
 #pragma unroll 1
-        for (int c = from; c < to; c += 16) {
-          uint32_t a[16], b[16];
-          float o[16];
-          tmem_ld_32x32b_x16n(t_o + c, a);
-          if (!f.two) tmem_ld_32x32b_x16n((t_o ^ 256u) + c, b);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) o[j] = (use_mine ? a_mine * __uint_as_float(a[j]) : 0.f) + (use_other ? a_other * __uint_as_float(b[j]) : 0.f);
-          if (on) {
-            if (odd) restore_odd<HD>(p, f, tree, node, max(f.page0 * kPage, ctx), end, c, o);
-            if (f.to < 0) {
-              __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + out_row + c;
-#pragma unroll
-              for (int k = 0; k < 2; ++k)
-                *reinterpret_cast<uint4*>(dst + k * 8) =
-                    make_uint4(pack_bf16x2(o[8 * k] * by, o[8 * k + 1] * by), pack_bf16x2(o[8 * k + 2] * by, o[8 * k + 3] * by),
-                               pack_bf16x2(o[8 * k + 4] * by, o[8 * k + 5] * by), pack_bf16x2(o[8 * k + 6] * by, o[8 * k + 7] * by));
+          for (int c = from; c < to; c += 64) {
+            uint4 v[8];
+            float o[32];
+            columns(c, o);
+            packed(o, v);
+            const bool wide = c + 32 < to;
+            if (wide) {
+              columns(c + 32, o);
+              packed(o, v + 4);
+              exchange<8>(v);
             } else {
+              exchange<4>(v);
+            }
+            const int n = wide ? 8 : 4, j = lane & (n - 1), r0 = lane - j;
 #pragma unroll
-              for (int k = 0; k < 4; ++k)
-                __stcg(reinterpret_cast<float4*>(ws.o + o_row + c) + k, make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
+            for (int k = 0; k < 8; ++k) {
+              if (k >= n) break;
+              const int at = __shfl_sync(0xffffffffu, out_row, r0 + k);
+              if (r0 + k < rows_on) out[static_cast<long long>(static_cast<unsigned int>(at)) + c / 8 + j] = v[k];
             }
           }
-          __syncwarp();
+        } else {
+#pragma unroll 1
+          for (int c = from; c < to; c += 32) {
+            uint4 v[8];
+            float o[32];
+            columns(c, o);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              v[k] = make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
+            exchange<8>(v);
+            const int j = lane & 7, r0 = lane - j;
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              if (r0 + k < rows_on) __stcg(reinterpret_cast<uint4*>(o_rows + (r0 + k) * HD + c) + j, v[k]);
+          }
         }
         if (on && f.to >= 0 && (f.two || slot == 0)) __stcg(ws.ml + static_cast<long long>(f.to) * 256 + (f.two ? slot * 128 : 0) + row, make_float2(ref, l));
       }
@@ -712,67 +828,101 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
 }
 
-// Rows of items that were cut: a warp per row, lanes over its pieces for the weights and over head_dim for the sums.
-constexpr int kJoinWarps = 8, kJoinParts = 8;
+// Rows of items that were cut, a warp each: lanes over its pieces for the weights and over head_dim for the sums. Every CTA works out
+// from all records which rows there are.
+constexpr int kJoinWarps = 8, kJoinPerSm = 4, kMostCtas = 256;
 template <int HD>
 __global__ void __launch_bounds__(kJoinWarps * 32) attn_tree_join_kernel(nfk_attn_tree_params p, Workspace ws, int ctas) {
-  constexpr int V = HD / 32;
+  constexpr int V = HD / 32, AHEAD = 8;
+  __shared__ int4 record_s[kMostCtas];
+  __shared__ int rows_s[kMostCtas + 1], warp_s[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.q_heads / p.kv_heads, per_slot = 128 / group;
   await_previous();
   let_next_start();
-  for (int work = blockIdx.x; work < ctas * kJoinParts; work += gridDim.x) {
-    const int c = work / kJoinParts, part = work - c * kJoinParts;
-    const int4 rec = __ldcg(reinterpret_cast<const int4*>(ws.records + c));
-    const int pieces = rec.x, tok = rec.y, nodes = rec.z, kvh = rec.w;
-    for (int b = part * kJoinWarps + warp; pieces > 0 && b < nodes * group; b += kJoinParts * kJoinWarps) {
-      const int node = b / group, hh = b - node * group, slot = node / per_slot;
-      const int row = slot * 128 + (node - slot * per_slot) * group + hh;
-      auto number = [&](int k) { return static_cast<long long>(k == 0 ? 2 * c + 1 : 2 * (c + k)) * 256 + row; };
-      float top = -INFINITY, odd = 0.f;
-      for (int k = lane; k < pieces; k += 32) {
-        const float2 ml = __ldcg(ws.ml + number(k));
-        top = fmaxf(top, ml.x);
-        if (ml.y != ml.y) odd = ml.y;
+  // ---- rows in front of each record ----
+  int4 rec = make_int4(0, 0, 0, 0);
+  if (static_cast<int>(threadIdx.x) < ctas) rec = __ldcg(reinterpret_cast<const int4*>(ws.records + threadIdx.x));
+  const int mine = rec.x > 0 ? rec.z * group : 0;
+  int sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, sum, o);
+    if (lane >= o) sum += v;
+  }
+  if (lane == 31) warp_s[warp] = sum;
+  __syncthreads();
+  int before = sum - mine, total = 0;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    if (w < warp) before += warp_s[w];
+    total += warp_s[w];
+  }
+  record_s[threadIdx.x] = rec;
+  rows_s[threadIdx.x] = before;
+  __syncthreads();
+  for (int work = blockIdx.x * kJoinWarps + warp; work < total; work += gridDim.x * kJoinWarps) {
+    int c = 0;                                   // the last record with rows_s <= work
+#pragma unroll
+    for (int step = kMostCtas / 2; step > 0; step >>= 1)
+      if (rows_s[c + step] <= work) c += step;
+    const int pieces = record_s[c].x, tok = record_s[c].y, kvh = record_s[c].w;
+    const int b = work - rows_s[c], node = b / group, hh = b - node * group, slot = node / per_slot;
+    const int row = slot * 128 + (node - slot * per_slot) * group + hh;
+    auto number = [&](int k) { return static_cast<long long>(k == 0 ? 2 * c + 1 : 2 * (c + k)) * 256 + row; };
+    auto load = [&](int k, float (&x)[V]) {
+      const float* from = ws.o + number(k) * HD + lane * V;
+      if constexpr (V == 4) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(from));
+        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
+      } else {
+        const float2 y = __ldcg(reinterpret_cast<const float2*>(from));
+        x[0] = y.x; x[1] = y.y;
       }
+    };
+    float x[AHEAD][V];
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      float sum = 0.f, acc[V];
-#pragma unroll
-      for (int v = 0; v < V; ++v) acc[v] = 0.f;
-      for (int k0 = 0; k0 < pieces; k0 += 32) {
-        float w = 0.f, l = 0.f;
-        if (k0 + lane < pieces) {
-          const float2 ml = __ldcg(ws.ml + number(k0 + lane));
-          w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-          l = ml.y;
-        }
-        sum += w != 0.f ? w * l : 0.f;
-        const int here = min(32, pieces - k0);
-#pragma unroll 4
-        for (int k = 0; k < here; ++k) {
-          const float by = __shfl_sync(0xffffffffu, w, k);
-          const float* from = ws.o + number(k0 + k) * HD + lane * V;
-          float x[V];
-          if (V == 4) {
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(from));
-            x[0] = y.x; x[1] = y.y; x[V - 2] = y.z; x[V - 1] = y.w;
-          } else {
-            const float2 y = __ldcg(reinterpret_cast<const float2*>(from));
-            x[0] = y.x; x[1] = y.y;
-          }
-#pragma unroll
-          for (int v = 0; v < V; ++v) acc[v] += by != 0.f ? by * x[v] : 0.f;
-        }
-      }
-      sum = warp_sum(sum);
-      // without weights: zeros, or NaN where the row sees something
-      odd = top == -INFINITY ? warp_sum(odd) : 0.f;
-      const float by = sum > 0.f ? 1.f / sum : sum + odd;
-      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<long long>(tok + node) * p.ld_out + (kvh * group + hh) * HD + lane * V);
-#pragma unroll
-      for (int v = 0; v < V; v += 2) dst[v / 2] = pack_bf16x2(acc[v] * by, acc[v + 1] * by);
+    for (int k = 0; k < AHEAD; ++k)
+      if (k < pieces) load(k, x[k]);
+    float2 ml = make_float2(-INFINITY, 0.f);     // the first 32 pieces'
+    if (lane < pieces) ml = __ldcg(ws.ml + number(lane));
+    float top = ml.x, odd = ml.y != ml.y ? ml.y : 0.f;
+    for (int k = 32 + lane; k < pieces; k += 32) {
+      const float2 far = __ldcg(ws.ml + number(k));
+      top = fmaxf(top, far.x);
+      if (far.y != far.y) odd = far.y;
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float total_l = 0.f, acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = 0.f;
+    for (int k0 = 0; k0 < pieces; k0 += 32) {
+      if (k0 > 0) ml = k0 + lane < pieces ? __ldcg(ws.ml + number(k0 + lane)) : make_float2(-INFINITY, 0.f);
+      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+      total_l += w != 0.f ? w * ml.y : 0.f;
+      const int here = min(32, pieces - k0);
+      for (int k1 = 0; k1 < here; k1 += AHEAD) {
+        if (k0 + k1 > 0)
+#pragma unroll
+          for (int k = 0; k < AHEAD; ++k)
+            if (k1 + k < here) load(k0 + k1 + k, x[k]);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const float by = __shfl_sync(0xffffffffu, w, (k1 + k) & 31);
+          if (k1 + k >= here) break;
+#pragma unroll
+          for (int v = 0; v < V; ++v) acc[v] += by != 0.f ? by * x[k][v] : 0.f;
+        }
+      }
+    }
+    total_l = warp_sum(total_l);
+    // without weights: zeros, or NaN where the row sees something
+    odd = top == -INFINITY ? warp_sum(odd) : 0.f;
+    const float by = total_l > 0.f ? 1.f / total_l : total_l + odd;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<long long>(tok + node) * p.ld_out + (kvh * group + hh) * HD + lane * V);
+#pragma unroll
+    for (int v = 0; v < V; v += 2) dst[v / 2] = pack_bf16x2(acc[v] * by, acc[v + 1] * by);
   }
 }
 
@@ -810,8 +960,8 @@ int launch(const nfk_attn_tree_params& p, cudaStream_t stream) {
   if (rc != NF_OK) return rc;
   Workspace ws;
   workspace_bytes(HD, &ws, p.workspace);
-  const int sms = device_sm_count(), ctas = p.num_ctas > 0 && p.num_ctas < sms ? p.num_ctas : sms;
-  int joins = ctas * kJoinParts;
+  const int sms = device_sm_count(), most = sms < kMostCtas ? sms : kMostCtas, ctas = p.num_ctas > 0 && p.num_ctas < most ? p.num_ctas : most;
+  int joins = sms * kJoinPerSm;
   if (p.num_ctas > 0 && p.num_ctas < joins) joins = p.num_ctas;
   if (launch_kernel(early_first(p.early_start), attn_tree_kernel<HD>, ctas, kThreads, C::kBytes, stream, 1, tm_q, tm_kv, p, ws) != cudaSuccess ||
       launch_kernel(early_further(p.early_start), attn_tree_join_kernel<HD>, joins, kJoinWarps * 32, 0, stream, 1, p, ws, ctas) != cudaSuccess) {
