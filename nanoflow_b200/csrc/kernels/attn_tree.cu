@@ -34,11 +34,9 @@ namespace {
 
 constexpr int kTile = 64;             // cached tokens per tile
 constexpr int kTilePages = kTile / kPage;
-constexpr int kThreads = 352;         // warps 0-3 slot 0, 4-7 slot 1, 8 copies, 9 and 10 products of either slot
-constexpr int kLoadWarp = 8, kMmaWarp = 9;
 constexpr float kGap = 8.f;           // log2 of how far a row's maximum may outgrow its reference
 // What an item's beginning and end cost, in pages: where the work is cut, the ends count too.
-constexpr int kLead = 8;
+constexpr int kLead = 16;
 // Pages that a CTA takes at least, so that the states of short requests do not outweigh their pages.
 constexpr int kLeast = 8;
 
@@ -55,21 +53,24 @@ struct Piece {
   int to;            // piece number, -1: the whole item
   int two;           // blocks of more than 128 rows: each slot its own
 };
-template <int HD>
+template <int HD, int SLOTS>
 struct Cfg {
+  // warps: four of softmax a slot, one that copies keys, one of products a slot, one that copies values
+  static constexpr int kSoftWarps = 4 * SLOTS, kKeyWarp = kSoftWarps, kMmaWarp = kKeyWarp + 1, kValueWarp = kMmaWarp + SLOTS, kThreads = 32 * (kValueWarp + 1);
   static constexpr int NH = HD / 64;
   static constexpr int kQHalf = 128 * 128, kHalf = kTile * 128;        // [128 rows or 64 tokens][64 elements]
   static constexpr int kQ = NH * kQHalf, kStage = NH * kHalf;  // a slot's queries; a tile of keys or of values
-  static constexpr int kStages = HD == 128 ? 8 : 16;           // (a power of two)
-  static constexpr int kRing = 2 * kQ;                         // (queries of both slots in front)
-  static constexpr int kMl = kRing + kStages * kStage;         // [2 slots][128] float2
-  static constexpr int kBars = kMl + 2 * 128 * 8;
+  static constexpr int kStages = (HD == 128 ? 2 : 4) * SLOTS;  // tiles of keys, and as many of values (a power of two)
+  static constexpr int kRing = SLOTS * kQ;
+  static constexpr int kOut = kRing + 2 * kStages * kStage;    // of each softmax warp [32 rows][32 columns] fp32: rows on their way out
+  static constexpr int kMl = kOut + kSoftWarps * 4096;         // [2 slots][128] float2; before that, where the CTA begins
+  static constexpr int kBars = kMl + (SLOTS == 2 ? 2 * 128 * 8 : 256);
   static constexpr int kBytes = kBars + 640;
   enum Bar : int {
-    FULL = 0, EMPTY = FULL + kStages, Q_FULL = EMPTY + kStages, Q_EMPTY, READ, O_FREE, LAST, CARE = LAST + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 4,
-    PV_DONE = P_FULL + 4, MERGE = PV_DONE + 4, kNum = MERGE + 4   // (S_FULL to PV_DONE: two to a slot, which its tiles use in turn)
+    K_FULL = 0, K_EMPTY = K_FULL + kStages, V_FULL = K_EMPTY + kStages, V_EMPTY = V_FULL + kStages, Q_FULL = V_EMPTY + kStages, Q_EMPTY, READ, O_FREE, LAST,
+    CARE = LAST + 2, S_FULL = CARE + 2, P_FULL = S_FULL + 4, PV_DONE = P_FULL + 4, MERGE = PV_DONE + 4, kNum = MERGE + 4   // (S_FULL to PV_DONE: two to a slot, which its tiles use in turn)
   };
-  static_assert(kNum * 8 + 20 + sizeof(Piece) <= 640 && kBytes <= 227 * 1024, "shared memory");
+  static_assert(kNum * 8 + 20 + sizeof(Piece) <= 640 && SLOTS * kBytes <= SLOTS * 227 * 1024 && (3 - SLOTS) * (kBytes + 1024) <= 228 * 1024, "shared memory");
 };
 
 // What a CTA leaves for the kernel that joins states: the item that begins with it and goes on behind it, if there is one.
@@ -79,18 +80,23 @@ struct Record {
 
 struct Workspace {
   Record* records;   // [CTAs]
-  float2* ml;        // [2 CTAs][256]: reference (of exponents to base 2) and sum
-  float* o;          // [2 CTAs][256][head_dim], not divided by the sum
+  float2* ml;        // [2 CTAs][rows of a block]: reference (of exponents to base 2) and sum
+  float* o;          // [2 CTAs][rows of a block][head_dim], not divided by the sum
 };
+// CTAs at most: two to an SM.
+int most_ctas() {
+  const int n = 2 * device_sm_count();
+  return n < 512 ? n : 512;
+}
 long long workspace_bytes(int head_dim, Workspace* w = nullptr, void* base = nullptr) {
-  const long long n = device_sm_count(), records = (n * static_cast<long long>(sizeof(Record)) + 255) / 256 * 256, ml = 2 * n * 256 * 8;
+  const long long n = most_ctas(), records = (n * static_cast<long long>(sizeof(Record)) + 255) / 256 * 256, ml = 2 * n * 128 * 8;
   if (w != nullptr) {
     char* at = static_cast<char*>(base);
     w->records = reinterpret_cast<Record*>(at);
     w->ml = reinterpret_cast<float2*>(at + records);
     w->o = reinterpret_cast<float*>(at + records + ml);
   }
-  return records + ml + 2 * n * 256 * head_dim * 4;
+  return records + ml + 2 * n * 128 * head_dim * 4;
 }
 
 // A request as the lists have it. Lists that are none: no query tokens, or no cached ones.
@@ -158,6 +164,18 @@ __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
 __device__ __forceinline__ void st_shared_v4(uint32_t addr, const uint4& v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
 __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* tm, uint64_t* bar, int x, int y, int z) {
   asm volatile(
       "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
@@ -173,6 +191,9 @@ __device__ __forceinline__ bool mbar_test(uint32_t bar, uint32_t parity) {
       : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
+__device__ __noinline__ bool wait_for(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, wait_or_abort(bar, parity, abort_flag)) != 0;
+}
 // bf16 pairs with an infinity or NaN in them
 __device__ __forceinline__ bool odd_pair(uint32_t w) { return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u; }
 __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
@@ -181,26 +202,6 @@ __device__ __forceinline__ uint32_t without_odd(uint32_t w) {
   return w;
 }
 
-// Of N x N pieces, N lanes with a row of them each: lane j gets piece j of all N rows.
-template <int N>
-__device__ __forceinline__ void exchange(uint4* v) {
-  const int lane = threadIdx.x & 31;
-#pragma unroll
-  for (int s = N / 2; s > 0; s >>= 1)
-#pragma unroll
-    for (int k = 0; k < N; ++k) {
-      if ((k & s) != 0) continue;
-      const bool up = (lane & s) != 0;
-      const uint4 give = up ? v[k] : v[k | s];
-      uint4 get;
-      get.x = __shfl_xor_sync(0xffffffffu, give.x, s);
-      get.y = __shfl_xor_sync(0xffffffffu, give.y, s);
-      get.z = __shfl_xor_sync(0xffffffffu, give.z, s);
-      get.w = __shfl_xor_sync(0xffffffffu, give.w, s);
-      if (up) v[k] = get;
-      else v[k | s] = get;
-    }
-}
 // Waits, for a while, until *count is `goal`; for a whole warp.
 __device__ __forceinline__ bool reached(volatile int* count, int goal, volatile int* abort_flag) {
   bool ok = false;
@@ -214,29 +215,31 @@ __device__ __forceinline__ long long divide(long long a, long long b) {
   return a / b;
 }
 
-// Infinities and NaN of the drafted tokens [from, end) that the row sees, in 32 columns: as terms of its sums they are what they are,
-// whatever their weights. (Only where there are some.)
+// Infinities and NaN of the drafted tokens [first, end) that the row sees, in its columns [from, to): as terms of its sums they are what
+// they are, whatever their weights, and are added to the row where it has been written. (Only where there are some.)
 template <int HD>
-__device__ __forceinline__ void restore_odd(const nfk_attn_tree_params& p, const Piece& f, const uint32_t* tree, int node, int from, int end, int c,
-                                         float (&o)[32]) {
-  for (int t = from; t < end; ++t) {
-    if ((seen_bits(tree, 2 * p.words, node, f.all, t - (f.len - f.all)) & 1u) == 0u) continue;
-    int page = p.kv_indices[f.list + t / kPage];
+__device__ __noinline__ void restore_odd(const nfk_attn_tree_params& p, const int* list, int kvh, const uint32_t* tree, int node, int all, int ctx, int first, int end,
+                                         int from, int to, float* sums, __nv_bfloat16* out) {
+  for (int t = first; t < end; ++t) {
+    if ((seen_bits(tree, 2 * p.words, node, all, t - ctx) & 1u) == 0u) continue;
+    int page = list[t / kPage];
     if (page < 0 || page >= p.num_pages) page = 0;               // (as it was read)
-    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.kv_pool) + (((static_cast<long long>(page) * 2 + 1) * p.kv_heads + f.kvh) * kPage + t % kPage) * HD + c;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) {
-      const float x = __bfloat162float(v[j]);
-      if (!isfinite(x)) o[j] += x;
+    const __nv_bfloat16* v = static_cast<const __nv_bfloat16*>(p.kv_pool) + (((static_cast<long long>(page) * 2 + 1) * p.kv_heads + kvh) * kPage + t % kPage) * HD;
+    for (int c = from; c < to; ++c) {
+      const float x = __bfloat162float(v[c]);
+      if (isfinite(x)) continue;
+      if (sums != nullptr) __stcg(sums + c, __ldcg(sums + c) + x);
+      else out[c] = __float2bfloat16(__bfloat162float(*const_cast<volatile __nv_bfloat16*>(out + c)) + x);
     }
   }
 }
 
-template <int HD>
-__global__ void __launch_bounds__(kThreads, 1)
-attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV, nfk_attn_tree_params p, Workspace ws) {
-  using C = Cfg<HD>;
-  constexpr int NH = C::NH, NST = C::kStages;
+template <int HD, int SLOTS>
+__global__ void __launch_bounds__(Cfg<HD, SLOTS>::kThreads, 3 - SLOTS)
+attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV,
+                 const __grid_constant__ nfk_attn_tree_params p, Workspace ws) {
+  using C = Cfg<HD, SLOTS>;
+  constexpr int NH = C::NH, NST = C::kStages, kKeyWarp = C::kKeyWarp, kMmaWarp = C::kMmaWarp, kValueWarp = C::kValueWarp, kThreads = C::kThreads;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sb = smem_u32(smem);
   float2* ml_s = reinterpret_cast<float2*>(smem + C::kMl);
@@ -249,9 +252,10 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   // (before the roles begin) sums of the warps' units, units in front of the CTA's first request, its number
   long long* scan_s = reinterpret_cast<long long*>(smem + C::kMl);
   long long* start_off_s = scan_s + kThreads / 32;
-  int* start_req_s = reinterpret_cast<int*>(start_off_s + 1);
+  Request* start_s = reinterpret_cast<Request*>(start_off_s + 1);
+  int* start_req_s = reinterpret_cast<int*>(start_s + 1);
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
-  const int group = p.q_heads / p.kv_heads, per_slot = 128 / group;                // tokens of a slot
+  const int group = p.q_heads / p.kv_heads, per_slot = 128 / group, per_block = SLOTS * per_slot;     // tokens of a slot, of a block of rows
   if ((sb & 1023u) != 0u) {                      // the operands' layouts need it; report instead of computing garbage
     await_previous();
     if (threadIdx.x == 0) {
@@ -262,8 +266,8 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   if (threadIdx.x == 0) {
     for (int b = 0; b < C::kNum; ++b) {
-      const int n = b == C::READ ? 10 : b == C::O_FREE ? 8 : (b >= C::P_FULL && b < C::PV_DONE) ? 4
-                    : b >= C::MERGE || b == C::Q_EMPTY || (b >= C::EMPTY && b < C::Q_FULL) ? 2 : 1;
+      const int n = b == C::READ ? C::kSoftWarps + SLOTS : b == C::O_FREE ? C::kSoftWarps : (b >= C::P_FULL && b < C::PV_DONE) ? 4 : b >= C::MERGE ? 2
+                    : b == C::Q_EMPTY || (b >= C::K_EMPTY && b < C::V_FULL) || (b >= C::V_EMPTY && b < C::Q_FULL) ? SLOTS : 1;
       mbar_init(&bars[b], n);
     }
     *abort_flag = 0;
@@ -275,14 +279,14 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   await_previous();                              // (before tensor memory is taken, which the kernel before may need)
   if (warp == kMmaWarp) {
-    tmem_alloc(tmem_slot, 512);                  // of each slot (256 columns): scores in [0, 64) and [64, 128), sums in [128, 128 + HD)
+    tmem_alloc(tmem_slot, 256 * SLOTS);                  // of each slot (256 columns): scores in [0, 64) and [64, 128), sums in [128, 128 + HD)
     tmem_relinquish();
   }
   // ---- where this CTA's share of the units begins: units of every thread's requests, scanned ----
   const int per_thread = (p.req_count + kThreads - 1) / kThreads;
   const int r0 = min(p.req_count, static_cast<int>(threadIdx.x) * per_thread), r1 = min(p.req_count, r0 + per_thread);
   long long mine = 0;
-  for (int r = r0; r < r1; ++r) mine += units_of(read_request(p, r, 2 * per_slot, blockIdx.x == 0)) * p.kv_heads;
+  for (int r = r0; r < r1; ++r) mine += units_of(read_request(p, r, per_block, blockIdx.x == 0)) * p.kv_heads;
   long long sum = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -307,8 +311,10 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   if (works && u0 >= before && u0 < before + mine) {           // one thread
     long long at = before;
     for (int r = r0; r < r1; ++r) {
-      const long long n = units_of(read_request(p, r, 2 * per_slot, false)) * p.kv_heads;
+      const Request q = read_request(p, r, per_block, false);
+      const long long n = units_of(q) * p.kv_heads;
       if (u0 < at + n) {
+        *start_s = q;
         *start_req_s = r;
         *start_off_s = at;
         break;
@@ -320,6 +326,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const uint32_t tmem = *tmem_slot;
   const int start_req = *start_req_s;
   const long long start_off = *start_off_s;
+  Request start = *start_s;
   __syncthreads();
   let_next_start();
 
@@ -330,24 +337,22 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   const uint32_t bars_at = smem_u32(bars);
   // for a whole warp; most barriers have been passed long before
   auto passed = [&](int bar, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_test(bars_at + bar * 8, parity)) != 0 || __all_sync(0xffffffffu, wait_or_abort(&bars[bar], parity, abort_flag)) != 0;
+    return __all_sync(0xffffffffu, mbar_test(bars_at + bar * 8, parity)) != 0 || wait_for(&bars[bar], parity, abort_flag);
   };
-  // Places of an item's tiles in the ring, in the order K0 K1 K2 K3 V0 K4 V1 K5 ... : keys are four tiles ahead, as far as both slots' scores
-  // are issued ahead of the second products.
-  auto k_at = [](int t) { return t + max(0, t - 3); };
-  auto v_at = [](int t, int n) { return t + min(n, t + 4); };
-
   if (!works || start_req < 0) {
     if (threadIdx.x == 0) ws.records[blockIdx.x] = Record{0, 0, 0, 0};
-  } else if (warp == kLoadWarp) {
-    // ------------------------------------------------------------------ copies (the warp walks, an elected lane issues)
+  } else if (warp == kKeyWarp || warp == kValueWarp) {
+    // ------------------------------------------------------------------ copies (a warp walks, an elected lane issues)
+    // Keys and values have a warp each, since a tile's eight copies and the wait for its place take most of the time that its bytes do.
+    const int part = warp == kKeyWarp ? 0 : 1, full = part == 0 ? C::K_FULL : C::V_FULL, empty = part == 0 ? C::K_EMPTY : C::V_EMPTY;
+    uint8_t* const tiles_at = smem + C::kRing + part * (NST * C::kStage);
     Record record{0, 0, 0, 0};
-    uint32_t ring = 0, n_item = 0;               // tiles so far (keys and values each), items so far
+    uint32_t ring = 0, n_item = 0;               // tiles and items so far
     const int no_row = static_cast<int>(min(static_cast<long long>(p.num_pages) * 2 * p.kv_heads * kPage, 0x7fffff00ll));   // behind the pool: zeros
     bool ok = true;
     long long at = start_off;                    // units in front of request r
     for (int r = start_req; ok && r < p.req_count && at < u1; ++r) {
-      const Request q = read_request(p, r, 2 * per_slot, false);
+      const Request q = r == start_req ? start : read_request(p, r, per_block, false);
       const long long span = kLead + q.pages, n_items = q.blocks * p.kv_heads;
       for (long long i = u0 > at ? divide(u0 - at, span) : 0; ok && i < n_items; ++i) {
         const long long s = at + i * span;       // the item's first unit
@@ -355,9 +360,9 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (s + span <= u0) continue;
         Piece f;
         f.kvh = static_cast<int>(divide(i, q.blocks));
-        f.node = static_cast<int>(i - f.kvh * q.blocks) * 2 * per_slot;
+        f.node = static_cast<int>(i - f.kvh * q.blocks) * per_block;
         f.tok = q.tok + f.node;
-        f.nodes = min(2 * per_slot, q.n - f.node);
+        f.nodes = min(per_block, q.n - f.node);
         f.all = q.n;
         f.list = q.list;
         f.len = q.len;
@@ -376,95 +381,85 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
         const int tiles = (f.pages + kTilePages - 1) / kTilePages;
         const int* list = p.kv_indices + q.list + f.page0;
-        // Page numbers of 32 pages (eight tiles) at a time, a lane each; keys are four tiles ahead of values, so that two such groups are held.
-        auto fetch = [&](int group_of_32) {
-          const int j = group_of_32 * 32 + lane;
-          int page = -1;
+        // Page numbers of 32 pages (eight tiles) at a time, a lane each.
+        int pages = 0;
+        auto fetch = [&](int tile) {
+          const int j = tile * kTilePages + lane;
+          pages = -1;
           if (j < f.pages) {
-            page = list[j];
-            if (page < 0 || page >= p.num_pages) {
+            pages = list[j];
+            if (pages < 0 || pages >= p.num_pages) {
               report_status(p.status, NF_ST_BAD_INDEX);
-              page = 0;
+              pages = 0;
             }
           }
-          return page;
         };
-        int held[2] = {-1, -1};
-        auto issue = [&](int pos, int tile, int part) {
-          const bool second = (tile >> 3 & 1) != 0;
-          if (part == 0 && (tile & 7) == 0) {
-            if (second) held[1] = fetch(tile >> 3);
-            else held[0] = fetch(tile >> 3);
-          }
-          const int pages = second ? held[1] : held[0];
-          const uint32_t at_ring = ring + pos, stage = at_ring % NST;
-          if (!passed(C::EMPTY + stage, (at_ring / NST & 1) ^ 1)) return false;
-          uint8_t* to = smem + C::kRing + stage * C::kStage;
+        fetch(0);
+        auto issue = [&](int tile) {
+          if (tile > 0 && (tile & 7) == 0) fetch(tile);
+          const uint32_t at_ring = ring + tile, stage = at_ring % NST;
           int rows[kTilePages];
 #pragma unroll
           for (int j = 0; j < kTilePages; ++j) {
             const int page = __shfl_sync(0xffffffffu, pages, (tile & 7) * kTilePages + j);
             rows[j] = page < 0 ? no_row : ((page * 2 + part) * p.kv_heads + f.kvh) * kPage;
           }
+          if (!passed(empty + stage, (at_ring / NST & 1) ^ 1)) return false;
+          uint8_t* to = tiles_at + stage * C::kStage;
           if (elect_one()) {
-            mbar_expect_tx(&bars[C::FULL + stage], C::kStage);
+            uint64_t* bar = &bars[full + stage];
+            mbar_expect_tx(bar, C::kStage);
 #pragma unroll
             for (int j = 0; j < kTilePages; ++j)
 #pragma unroll
-              for (int h = 0; h < NH; ++h)
-                tma_load_2d(to + h * C::kHalf + j * (kPage * 128), &tmKV, &bars[C::FULL + stage], h * 64, rows[j]);
+              for (int h = 0; h < NH; ++h) tma_load_2d(to + h * C::kHalf + j * (kPage * 128), &tmKV, bar, h * 64, rows[j]);
           }
           __syncwarp();
           return true;
         };
-        // the first tiles are on their way before the queries, which wait for the item before
-        auto issue_at = [&](int pos) {           // the inverse of k_at, v_at
-          if (pos < min(tiles, 4)) return issue(pos, pos, 0);
-          if (pos >= 2 * tiles - 4) return issue(pos, pos - tiles, 1);
-          return (pos & 1) != 0 ? issue(pos, (pos + 3) / 2, 0) : issue(pos, pos / 2 - 2, 1);
-        };
-        int pos = 0;
-        if (n_item > 0)
-          for (; ok && pos < min(tiles, 4); ++pos) ok = issue_at(pos);
-        if (!ok || !passed(C::READ, (n_item & 1) ^ 1) || !passed(C::Q_EMPTY, (n_item & 1) ^ 1)) {
-          ring += pos;
-          ok = false;
-          break;
-        }
-        if (elect_one()) {
-          *piece_s = f;
-          const int slots = f.two ? 2 : 1;
-          mbar_expect_tx(&bars[C::Q_FULL], slots * NH * per_slot * group * 128);
-          for (int slot = 0; slot < slots; ++slot)
+        int tile = 0;
+        if (part == 0) {
+          // the first tiles are on their way before the queries, which wait for the item before
+          if (n_item > 0)
+            for (; ok && tile < min(tiles, NST); ++tile) ok = issue(tile);
+          ok = ok && passed(C::READ, (n_item & 1) ^ 1) && passed(C::Q_EMPTY, (n_item & 1) ^ 1);
+          if (ok) {
+            if (elect_one()) {
+              *piece_s = f;
+              const int slots = f.two ? 2 : 1;
+              mbar_expect_tx(&bars[C::Q_FULL], slots * NH * per_slot * group * 128);
+              for (int slot = 0; slot < slots; ++slot)
 #pragma unroll
-            for (int h = 0; h < NH; ++h)
-              tma_load_3d(smem + slot * C::kQ + h * C::kQHalf, &tmQ, &bars[C::Q_FULL], h * 64, f.kvh * group, f.tok + slot * per_slot);
+                for (int h = 0; h < NH; ++h)
+                  tma_load_3d(smem + slot * C::kQ + h * C::kQHalf, &tmQ, &bars[C::Q_FULL], h * 64, f.kvh * group, f.tok + slot * per_slot);
+            }
+            __syncwarp();
+            ++n_item;
+          }
         }
-        __syncwarp();
-        ++n_item;
-        for (; ok && pos < 2 * tiles; ++pos) ok = issue_at(pos);
-        ring += pos;
+        for (; ok && tile < tiles; ++tile) ok = issue(tile);
+        ring += tile;
       }
       at += n_items * span;
     }
     if (!ok) fail(NF_ST_TIMEOUT_SMEM_EMPTY);
-    if (lane == 0) ws.records[blockIdx.x] = record;
-    if (ok && passed(C::READ, (n_item & 1) ^ 1) && passed(C::Q_EMPTY, (n_item & 1) ^ 1)) {
+    if (part == 0 && lane == 0) ws.records[blockIdx.x] = record;
+    if (part == 0 && ok && passed(C::READ, (n_item & 1) ^ 1) && passed(C::Q_EMPTY, (n_item & 1) ^ 1)) {
       if (elect_one()) {                         // no more pieces
         piece_s->nodes = 0;
         mbar_arrive(&bars[C::Q_FULL]);
       }
       __syncwarp();
-    } else if (n_item > 0) {
+    } else if (part == 0 && n_item > 0) {
       (void)mbar_wait(&bars[C::Q_FULL], (n_item - 1) & 1);
     }
     // copies still in flight must have landed before the CTA gives its shared memory back
-    for (uint32_t k = ring > NST ? ring - NST : 0; k < ring; ++k) (void)mbar_wait(&bars[C::FULL + k % NST], k / NST & 1);
-  } else if (warp >= kMmaWarp) {
+    for (uint32_t k = ring > NST ? ring - NST : 0; k < ring; ++k) (void)mbar_wait(&bars[full + k % NST], k / NST & 1);
+  } else if (warp >= kMmaWarp && warp < kValueWarp) {
     // ------------------------------------------------------------------ products (the warp walks, an elected lane issues)
     const uint32_t idesc_s = umma_idesc_bf16(128, kTile), idesc_o = umma_idesc_bf16(128, HD) | kIdescBMnMajor;
     const uint64_t q_desc = umma_desc_k_sw128(sb), k_desc = umma_desc_k_sw128(sb + C::kRing);
-    const uint64_t v_desc = umma_desc_mn_sw128(sb + C::kRing, C::kHalf, 1024);
+    const uint64_t v_desc = umma_desc_mn_sw128(sb + C::kRing + NST * C::kStage, C::kHalf, 1024);
     // A warp per slot: what it spends is not the products but the waits in front of them (some 100 cycles each, also where the barrier has
     // long been passed), and one warp for both took 2600 cycles for a tile of both.
     const int slot = warp - kMmaWarp;
@@ -474,34 +469,31 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     bool ok = true;
     for (;;) {
       if (!passed(C::Q_FULL, n_item & 1)) { ok = false; break; }
-      const int nodes = piece_s->nodes, pages = piece_s->pages, two = piece_s->two, page0 = piece_s->page0;
+      const int nodes = piece_s->nodes, pages = piece_s->pages, page0 = piece_s->page0;
+      const bool two = SLOTS == 2 && piece_s->two != 0, every = SLOTS == 1 || two;      // whether the slot takes every tile
       const int care_from = min(piece_s->len - piece_s->all, min(piece_s->len, (page0 + pages) * kPage));
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars[C::READ]);
       if (nodes == 0) break;
       const int tiles = (pages + kTilePages - 1) / kTilePages;
-      const int n = two ? tiles : (tiles + 1 - slot) / 2;
+      const int n = every ? tiles : (tiles + 1 - slot) / 2;
       const uint64_t qd = q_desc + static_cast<uint64_t>((two ? slot : 0) * (C::kQ >> 4));
-      // The other slot's tiles pass by: both warps wait for all of the ring's places in their order, since a parity tells only neighbouring
+      // The other slot's tiles pass by: both warps wait for all of a ring's places in their order, since a parity tells only neighbouring
       // phases apart.
-      auto pass_by = [&](uint32_t place) {
-        if (!passed(C::FULL + place % NST, place / NST & 1)) return false;
-        if (lane == 0) mbar_arrive(&bars[C::EMPTY + place % NST]);
+      auto pass_by = [&](int full, int empty, int tile) {
+        if (every || tile >= tiles) return true;
+        const uint32_t at = ring + tile;
+        if (!passed(full + at % NST, at / NST & 1)) return false;
+        if (lane == 0) mbar_arrive(&bars[empty + at % NST]);
         return true;
       };
-      auto other_keys = [&](int i) {
-        const int tile = 2 * i + (slot ^ 1);
-        return two || tile >= tiles || pass_by(ring + k_at(tile));
-      };
-      auto other_values = [&](int i) {
-        const int tile = 2 * i + (slot ^ 1);
-        return two || tile >= tiles || pass_by(ring + v_at(tile, tiles));
-      };
+      auto other_keys = [&](int i) { return pass_by(C::K_FULL, C::K_EMPTY, 2 * i + (slot ^ 1)); };
+      auto other_values = [&](int i) { return pass_by(C::V_FULL, C::V_EMPTY, 2 * i + (slot ^ 1)); };
       // S(i) goes over the weights of the slot's tile before the last one, which that one's second product reads: it must have ended
       auto scores = [&](int i) {
-        const uint32_t k = ring + k_at(two ? i : 2 * i + slot), g = n_tile + i, at = slot * 2 + (g & 1);
+        const uint32_t k = ring + (every ? i : 2 * i + slot), g = n_tile + i, at = slot * 2 + (g & 1);
         if (g >= 2 && !passed(C::PV_DONE + at, ((g >> 1) - 1) & 1)) return false;
-        if (!passed(C::FULL + k % NST, k / NST & 1)) return false;
+        if (!passed(C::K_FULL + k % NST, k / NST & 1)) return false;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t kd = k_desc + static_cast<uint64_t>(k % NST * (C::kStage >> 4));
@@ -511,18 +503,18 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             for (int s = 0; s < 4; ++s)
               umma_bf16_ss(t_s + (g & 1) * kTile, qd + ((h * C::kQHalf + s * 32) >> 4), kd + ((h * C::kHalf + s * 32) >> 4), idesc_s, (h | s) ? 1u : 0u);
           umma_commit(&bars[C::S_FULL + at]);
-          umma_commit(&bars[C::EMPTY + k % NST]);
+          umma_commit(&bars[C::K_EMPTY + k % NST]);
           if (i == n - 1) umma_commit(&bars[C::Q_EMPTY]);
         }
         __syncwarp();
         return true;
       };
       auto sums = [&](int i) {
-        const int tile = two ? i : 2 * i + slot;
-        const uint32_t v = ring + v_at(tile, tiles), g = n_tile + i, at = slot * 2 + (g & 1);
+        const int tile = every ? i : 2 * i + slot;
+        const uint32_t v = ring + tile, g = n_tile + i, at = slot * 2 + (g & 1);
         // the item before must have been read out of both slots' sums
         if (i == 0 && !passed(C::O_FREE, (n_item & 1) ^ 1)) return false;
-        if (!passed(C::FULL + v % NST, v / NST & 1)) return false;
+        if (!passed(C::V_FULL + v % NST, v / NST & 1)) return false;
         if (page0 * kPage + (tile + 1) * kTile > care_from) {    // the values are gone through first, by slot 0 for both if both have them
           if (!two || slot == 0) {
             if (lane == 0) mbar_arrive(&bars[C::CARE + slot]);
@@ -538,7 +530,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           for (int s = 0; s < kTile / 16; ++s)
             umma_bf16_ts(t_o, t_s + (g & 1) * kTile + s * 8, vd + ((s * 2048) >> 4), idesc_o, (i | s) ? 1u : 0u);
           umma_commit(&bars[C::PV_DONE + at]);
-          umma_commit(&bars[C::EMPTY + v % NST]);
+          umma_commit(&bars[C::V_EMPTY + v % NST]);
         }
         __syncwarp();
         return true;
@@ -550,10 +542,10 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         ok = scores(0);
       }
       ok = ok && other_keys(0);
-      for (int i = 0; ok && i < (two ? tiles : (tiles + 1) / 2); ++i)
+      for (int i = 0; ok && i < (every ? tiles : (tiles + 1) / 2); ++i)
         ok = (i + 1 >= n || scores(i + 1)) && other_keys(i + 1) && (i >= n || sums(i)) && other_values(i);
       if (!ok) break;
-      ring += 2 * tiles;
+      ring += tiles;
       n_tile += n;
       ++n_item;
     }
@@ -572,7 +564,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     uint32_t ring = 0, n_item = 0, n_done = 0, n_merge = 0, n_care = 0;
     // States that will not be formed are NaN, and not what an earlier call left in the workspace.
 #pragma unroll
-    for (int k = 0; k < 2; ++k) __stcg(ws.ml + (2 * blockIdx.x + k) * 256 + slot * 128 + row, make_float2(0.f, __uint_as_float(0x7fc00000u)));
+    for (int k = 0; k < 2; ++k) __stcg(ws.ml + ((2 * blockIdx.x + k) * SLOTS + slot) * 128 + row, make_float2(0.f, __uint_as_float(0x7fc00000u)));
     for (;;) {
       if (!passed(C::Q_FULL, n_item & 1)) { fail(NF_ST_TIMEOUT_SMEM_FULL); break; }
       const Piece f = *piece_s;
@@ -580,8 +572,9 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       if (lane == 0) mbar_arrive(&bars[C::READ]);
       if (f.nodes == 0) break;
       const int tiles = (f.pages + kTilePages - 1) / kTilePages;
-      const int n_mine = f.two ? tiles : (tiles + 1 - slot) / 2;
-      const int node_in = in_slot + (f.two ? slot * per_slot : 0);       // of the block
+      const bool two = SLOTS == 2 && f.two != 0, every = SLOTS == 1 || two;
+      const int n_mine = every ? tiles : (tiles + 1 - slot) / 2;
+      const int node_in = in_slot + (two ? slot * per_slot : 0);       // of the block
       const bool on = in_slot < per_slot && node_in < f.nodes;
       const bool warp_on = __any_sync(0xffffffffu, on);
       const int node = f.node + node_in, ctx = f.len - f.all;
@@ -590,7 +583,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       float ref = -INFINITY, l = 0.f;
       bool sees = false, ok = true;
       for (int i = 0; i < n_mine; ++i) {
-        const int tile = f.two ? i : 2 * i + slot;
+        const int tile = every ? i : 2 * i + slot;
         const int at = f.page0 * kPage + tile * kTile;                   // the tile's first token
         const bool care = at + kTile > min(ctx, end);
         uint32_t bits[2] = {~0u, ~0u};
@@ -604,15 +597,15 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int b = slot * 2 + (n_done & 1);
         const uint32_t t_s = t_slot + (n_done & 1) * kTile;
         if (!passed(C::S_FULL + b, n_done >> 1 & 1)) { ok = false; break; }
-        if (care && (!f.two || slot == 0)) {
+        if (care && (!two || slot == 0)) {
           // ---- values of the tile: two threads per token ----
           // (by way of the warp that waits for all of the ring's places in their order)
-          const uint32_t v = ring + v_at(tile, tiles);
-          if (!passed(C::CARE + slot, n_care & 1) || !passed(C::FULL + v % NST, v / NST & 1)) { ok = false; break; }
+          const uint32_t v = ring + tile;
+          if (!passed(C::CARE + slot, n_care & 1) || !passed(C::V_FULL + v % NST, v / NST & 1)) { ok = false; break; }
           ++n_care;
           const int in_tile = row & (kTile - 1), token = at + in_tile;
           if (token >= ctx) {
-            const uint32_t v_row = sb + C::kRing + v % NST * C::kStage + in_tile * 128;
+            const uint32_t v_row = sb + C::kRing + NST * C::kStage + v % NST * C::kStage + in_tile * 128;
             bool odd = false;
 #pragma unroll
             for (int k = 0; k < HD / 16; ++k) {
@@ -633,7 +626,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           }
           fence_proxy_async_smem();
           __syncwarp();
-          if (f.two && lane == 0) {
+          if (two && lane == 0) {
             __threadfence_block();
             atomicAdd(cleared, 1);
           }
@@ -655,16 +648,38 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           } else {
             sees = true;
           }
-          float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) mq[2 * c + (j >> 1 & 1)] = max3(mq[2 * c + (j >> 1 & 1)], __uint_as_float(x[c][j]), __uint_as_float(x[c][j + 1]));
-          const float mx = fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])) * scale;
-          const bool grow = mx > ref + kGap || (ref == -INFINITY && mx > -INFINITY);
+          float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (NaN where there is one)
+          auto more = [&](int j) { mq[j & 3] = max3_nan(mq[j & 3], __uint_as_float(x[j >> 4][2 * (j & 15)]), __uint_as_float(x[j >> 4][2 * (j & 15) + 1])); };
+          auto largest = [&]() {
+            const float mx = max3_nan(max3_nan(mq[0], mq[1], mq[2]), mq[3], mq[3]) * scale;
+            if (mx < INFINITY) return mx;
+            l = __uint_as_float(0x7fc00000u);    // a score of infinity, or none
+            return 0.f;
+          };
           if (i == 0) {
-            ref = mx;
-          } else if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) more(j);
+            ref = largest();
+          }
+          // Weights relative to the reference as it is, while the largest score is found beside them: there is seldom more than one pass.
+          f32x2 rs[2];
+          uint32_t pk[32];                       // column j: tokens 2j, 2j + 1
+          for (;;) {
+            const float ms = ref == -INFINITY ? 0.f : ref;
+            const f32x2 scale2 = pair(scale, scale), ms2 = pair(-ms, -ms);
+            rs[0] = rs[1] = pair(0.f, 0.f);
+            mq[0] = mq[1] = mq[2] = mq[3] = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              more(j);
+              const float2 y = halves(fma2(pair(__uint_as_float(x[j >> 4][2 * (j & 15)]), __uint_as_float(x[j >> 4][2 * (j & 15) + 1])), scale2, ms2));
+              const float e0 = fast_exp2(y.x), e1 = fast_exp2(y.y);
+              rs[j & 1] = add2(rs[j & 1], pair(e0, e1));
+              pk[j] = pack_bf16x2(e0, e1);
+            }
+            const float mx = largest();
+            const bool grow = mx > ref + kGap || (ref == -INFINITY && mx > -INFINITY);
+            if (!__any_sync(0xffffffffu, grow)) break;
             // Sums may be touched between two products only: that of the tile before is the last one issued (this tile's needs its weights)
             if (!passed(C::PV_DONE + slot * 2 + ((n_done - 1) & 1), (n_done - 1) >> 1 & 1)) { ok = false; break; }
             tc_fence_after();
@@ -676,27 +691,13 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               tmem_ld_wait();
 #pragma unroll
               for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-              asm volatile(
-                  "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(t_o + c * 16),
-                  "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]), "r"(o[8]), "r"(o[9]), "r"(o[10]),
-                  "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15])
-                  : "memory");
+              tmem_st_32x32b_x16(t_o + c * 16, o);
             }
             tmem_st_wait();
             l *= alpha;
             if (grow) ref = mx;
           }
-          const float ms = ref == -INFINITY ? 0.f : ref;
-          const f32x2 scale2 = pair(scale, scale), ms2 = pair(-ms, -ms);
-          f32x2 rs[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
-          uint32_t pk[32];                       // column j: tokens 2j, 2j + 1
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float2 y = halves(fma2(pair(__uint_as_float(x[j >> 4][2 * (j & 15)]), __uint_as_float(x[j >> 4][2 * (j & 15) + 1])), scale2, ms2));
-            const float e0 = fast_exp2(y.x), e1 = fast_exp2(y.y);
-            rs[j & 1] = add2(rs[j & 1], pair(e0, e1));
-            pk[j] = pack_bf16x2(e0, e1);
-          }
+          if (!ok) break;
           tmem_st_32x32b_x32(t_s, pk);
           const float2 t = halves(add2(rs[0], rs[1]));
           l += t.x + t.y;
@@ -708,14 +709,14 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         ++n_done;
       }
       if (!ok) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
-      ring += 2 * tiles;
+      ring += tiles;
       if (n_mine > 0 && !passed(C::PV_DONE + slot * 2 + ((n_done - 1) & 1), (n_done - 1) >> 1 & 1)) { fail(NF_ST_TIMEOUT_TMEM_FULL); break; }
       tc_fence_after();
       if (sees && l == 0.f) l = __uint_as_float(0x7fc00000u);            // all that it sees has a score of minus infinity
       // ---- sums of the row: columns [from, to), a0 times those of slot 0 and a1 times those of slot 1 ----
       float a_mine = 1.f, a_other = 0.f;
       int from = 0, to = HD;
-      if (!f.two) {
+      if (!every) {
         // (one without tiles does not write, it may be an item ahead of the other's reads)
         if (n_mine > 0) ml_s[slot * 128 + row] = make_float2(ref, l);
         tc_fence_before();
@@ -730,10 +731,10 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (top == -INFINITY) {
           a_mine = 0.f;
           l += other.y;
-        } else {                                 // (NaN where a score is infinite)
+        } else {                                 // (a sum of NaN counts whatever its weight, but for a slot without weights)
           a_mine = ref == -INFINITY ? 0.f : fast_exp2(ref - top);
           a_other = other.x == -INFINITY ? 0.f : fast_exp2(other.x - top);
-          l = (a_mine != 0.f ? a_mine * l : 0.f) + (a_other != 0.f ? a_other * other.y : 0.f);
+          l = (ref == -INFINITY ? 0.f : a_mine * l) + (other.x == -INFINITY ? 0.f : a_other * other.y);
         }
         ref = top;
         from = slot * (HD / 2);
@@ -748,70 +749,56 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int out_row = static_cast<int>((static_cast<long long>(f.tok + node_in) * p.ld_out + (f.kvh * group + hh) * HD) >> 3);
       if (warp_on) {
         const bool use_mine = a_mine != 0.f, use_other = a_other != 0.f;
-        const int rows_on = min(per_slot, f.nodes - (f.two ? slot * per_slot : 0)) * group - (warp & 3) * 32;   // of this warp
-        float* o_rows = ws.o + ((static_cast<long long>(f.to) * 256 + (f.two ? slot * 128 : 0) + (warp & 3) * 32) * HD);
-        auto columns = [&](int c, float (&o)[32]) {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            uint32_t a[16], other[16];
-            tmem_ld_32x32b_x16n(t_o + c + 16 * k, a);
-            if (!f.two) tmem_ld_32x32b_x16n((t_o ^ 256u) + c + 16 * k, other);
-            tmem_ld_wait();
-#pragma unroll
-            for (int j = 0; j < 16; ++j)
-              o[16 * k + j] = (use_mine ? a_mine * __uint_as_float(a[j]) : 0.f) + (use_other ? a_other * __uint_as_float(other[j]) : 0.f);
-          }
-          if (odd && on) restore_odd<HD>(p, f, tree, node, max(f.page0 * kPage, ctx), end, c, o);
-        };
-        // A thread has its own row; eight lanes exchange theirs, so that a store is of 128 bytes of four rows (each thread its own: 2.2 us
-        // longer, the stores' 32 lines at a time).
-        if (f.to < 0) {
-          auto packed = [&](const float (&o)[32], uint4* v) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              v[k] = make_uint4(pack_bf16x2(o[8 * k] * by, o[8 * k + 1] * by), pack_bf16x2(o[8 * k + 2] * by, o[8 * k + 3] * by),
-                                pack_bf16x2(o[8 * k + 4] * by, o[8 * k + 5] * by), pack_bf16x2(o[8 * k + 6] * by, o[8 * k + 7] * by));
-          };
-          uint4* out = static_cast<uint4*>(p.out);
+        const int rows_on = min(per_slot, f.nodes - (two ? slot * per_slot : 0)) * group - (warp & 3) * 32;   // of this warp
+        float* o_rows = ws.o + ((static_cast<long long>(f.to) * SLOTS + (two ? slot : 0)) * 128 + (warp & 3) * 32) * HD;
+        // A thread has its own row; by way of shared memory, so that a store is of 128 (or, in bf16, 64) bytes of some rows at once. In few
+        // instructions, which an item meets for the first time.
+        const float times = f.to < 0 ? by : 1.f;
+        const uint32_t via = sb + C::kOut + warp * 4096;
 #pragma unroll 1
-          for (int c = from; c < to; c += 64) {
-            uint4 v[8];
-            float o[32];
-            columns(c, o);
-            packed(o, v);
-            const bool wide = c + 32 < to;
-            if (wide) {
-              columns(c + 32, o);
-              packed(o, v + 4);
-              exchange<8>(v);
-            } else {
-              exchange<4>(v);
-            }
-            const int n = wide ? 8 : 4, j = lane & (n - 1), r0 = lane - j;
+        for (int c = from; c < to; c += 32) {
+          uint32_t a[32], other[32];
+          tmem_ld_32x32b_x32(t_o + c, a);
+          if (!every) tmem_ld_32x32b_x32((t_o ^ 256u) + c, other);
+          tmem_ld_wait();
+          __syncwarp();                          // (the columns before have been read)
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              if (k >= n) break;
-              const int at = __shfl_sync(0xffffffffu, out_row, r0 + k);
-              if (r0 + k < rows_on) out[static_cast<long long>(static_cast<unsigned int>(at)) + c / 8 + j] = v[k];
-            }
+          for (int k = 0; k < 8; ++k) {
+            uint32_t o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              o[j] = __float_as_uint(((use_mine ? a_mine * __uint_as_float(a[4 * k + j]) : 0.f) + (use_other ? a_other * __uint_as_float(other[4 * k + j]) : 0.f)) * times);
+            st_shared_v4(via + lane * 128 + ((k ^ (lane & 7)) << 4), make_uint4(o[0], o[1], o[2], o[3]));
           }
-        } else {
-#pragma unroll 1
-          for (int c = from; c < to; c += 32) {
-            uint4 v[8];
-            float o[32];
-            columns(c, o);
+          __syncwarp();
+          if (f.to < 0) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              v[k] = make_uint4(__float_as_uint(o[4 * k]), __float_as_uint(o[4 * k + 1]), __float_as_uint(o[4 * k + 2]), __float_as_uint(o[4 * k + 3]));
-            exchange<8>(v);
-            const int j = lane & 7, r0 = lane - j;
+            for (int i = 0; i < 4; ++i) {
+              const int r = i * 8 + (lane >> 2), j = 2 * (lane & 3);
+              const int at = __shfl_sync(0xffffffffu, out_row, r);
+              const uint4 lo = ld_shared_v4(via + r * 128 + ((j ^ (r & 7)) << 4)), hi = ld_shared_v4(via + r * 128 + (((j + 1) ^ (r & 7)) << 4));
+              if (r < rows_on)
+                static_cast<uint4*>(p.out)[static_cast<long long>(static_cast<unsigned int>(at)) + c / 8 + j / 2] =
+                    make_uint4(pack_bf16x2(__uint_as_float(lo.x), __uint_as_float(lo.y)), pack_bf16x2(__uint_as_float(lo.z), __uint_as_float(lo.w)),
+                               pack_bf16x2(__uint_as_float(hi.x), __uint_as_float(hi.y)), pack_bf16x2(__uint_as_float(hi.z), __uint_as_float(hi.w)));
+            }
+          } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              if (r0 + k < rows_on) __stcg(reinterpret_cast<uint4*>(o_rows + (r0 + k) * HD + c) + j, v[k]);
+            for (int i = 0; i < 8; ++i) {
+              const int r = i * 4 + (lane >> 3), j = lane & 7;
+              const uint4 w = ld_shared_v4(via + r * 128 + ((j ^ (r & 7)) << 4));
+              if (r < rows_on) __stcg(reinterpret_cast<uint4*>(o_rows + r * HD + c) + j, w);
+            }
           }
         }
-        if (on && f.to >= 0 && (f.two || slot == 0)) __stcg(ws.ml + static_cast<long long>(f.to) * 256 + (f.two ? slot * 128 : 0) + row, make_float2(ref, l));
+        if (__any_sync(0xffffffffu, odd)) {
+          __syncwarp();
+          if (on)
+            restore_odd<HD>(p, p.kv_indices + f.list, f.kvh, tree, node, f.all, ctx, max(f.page0 * kPage, ctx), end, from, to,
+                            f.to < 0 ? nullptr : o_rows + lane * HD,
+                            static_cast<__nv_bfloat16*>(p.out) + static_cast<long long>(static_cast<unsigned int>(out_row)) * 8);
+        }
+        if (on && f.to >= 0 && (every || slot == 0)) __stcg(ws.ml + (static_cast<long long>(f.to) * SLOTS + (two ? slot : 0)) * 128 + row, make_float2(ref, l));
       }
       tc_fence_before();
       __syncwarp();
@@ -824,26 +811,102 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   __syncthreads();
   if (warp == kMmaWarp) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, 256 * SLOTS);
   }
 }
 
-// Rows of items that were cut, a warp each: lanes over its pieces for the weights and over head_dim for the sums. Every CTA works out
-// from all records which rows there are.
-constexpr int kJoinWarps = 8, kJoinPerSm = 4, kMostCtas = 256;
-template <int HD>
-__global__ void __launch_bounds__(kJoinWarps * 32) attn_tree_join_kernel(nfk_attn_tree_params p, Workspace ws, int ctas) {
-  constexpr int V = HD / 32, AHEAD = 8;
+// Rows of items that were cut: LANES lanes each, over its pieces for the weights and over head_dim, a float4 or two a lane, for the sums.
+constexpr int kJoinWarps = 8, kJoinPerSm = 4, kMostCtas = 2 * kJoinWarps * 32;
+template <int HD, int SLOTS, int LANES, int AHEAD>         // AHEAD: pieces on their way at once
+__device__ __forceinline__ void join_rows(const nfk_attn_tree_params& p, const Workspace& ws, const int4* record_s, const int* rows_s, int total, int warp, int lane) {
+  constexpr int V = HD / 4 / LANES, ROWS = 32 / LANES;
+  const int sub = lane & (LANES - 1), group = p.q_heads / p.kv_heads, per_slot = 128 / group;
+  for (int first = (blockIdx.x * kJoinWarps + warp) * ROWS; first < total; first += gridDim.x * kJoinWarps * ROWS) {
+    const int work = min(first + lane / LANES, total - 1);       // (the last row again, where there are no others beside it)
+    int c = 0;                                   // the last record with rows_s <= work
+#pragma unroll
+    for (int step = kMostCtas / 2; step > 0; step >>= 1)
+      if (rows_s[c + step] <= work) c += step;
+    const int pieces = record_s[c].x, tok = record_s[c].y, kvh = record_s[c].w;
+    int most = pieces;
+#pragma unroll
+    for (int o = 16; o >= LANES; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    const int b = work - rows_s[c], node = b / group, hh = b - node * group, slot = node / per_slot;
+    const int row = slot * 128 + (node - slot * per_slot) * group + hh;
+    auto number = [&](int k) { return static_cast<long long>(k == 0 ? 2 * c + 1 : 2 * (c + k)) * (128 * SLOTS) + row; };
+    float4 x[AHEAD][V];
+    auto load = [&](int k0) {
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k)
+        if (k0 + k < pieces)
+#pragma unroll
+          for (int v = 0; v < V; ++v) x[k][v] = __ldcg(reinterpret_cast<const float4*>(ws.o + number(k0 + k) * HD) + v * LANES + sub);
+    };
+    load(0);
+    float2 ml = make_float2(-INFINITY, 0.f);     // the first pieces', one a lane
+    if (sub < pieces) ml = __ldcg(ws.ml + number(sub));
+    float top = ml.x, odd = ml.y != ml.y ? ml.y : 0.f;
+    for (int k = LANES + sub; k < pieces; k += LANES) {
+      const float2 far = __ldcg(ws.ml + number(k));
+      top = fmaxf(top, far.x);
+      if (far.y != far.y) odd = far.y;
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float total_l = 0.f;
+    float4 acc[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = 0; k0 < most; k0 += LANES) {
+      if (k0 > 0) ml = k0 + sub < pieces ? __ldcg(ws.ml + number(k0 + sub)) : make_float2(-INFINITY, 0.f);
+      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
+      total_l += ml.x == -INFINITY ? 0.f : w * ml.y;             // (a sum of NaN counts whatever its weight)
+      for (int k1 = k0; k1 < min(k0 + LANES, most); k1 += AHEAD) {
+        if (k1 > 0) load(k1);
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+          const float by = __shfl_sync(0xffffffffu, w, (lane & ~(LANES - 1)) | ((k1 + k) & (LANES - 1)));
+          if (by != 0.f)                         // (zero behind the last piece)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+              acc[v].x += by * x[k][v].x;
+              acc[v].y += by * x[k][v].y;
+              acc[v].z += by * x[k][v].z;
+              acc[v].w += by * x[k][v].w;
+            }
+        }
+      }
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+      total_l += __shfl_xor_sync(0xffffffffu, total_l, o);
+      odd += __shfl_xor_sync(0xffffffffu, odd, o);
+    }
+    // without weights: zeros, or NaN where the row sees something
+    const float by = total_l > 0.f ? 1.f / total_l : total_l + (top == -INFINITY ? odd : 0.f);
+    uint2* dst = reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<long long>(tok + node) * p.ld_out + (kvh * group + hh) * HD);
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      dst[v * LANES + sub] = make_uint2(pack_bf16x2(acc[v].x * by, acc[v].y * by), pack_bf16x2(acc[v].z * by, acc[v].w * by));
+  }
+}
+// Every CTA works out from all records which rows there are.
+template <int HD, int SLOTS>
+__global__ void __launch_bounds__(kJoinWarps * 32, kJoinPerSm) attn_tree_join_kernel(const __grid_constant__ nfk_attn_tree_params p, Workspace ws, int ctas) {
   __shared__ int4 record_s[kMostCtas];
-  __shared__ int rows_s[kMostCtas + 1], warp_s[kJoinWarps];
+  __shared__ int rows_s[kMostCtas], warp_s[kJoinWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = p.q_heads / p.kv_heads, per_slot = 128 / group;
+  const int group = p.q_heads / p.kv_heads;
   await_previous();
   let_next_start();
   // ---- rows in front of each record ----
-  int4 rec = make_int4(0, 0, 0, 0);
-  if (static_cast<int>(threadIdx.x) < ctas) rec = __ldcg(reinterpret_cast<const int4*>(ws.records + threadIdx.x));
-  const int mine = rec.x > 0 ? rec.z * group : 0;
+  int4 rec[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const int c = 2 * threadIdx.x + k;
+    rec[k] = c < ctas ? __ldcg(reinterpret_cast<const int4*>(ws.records + c)) : make_int4(0, 0, 0, 0);
+  }
+  const int mine0 = rec[0].x > 0 ? rec[0].z * group : 0, mine = mine0 + (rec[1].x > 0 ? rec[1].z * group : 0);
   int sum = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -858,72 +921,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32) attn_tree_join_kernel(nfk_att
     if (w < warp) before += warp_s[w];
     total += warp_s[w];
   }
-  record_s[threadIdx.x] = rec;
-  rows_s[threadIdx.x] = before;
+  record_s[2 * threadIdx.x] = rec[0];
+  record_s[2 * threadIdx.x + 1] = rec[1];
+  rows_s[2 * threadIdx.x] = before;
+  rows_s[2 * threadIdx.x + 1] = before + mine0;
   __syncthreads();
-  for (int work = blockIdx.x * kJoinWarps + warp; work < total; work += gridDim.x * kJoinWarps) {
-    int c = 0;                                   // the last record with rows_s <= work
-#pragma unroll
-    for (int step = kMostCtas / 2; step > 0; step >>= 1)
-      if (rows_s[c + step] <= work) c += step;
-    const int pieces = record_s[c].x, tok = record_s[c].y, kvh = record_s[c].w;
-    const int b = work - rows_s[c], node = b / group, hh = b - node * group, slot = node / per_slot;
-    const int row = slot * 128 + (node - slot * per_slot) * group + hh;
-    auto number = [&](int k) { return static_cast<long long>(k == 0 ? 2 * c + 1 : 2 * (c + k)) * 256 + row; };
-    auto load = [&](int k, float (&x)[V]) {
-      const float* from = ws.o + number(k) * HD + lane * V;
-      if constexpr (V == 4) {
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(from));
-        x[0] = y.x; x[1] = y.y; x[2] = y.z; x[3] = y.w;
-      } else {
-        const float2 y = __ldcg(reinterpret_cast<const float2*>(from));
-        x[0] = y.x; x[1] = y.y;
-      }
-    };
-    float x[AHEAD][V];
-#pragma unroll
-    for (int k = 0; k < AHEAD; ++k)
-      if (k < pieces) load(k, x[k]);
-    float2 ml = make_float2(-INFINITY, 0.f);     // the first 32 pieces'
-    if (lane < pieces) ml = __ldcg(ws.ml + number(lane));
-    float top = ml.x, odd = ml.y != ml.y ? ml.y : 0.f;
-    for (int k = 32 + lane; k < pieces; k += 32) {
-      const float2 far = __ldcg(ws.ml + number(k));
-      top = fmaxf(top, far.x);
-      if (far.y != far.y) odd = far.y;
-    }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float total_l = 0.f, acc[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) acc[v] = 0.f;
-    for (int k0 = 0; k0 < pieces; k0 += 32) {
-      if (k0 > 0) ml = k0 + lane < pieces ? __ldcg(ws.ml + number(k0 + lane)) : make_float2(-INFINITY, 0.f);
-      const float w = ml.x == -INFINITY ? 0.f : fast_exp2(ml.x - top);
-      total_l += w != 0.f ? w * ml.y : 0.f;
-      const int here = min(32, pieces - k0);
-      for (int k1 = 0; k1 < here; k1 += AHEAD) {
-        if (k0 + k1 > 0)
-#pragma unroll
-          for (int k = 0; k < AHEAD; ++k)
-            if (k1 + k < here) load(k0 + k1 + k, x[k]);
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-          const float by = __shfl_sync(0xffffffffu, w, (k1 + k) & 31);
-          if (k1 + k >= here) break;
-#pragma unroll
-          for (int v = 0; v < V; ++v) acc[v] += by != 0.f ? by * x[k][v] : 0.f;
-        }
-      }
-    }
-    total_l = warp_sum(total_l);
-    // without weights: zeros, or NaN where the row sees something
-    odd = top == -INFINITY ? warp_sum(odd) : 0.f;
-    const float by = total_l > 0.f ? 1.f / total_l : total_l + odd;
-    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<__nv_bfloat16*>(p.out) + static_cast<long long>(tok + node) * p.ld_out + (kvh * group + hh) * HD + lane * V);
-#pragma unroll
-    for (int v = 0; v < V; v += 2) dst[v / 2] = pack_bf16x2(acc[v] * by, acc[v + 1] * by);
-  }
+  // few rows of many pieces, or many of few: a lane's loads are latency's in the one case, throughput's in the other
+  if (total <= static_cast<int>(gridDim.x) * kJoinWarps) join_rows<HD, SLOTS, HD / 4, 8>(p, ws, record_s, rows_s, total, warp, lane);
+  else join_rows<HD, SLOTS, HD / 8, 4>(p, ws, record_s, rows_s, total, warp, lane);
 }
 
 int encode(CUtensorMap* out, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
@@ -935,13 +940,14 @@ int encode(CUtensorMap* out, int rank, const void* base, const cuuint64_t* dims,
              ? NF_OK : NF_ERR_CUDA;
 }
 
-template <int HD>
+template <int HD, int SLOTS>
 int launch(const nfk_attn_tree_params& p, cudaStream_t stream) {
-  using C = Cfg<HD>;
+  using C = Cfg<HD, SLOTS>;
+  const auto kernel = attn_tree_kernel<HD, SLOTS>;
   static bool attr_dev[kMaxDevices] = {false};
   bool& attr = attr_dev[device_slot()];
   if (!attr) {
-    if (cudaFuncSetAttribute(attn_tree_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes) != cudaSuccess) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kBytes) != cudaSuccess) {
       (void)cudaGetLastError();
       return NF_ERR_CUDA;
     }
@@ -960,11 +966,11 @@ int launch(const nfk_attn_tree_params& p, cudaStream_t stream) {
   if (rc != NF_OK) return rc;
   Workspace ws;
   workspace_bytes(HD, &ws, p.workspace);
-  const int sms = device_sm_count(), most = sms < kMostCtas ? sms : kMostCtas, ctas = p.num_ctas > 0 && p.num_ctas < most ? p.num_ctas : most;
+  const int sms = most_ctas() / 2, most = sms * (3 - SLOTS), ctas = p.num_ctas > 0 && p.num_ctas < most ? p.num_ctas : most;
   int joins = sms * kJoinPerSm;
   if (p.num_ctas > 0 && p.num_ctas < joins) joins = p.num_ctas;
-  if (launch_kernel(early_first(p.early_start), attn_tree_kernel<HD>, ctas, kThreads, C::kBytes, stream, 1, tm_q, tm_kv, p, ws) != cudaSuccess ||
-      launch_kernel(early_further(p.early_start), attn_tree_join_kernel<HD>, joins, kJoinWarps * 32, 0, stream, 1, p, ws, ctas) != cudaSuccess) {
+  if (launch_kernel(early_first(p.early_start), kernel, ctas, C::kThreads, C::kBytes, stream, 1, tm_q, tm_kv, p, ws) != cudaSuccess ||
+      launch_kernel(early_further(p.early_start), attn_tree_join_kernel<HD, SLOTS>, joins, kJoinWarps * 32, 0, stream, 1, p, ws, ctas) != cudaSuccess) {
     (void)cudaGetLastError();
     return NF_ERR_CUDA;
   }
@@ -994,5 +1000,8 @@ extern "C" int nfk_attn_tree(const nfk_attn_tree_params* p, cudaStream_t stream)
       (p->tree != nullptr && (p->words < 1 || p->words > NFK_TREE_NODES / 64)) ||
       static_cast<long long>(p->num_pages) * 2 * p->kv_heads * kPage > 0x7fff0000ll)
     return NF_ERR_BAD_ARG;
-  return p->head_dim == 128 ? launch<128>(*p, stream) : launch<64>(*p, stream);
+  // Blocks of two slots where requests have more than 128 rows on average.
+  const bool wide = static_cast<long long>(p->num_tokens) * (p->q_heads / p->kv_heads) > 128ll * p->req_count;
+  if (p->head_dim == 128) return wide ? launch<128, 2>(*p, stream) : launch<128, 1>(*p, stream);
+  return wide ? launch<64, 2>(*p, stream) : launch<64, 1>(*p, stream);
 }
