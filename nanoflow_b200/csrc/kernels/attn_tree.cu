@@ -34,7 +34,8 @@ namespace {
 
 constexpr int kTile = 64;             // cached tokens per tile
 constexpr int kTilePages = kTile / kPage;
-constexpr float kGap = 8.f;           // log2 of how far a row's maximum may outgrow its reference
+constexpr float kGap = 8.f;           // log2 of how far a row's largest score may outgrow its reference where it is looked for,
+constexpr float kMostWeight = 16384.f;           // and the sum of a tile's weights from which on it is
 // What an item's beginning and end cost, in pages: where the work is cut, the ends count too.
 constexpr int kLead = 16;
 // Pages that a CTA takes at least, so that the states of short requests do not outweigh their pages.
@@ -648,38 +649,43 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           } else {
             sees = true;
           }
-          float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (NaN where there is one)
-          auto more = [&](int j) { mq[j & 3] = max3_nan(mq[j & 3], __uint_as_float(x[j >> 4][2 * (j & 15)]), __uint_as_float(x[j >> 4][2 * (j & 15) + 1])); };
           auto largest = [&]() {
+            float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (NaN where there is one)
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              mq[j & 3] = max3_nan(mq[j & 3], __uint_as_float(x[j >> 4][2 * (j & 15)]), __uint_as_float(x[j >> 4][2 * (j & 15) + 1]));
             const float mx = max3_nan(max3_nan(mq[0], mq[1], mq[2]), mq[3], mq[3]) * scale;
             if (mx < INFINITY) return mx;
             l = __uint_as_float(0x7fc00000u);    // a score of infinity, or none
             return 0.f;
           };
-          if (i == 0) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) more(j);
-            ref = largest();
-          }
-          // Weights relative to the reference as it is, while the largest score is found beside them: there is seldom more than one pass.
-          f32x2 rs[2];
-          uint32_t pk[32];                       // column j: tokens 2j, 2j + 1
-          for (;;) {
+          if (i == 0) ref = largest();
+          // Weights relative to the reference as it is. Only where their sum says that it has been left far behind (or that there is none
+          // yet, or a NaN) is the largest score looked for, and the weights are formed once more.
+          float sum;
+          for (bool again = false;; again = true) {
             const float ms = ref == -INFINITY ? 0.f : ref;
             const f32x2 scale2 = pair(scale, scale), ms2 = pair(-ms, -ms);
-            rs[0] = rs[1] = pair(0.f, 0.f);
-            mq[0] = mq[1] = mq[2] = mq[3] = -INFINITY;
+            f32x2 rs[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              more(j);
-              const float2 y = halves(fma2(pair(__uint_as_float(x[j >> 4][2 * (j & 15)]), __uint_as_float(x[j >> 4][2 * (j & 15) + 1])), scale2, ms2));
-              const float e0 = fast_exp2(y.x), e1 = fast_exp2(y.y);
-              rs[j & 1] = add2(rs[j & 1], pair(e0, e1));
-              pk[j] = pack_bf16x2(e0, e1);
+            for (int h = 0; h < 2; ++h) {
+              uint32_t pk[16];                   // column j: tokens 2j, 2j + 1
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const float2 y = halves(fma2(pair(__uint_as_float(x[h][2 * j]), __uint_as_float(x[h][2 * j + 1])), scale2, ms2));
+                const float e0 = fast_exp2(y.x), e1 = fast_exp2(y.y);
+                rs[j & 1] = add2(rs[j & 1], pair(e0, e1));
+                pk[j] = pack_bf16x2(e0, e1);
+              }
+              tmem_st_32x32b_x16(t_s + 16 * h, pk);
             }
+            const float2 both = halves(add2(rs[0], rs[1]));
+            sum = both.x + both.y;
+            const bool look = on && (!(sum < kMostWeight) || ref == -INFINITY);
+            if (again || !__any_sync(0xffffffffu, look)) break;
             const float mx = largest();
             const bool grow = mx > ref + kGap || (ref == -INFINITY && mx > -INFINITY);
-            if (!__any_sync(0xffffffffu, grow)) break;
+            if (i == 0 || !__any_sync(0xffffffffu, grow)) break;
             // Sums may be touched between two products only: that of the tile before is the last one issued (this tile's needs its weights)
             if (!passed(C::PV_DONE + slot * 2 + ((n_done - 1) & 1), (n_done - 1) >> 1 & 1)) { ok = false; break; }
             tc_fence_after();
@@ -693,14 +699,11 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
               tmem_st_32x32b_x16(t_o + c * 16, o);
             }
-            tmem_st_wait();
             l *= alpha;
             if (grow) ref = mx;
           }
           if (!ok) break;
-          tmem_st_32x32b_x32(t_s, pk);
-          const float2 t = halves(add2(rs[0], rs[1]));
-          l += t.x + t.y;
+          l += sum;
           tmem_st_wait();
           tc_fence_before();
         }
