@@ -13,9 +13,11 @@ namespace nf {
 namespace {
 
 constexpr int kPage = 16;
-constexpr int kThreads = 512;
+constexpr int kMostThreads = 1024, kMine = NFK_TABLES_REQUESTS / kMostThreads;   // requests of a thread at most
+// Threads of a CTA: barriers of many take longer, and few requests need no more.
+constexpr int kFewThreads = 256;
 // entries of the lists that a thread writes before there are further CTAs
-constexpr int kPerThread = 4;
+constexpr int kPerThread = 2;
 
 __device__ __forceinline__ int pages_of(int tokens) { return (tokens + kPage - 1) / kPage; }
 
@@ -37,50 +39,53 @@ __device__ __forceinline__ Sums sums_in(uint8_t* smem, int requests) {
 }
 int smem_bytes(int requests, int max_requests) { return (5 * requests + 3 + (max_requests + 31) / 32) * 4; }
 
-// at[k][r] = sum of what[k] of the requests in front of r; false where one does not fit 32 bits. Entries hold `what` before.
-__device__ __forceinline__ bool scan(const Sums& s, int requests, long long (&total)[3]) {
-  __shared__ long long warp_sum[3][kThreads / 32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int per = (requests + kThreads - 1) / kThreads, r0 = min(requests, static_cast<int>(threadIdx.x) * per), r1 = min(requests, r0 + per);
-  long long mine[3] = {0, 0, 0}, sum[3];
+// at[k][r] = sum of what[k] of the requests in front of r, `total` of all; entries hold `what` before, none negative. Sums end at the
+// largest int: a total of that says that they do not fit, and nothing else then means anything.
+constexpr unsigned int kFull = 0x7fffffffu;
+__device__ __forceinline__ unsigned int add(unsigned int a, unsigned int b) { return min(a + b, kFull); }
+__device__ __forceinline__ void scan(const Sums& s, int requests, int (&total)[3]) {
+  __shared__ unsigned int warp_sum[3][kMostThreads / 32];
+  const int threads = blockDim.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (requests + threads - 1) / threads, r0 = min(requests, static_cast<int>(threadIdx.x) * per), r1 = min(requests, r0 + per);
+  unsigned int mine[3] = {0, 0, 0}, sum[3];
   for (int r = r0; r < r1; ++r)
 #pragma unroll
-    for (int k = 0; k < 3; ++k) mine[k] += s.at[k][r];
+    for (int k = 0; k < 3; ++k) mine[k] = add(mine[k], s.at[k][r]);
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    sum[k] = mine[k];
+  for (int k = 0; k < 3; ++k) sum[k] = mine[k];
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long v = __shfl_up_sync(0xffffffffu, sum[k], o);
-      if (lane >= o) sum[k] += v;
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const unsigned int v = __shfl_up_sync(0xffffffffu, sum[k], o);
+      if (lane >= o) sum[k] = add(sum[k], v);
     }
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
     if (lane == 31) warp_sum[k][warp] = sum[k];
-  }
   __syncthreads();
-  bool fits = true;
+  unsigned int own[3], up[3];                    // the warps' sums, by every warp for itself
+#pragma unroll
+  for (int k = 0; k < 3; ++k) own[k] = up[k] = lane < threads / 32 ? warp_sum[k][lane] : 0u;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1)
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      const unsigned int v = __shfl_up_sync(0xffffffffu, up[k], o);
+      if (lane >= o) up[k] = add(up[k], v);
+    }
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
-    long long before = sum[k] - mine[k];
-    total[k] = 0;
-#pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) {
-      const long long v = warp_sum[k][w];
-      if (w < warp) before += v;
-      total[k] += v;
+    total[k] = static_cast<int>(__shfl_sync(0xffffffffu, up[k], 31));
+    unsigned int a = __shfl_sync(0xffffffffu, up[k] - own[k], warp) + sum[k] - mine[k];
+    for (int r = r0; r < r1; ++r) {
+      const unsigned int n = s.at[k][r];
+      s.at[k][r] = static_cast<int>(a);
+      a += n;
     }
-    fits = fits && total[k] <= 0x7fffffff;
-    if (total[k] <= 0x7fffffff) {
-      int a = static_cast<int>(before);
-      for (int r = r0; r < r1; ++r) {
-        const int n = s.at[k][r];
-        s.at[k][r] = a;
-        a += n;
-      }
-      if (threadIdx.x == 0) s.at[k][requests] = static_cast<int>(total[k]);
-    }
+    if (threadIdx.x == 0) s.at[k][requests] = total[k];
   }
   __syncthreads();
-  return fits;
 }
 // The request that entry e belongs to: the last one with at[r] <= e.
 __device__ __forceinline__ int holder(const int* at, int requests, int e) {
@@ -98,40 +103,49 @@ __device__ __forceinline__ int holder(const int* at, int requests, int e) {
 }
 // Requests as they come, into row, old and at[0] (tokens); false, for all threads, where one is none.
 __device__ __forceinline__ bool read_requests(const nfk_tables_params& p, const Sums& s) {
-  const int words = (p.max_requests + 31) / 32;
-  for (int w = threadIdx.x; w < words; w += kThreads) s.taken[w] = 0;
+  const int words = (p.max_requests + 31) / 32, threads = blockDim.x;
+  for (int w = threadIdx.x; w < words; w += threads) s.taken[w] = 0;
+  int row[kMine], n[kMine], old[kMine];          // all of a thread's loads on their way at once
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int r = threadIdx.x + k * threads;
+    row[k] = r < p.requests ? p.rows[r] : -1;
+    n[k] = r < p.requests ? p.tokens[r] : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) old[k] = row[k] >= 0 && row[k] < p.max_requests ? p.lengths[row[k]] : -1;
   __syncthreads();
   bool bad = false;
-  for (int r = threadIdx.x; r < p.requests; r += kThreads) {
-    const int row = p.rows[r], n = p.tokens[r];
-    bool ok = row >= 0 && row < p.max_requests && n >= 0;
-    if (ok) ok = (atomicOr(&s.taken[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u) == 0u;
-    const int old = ok ? p.lengths[row] : 0;
-    ok = ok && old >= 0 && old <= p.max_pages * kPage;
-    s.row[r] = row;
-    s.old[r] = old;
-    s.at[0][r] = n;
+#pragma unroll
+  for (int k = 0; k < kMine; ++k) {
+    const int r = threadIdx.x + k * threads;
+    if (r >= p.requests) continue;
+    bool ok = old[k] >= 0 && old[k] <= p.max_pages * kPage && n[k] >= 0;
+    if (ok) ok = (atomicOr(&s.taken[row[k] >> 5], 1u << (row[k] & 31)) >> (row[k] & 31) & 1u) == 0u;
+    s.row[r] = row[k];
+    s.old[r] = ok ? old[k] : 0;
+    s.at[0][r] = n[k];
     bad = bad || !ok;
   }
   return __syncthreads_or(bad) == 0;
 }
-// Whether this CTA is the last one to have read what the call changes; all threads.
-__device__ __forceinline__ bool last_reader(unsigned int* ticket) {
-  if (gridDim.x == 1) return true;               // (behind a barrier of the block)
-  __shared__ int last;
-  if (threadIdx.x == 0) {
+// How many CTAs before this one have read what the call changes: asked behind a barrier of the block, by thread 0, and looked at in the end.
+__device__ __forceinline__ unsigned int take_ticket(unsigned int* ticket) {
+  if (threadIdx.x != 0 || gridDim.x == 1) return 0;
+  __threadfence();
+  return atomicAdd(ticket, 1u);
+}
+// Whether this CTA was the last of them; for all threads.
+__device__ __forceinline__ bool last_reader(unsigned int* ticket, unsigned int mine) {
+  const bool last = __syncthreads_or(threadIdx.x == 0 && mine == gridDim.x - 1) != 0;
+  if (last && threadIdx.x == 0 && gridDim.x > 1) {
+    *ticket = 0;
     __threadfence();
-    last = atomicAdd(ticket, 1u) == gridDim.x - 1;
-    if (last) {
-      *ticket = 0;
-      __threadfence();
-    }
   }
-  __syncthreads();
-  return last != 0;
+  return last;
 }
 
-__global__ void __launch_bounds__(kThreads) tables_grow_kernel(nfk_tables_params p) {
+__global__ void __launch_bounds__(kMostThreads) tables_grow_kernel(const __grid_constant__ nfk_tables_params p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const Sums s = sums_in(smem, p.requests);
   const int R = p.requests;
@@ -139,10 +153,10 @@ __global__ void __launch_bounds__(kThreads) tables_grow_kernel(nfk_tables_params
   await_previous();
   const int free_count = *p.free_count;
   bool ok = read_requests(p, s) && free_count >= 0 && free_count <= p.num_pages;
-  long long total[3] = {0, 0, 0};                // tokens, pages, pages taken
+  int total[3] = {0, 0, 0};                      // tokens, pages, pages taken
   if (ok) {
     bool bad = false;
-    for (int r = threadIdx.x; r < R; r += kThreads) {
+    for (int r = threadIdx.x; r < R; r += blockDim.x) {
       const int old = s.old[r], n = s.at[0][r];
       if (n > p.max_pages * kPage - old) {
         bad = true;
@@ -153,13 +167,17 @@ __global__ void __launch_bounds__(kThreads) tables_grow_kernel(nfk_tables_params
     }
     ok = __syncthreads_or(bad) == 0;
   }
-  if (ok) ok = scan(s, R, total) && total[0] <= p.num_tokens && total[1] <= p.num_indices && total[2] <= free_count;
-  const bool last = last_reader(p.ticket);
+  if (ok) {
+    scan(s, R, total);
+    const int most = static_cast<int>(kFull) - 1;
+    ok = total[0] <= min(p.num_tokens, most) && total[1] <= min(p.num_indices, most) && total[2] <= free_count;
+  }
+  const unsigned int ticket = take_ticket(p.ticket);
   if (!ok) {
     total[0] = total[1] = 0;
-    if (last && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
+    if (blockIdx.x == 0 && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
   }
-  const int at = blockIdx.x * kThreads + threadIdx.x, step = gridDim.x * kThreads;
+  const int at = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
   for (int r = at; r <= R; r += step) {
     p.qo_indptr[r] = ok ? s.at[0][r] : 0;
     p.kv_indptr[r] = ok ? s.at[1][r] : 0;
@@ -173,14 +191,14 @@ __global__ void __launch_bounds__(kThreads) tables_grow_kernel(nfk_tables_params
     const int had = pages_of(s.old[r]);
     return i < had ? p.table[static_cast<long long>(s.row[r]) * p.max_pages + i] : p.free_pages[free_count - 1 - (s.at[2][r] + i - had)];
   };
-  for (int e = at; e < static_cast<int>(total[1]); e += step) {
+  for (int e = at; e < total[1]; e += step) {
     const int r = holder(s.at[1], R, e), i = e - s.at[1][r], id = page(r, i);
     p.kv_indices[e] = id;
     if (i >= pages_of(s.old[r])) p.table[static_cast<long long>(s.row[r]) * p.max_pages + i] = id;
   }
   for (int t = at; t < p.num_tokens; t += step) {
     int pos = 0, req = -1, slot = -1;
-    if (t < static_cast<int>(total[0])) {
+    if (t < total[0]) {
       req = holder(s.at[0], R, t);
       pos = s.old[req] + t - s.at[0][req];
       slot = page(req, pos / kPage) * kPage + pos % kPage;
@@ -189,13 +207,13 @@ __global__ void __launch_bounds__(kThreads) tables_grow_kernel(nfk_tables_params
     p.token_req[t] = req;
     p.slots[t] = slot;
   }
-  if (last && ok) {
-    for (int r = threadIdx.x; r < R; r += kThreads) p.lengths[s.row[r]] = s.old[r] + s.at[0][r + 1] - s.at[0][r];
-    if (threadIdx.x == 0) *p.free_count = free_count - static_cast<int>(total[2]);
+  if (last_reader(p.ticket, ticket) && ok) {
+    for (int r = threadIdx.x; r < R; r += blockDim.x) p.lengths[s.row[r]] = s.old[r] + s.at[0][r + 1] - s.at[0][r];
+    if (threadIdx.x == 0) *p.free_count = free_count - total[2];
   }
 }
 
-__global__ void __launch_bounds__(kThreads) tables_trim_kernel(nfk_tables_params p) {
+__global__ void __launch_bounds__(kMostThreads) tables_trim_kernel(const __grid_constant__ nfk_tables_params p) {
   extern __shared__ __align__(16) uint8_t smem[];
   const Sums s = sums_in(smem, p.requests);
   const int R = p.requests;
@@ -203,9 +221,9 @@ __global__ void __launch_bounds__(kThreads) tables_trim_kernel(nfk_tables_params
   await_previous();
   const int free_count = *p.free_count;
   bool ok = read_requests(p, s) && free_count >= 0 && free_count <= p.num_pages;
-  long long total[3] = {0, 0, 0};                // new lengths (their sums are not looked at), unused, pages that come free
+  int total[3] = {0, 0, 0};                      // new lengths (their sums are not looked at), unused, pages that come free
   if (ok) {
-    for (int r = threadIdx.x; r < R; r += kThreads) {
+    for (int r = threadIdx.x; r < R; r += blockDim.x) {
       const int old = s.old[r], length = old - min(s.at[0][r], old);
       s.at[0][r] = length;
       s.at[1][r] = 0;
@@ -213,21 +231,18 @@ __global__ void __launch_bounds__(kThreads) tables_trim_kernel(nfk_tables_params
       s.old[r] = length;
     }
     __syncthreads();
-    (void)scan(s, R, total);
+    scan(s, R, total);
     ok = total[2] <= p.num_pages - free_count;
   }
-  const bool last = last_reader(p.ticket);
-  if (!ok) {
-    if (last && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
-    return;
-  }
-  const int n = static_cast<int>(total[2]);
-  for (int e = blockIdx.x * kThreads + threadIdx.x; e < n; e += gridDim.x * kThreads) {
+  const unsigned int ticket = take_ticket(p.ticket);
+  if (!ok && blockIdx.x == 0 && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
+  const int n = ok ? total[2] : 0;
+  for (int e = blockIdx.x * blockDim.x + threadIdx.x; e < n; e += gridDim.x * blockDim.x) {
     const int r = holder(s.at[2], R, e);
     p.free_pages[free_count + n - 1 - e] = p.table[static_cast<long long>(s.row[r]) * p.max_pages + pages_of(s.old[r]) + e - s.at[2][r]];
   }
-  if (last) {
-    for (int r = threadIdx.x; r < R; r += kThreads) p.lengths[s.row[r]] = s.old[r];
+  if (last_reader(p.ticket, ticket) && ok) {
+    for (int r = threadIdx.x; r < R; r += blockDim.x) p.lengths[s.row[r]] = s.old[r];
     if (threadIdx.x == 0) *p.free_count = free_count + n;
   }
 }
@@ -245,10 +260,11 @@ int launch(const nfk_tables_params& p, long long entries, cudaStream_t stream) {
     }
     attr = true;
   }
-  long long ctas = (entries + kThreads * kPerThread - 1) / (kThreads * kPerThread);
+  const int threads = p.requests <= kFewThreads && entries <= 8ll * kFewThreads * kPerThread ? kFewThreads : kMostThreads;
+  long long ctas = (entries + threads * kPerThread - 1) / (threads * kPerThread);
   if (ctas > device_sm_count()) ctas = device_sm_count();
   if (ctas < 1) ctas = 1;
-  if (launch_kernel(early_first(p.early_start), kernel, static_cast<int>(ctas), kThreads, bytes, stream, 1, p) == cudaSuccess) return NF_OK;
+  if (launch_kernel(early_first(p.early_start), kernel, static_cast<int>(ctas), threads, bytes, stream, 1, p) == cudaSuccess) return NF_OK;
   (void)cudaGetLastError();
   return NF_ERR_CUDA;
 }
@@ -278,5 +294,5 @@ extern "C" int nfk_tables_trim(const nfk_tables_params* p, cudaStream_t stream) 
   const int rc = check(p);
   if (rc != NF_OK) return rc;
   if (p->requests == 0) return NF_OK;
-  return launch<false>(*p, static_cast<long long>(p->requests) * 64, stream);
+  return launch<false>(*p, static_cast<long long>(p->requests) * 16, stream);
 }

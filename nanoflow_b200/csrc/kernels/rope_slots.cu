@@ -21,35 +21,25 @@ __device__ __forceinline__ float2 turn(int pos, float w, float factor) {
   sincospif(2.f * static_cast<float>(t - rint(t)), &s, &c);
   return make_float2(c * factor, s * factor);
 }
-__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
-  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    f[2 * j] = __uint_as_float(w[j] << 16);
-    f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-  }
-}
-__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
-  return make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-}
+// Two neighbouring elements of a word, and back.
+__device__ __forceinline__ float2 elements(uint32_t w) { return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
 
 // Which elements a thread's two vectors of eight hold: HALVES the two of its eight pairs (pairs a multiple of eight), NEIGHBOURS and
-// SCATTERED 16 elements in a row; SCATTERED (half layout, any number of pairs) fetches each element's partner by itself.
+// SCATTERED 16 elements in a row; SCATTERED (half layout, any number of pairs) finds each element's partner in shared memory.
 enum { HALVES, NEIGHBOURS, SCATTERED };
 
 // A CTA per token, HD / 16 threads per head, the same elements of each head that they take, so that their cosines and sines stay in
-// registers. Three heads a thread are requested before the token's angles are worked out.
+// registers. Three heads a thread are requested before the token's angles are worked out; what hides their latency beyond that is the
+// number of CTAs, of which 64 registers let eight share an SM.
 template <int HD, int LAYOUT>
-__global__ void __launch_bounds__(kThreads) rope_slots_kernel(nfk_rope_slots_params p) {
+__global__ void __launch_bounds__(kThreads, LAYOUT == SCATTERED ? 6 : 8) rope_slots_kernel(const __grid_constant__ nfk_rope_slots_params p) {
   constexpr int LPH = HD / 16, AT_ONCE = kThreads / LPH, BATCH = 3;
   __shared__ __align__(16) float cosines[HD / 2], sines[HD / 2];
+  __shared__ __align__(16) __nv_bfloat16 raw[LAYOUT == SCATTERED ? AT_ONCE : 1][HD];     // of the heads at hand
   const int l = threadIdx.x % LPH, h0 = threadIdx.x / LPH, t = blockIdx.x, rot = 2 * p.pairs;
   const int heads = p.q_heads + 2 * p.kv_heads;
-  int ea = 16 * l, eb = 16 * l + 8;
-  if (LAYOUT == HALVES && 16 * l < rot) {
-    ea = 8 * l;
-    eb = 8 * l + p.pairs;
-  }
+  const bool apart = LAYOUT == HALVES && 16 * l < rot;
+  const int ea = apart ? 8 * l : 16 * l, eb = apart ? 8 * l + p.pairs : 16 * l + 8;
   const __nv_bfloat16* row = static_cast<const __nv_bfloat16*>(p.qkv) + t * p.ld_qkv;
   auto source = [&](int h) {
     return row + (h < p.q_heads ? p.q_off + h * HD : h < p.q_heads + p.kv_heads ? p.k_off + (h - p.q_heads) * HD
@@ -61,8 +51,8 @@ __global__ void __launch_bounds__(kThreads) rope_slots_kernel(nfk_rope_slots_par
     for (int i = 0; i < BATCH; ++i) {
       const int h = first + i * AT_ONCE + h0;
       if (h >= heads) continue;
-      a[i] = *reinterpret_cast<const uint4*>(source(h) + ea);
-      b[i] = *reinterpret_cast<const uint4*>(source(h) + eb);
+      a[i] = __ldcs(reinterpret_cast<const uint4*>(source(h) + ea));
+      b[i] = __ldcs(reinterpret_cast<const uint4*>(source(h) + eb));
     }
   };
   let_next_start();
@@ -77,27 +67,75 @@ __global__ void __launch_bounds__(kThreads) rope_slots_kernel(nfk_rope_slots_par
   __syncthreads();
   const bool cached = slot >= 0 && slot < p.num_pages * kPage;
   if (slot >= p.num_pages * kPage && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
-  // element e turns with its partner: f e' = e c + partner s, s negative for the first one of a pair
-  float c[16], s[16];
+  // of the thread's eight pairs; of those that do not turn, what leaves them as they are is not (0 times infinity), so there is a bit each
+  constexpr int N = LAYOUT == SCATTERED ? 16 : 8;
+  float c[N], s[N];
   uint32_t turning = 0;
 #pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    const int e = j < 8 ? ea + j : eb + j - 8;
-    const bool turns = e < rot;
-    const int i = LAYOUT == NEIGHBOURS ? e >> 1 : e < p.pairs ? e : e - p.pairs;
-    const bool second = LAYOUT == NEIGHBOURS ? (e & 1) != 0 : e >= p.pairs;
-    c[j] = turns ? cosines[i] : 1.f;
-    s[j] = turns ? (second ? sines[i] : -sines[i]) : 0.f;
-    turning |= turns ? 1u << j : 0u;
+  for (int j = 0; j < N; ++j) {
+    if (LAYOUT == SCATTERED) {
+      const int e = 16 * l + j, i = e < p.pairs ? e : e - p.pairs;
+      const bool turns = e < rot;
+      c[j] = turns ? cosines[i] : 0.f;
+      s[j] = turns ? (e < p.pairs ? -sines[i] : sines[i]) : 0.f;
+      turning |= turns ? 1u << j : 0u;
+    } else {
+      const int i = 8 * l + j;
+      const bool turns = i < p.pairs;
+      c[j] = turns ? cosines[i] : 0.f;
+      s[j] = turns ? sines[i] : 0.f;
+      turning |= turns ? 1u << j : 0u;
+    }
   }
   for (int first = 0; first < heads; first += BATCH * AT_ONCE) {
     if (first > 0) load(first);
 #pragma unroll
     for (int i = 0; i < BATCH; ++i) {
+      if (first + i * AT_ONCE >= heads) break;   // (the same for all threads)
       const int h = first + i * AT_ONCE + h0;
-      if (h >= heads) continue;
-      const bool is_q = h < p.q_heads, is_v = h >= p.q_heads + p.kv_heads;
-      if (!is_q && !cached) continue;
+      const bool on = h < heads, is_q = h < p.q_heads, is_v = h >= p.q_heads + p.kv_heads;
+      uint32_t va[4] = {a[i].x, a[i].y, a[i].z, a[i].w}, vb[4] = {b[i].x, b[i].y, b[i].z, b[i].w};
+      if (LAYOUT == SCATTERED) {
+        __syncwarp();                            // (a head's threads are of one warp)
+        if (on) {
+          *reinterpret_cast<uint4*>(&raw[h0][ea]) = a[i];
+          *reinterpret_cast<uint4*>(&raw[h0][eb]) = b[i];
+        }
+        __syncwarp();
+      }
+      if (!on || (!is_q && !cached)) continue;
+      if (!is_v && turning != 0u) {
+        if (LAYOUT == HALVES) {                  // (all eight pairs turn or none does)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float2 x = elements(va[k]), y = elements(vb[k]);
+            va[k] = pack_bf16x2(fmaf(y.x, -s[2 * k], x.x * c[2 * k]), fmaf(y.y, -s[2 * k + 1], x.y * c[2 * k + 1]));
+            vb[k] = pack_bf16x2(fmaf(x.x, s[2 * k], y.x * c[2 * k]), fmaf(x.y, s[2 * k + 1], y.y * c[2 * k + 1]));
+          }
+        } else if (LAYOUT == NEIGHBOURS) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            uint32_t& w = k < 4 ? va[k & 3] : vb[k & 3];
+            const float2 x = elements(w);
+            if ((turning >> k & 1u) != 0u) w = pack_bf16x2(fmaf(x.y, -s[k], x.x * c[k]), fmaf(x.x, s[k], x.y * c[k]));
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            uint32_t& w = k < 4 ? va[k & 3] : vb[k & 3];
+            float2 x = elements(w);
+            float* const at[2] = {&x.x, &x.y};
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              const int j = 2 * k + q, e = 16 * l + j;
+              if ((turning >> (j & (N - 1)) & 1u) == 0u) continue;
+              const float other = __bfloat162float(raw[h0][e < p.pairs ? e + p.pairs : e - p.pairs]);
+              *at[q] = fmaf(other, s[j & (N - 1)], *at[q] * c[j & (N - 1)]);
+            }
+            if ((turning >> (2 * k & (N - 1)) & 3u) != 0u) w = pack_bf16x2(x.x, x.y);
+          }
+        }
+      }
       __nv_bfloat16* dst;
       if (is_q) {
         dst = static_cast<__nv_bfloat16*>(p.q_out) + (static_cast<long long>(t) * p.q_heads + h) * HD;
@@ -105,33 +143,8 @@ __global__ void __launch_bounds__(kThreads) rope_slots_kernel(nfk_rope_slots_par
         const int hh = h - p.q_heads - (is_v ? p.kv_heads : 0);
         dst = static_cast<__nv_bfloat16*>(p.kv_pool) + (((static_cast<long long>(slot / kPage) * 2 + (is_v ? 1 : 0)) * p.kv_heads + hh) * kPage + slot % kPage) * HD;
       }
-      uint4 va = a[i], vb = b[i];
-      if (!is_v) {
-        float x[8], y[8], u[8], v[8];
-        unpack8(va, x);
-        unpack8(vb, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float px, py;                          // partners
-          if (LAYOUT == HALVES) {
-            px = y[j];
-            py = x[j];
-          } else if (LAYOUT == NEIGHBOURS) {
-            px = x[j ^ 1];
-            py = y[j ^ 1];
-          } else {
-            const int e0 = ea + j, e1 = eb + j;
-            px = e0 < rot ? __bfloat162float(source(h)[e0 < p.pairs ? e0 + p.pairs : e0 - p.pairs]) : 0.f;
-            py = e1 < rot ? __bfloat162float(source(h)[e1 < p.pairs ? e1 + p.pairs : e1 - p.pairs]) : 0.f;
-          }
-          u[j] = (turning >> j & 1u) != 0u ? fmaf(px, s[j], x[j] * c[j]) : x[j];
-          v[j] = (turning >> (8 + j) & 1u) != 0u ? fmaf(py, s[8 + j], y[j] * c[8 + j]) : y[j];
-        }
-        va = pack8(u);
-        vb = pack8(v);
-      }
-      *reinterpret_cast<uint4*>(dst + ea) = va;
-      *reinterpret_cast<uint4*>(dst + eb) = vb;
+      *reinterpret_cast<uint4*>(dst + ea) = make_uint4(va[0], va[1], va[2], va[3]);
+      *reinterpret_cast<uint4*>(dst + eb) = make_uint4(vb[0], vb[1], vb[2], vb[3]);
     }
   }
 }

@@ -123,20 +123,21 @@ __global__ void __launch_bounds__(kAcceptWarps * 32) tree_accept_kernel(nfk_tree
 }
 
 // A CTA per (request, pool). A thread moves the same 16 bytes of the same head of every token, in the order of the path: token path[k] never
-// lies in front of place k, so that what a move overwrites has been moved before; eight moves' loads are on their way at once.
-constexpr int kKeepThreads = 256, kAhead = 8;
-__global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(nfk_kv_keep_params p) {
+// lies in front of place k, so that what a move overwrites has been moved before; four moves' loads are on their way at once. A chain of
+// loads (lists and path, slots, vectors) takes most of a CTA's time, which other CTAs fill: registers for six to an SM (48 requests of up
+// to 60 tokens, 32 pools: with eight loads and four CTAs 2 us longer, with two pools to a CTA 4).
+constexpr int kKeepThreads = 256, kAhead = 4;
+__global__ void __launch_bounds__(kKeepThreads, 6) kv_keep_kernel(const __grid_constant__ nfk_kv_keep_params p) {
   __shared__ int from_s[NFK_TREE_NODES], to_s[NFK_TREE_NODES], moves_s;
   const int r = blockIdx.x / p.num_pools, pool = blockIdx.x - r * p.num_pools;
   let_next_start();
   await_previous();
   const int a = p.qo_indptr[r], b = p.qo_indptr[r + 1];
+  const int* path = p.path + static_cast<long long>(r) * p.max_path;
+  const int first = threadIdx.x < static_cast<unsigned int>(p.max_path) ? path[threadIdx.x] : -1;      // (with the lists, not behind them)
   int count = p.counts[r];
   bool bad = a < 0 || b < a || b > p.num_tokens || count < 0 || count > p.max_path || count > b - a || count > NFK_TREE_NODES;
   if (bad) count = 0;
-  const int* path = p.path + static_cast<long long>(r) * p.max_path;
-  if (threadIdx.x == 0) moves_s = 0;
-  __syncthreads();
   // moves that change something, in their order; by one warp
   if (threadIdx.x < 32) {
     int moves = 0;
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kKeepThreads) kv_keep_kernel(nfk_kv_keep_param
       const int k = k0 + threadIdx.x;
       int from = -1, to = -1;
       if (k < count) {
-        const int i = path[k];
+        const int i = k0 == 0 ? first : path[k];
         const bool ok = i >= k && i < b - a;
         if (ok && i != k) {
           from = p.slots[a + i];
