@@ -32,7 +32,7 @@ enum { HALVES, NEIGHBOURS, SCATTERED };
 // registers. Three heads a thread are requested before the token's angles are worked out; what hides their latency beyond that is the
 // number of CTAs, of which 64 registers let eight share an SM.
 template <int HD, int LAYOUT>
-__global__ void __launch_bounds__(kThreads, LAYOUT == SCATTERED ? 6 : 8) rope_slots_kernel(const __grid_constant__ nfk_rope_slots_params p) {
+__global__ void __launch_bounds__(kThreads, 8) rope_slots_kernel(const __grid_constant__ nfk_rope_slots_params p) {
   constexpr int LPH = HD / 16, AT_ONCE = kThreads / LPH, BATCH = 3;
   __shared__ __align__(16) float cosines[HD / 2], sines[HD / 2];
   __shared__ __align__(16) __nv_bfloat16 raw[LAYOUT == SCATTERED ? AT_ONCE : 1][HD];     // of the heads at hand
@@ -68,18 +68,13 @@ __global__ void __launch_bounds__(kThreads, LAYOUT == SCATTERED ? 6 : 8) rope_sl
   const bool cached = slot >= 0 && slot < p.num_pages * kPage;
   if (slot >= p.num_pages * kPage && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
   // of the thread's eight pairs; of those that do not turn, what leaves them as they are is not (0 times infinity), so there is a bit each
-  constexpr int N = LAYOUT == SCATTERED ? 16 : 8;
-  float c[N], s[N];
+  float c[8], s[8];
   uint32_t turning = 0;
+  if (LAYOUT == SCATTERED) {
+    turning = 16 * l < rot ? 1u : 0u;            // (its cosines and sines stay in shared memory)
+  } else {
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    if (LAYOUT == SCATTERED) {
-      const int e = 16 * l + j, i = e < p.pairs ? e : e - p.pairs;
-      const bool turns = e < rot;
-      c[j] = turns ? cosines[i] : 0.f;
-      s[j] = turns ? (e < p.pairs ? -sines[i] : sines[i]) : 0.f;
-      turning |= turns ? 1u << j : 0u;
-    } else {
+    for (int j = 0; j < 8; ++j) {
       const int i = 8 * l + j;
       const bool turns = i < p.pairs;
       c[j] = turns ? cosines[i] : 0.f;
@@ -105,14 +100,14 @@ __global__ void __launch_bounds__(kThreads, LAYOUT == SCATTERED ? 6 : 8) rope_sl
       }
       if (!on || (!is_q && !cached)) continue;
       if (!is_v && turning != 0u) {
-        if (LAYOUT == HALVES) {                  // (all eight pairs turn or none does)
+        if constexpr (LAYOUT == HALVES) {        // (all eight pairs turn or none does)
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const float2 x = elements(va[k]), y = elements(vb[k]);
             va[k] = pack_bf16x2(fmaf(y.x, -s[2 * k], x.x * c[2 * k]), fmaf(y.y, -s[2 * k + 1], x.y * c[2 * k + 1]));
             vb[k] = pack_bf16x2(fmaf(x.x, s[2 * k], y.x * c[2 * k]), fmaf(x.y, s[2 * k + 1], y.y * c[2 * k + 1]));
           }
-        } else if (LAYOUT == NEIGHBOURS) {
+        } else if constexpr (LAYOUT == NEIGHBOURS) {
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             uint32_t& w = k < 4 ? va[k & 3] : vb[k & 3];
@@ -123,16 +118,15 @@ __global__ void __launch_bounds__(kThreads, LAYOUT == SCATTERED ? 6 : 8) rope_sl
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
             uint32_t& w = k < 4 ? va[k & 3] : vb[k & 3];
+            const int e0 = 16 * l + 2 * k;
+            if (e0 >= rot) continue;
             float2 x = elements(w);
-            float* const at[2] = {&x.x, &x.y};
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const int j = 2 * k + q, e = 16 * l + j;
-              if ((turning >> (j & (N - 1)) & 1u) == 0u) continue;
-              const float other = __bfloat162float(raw[h0][e < p.pairs ? e + p.pairs : e - p.pairs]);
-              *at[q] = fmaf(other, s[j & (N - 1)], *at[q] * c[j & (N - 1)]);
-            }
-            if ((turning >> (2 * k & (N - 1)) & 3u) != 0u) w = pack_bf16x2(x.x, x.y);
+            auto turned = [&](int e, float own) {
+              const int i = e < p.pairs ? e : e - p.pairs;
+              const float other = __bfloat162float(raw[h0][e < p.pairs ? e + p.pairs : i]);
+              return fmaf(other, e < p.pairs ? -sines[i] : sines[i], own * cosines[i]);
+            };
+            w = pack_bf16x2(turned(e0, x.x), turned(e0 + 1, x.y));       // (rot is even)
           }
         }
       }
