@@ -1,25 +1,35 @@
 // Attention of drafted tokens (trees or chains, one to some hundred tokens a request) over the paged bf16 cache, on the 5th-generation
 // tensor cores:  o = sum_j e^(s_j) v_j / sum_j e^(s_j),  s_j = sm_scale q.k_j  over the tokens j that the query's token sees.
 //
-// The rows of an item are those query rows of a request that share a KV head (tokens x group), in blocks of up to 256. Every key and
-// value is read once per block, 4 head_dim operations a row for 4 head_dim bytes: the cache's bytes bound it below some 250 rows, the
-// products (and 2^x, 16 a clock and SM, which takes as long as both products of a tile) above.
+// The rows of an item are those query rows of a request that share a KV head (tokens x group), in blocks of 128 (one slot) or of up to 256
+// (two). Every key and value is read once per block, 4 head_dim operations a row for 4 head_dim bytes: the cache's bytes bound it below some
+// 250 rows, the products above. In between and beyond, what a tile waits for is what counts: scores, their 2^x (16 a clock and SM, which
+// takes as long as both products at their full rate), weights, sums follow one another, and no stage of it is ever the only one.
 //
-// A CTA has an SM to itself and two slots of 128 rows, each with scores and sums of its own in tensor memory, so that one slot's softmax
-// runs under the other's products. Up to 128 rows, both slots hold the same rows and take turns at the tiles of 128 tokens, and their
-// states are joined at the end; up to 256, each has its own rows and both take every tile.
-//
-//   8 warps     softmax, a thread per row: a tile's 128 scores to registers, running maximum and sum, weights as bf16 pairs back over
-//               the scores' columns, the A operand of the second product
-//   1 warp      copies (TMA, no multicast): queries, and keys and values page by page into a ring; walks the work
-//   1 warp      tcgen05.mma
+// Tiles are of 64 tokens, and a slot has two buffers of scores in tensor memory: the next tile's scores are formed while the softmax goes
+// through this one's. Weights (bf16 pairs) go over the scores that they come from and are the second product's A operand from there.
+//   One slot:   two CTAs to an SM, of 7 warps: four of softmax (a thread per row), one that copies keys (TMA, page by page into a ring),
+//               one that copies values, one of products. A CTA's softmax runs under the other's products.
+//   Two slots:  a CTA to an SM, of 12 warps: eight of softmax, the two of copies, one of products for each slot. Up to 128 rows both
+//               slots hold the same rows and take turns at the tiles, and their states are joined at the end; up to 256 each has its own
+//               rows and both take every tile.
+// A product of 128 x 64 x 16 takes as long as one of 128 x 128 x 16 (63 clocks), so that scores run at half the tensor cores' rate; tiles
+// of 128 tokens leave room for one buffer of scores only, and cost more than they gain: with the weights over the scores 32 x 64 tokens
+// of 512 rows take 470 us against 287, with the weights by way of shared memory 339 (of which rings of a tile and a half are the most).
+// Two threads to a row, 375. Of those 287 us 2^x is worth 12, half of the scores' products 13, the cache's way from HBM instead of the L2 10.
 //
 // Work is a row of pages of all requests, KV heads and blocks, cut evenly over the CTAs whatever the requests' lengths; an item that is
-// cut leaves a state (maximum, sum, sums of values) per piece, which a second kernel joins, in the order of the pieces: results do not
+// cut leaves a state (reference, sum, sums of values) per piece, which a second kernel joins, in the order of the pieces: results do not
 // depend on the order in which anything runs.
 //
-// Weights are rounded to bf16 (2^-9 of each on average), the type of the values that they meet in the product. Scores, maxima, sums and
-// states are fp32. The reference that weights are relative to moves (and sums are rescaled) where a row's maximum outgrows it by 2^8.
+// Weights are rounded to bf16 (at most 2^-8 of each), the type of the values that they meet in the product. Scores, references, sums and
+// states are fp32. Weights are relative to a reference, at first the first tile's largest score. The largest score of a further tile is
+// looked for only where the sum of its weights reaches 2^14, and the reference moves (sums are rescaled, the tile's weights formed anew)
+// where that score is above it by 2^8 or more: 286 us instead of 296 with a search in every tile.
+//
+// Measured (32 query and 8 KV heads of 128, a launch of both kernels in a graph): 64 requests of 5 tokens behind up to 4000 70 us (5.2 TB/s),
+// 256 single tokens behind up to 2000 147 us (5.9 TB/s), one of 60 behind 100000 115 us; with 64 query heads 32 of 64 tokens behind up to
+// 8000 287 us (0.85 PFLOP/s); one of 26 behind 2000 16 us, which is two launches, the scan of the lists and one tile's way through all of it.
 //
 // Only tiles with drafted tokens or the end of a piece need care: masks of 128 bits a row; and values that a row does not see must not
 // reach it as 0 * inf, so rows of values behind the end become zeros, as do infinities and NaN of drafted tokens, which the rows that do
@@ -35,10 +45,11 @@ namespace {
 constexpr int kTile = 64;             // cached tokens per tile
 constexpr int kTilePages = kTile / kPage;
 constexpr float kGap = 8.f;           // log2 of how far a row's largest score may outgrow its reference where it is looked for,
-constexpr float kMostWeight = 16384.f;           // and the sum of a tile's weights from which on it is
-// What an item's beginning and end cost, in pages: where the work is cut, the ends count too.
+constexpr float kMostWeight = 16384.f;           // and the sum of a tile's weights from which on it is: 64 weights of 2^kGap
+// What an item's beginning and end cost, in pages: where the work is cut, the ends count too. (8 or 24 change little, 0 leaves CTAs with
+// many short requests behind the others.)
 constexpr int kLead = 16;
-// Pages that a CTA takes at least, so that the states of short requests do not outweigh their pages.
+// Pages that a CTA takes at least, so that the states of short requests do not outweigh their pages. (4 and 16 take the same time within 3 %.)
 constexpr int kLeast = 8;
 
 // What the roles need to know of a piece.
@@ -1003,8 +1014,12 @@ extern "C" int nfk_attn_tree(const nfk_attn_tree_params* p, cudaStream_t stream)
       (p->tree != nullptr && (p->words < 1 || p->words > NFK_TREE_NODES / 64)) ||
       static_cast<long long>(p->num_pages) * 2 * p->kv_heads * kPage > 0x7fff0000ll)
     return NF_ERR_BAD_ARG;
-  // Blocks of two slots where requests have more than 128 rows on average.
+  // 128 elements a head: two slots to a CTA where requests have more than 128 rows on average, since both take every tile that has been
+  // read (32 requests of 64 tokens, 512 rows each: 287 us, by two CTAs of a slot 317; one of 240 rows behind 100000 tokens: 115 and 143;
+  // 8 of 160 rows behind 6000: 64.5 and 67.5; short contexts are the other way, 128 of 200 rows behind 350: 118 and 114; requests of one
+  // block of 128 take either form's one slot). 64 elements: always one slot, as its tiles are half as much to read and two CTAs wait less
+  // for one another than two slots (64 requests of 256 rows: 119 us against 135; 32 of 512: 211 and 243; one of 240 behind 100000: 92 and 107).
   const bool wide = static_cast<long long>(p->num_tokens) * (p->q_heads / p->kv_heads) > 128ll * p->req_count;
-  if (p->head_dim == 128) return wide ? launch<128, 2>(*p, stream) : launch<128, 1>(*p, stream);
-  return wide ? launch<64, 2>(*p, stream) : launch<64, 1>(*p, stream);
+  if (p->head_dim == 64) return launch<64, 1>(*p, stream);
+  return wide ? launch<128, 2>(*p, stream) : launch<128, 1>(*p, stream);
 }
