@@ -15,8 +15,9 @@
 //               rows and both take every tile.
 // A product of 128 x 64 x 16 takes as long as one of 128 x 128 x 16 (63 clocks), so that scores run at half the tensor cores' rate; tiles
 // of 128 tokens leave room for one buffer of scores only, and cost more than they gain: with the weights over the scores 32 x 64 tokens
-// of 512 rows take 470 us against 287, with the weights by way of shared memory 339 (of which rings of a tile and a half are the most).
-// Two threads to a row, 375. Of those 287 us 2^x is worth 12, half of the scores' products 13, the cache's way from HBM instead of the L2 10.
+// of 512 rows take 470 us against 287, with the weights by way of shared memory 339 (with rings of a tile and a half). Tiles of 64 tokens
+// with the weights by way of shared memory, so that nothing has to wait for the place of the scores: 325, since both products then read all
+// operands from there. Two threads to a row, 375. Of those 287 us 2^x is worth 12, half of the scores' products 13, the cache's way from HBM instead of the L2 10.
 //
 // Work is a row of pages of all requests, KV heads and blocks, cut evenly over the CTAs whatever the requests' lengths; an item that is
 // cut leaves a state (reference, sum, sums of values) per piece, which a second kernel joins, in the order of the pieces: results do not
@@ -24,7 +25,7 @@
 //
 // Weights are rounded to bf16 (at most 2^-8 of each), the type of the values that they meet in the product. Scores, references, sums and
 // states are fp32. Weights are relative to a reference, at first the first tile's largest score. The largest score of a further tile is
-// looked for only where the sum of its weights reaches 2^14, and the reference moves (sums are rescaled, the tile's weights formed anew)
+// looked for only where the sum of its weights reaches 2^14 times the weight of that, and the reference moves (sums are rescaled, the tile's weights formed anew)
 // where that score is above it by 2^8 or more: 286 us instead of 296 with a search in every tile.
 //
 // Measured (32 query and 8 KV heads of 128, a launch of both kernels in a graph): 64 requests of 5 tokens behind up to 4000 70 us (5.2 TB/s),
@@ -45,7 +46,10 @@ namespace {
 constexpr int kTile = 64;             // cached tokens per tile
 constexpr int kTilePages = kTile / kPage;
 constexpr float kGap = 8.f;           // log2 of how far a row's largest score may outgrow its reference where it is looked for,
-constexpr float kMostWeight = 16384.f;           // and the sum of a tile's weights from which on it is: 64 weights of 2^kGap
+// Weights are 2^-kSpare of what they would be: sums of many tokens with values next to bf16's largest stay finite, and a weight is lost
+// only where it is 2^-94 of the largest.
+constexpr float kSpare = 32.f;
+constexpr float kMostWeight = 16384.f / 4294967296.f;        // the sum of a tile's weights from which on it is: 64 weights of 2^kGap
 // What an item's beginning and end cost, in pages: where the work is cut, the ends count too. (8 or 24 change little, 0 leaves CTAs with
 // many short requests behind the others.)
 constexpr int kLead = 16;
@@ -675,7 +679,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           // yet, or a NaN) is the largest score looked for, and the weights are formed once more.
           float sum;
           for (bool again = false;; again = true) {
-            const float ms = ref == -INFINITY ? 0.f : ref;
+            const float ms = ref == -INFINITY ? 0.f : ref + kSpare;
             const f32x2 scale2 = pair(scale, scale), ms2 = pair(-ms, -ms);
             f32x2 rs[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll

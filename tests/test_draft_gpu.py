@@ -369,6 +369,16 @@ def test_masked_tokens_do_not_reach_a_row(value, side, lengths, nodes, H, G, d):
         assert seen.isnan().all()
 
 
+@pytest.mark.parametrize("lengths,nodes,H,G,d", [([30000], [64], 32, 8, 128), ([3000, 90], [20, 3], 8, 2, 128), ([5000, 2], [64, 1], 32, 8, 64)])
+def test_sums_of_the_largest_values_stay_finite(lengths, nodes, H, G, d):
+    """Values up to 2^127 (of either sign, so that what a row's sums pass through is larger than the row), one KV head of them all alike."""
+    b = _batch(18, lengths, nodes, H, G, d)
+    b["kv_pool"][:, 1] = (b["kv_pool"][:, 1].float().clamp(-4, 4) * 2.0 ** 125).to(torch.bfloat16)
+    b["kv_pool"][:, 1, 0] = 2.0 ** 127
+    ops.attn_tree(**b)
+    _near(b["out"], *_want(b))
+
+
 def test_rows_that_only_see_minus_infinity():
     b = _batch(10, [1, 2, 20], [1, 1, 1], 2, 1, 64, chain=True)
     b["q"].abs_()
