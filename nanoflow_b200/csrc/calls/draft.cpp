@@ -227,7 +227,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       p.words = static_cast<int>(tree->size(1));
     }
     p.sm_scale = a[11] == Py_None ? (c.head_dim == 128 ? 0.08838834764831845f : 0.125f) : real(a[11], what, "sm_scale");
-    if (!(p.sm_scale > 0.f) || p.sm_scale > 3e38f) refuse(what, "sm_scale must be positive and finite");
+    if (!(p.sm_scale > 0.f) || p.sm_scale > 2e38f) refuse(what, "sm_scale must be positive, up to 2e38");
+    if (q.size(0) > 0 && p.ld_out / 8 > 0xffffffffll / q.size(0)) refuse(what, "rows of out reach over more than 64 GB");
     p.num_ctas = whole(a[12], what, "num_ctas");
     if (a[13] == Py_None) refuse(what, "needs a workspace (tree_workspace)");
     const Tensor& workspace = checked(what, "workspace", a[13], at::kByte, device);

@@ -1014,7 +1014,9 @@ extern "C" int nfk_attn_tree(const nfk_attn_tree_params* p, cudaStream_t stream)
       off(p->out) || off(p->kv_pool) || (reinterpret_cast<uintptr_t>(p->workspace) & 255) != 0 || (reinterpret_cast<uintptr_t>(p->tree) & 7) != 0)
     return NF_ERR_BAD_ARG;
   if (p->num_tokens < 0 || p->num_pages <= 0 || p->num_indices < 0 || p->ld_q % 8 != 0 || p->ld_out % 8 != 0 || p->ld_q < row || p->ld_out < row ||
-      p->req_begin > 0x7fffffff - p->req_count || !(p->sm_scale > 0.f) || p->sm_scale > 3e38f || p->workspace_bytes < workspace_bytes(p->head_dim) ||
+      p->req_begin > 0x7fffffff - p->req_count || !(p->sm_scale > 0.f) || p->sm_scale > 2e38f ||
+      p->ld_q > (1ll << 38) || p->ld_out / 8 > 0xffffffffll / p->num_tokens ||             // (places of output rows: 16 bytes each, in 32 bits)
+      p->workspace_bytes < workspace_bytes(p->head_dim) ||
       (p->tree != nullptr && (p->words < 1 || p->words > NFK_TREE_NODES / 64)) ||
       static_cast<long long>(p->num_pages) * 2 * p->kv_heads * kPage > 0x7fff0000ll)
     return NF_ERR_BAD_ARG;

@@ -162,6 +162,8 @@ def rope_frequencies(rot_dim: int, theta: float, scaling: Optional[dict] = None,
     ``yarn``, ``longrope`` (short or long factors by ``length``)."""
     if rot_dim < 2 or rot_dim % 2:
         raise RuntimeError("rope_frequencies: rot_dim must be even")
+    if not theta > 1:
+        raise RuntimeError("rope_frequencies: theta must be above 1")
     scaling = scaling or {}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
     i = torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim
@@ -171,6 +173,17 @@ def rope_frequencies(rot_dim: int, theta: float, scaling: Optional[dict] = None,
         raise RuntimeError(f"rope_frequencies: unknown scaling {kind}")
     if kind in ("dynamic", "yarn", "longrope") and not original:
         raise RuntimeError(f"rope_frequencies: {kind} needs max_position or original_max_position_embeddings")
+    needed = {"linear": ("factor",), "dynamic": ("factor",), "llama3": ("factor",), "longrope": ("short_factor", "long_factor"),
+              "yarn": () if max_position else ("factor",)}
+    for name in needed.get(kind, ()):
+        if name not in scaling:
+            raise RuntimeError(f"rope_frequencies: {kind} needs {name}")
+    if scaling.get("factor") is not None and not float(scaling["factor"]) > 0:
+        raise RuntimeError("rope_frequencies: factor must be positive")
+    if kind == "dynamic" and rot_dim == 2:
+        raise RuntimeError("rope_frequencies: dynamic has no form for a single pair")
+    if kind == "longrope" and not len(scaling["short_factor"]) == len(scaling["long_factor"]) == rot_dim // 2:
+        raise RuntimeError("rope_frequencies: longrope needs a factor for each pair")
     if kind == "linear":
         inv = inv / float(scaling["factor"])
     elif kind == "dynamic":
@@ -263,7 +276,7 @@ def tree_masks(parents: torch.Tensor, qo_indptr: torch.Tensor, mask: torch.Tenso
                status: Optional[torch.Tensor] = None, early_start: int = EARLY_FIRST) -> torch.Tensor:
     """``mask`` (int64 ``[tokens, words]``) = bits of each token and of those that it descends from. ``parents[t]``: place of t's parent among
     its request's tokens, in front of its own; -1: none (anything else is reported and taken for it). ``positions``: of which each request's
-    first is right; the others become that plus the token's depth. Tokens behind a mask's last bit (64 words, up to 512) see none of the others
+    first is right; the others become that plus the token's depth. Tokens behind a mask's last bit (64 a word, up to 512) see none of the others
     and are reported; rows of tokens of no request are left as they were."""
     _calls().masks(parents, qo_indptr, mask, positions, status, early_start)
     return mask

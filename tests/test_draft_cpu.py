@@ -53,7 +53,13 @@ def test_frequencies_without_scaling():
     inv, out = ops.rope_frequencies(128, 500000.0, device="cpu")
     torch.testing.assert_close(inv, ref.rope_inv_freq(128, 500000.0), rtol=0, atol=0)
     assert out == 1.0
-    for bad in (dict(rot_dim=7), dict(rot_dim=64, scaling={"rope_type": "other"}), dict(rot_dim=64, scaling={"rope_type": "yarn", "factor": 2.0})):
+    for bad in (dict(rot_dim=7), dict(rot_dim=64, scaling={"rope_type": "other"}), dict(rot_dim=64, scaling={"rope_type": "yarn", "factor": 2.0}),
+                dict(rot_dim=64, scaling={"rope_type": "linear"}), dict(rot_dim=64, scaling={"rope_type": "dynamic"}, max_position=4096),
+                dict(rot_dim=2, scaling={"rope_type": "dynamic", "factor": 2.0}, max_position=4096), dict(rot_dim=64, theta=1.0), dict(rot_dim=64, theta=-2.0),
+                dict(rot_dim=64, scaling={"rope_type": "linear", "factor": 0.0}), dict(rot_dim=64, scaling={"rope_type": "longrope"}, max_position=4096),
+                dict(rot_dim=64, scaling={"rope_type": "longrope", "short_factor": [1.0] * 31, "long_factor": [1.0] * 31}, max_position=4096),
+                dict(rot_dim=64, scaling={"rope_type": "llama3"}), dict(rot_dim=64, scaling={"rope_type": "yarn", "original_max_position_embeddings": 4096}),
+                dict(rot_dim=64, scaling={"rope_type": "yarn", "factor": -4.0, "original_max_position_embeddings": 4096})):
         with pytest.raises(RuntimeError, match="rope_frequencies"):
             ops.rope_frequencies(**{"theta": 10000.0, "device": "cpu", **bad})
 
@@ -117,7 +123,7 @@ def test_rotation_refuses_before_any_launch(change, rc):
     (dict(head_dim=96), 3), (dict(q_heads=7), 3), (dict(q_heads=258), 3), (dict(kv_heads=0), 3), (dict(req_count=-1), 1), (dict(req_begin=-1), 1),
     (dict(req_count=0), 0), (dict(num_tokens=0), 0), (dict(num_ctas=-1), 1), (dict(q=0), 1), (dict(out=4104), 1), (dict(workspace=4112), 1), (dict(workspace_bytes=1000), 1),
     (dict(tree=4100), 1), (dict(words=0), 1), (dict(words=9), 1), (dict(ld_q=1000), 1), (dict(ld_out=1028), 1), (dict(sm_scale=0.0), 1),
-    (dict(sm_scale=float("nan")), 1), (dict(sm_scale=float("inf")), 1), (dict(num_pages=0), 1), (dict(num_pages=2 ** 26), 1), (dict(num_indices=-1), 1), (dict(req_begin=2 ** 31 - 2), 1)])
+    (dict(sm_scale=2.5e38), 1), (dict(ld_out=2 ** 35 // 3 + 8), 1), (dict(ld_out=2 ** 62), 1), (dict(ld_q=2 ** 40), 1), (dict(sm_scale=float("nan")), 1), (dict(sm_scale=float("inf")), 1), (dict(num_pages=0), 1), (dict(num_pages=2 ** 26), 1), (dict(num_indices=-1), 1), (dict(req_begin=2 ** 31 - 2), 1)])
 def test_attention_refuses_before_any_launch(change, rc):
     pointers = ("q", "out", "kv_pool", "qo_indptr", "kv_indptr", "kv_indices", "kv_last_page_len", "tree", "workspace")
     values = dict(ld_q=1024, ld_out=1024, q_heads=8, kv_heads=2, head_dim=128, num_pages=4, num_tokens=3, num_indices=4, req_count=3, words=1, sm_scale=0.1,
