@@ -15,9 +15,11 @@
 //               rows and both take every tile.
 // A product of 128 x 64 x 16 takes as long as one of 128 x 128 x 16 (63 clocks), so that scores run at half the tensor cores' rate; tiles
 // of 128 tokens leave room for one buffer of scores only, and cost more than they gain: with the weights over the scores 32 x 64 tokens
-// of 512 rows take 470 us against 287, with the weights by way of shared memory 339 (with rings of a tile and a half). Tiles of 64 tokens
+// of 512 rows take 470 us against 279, with the weights by way of shared memory 339 (with rings of a tile and a half). Tiles of 64 tokens
 // with the weights by way of shared memory, so that nothing has to wait for the place of the scores: 325, since both products then read all
-// operands from there. Two threads to a row, 375. Of those 287 us 2^x is worth 12, half of the scores' products 13, the cache's way from HBM instead of the L2 10.
+// operands from there. Two threads to a row, 375. What is left is the softmax's own chain, some 2200 clocks a tile for the two warps of a
+// scheduler, 1040 of them 2^x: without 2^x the same case takes 12 us less, with half of the scores' products 13, with the cache in the L2
+// 10; letting the two warps take turns at 2^x makes it 302.
 //
 // Work is a row of pages of all requests, KV heads and blocks, cut evenly over the CTAs whatever the requests' lengths; an item that is
 // cut leaves a state (reference, sum, sums of values) per piece, which a second kernel joins, in the order of the pieces: results do not
@@ -25,12 +27,12 @@
 //
 // Weights are rounded to bf16 (at most 2^-8 of each), the type of the values that they meet in the product. Scores, references, sums and
 // states are fp32. Weights are relative to a reference, at first the first tile's largest score. The largest score of a further tile is
-// looked for only where the sum of its weights reaches 2^14 times the weight of that, and the reference moves (sums are rescaled, the tile's weights formed anew)
-// where that score is above it by 2^8 or more: 286 us instead of 296 with a search in every tile.
+// looked for only where its weights' sum reaches 2^14 times the reference's own weight, and the reference moves (sums are rescaled, the
+// tile's weights formed anew) where that score is above it by 2^8 or more: 286 us instead of 296 with a search in every tile.
 //
 // Measured (32 query and 8 KV heads of 128, a launch of both kernels in a graph): 64 requests of 5 tokens behind up to 4000 70 us (5.2 TB/s),
 // 256 single tokens behind up to 2000 147 us (5.9 TB/s), one of 60 behind 100000 115 us; with 64 query heads 32 of 64 tokens behind up to
-// 8000 287 us (0.85 PFLOP/s); one of 26 behind 2000 16 us, which is two launches, the scan of the lists and one tile's way through all of it.
+// 8000 279 us (0.87 PFLOP/s); one of 26 behind 2000 16 us, which is two launches, the scan of the lists and one tile's way through all of it.
 //
 // Only tiles with drafted tokens or the end of a piece need care: masks of 128 bits a row; and values that a row does not see must not
 // reach it as 0 * inf, so rows of values behind the end become zeros, as do infinities and NaN of drafted tokens, which the rows that do
@@ -255,6 +257,9 @@ __global__ void __launch_bounds__(Cfg<HD, SLOTS>::kThreads, 3 - SLOTS)
 attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmKV,
                  const __grid_constant__ nfk_attn_tree_params p, Workspace ws) {
   using C = Cfg<HD, SLOTS>;
+  // Exponents by two to an instruction or by one: the one needs pairs of registers, which cost moves; the same values. (One slot: 128
+  // requests of 64 rows 59.6 us by two, 62 by one. Two slots: 32 requests of 512 rows 290 and 279.)
+  constexpr bool kInPairs = SLOTS == 1;
   constexpr int NH = C::NH, NST = C::kStages, kKeyWarp = C::kKeyWarp, kMmaWarp = C::kMmaWarp, kValueWarp = C::kValueWarp, kThreads = C::kThreads;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sb = smem_u32(smem);
@@ -687,7 +692,8 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               uint32_t pk[16];                   // column j: tokens 2j, 2j + 1
 #pragma unroll
               for (int j = 0; j < 16; ++j) {
-                const float2 y = halves(fma2(pair(__uint_as_float(x[h][2 * j]), __uint_as_float(x[h][2 * j + 1])), scale2, ms2));
+                const float x0 = __uint_as_float(x[h][2 * j]), x1 = __uint_as_float(x[h][2 * j + 1]);
+                const float2 y = kInPairs ? halves(fma2(pair(x0, x1), scale2, ms2)) : make_float2(fmaf(x0, scale, -ms), fmaf(x1, scale, -ms));
                 const float e0 = fast_exp2(y.x), e1 = fast_exp2(y.y);
                 rs[j & 1] = add2(rs[j & 1], pair(e0, e1));
                 pk[j] = pack_bf16x2(e0, e1);
@@ -1021,7 +1027,7 @@ extern "C" int nfk_attn_tree(const nfk_attn_tree_params* p, cudaStream_t stream)
       static_cast<long long>(p->num_pages) * 2 * p->kv_heads * kPage > 0x7fff0000ll)
     return NF_ERR_BAD_ARG;
   // 128 elements a head: two slots to a CTA where requests have more than 128 rows on average, since both take every tile that has been
-  // read (32 requests of 64 tokens, 512 rows each: 287 us, by two CTAs of a slot 317; one of 240 rows behind 100000 tokens: 115 and 143;
+  // read (32 requests of 64 tokens, 512 rows each: 279 us, by two CTAs of a slot 317; one of 240 rows behind 100000 tokens: 115 and 143;
   // 8 of 160 rows behind 6000: 64.5 and 67.5; short contexts are the other way, 128 of 200 rows behind 350: 118 and 114; requests of one
   // block of 128 take either form's one slot). 64 elements: always one slot, as its tiles are half as much to read and two CTAs wait less
   // for one another than two slots (64 requests of 256 rows: 119 us against 135; 32 of 512: 211 and 243; one of 240 behind 100000: 92 and 107).

@@ -2,7 +2,9 @@
 //
 //   (x, y) -> f (x c - y s, y c + x s),  c, s = cos, sin(pos w_i),  (x, y) = (x_i, x_(i + pairs)) or (x_2i, x_(2i+1)),  i < pairs;
 // what lies behind the first 2 pairs elements of a head stays as it is, as do values. All in fp32 from the bf16 inputs, rounded once.
-// Memory-bound: every element is read once and written once.
+// Memory-bound: every element is read once and written once. In a graph, heads of 128: 8192 tokens of 32 query and 8 KV heads 36.2 us
+// (201 MB, 5.6 TB/s; floor 30.8), any number of pairs 54, by way of shared memory for each element's partner; 1215 tokens of 64 and 8 heads
+// 12.2 (floor 7.6: a token's CTA has a chain of position, angles and heads to itself, and there is one turn of them); 26 tokens 2.6.
 #include "cache_q8.cuh"
 #include "common.cuh"
 #include "kernels.h"
