@@ -778,6 +778,29 @@ def _begun(loop):
     ops.check_status(loop.status)
 
 
+def test_two_calls_at_once():
+    """Two streams, a workspace each, one of them with a captured graph: as one after the other."""
+    torch.cuda.synchronize()
+    calls = [_batch(30, [900, 300, 2000], [60, 64, 33], 32, 8, 128), _batch(31, [700] * 20, [5] * 20, 32, 8, 128), _batch(32, [1500, 40], [100, 3], 16, 2, 64)]
+    want = [ops.attn_tree(**b).clone() for b in calls]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attn_tree(**calls[0])
+    one, other = torch.cuda.Stream(), torch.cuda.Stream()
+    for b in calls:
+        b["out"].fill_(1.0)
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(one):
+            graph.replay()
+            ops.attn_tree(**calls[2])
+        with torch.cuda.stream(other):
+            ops.attn_tree(**calls[1])
+    torch.cuda.synchronize()
+    for b, w in zip(calls, want):
+        assert torch.equal(b["out"], w)
+
+
 @pytest.mark.parametrize("captured", [False, True])
 def test_a_run_of_all_of_them(captured):
     loop = Loop([1, 30, 16, 100, 47], 256, 4)
