@@ -7,7 +7,7 @@
 // itself, in shared memory, and then writes its share of the lists, an entry's request found by bisection. What the call changes
 // is written by the CTA that is the last to have read it, known by a ticket.
 //
-// A step's growth and the way back together, in a graph: 1 request 6.6 us, 256 of up to 6000 tokens 11.2, 2048 of up to 4000 19.9, of which
+// A step's growth and the way back together, in a graph: 1 request 6.6 us, 256 of up to 6000 tokens 10.2, 2048 of up to 4000 19.9, of which
 // bytes need 0.3: loads of rows, lengths and pages behind one another, the barriers of the scan, eleven steps of bisection.
 #include "common.cuh"
 #include "kernels.h"
@@ -17,7 +17,8 @@ namespace {
 
 constexpr int kPage = 16;
 constexpr int kMostThreads = 1024, kMine = NFK_TABLES_REQUESTS / kMostThreads;   // requests of a thread at most
-// Threads of a CTA: barriers of many take longer, and few requests need no more.
+// Threads of a CTA: barriers of many take longer, and few requests need no more (256 requests 10.2 us, with 1024 threads 11.3; 512 requests
+// the other way, 16.8, with 256 threads 20.3).
 constexpr int kFewThreads = 256;
 // entries of the lists that a thread writes before there are further CTAs
 constexpr int kPerThread = 2;
@@ -263,7 +264,7 @@ int launch(const nfk_tables_params& p, long long entries, cudaStream_t stream) {
     }
     attr = true;
   }
-  const int threads = p.requests <= kFewThreads && entries <= 8ll * kFewThreads * kPerThread ? kFewThreads : kMostThreads;
+  const int threads = p.requests <= kFewThreads ? kFewThreads : kMostThreads;
   long long ctas = (entries + threads * kPerThread - 1) / (threads * kPerThread);
   if (ctas > device_sm_count()) ctas = device_sm_count();
   if (ctas < 1) ctas = 1;
