@@ -32,7 +32,7 @@
 //
 // Measured (32 query and 8 KV heads of 128, a launch of both kernels in a graph): 64 requests of 5 tokens behind up to 4000 70 us (5.2 TB/s),
 // 256 single tokens behind up to 2000 147 us (5.9 TB/s), one of 60 behind 100000 115 us; with 64 query heads 32 of 64 tokens behind up to
-// 8000 279 us (0.87 PFLOP/s); one of 26 behind 2000 16 us, which is two launches, the scan of the lists and one tile's way through all of it.
+// 8000 279 us (0.87 PFLOP/s); one of 26 behind 2000 15 us, which is two launches, the scan of the lists and one tile's way through all of it.
 //
 // Only tiles with drafted tokens or the end of a piece need care: masks of 128 bits a row; and values that a row does not see must not
 // reach it as 0 * inf, so rows of values behind the end become zeros, as do infinities and NaN of drafted tokens, which the rows that do
@@ -52,11 +52,10 @@ constexpr float kGap = 8.f;           // log2 of how far a row's largest score m
 // only where it is 2^-94 of the largest.
 constexpr float kSpare = 32.f;
 constexpr float kMostWeight = 16384.f / 4294967296.f;        // the sum of a tile's weights from which on it is: 64 weights of 2^kGap
-// What an item's beginning and end cost, in pages: where the work is cut, the ends count too. (8 or 24 change little, 0 leaves CTAs with
-// many short requests behind the others.)
+// What an item's beginning and end cost, in pages: where the work is cut, the ends count too. (64 requests of 5 tokens 69.8 us, with 8 pages
+// 72.1, with 4 76.7; 24 cost single tokens 1 % and give batches of short contexts 2 to 5.) It is also the least share of a CTA: 1 x 26
+// tokens behind 2000 take 14.9 us, with shares of 24 15.9; fewer make more pieces than they save tiles.
 constexpr int kLead = 16;
-// Pages that a CTA takes at least, so that the states of short requests do not outweigh their pages. (4 and 16 take the same time within 3 %.)
-constexpr int kLeast = 8;
 
 // What the roles need to know of a piece.
 struct Piece {
@@ -149,7 +148,7 @@ struct Cut {
   long long total;
   int w;
   __device__ __forceinline__ Cut(long long t, int ctas) : total(t) {
-    const long long most = (t + kLead + kLeast - 1) / (kLead + kLeast);
+    const long long most = (t + kLead - 1) / kLead;
     w = static_cast<int>(most < ctas ? (most > 0 ? most : 1) : ctas);
   }
   __device__ __forceinline__ long long begin(int c) const { return total * c / w; }
