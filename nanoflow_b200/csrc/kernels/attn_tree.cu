@@ -32,7 +32,7 @@
 //
 // Measured (32 query and 8 KV heads of 128, a launch of both kernels in a graph): 64 requests of 5 tokens behind up to 4000 70 us (5.2 TB/s),
 // 256 single tokens behind up to 2000 147 us (5.9 TB/s), one of 60 behind 100000 115 us; with 64 query heads 32 of 64 tokens behind up to
-// 8000 279 us (0.87 PFLOP/s); one of 26 behind 2000 15 us, which is two launches, the scan of the lists and one tile's way through all of it.
+// 8000 280 us (0.87 PFLOP/s; for seconds 326, at the power cap and 1610 MHz); one of 26 behind 2000 15 us, which is two launches, the scan of the lists and one tile's way through all of it.
 //
 // Only tiles with drafted tokens or the end of a piece need care: masks of 128 bits a row; and values that a row does not see must not
 // reach it as 0 * inf, so rows of values behind the end become zeros, as do infinities and NaN of drafted tokens, which the rows that do
