@@ -26,15 +26,16 @@
 // depend on the order in which anything runs.
 //
 // Weights are rounded to bf16 (at most 2^-8 of each), the type of the values that they meet in the product. Scores, references, sums and
-// states are fp32. Weights are relative to a reference, at first the first tile's largest score. The largest score of a further tile is
-// looked for only where its weights' sum reaches 2^14 times the reference's own weight, and the reference moves (sums are rescaled, the
-// tile's weights formed anew) where that score is above it by 2^8 or more: 286 us instead of 296 with a search in every tile.
+// states are fp32. Weights are relative to a reference, at first the first tile's largest score (and 2^32, kSpare). The largest score of a
+// further tile is looked for only where its weights' sum reaches 2^14 of the first one's largest, and the reference moves (sums are rescaled,
+// the tile's weights formed anew) where that score is above it by 2^8 or more: 286 us instead of 296 with a search in every tile.
 //
 // Measured (32 query and 8 KV heads of 128, a launch of both kernels in a graph): 64 requests of 5 tokens behind up to 4000 70 us (5.2 TB/s),
 // 256 single tokens behind up to 2000 147 us (5.9 TB/s), one of 60 behind 100000 115 us; with 64 query heads 32 of 64 tokens behind up to
-// 8000 280 us (0.87 PFLOP/s; for seconds 326, at the power cap and 1610 MHz); one of 26 behind 2000 15 us, which is two launches, the scan of the lists and one tile's way through all of it.
+// 8000 280 us (0.87 PFLOP/s; for seconds 326, at the power cap and 1610 MHz); one of 26 behind 2000 15 us, which is two launches, the scan
+// of the lists and a few tiles' way through all of it.
 //
-// Only tiles with drafted tokens or the end of a piece need care: masks of 128 bits a row; and values that a row does not see must not
+// Only tiles with drafted tokens or the end of a piece need care: masks of 64 bits a row; and values that a row does not see must not
 // reach it as 0 * inf, so rows of values behind the end become zeros, as do infinities and NaN of drafted tokens, which the rows that do
 // see them get back at the end (restore_odd).
 #include "attn_mma.cuh"
@@ -668,13 +669,13 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           } else {
             sees = true;
           }
-          auto largest = [&]() {
+          auto largest = [&]() {                 // as a reference
             float mq[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // (NaN where there is one)
 #pragma unroll
             for (int j = 0; j < 32; ++j)
               mq[j & 3] = max3_nan(mq[j & 3], __uint_as_float(x[j >> 4][2 * (j & 15)]), __uint_as_float(x[j >> 4][2 * (j & 15) + 1]));
             const float mx = max3_nan(max3_nan(mq[0], mq[1], mq[2]), mq[3], mq[3]) * scale;
-            if (mx < INFINITY) return mx;
+            if (mx < INFINITY) return mx + kSpare;
             l = __uint_as_float(0x7fc00000u);    // a score of infinity, or none
             return 0.f;
           };
@@ -683,7 +684,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           // yet, or a NaN) is the largest score looked for, and the weights are formed once more.
           float sum;
           for (bool again = false;; again = true) {
-            const float ms = ref == -INFINITY ? 0.f : ref + kSpare;
+            const float ms = ref == -INFINITY ? 0.f : ref;
             const f32x2 scale2 = pair(scale, scale), ms2 = pair(-ms, -ms);
             f32x2 rs[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
