@@ -20,7 +20,7 @@ __device__ __forceinline__ int2 tokens_of(const int* qo_indptr, int r, int num_t
 }
 
 // mask(i) = bit i or mask(parent(i)), by doubling: with masks that reach up 2^k steps and the ancestor after so many, one step more
-// joins the two halves of 2^(k+1). A CTA per request, a thread per token.
+// joins the two halves of 2^(k+1). A CTA per request, a thread per token; W: words of a mask, or the next power of two.
 template <int W>
 __global__ void __launch_bounds__(W * 64) tree_masks_kernel(nfk_tree_masks_params p) {
   constexpr int N = W * 64;
@@ -30,8 +30,8 @@ __global__ void __launch_bounds__(W * 64) tree_masks_kernel(nfk_tree_masks_param
   let_next_start();
   await_previous();
   const int2 own = tokens_of(p.qo_indptr, blockIdx.x, p.num_tokens, p.status);
-  const int n = min(own.y, N);
-  if (own.y > N) {                               // tokens behind the last that a mask has bits for see the context only
+  const int bits = p.words * 64, n = min(own.y, bits);
+  if (own.y > bits) {                            // tokens behind the last that a mask has bits for see the context only
     if (i == 0) report_status(p.status, NF_ST_BAD_INDEX);
     for (int t = n + i; t < own.y; t += N) {
       for (int w = 0; w < p.words; ++w) p.mask[static_cast<long long>(own.x + t) * p.words + w] = 0ull;

@@ -542,10 +542,10 @@ def attn_tree(q, kv_pool, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tr
 
 
 def tree_masks(parents, qo_indptr, words):
-    """(mask words, depths)."""
+    """(mask words, depths); zeros behind a mask's last bit."""
     mask, depth = torch.zeros(parents.numel(), words, dtype=torch.int64), torch.zeros(parents.numel(), dtype=torch.int32)
     for a, b in zip(qo_indptr.tolist(), qo_indptr.tolist()[1:]):
-        for i in range(b - a):
+        for i in range(min(b - a, 64 * words)):
             j, bits, steps = i, 0, -1
             while j >= 0:
                 bits, steps, j = bits | 1 << j, steps + 1, int(parents[a + j])
