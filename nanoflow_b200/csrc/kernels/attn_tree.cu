@@ -305,7 +305,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   // ---- where this CTA's share of the units begins: units of every thread's requests, scanned ----
   const int per_thread = (p.req_count + kThreads - 1) / kThreads;
-  const int r0 = min(p.req_count, static_cast<int>(threadIdx.x) * per_thread), r1 = min(p.req_count, r0 + per_thread);
+  const int r0 = min(p.req_count, static_cast<int>(threadIdx.x) * per_thread), r1 = r0 + min(per_thread, p.req_count - r0);
   long long mine = 0;
   for (int r = r0; r < r1; ++r) mine += units_of(read_request(p, r, per_block, blockIdx.x == 0)) * p.kv_heads;
   long long sum = mine;
@@ -1010,7 +1010,8 @@ extern "C" long long nfk_attn_tree_workspace(const nfk_attn_tree_params* p) {
 
 extern "C" int nfk_attn_tree(const nfk_attn_tree_params* p, cudaStream_t stream) {
   using namespace nf;
-  if (p == nullptr || p->req_count < 0 || p->req_begin < 0 || p->num_ctas < 0) return NF_ERR_BAD_ARG;
+  if (p == nullptr || p->req_count < 0 || p->req_count > NFK_DRAFT_ENTRIES || p->num_tokens > NFK_DRAFT_ENTRIES || p->req_begin < 0 || p->num_ctas < 0)
+    return NF_ERR_BAD_ARG;
   if ((p->head_dim != 64 && p->head_dim != 128) || p->kv_heads <= 0 || p->q_heads <= 0 || p->q_heads % p->kv_heads != 0 || p->q_heads / p->kv_heads > 128)
     return NF_ERR_UNSUPPORTED;
   if (p->req_count == 0 || p->num_tokens == 0) return NF_OK;

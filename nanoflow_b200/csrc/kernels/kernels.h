@@ -330,7 +330,8 @@ int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream);
 // ------------------------------------------------------------------------------------------------
 // Drafted tokens (page_tables.cu, rope_slots.cu, attn_tree.cu, tree.cu): a step in which each request brings a tree or a chain of
 // tokens that the model is to check. bf16 cache pools [num_pages][2][kv_heads][16][head_dim]; a token's place in a pool is
-// its slot, page * 16 + place in the page.
+// its slot, page * 16 + place in the page. Requests of a call, and entries of a list, number up to NFK_DRAFT_ENTRIES: 32 bits with room for a
+// loop's step behind the last one.
 // ------------------------------------------------------------------------------------------------
 // Page tables: row r holds the pages of one request, table[r * max_pages + i] those of its tokens 16 i .. 16 i + 15. Free pages are a
 // stack; `ticket` is a word of the tables' own, zero between calls.
@@ -342,7 +343,7 @@ int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream);
 // free_pages[free_count + n - 1 - k]: a trim takes back the grow before it. The lists are not looked at.
 // A row that is none or comes twice, a negative count, or a size that does not fit (pages of a row, free pages, lists): nothing
 // changes, all lists are empty, and `status` says so.
-enum { NFK_TABLES_REQUESTS = 4096, NFK_TABLES_ROWS = 65536 };
+enum { NFK_DRAFT_ENTRIES = 0x7ff00000, NFK_TABLES_REQUESTS = 4096, NFK_TABLES_ROWS = 65536 };
 typedef struct nfk_tables_params {
   int* table; int* lengths; int* free_pages; int* free_count; unsigned int* ticket;
   const int* rows; const int* tokens;

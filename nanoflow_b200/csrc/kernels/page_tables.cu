@@ -287,7 +287,7 @@ extern "C" int nfk_tables_grow(const nfk_tables_params* p, cudaStream_t stream) 
   const int rc = check(p);
   if (rc != NF_OK) return rc;
   if (!p->qo_indptr || !p->kv_indptr || !p->kv_indices || !p->kv_last_page_len || !p->positions || !p->token_req || !p->slots ||
-      p->num_indices < 0 || p->num_tokens < 0)
+      p->num_indices < 0 || p->num_indices > NFK_DRAFT_ENTRIES || p->num_tokens < 0 || p->num_tokens > NFK_DRAFT_ENTRIES)
     return NF_ERR_BAD_ARG;
   // (lists of a captured graph may be far longer than what a step fills, so that both count)
   return launch<true>(*p, static_cast<long long>(p->num_indices) + p->num_tokens, stream);

@@ -191,6 +191,7 @@ __global__ void __launch_bounds__(kKeepThreads, 6) kv_keep_kernel(const __grid_c
   }
 }
 
+bool fits(int entries) { return entries >= 0 && entries <= NFK_DRAFT_ENTRIES; }
 int started(cudaError_t e) {
   if (e == cudaSuccess) return NF_OK;
   (void)cudaGetLastError();
@@ -202,7 +203,7 @@ int started(cudaError_t e) {
 
 extern "C" int nfk_tree_masks(const nfk_tree_masks_params* p, cudaStream_t stream) {
   using namespace nf;
-  if (p == nullptr || p->requests < 0 || p->num_tokens < 0 || p->words < 1 || p->words > NFK_TREE_NODES / 64) return NF_ERR_BAD_ARG;
+  if (p == nullptr || !fits(p->requests) || !fits(p->num_tokens) || p->words < 1 || p->words > NFK_TREE_NODES / 64) return NF_ERR_BAD_ARG;
   if (p->requests == 0 || p->num_tokens == 0) return NF_OK;
   if (!p->parents || !p->qo_indptr || !p->mask || (reinterpret_cast<uintptr_t>(p->mask) & 7) != 0) return NF_ERR_BAD_ARG;
   const auto run = [&](auto kernel, int words) { return started(launch_kernel(early_first(p->early_start), kernel, p->requests, words * 64, 0, stream, 1, *p)); };
@@ -214,7 +215,7 @@ extern "C" int nfk_tree_masks(const nfk_tree_masks_params* p, cudaStream_t strea
 
 extern "C" int nfk_tree_accept(const nfk_tree_accept_params* p, cudaStream_t stream) {
   using namespace nf;
-  if (p == nullptr || p->requests < 0 || p->num_tokens < 0 || p->max_path < 0) return NF_ERR_BAD_ARG;
+  if (p == nullptr || !fits(p->requests) || !fits(p->num_tokens) || !fits(p->max_path)) return NF_ERR_BAD_ARG;
   if (p->requests == 0) return NF_OK;
   if (!p->qo_indptr || !p->counts || !p->next_tokens || (p->max_path > 0 && !p->path) ||
       (p->num_tokens > 0 && (!p->tokens || !p->parents || !p->targets)))
@@ -225,7 +226,8 @@ extern "C" int nfk_tree_accept(const nfk_tree_accept_params* p, cudaStream_t str
 
 extern "C" int nfk_kv_keep(const nfk_kv_keep_params* p, cudaStream_t stream) {
   using namespace nf;
-  if (p == nullptr || p->requests < 0 || p->num_tokens < 0 || p->max_path < 0 || p->num_pools < 0 || p->num_pools > NFK_KEEP_POOLS) return NF_ERR_BAD_ARG;
+  if (p == nullptr || !fits(p->requests) || !fits(p->num_tokens) || !fits(p->max_path) || p->num_pools < 0 || p->num_pools > NFK_KEEP_POOLS)
+    return NF_ERR_BAD_ARG;
   if (p->head_dim < 8 || p->head_dim % 8 != 0 || p->head_dim > 1024) return NF_ERR_UNSUPPORTED;
   if (p->requests == 0 || p->num_pools == 0 || p->max_path == 0 || p->num_tokens == 0) return NF_OK;
   if (!p->slots || !p->path || !p->counts || !p->qo_indptr || p->num_pages <= 0 || p->num_pages > 0x7fffffff / kPage || p->kv_heads <= 0 ||

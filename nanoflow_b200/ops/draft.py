@@ -17,8 +17,9 @@ Caches are the bf16 pools ``[num_pages, 2, kv_heads, 16, head_dim]`` of :func:`n
 be captured into a CUDA graph; lists longer than a step needs hold tokens of no request, which the other calls leave alone.
 
 No tensor that a call writes may overlap another one of its tensors. Lists that are none are reported in ``status`` and touch nothing
-outside the call's tensors. ``early_start`` (EARLY_*): kernels may be launched while the one before them on the stream still runs, and
-wait for it there; 0 keeps the SMs free until then, for another stream's kernels beside it.
+outside the call's tensors. Requests of a call, and entries of a list, number up to 2^31 - 2^20. ``early_start`` (EARLY_*): kernels may be
+launched while the one before them on the stream still runs, and wait for it there; 0 keeps the SMs free until then, for another stream's
+kernels beside it.
 """
 from __future__ import annotations
 
