@@ -112,6 +112,9 @@ PyObject* grow(PyObject*, PyObject* const* a, Py_ssize_t n) {
     t.p.positions = ints(positions);
     t.p.token_req = ints(token_req);
     t.p.slots = ints(slots);
+    t.p.num_qo = count(what, qo, "qo_indptr");
+    t.p.num_kv = count(what, kv, "kv_indptr");
+    t.p.num_last = count(what, last, "kv_last_page_len");
     t.p.num_indices = count(what, indices, "kv_indices");
     t.p.num_tokens = count(what, slots, "slots");
     t.p.status = word(status);

@@ -338,7 +338,8 @@ int nfk_attn_decode_q8(const nfk_attn_q8_params* p, cudaStream_t stream);
 //
 // nfk_tables_grow: lengths[rows[r]] += tokens[r]; the k-th page that the call takes, requests in their order, is
 // free_pages[free_count - 1 - k]. Lists of the requests as they are afterwards; of the new tokens their positions, requests and slots
-// (entries behind the last token: 0, -1, -1).
+// (entries behind the last token: 0, -1, -1). Lists of requests may be longer than the batch, qo_indptr and kv_indptr have an entry more
+// than it at least: what is behind its last request are requests of nothing.
 // nfk_tables_trim: lengths[rows[r]] -= min(tokens[r], lengths[rows[r]]); the k-th of the n pages that come free goes to
 // free_pages[free_count + n - 1 - k]: a trim takes back the grow before it. The lists are not looked at.
 // A row that is none or comes twice, a negative count, or a size that does not fit (pages of a row, free pages, lists): nothing
@@ -351,6 +352,7 @@ typedef struct nfk_tables_params {
   int requests, max_requests, max_pages, num_pages, num_indices, num_tokens;   // entries of kv_indices; of positions, token_req, slots
   int early_start;
   unsigned int* status;
+  int num_qo, num_kv, num_last;   // entries of qo_indptr, kv_indptr and kv_last_page_len (fewer than the batch needs: that many)
 } nfk_tables_params;
 int nfk_tables_grow(const nfk_tables_params* p, cudaStream_t stream);
 int nfk_tables_trim(const nfk_tables_params* p, cudaStream_t stream);

@@ -182,11 +182,12 @@ __global__ void __launch_bounds__(kMostThreads) tables_grow_kernel(const __grid_
     if (blockIdx.x == 0 && threadIdx.x == 0) report_status(p.status, NF_ST_BAD_INDEX);
   }
   const int at = blockIdx.x * blockDim.x + threadIdx.x, step = gridDim.x * blockDim.x;
-  for (int r = at; r <= R; r += step) {
-    p.qo_indptr[r] = ok ? s.at[0][r] : 0;
-    p.kv_indptr[r] = ok ? s.at[1][r] : 0;
-    if (r < R) {
-      const int length = ok ? s.old[r] + s.at[0][r + 1] - s.at[0][r] : 0;
+  // requests, and requests of nothing behind the last one, to the lists' ends
+  for (int r = at; r <= max(R, max(max(p.num_qo, p.num_kv) - 1, p.num_last)); r += step) {
+    if (r <= R || r < p.num_qo) p.qo_indptr[r] = ok ? s.at[0][min(r, R)] : 0;
+    if (r <= R || r < p.num_kv) p.kv_indptr[r] = ok ? s.at[1][min(r, R)] : 0;
+    if (r < R || r < p.num_last) {
+      const int length = ok && r < R ? s.old[r] + s.at[0][r + 1] - s.at[0][r] : 0;
       p.kv_last_page_len[r] = length - max(pages_of(length) - 1, 0) * kPage;
     }
   }
@@ -287,7 +288,8 @@ extern "C" int nfk_tables_grow(const nfk_tables_params* p, cudaStream_t stream) 
   const int rc = check(p);
   if (rc != NF_OK) return rc;
   if (!p->qo_indptr || !p->kv_indptr || !p->kv_indices || !p->kv_last_page_len || !p->positions || !p->token_req || !p->slots ||
-      p->num_indices < 0 || p->num_indices > NFK_DRAFT_ENTRIES || p->num_tokens < 0 || p->num_tokens > NFK_DRAFT_ENTRIES)
+      p->num_indices < 0 || p->num_indices > NFK_DRAFT_ENTRIES || p->num_tokens < 0 || p->num_tokens > NFK_DRAFT_ENTRIES ||
+      p->num_qo > NFK_DRAFT_ENTRIES || p->num_kv > NFK_DRAFT_ENTRIES || p->num_last > NFK_DRAFT_ENTRIES)
     return NF_ERR_BAD_ARG;
   // (lists of a captured graph may be far longer than what a step fills, so that both count)
   return launch<true>(*p, static_cast<long long>(p->num_indices) + p->num_tokens, stream);

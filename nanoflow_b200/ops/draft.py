@@ -14,7 +14,8 @@ One step, for the requests in rows ``rows`` of the tables, ``new_tokens`` tokens
 
 Caches are the bf16 pools ``[num_pages, 2, kv_heads, 16, head_dim]`` of :func:`nanoflow_b200.ops.rope_append` and
 :func:`nanoflow_b200.ops.attn_decode`. A token's slot is ``page * 16 + place in the page``. Nothing here waits for the GPU, and all calls can
-be captured into a CUDA graph; lists longer than a step needs hold tokens of no request, which the other calls leave alone.
+be captured into a CUDA graph; lists longer than a step needs hold tokens of no request and requests of nothing, which the other calls
+leave alone (of a request of nothing, :func:`tree_accept` says so).
 
 No tensor that a call writes may overlap another one of its tensors. Lists that are none are reported in ``status`` and touch nothing
 outside the call's tensors. Requests of a call, and entries of a list, number up to 2^31 - 2^20. ``early_start`` (EARLY_*): kernels may be
@@ -41,7 +42,7 @@ class TablesParams(Structure):
     _fields_ = [(n, c_void_p) for n in ("table", "lengths", "free_pages", "free_count", "ticket", "rows", "tokens", "qo_indptr", "kv_indptr",
                                         "kv_indices", "kv_last_page_len", "positions", "token_req", "slots")] + \
                [(n, c_int) for n in ("requests", "max_requests", "max_pages", "num_pages", "num_indices", "num_tokens", "early_start")] + \
-               [("status", c_void_p)]
+               [("status", c_void_p)] + [(n, c_int) for n in ("num_qo", "num_kv", "num_last")]
 
 
 class RopeSlotsParams(Structure):
@@ -96,10 +97,10 @@ class BatchLists:
     """What :func:`tables_grow` writes, int32: lists of the batch's requests as ``attn_decode`` and :func:`attn_tree` read them, and
     of each new token its position, its request (-1: none) and its slot (-1: none)."""
 
-    qo_indptr: torch.Tensor           # [requests + 1]
-    kv_indptr: torch.Tensor           # [requests + 1]
+    qo_indptr: torch.Tensor           # [requests at most + 1]
+    kv_indptr: torch.Tensor           # [requests at most + 1]
     kv_indices: torch.Tensor          # [pages at most]
-    kv_last_page_len: torch.Tensor    # [requests]
+    kv_last_page_len: torch.Tensor    # [requests at most]
     positions: torch.Tensor           # [tokens at most]
     token_req: torch.Tensor
     slots: torch.Tensor
@@ -113,7 +114,7 @@ def page_tables(rows: int, max_pages: int, num_pages: int, device="cuda") -> Pag
 
 
 def batch_lists(requests: int, tokens: int, pages: int, device="cuda") -> BatchLists:
-    """Lists of ``requests`` requests with up to ``tokens`` new tokens and ``pages`` pages in all."""
+    """Lists of up to ``requests`` requests with up to ``tokens`` new tokens and ``pages`` pages in all."""
     i32 = dict(dtype=torch.int32, device=device)
     return BatchLists(torch.zeros(requests + 1, **i32), torch.zeros(requests + 1, **i32), torch.zeros(pages, **i32), torch.zeros(requests, **i32),
                       torch.zeros(tokens, **i32), torch.full((tokens,), -1, **i32), torch.full((tokens,), -1, **i32))
@@ -140,7 +141,8 @@ def _calls():
 def tables_grow(tables: PageTables, rows: torch.Tensor, new_tokens: torch.Tensor, lists: BatchLists, *, status: Optional[torch.Tensor] = None,
                 early_start: int = EARLY_FIRST) -> BatchLists:
     """Request i of the batch, in row ``rows[i]``, grows by ``new_tokens[i]`` tokens: pages are taken for them, requests in their order,
-    and the lists are written. ``lists.kv_indices`` behind the last page is left as it was.
+    and the lists are written: to their ends, tokens of no request and requests of nothing behind the last ones, but for ``lists.kv_indices``,
+    which behind the last page is left as it was.
 
     Nothing changes, all lists are empty, and ``status`` says so, if a row does not exist or comes twice, a number is negative, or something
     does not fit: a row's pages, the free pages, the lists. Up to 4096 requests."""

@@ -36,3 +36,8 @@ def test_trees_of_more_than_a_step_leaves_room_for_are_refused(entries):
             assert ops.lib().nfk_tree_masks(base._filled(draft.TreeMasksParams, ("parents", "qo_indptr", "mask"), masks, {field: entries}), c_void_p(0)) == 1
         pointers = ("tokens", "parents", "targets", "qo_indptr", "path", "counts", "next_tokens")
         assert ops.lib().nfk_tree_accept(base._filled(draft.TreeAcceptParams, pointers, accept, {field: entries}), c_void_p(0)) == 1
+
+
+@pytest.mark.parametrize("field", ["num_qo", "num_kv", "num_last"])
+def test_lists_of_requests_without_room_for_a_step_are_refused(field):
+    test_lists_of_tables_without_room_for_a_step_are_refused(field, MOST + 1)

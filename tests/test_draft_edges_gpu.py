@@ -39,3 +39,59 @@ def test_tokens_behind_a_masks_last_bit(words, tokens, chain):
             assert int(mask[a + i, i // 64]) >> (i % 64) & 1              # each sees itself
         assert not mask[b:qo[k + 1]].any() and (positions[b:qo[k + 1]] == first[k]).all()
         assert not want[b:qo[k + 1]].any() and not depth[b:qo[k + 1]].any()
+
+
+# ---- lists of more requests than a step has -------------------------------------------------------------------------------------
+@pytest.mark.parametrize("earlier,step", [([10] * 8, [40, 40]), ([10] * 8, [4, 4]), ([1] * 8, [30, 60, 2]), ([10] * 8, [0, 5]), ([10] * 8, [])])
+def test_lists_of_more_requests_than_the_step_has(earlier, step):
+    """A step in lists that an earlier one with more requests filled: entries behind its last request are requests of nothing, and rows and
+    tokens behind the last one are left alone, as with lists of its own."""
+    H, G, d, R, C, T, pages = 8, 2, 64, len(step), 8, 140, 100
+    lengths = [100, 33, 16, 5, 47, 64, 1, 200]
+    t, _ = base._tables(C, 24, 160, lengths)
+    g, r = base.gen(3), base.random.Random(1)
+    pool = base.normal(g, 160, 2, G, 16, d)
+    q = base.normal(g, T, H * d)
+    tokens, targets = (torch.randint(0, 3, (T,), generator=g, device="cuda").to(torch.int32) for _ in range(2))
+    parents = base.i32([p for n in step for p in base._parents(r, n)] + [0] * (T - sum(step)))
+    lists = ops.batch_lists(C, T, pages)
+    everyone = base.i32(list(range(C)))
+    ops.tables_grow(t, everyone, base.i32(earlier), lists)
+    ops.tables_trim(t, everyone, base.i32(earlier))
+    ws = ops.tree_workspace(q_heads=H, kv_heads=G, head_dim=d)
+
+    def run(li, requests):
+        out, mask = torch.full((T, H * d), 7.0, dtype=torch.bfloat16, device="cuda"), torch.zeros(T, 1, dtype=torch.int64, device="cuda")
+        path, counts, following, dropped = (torch.full(s, 9, dtype=torch.int32, device="cuda") for s in ((requests, 6), (requests,), (requests,), (requests,)))
+        cache, status = pool.clone(), ops.new_status()
+        ops.tables_grow(t, everyone[:R], base.i32(step), li, status=status)
+        ops.tree_masks(parents, li.qo_indptr, mask, positions=li.positions, status=status)
+        ops.attn_tree(q, out, cache, li.qo_indptr, li.kv_indptr, li.kv_indices, li.kv_last_page_len, mask, q_heads=H, workspace=ws, status=status)
+        ops.tree_accept(tokens, parents, targets, li.qo_indptr, path, counts, following, dropped=dropped, status=status)
+        ops.kv_keep([cache], li.slots, path, counts, li.qo_indptr, status=status)
+        ops.tables_trim(t, everyone[:R], base.i32(step), status=status)
+        torch.cuda.synchronize()
+        return [out, mask, li.positions.clone(), cache, path[:R], counts[:R], following[:R], dropped[:R]], [path[R:], counts[R:], following[R:], dropped[R:]], status
+
+    fitting, _, status = run(ops.batch_lists(R, T, pages), R)
+    ops.check_status(status)
+    same, behind, status = run(lists, C)
+    n = sum(step)
+    assert (fitting[0][n:] == 7).all() and (n == 0 or not (fitting[0][:n] == 7).all())
+    assert lists.qo_indptr[R:].tolist() == [n] * (C + 1 - R)
+    assert lists.kv_indptr[R:].tolist() == [int(lists.kv_indptr[R])] * (C + 1 - R) and not lists.kv_last_page_len[R:].any()
+    for a, b in zip(fitting, same):
+        assert torch.equal(a, b)
+    ops.check_status(status)
+    assert [x.unique().tolist() for x in behind] == [[-1], [0], [-1], [0]]
+
+
+def test_lists_of_a_step_that_does_not_fit_are_empty_to_their_ends():
+    t, _ = base._tables(6, 20, 90, [0, 15, 16, 100, 31, 64])
+    lists = ops.batch_lists(6, 40, 40)
+    ops.tables_grow(t, base.i32([0, 1, 2, 3, 4, 5]), base.i32([3] * 6), lists)
+    status = ops.new_status()
+    ops.tables_grow(t, base.i32([2, 2]), base.i32([1, 1]), lists, status=status)
+    with pytest.raises(RuntimeError, match="index"):
+        ops.check_status(status)
+    assert not any(x.any() for x in (lists.qo_indptr, lists.kv_indptr, lists.kv_last_page_len, lists.positions)) and (lists.slots == -1).all()
