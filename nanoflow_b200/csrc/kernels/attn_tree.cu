@@ -722,6 +722,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             }
             l *= alpha;
             if (grow) ref = mx;
+            tmem_st_wait();                      // (the weights go over those of the first pass: two stores have no order of their own)
           }
           if (!ok) break;
           l += sum;

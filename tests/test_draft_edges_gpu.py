@@ -95,3 +95,27 @@ def test_lists_of_a_step_that_does_not_fit_are_empty_to_their_ends():
     with pytest.raises(RuntimeError, match="index"):
         ops.check_status(status)
     assert not any(x.any() for x in (lists.qo_indptr, lists.kv_indptr, lists.kv_last_page_len, lists.positions)) and (lists.slots == -1).all()
+
+
+# ---- scores ---------------------------------------------------------------------------------------------------------------------
+SHAPES = [([900, 40, 2000], [20, 33, 64], 8, 2, 128), ([700, 64], [40, 64], 64, 8, 128), ([900, 2, 300], [20, 1, 130], 8, 2, 64)]
+
+
+@pytest.mark.parametrize("lengths,nodes,H,G,d", SHAPES)
+def test_scores_that_grow_from_tile_to_tile(lengths, nodes, H, G, d):
+    """The reference moves in every tile, and each tile's weights are formed twice: the same result in every run. (Scores of a tile's best
+    tokens are above those of the tiles in front by some 2^4 or more.)"""
+    b = base._batch(25, lengths, nodes, H, G, d)
+    b["q"].abs_()
+    for r, n in enumerate(lengths):
+        first = int(b["kv_indptr"][r])
+        pages = b["kv_indices"][first:int(b["kv_indptr"][r + 1])].long()
+        b["kv_pool"][pages, 0] = (b["kv_pool"][pages, 0].float() * 0.1 + torch.arange(len(pages), device="cuda")[:, None, None, None] * (20.0 / d)).to(torch.bfloat16)
+    want, size = base._want(b)
+    first = ops.attn_tree(**b).clone()
+    # sum |q k| scale is below 250 here, so that scores are off by 2^-24 128 250 < 2^-9, and weights and their sum by as much each
+    got = first.double().cpu().reshape(want.shape)
+    assert ((got - want).abs() <= want.abs() * 2.0 ** -8 + size * (2.0 ** -8 + 2.0 ** -10 + 2.0 ** -8)).all()
+    for _ in range(20):
+        b["out"].fill_(7)
+        assert torch.equal(ops.attn_tree(**b), first)
