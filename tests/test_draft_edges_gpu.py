@@ -119,3 +119,57 @@ def test_scores_that_grow_from_tile_to_tile(lengths, nodes, H, G, d):
     for _ in range(20):
         b["out"].fill_(7)
         assert torch.equal(ops.attn_tree(**b), first)
+
+
+def _whole(b, seed, most=3):
+    """Queries and keys of small whole numbers: their products are exact in fp32, scores differ by the scale or not at all."""
+    g = base.gen(seed)
+    b["q"].copy_(torch.randint(-most, most + 1, b["q"].shape, generator=g, device="cuda"))
+    b["kv_pool"][:, 0] = torch.randint(-most, most + 1, b["kv_pool"][:, 0].shape, generator=g, device="cuda").to(torch.bfloat16)
+    return b
+
+
+@pytest.mark.parametrize("sm_scale", [1e3, 3e7, 1e8, 1e9, 3e9, 1e10, 1e12, 1e20, 1e35])
+@pytest.mark.parametrize("lengths,nodes,H,G,d", SHAPES)
+@pytest.mark.parametrize("num_ctas", [0, 1])
+def test_rows_of_large_scores(lengths, nodes, H, G, d, sm_scale, num_ctas):
+    """Rows are the mean of the values with the largest score, in items of one piece (a single CTA) and in cut ones. Scores are below 3.4e38 /
+    log2(e): products are at most 9 d."""
+    b = _whole(base._batch(21, lengths, nodes, H, G, d), 5)
+    ops.attn_tree(**b, sm_scale=sm_scale, num_ctas=num_ctas)
+    base._near(b["out"], *base._want(b, sm_scale))
+
+
+@pytest.mark.parametrize("lengths,nodes,H,G,d", SHAPES)
+def test_rows_of_scores_far_below_zero(lengths, nodes, H, G, d):
+    b = _whole(base._batch(22, lengths, nodes, H, G, d), 6)
+    b["q"].abs_()
+    b["kv_pool"][:, 0] = -b["kv_pool"][:, 0].abs()
+    b["kv_pool"][:, 0, :, :, 0], b["q"][:, ::d] = -1, 1            # (none is zero)
+    ops.attn_tree(**b, sm_scale=1e11)
+    base._near(b["out"], *base._want(b, 1e11))
+
+
+@pytest.mark.parametrize("lengths,nodes,H,G,d", SHAPES)
+@pytest.mark.parametrize("num_ctas", [0, 1])
+def test_rows_of_small_and_large_scores_side_by_side(lengths, nodes, H, G, d, num_ctas):
+    """Rows whose scores go from some ten to 1e32, neighbours of one warp among them. Powers of two leave the products exact; where scores of a
+    row are some 2^k apart at least (k from 8 on), weights are those of ties; below, scores of 3000 at most are off by 2^-24 of themselves."""
+    b = _whole(base._batch(23, lengths, nodes, H, G, d), 7)
+    T = sum(nodes)
+    k = torch.tensor([0, 2, 8, 16, 19, 20, 21, 22, 24, 30, 40, 60, 100], device="cuda")
+    rows = b["q"].view(T, H, d)
+    rows *= (2.0 ** k[(torch.arange(T, device="cuda")[:, None] * 5 + torch.arange(H, device="cuda")) % len(k)])[..., None].to(torch.bfloat16)
+    ops.attn_tree(**b, sm_scale=0.125, num_ctas=num_ctas)
+    base._near(b["out"], *base._want(b, 0.125))
+
+
+def test_sums_of_the_largest_values_with_large_scores_stay_finite():
+    """Scores of 1e8 to 1e12 that are all the same, values of 2^127: the mean is as large, the sum of 3000 of them fp32 does not hold."""
+    for scale in (1e6, 1e8, 3e8, 1e9, 1e12):
+        b = base._batch(24, [3000, 70], [20, 30], 8, 2, 128)
+        b["q"].fill_(1)
+        b["kv_pool"][:, 0] = 1
+        b["kv_pool"][:, 1] = 2.0 ** 127
+        ops.attn_tree(**b, sm_scale=scale)
+        base._near(b["out"], *base._want(b, scale))
