@@ -341,6 +341,7 @@ PyObject* keep(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const Pool d = bf16_pool(what, items[i], true);
       if (d.pool.sizes() != c.pool.sizes() || d.pool.device() != device) refuse(what, "pools must be of one size, on one device");
       const char* at = static_cast<const char*>(d.pool.data_ptr());
+      if ((reinterpret_cast<uintptr_t>(at) & 15) != 0) refuse(what, "pools must begin at 16 bytes");       // (before the first launch)
       spans.emplace_back(at, at + d.pool.nbytes());
     }
     const Tensor& slots = int32(what, "slots", a[1], device);

@@ -173,3 +173,14 @@ def test_sums_of_the_largest_values_with_large_scores_stay_finite():
         b["kv_pool"][:, 1] = 2.0 ** 127
         ops.attn_tree(**b, sm_scale=scale)
         base._near(b["out"], *base._want(b, scale))
+
+
+def test_a_pool_that_is_not_aligned_is_refused_before_anything_moves():
+    """The last of more pools than a launch takes."""
+    pools = [base.normal(base.gen(k), 1, 2, 1, 16, 64) for k in range(64)]
+    pools.append(torch.zeros(2049, dtype=torch.bfloat16, device="cuda")[1:].view(1, 2, 1, 16, 64))
+    before = [p.clone() for p in pools]
+    with pytest.raises(RuntimeError, match="kv_keep"):
+        ops.kv_keep(pools, base.i32([0, 1, 2]), base.i32([[0, 2, -1]]), base.i32([2]), base.i32([0, 3]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(before, pools))
