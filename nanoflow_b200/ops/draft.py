@@ -162,12 +162,12 @@ def rope_frequencies(rot_dim: int, theta: float, scaling: Optional[dict] = None,
                      max_position: Optional[int] = None, device="cuda") -> Tuple[torch.Tensor, float]:
     """Inverse frequencies (fp32 ``[rot_dim / 2]``) and the factor of cosines and sines for :func:`rope_append_slots`, from a model's
     configuration (``rope_scaling`` of its config.json). Types: none, ``linear``, ``dynamic`` (by ``length``, above ``max_position``), ``llama3``,
-    ``yarn``, ``longrope`` (short or long factors by ``length``)."""
+    ``yarn``, ``longrope`` (short or long factors by ``length``). An entry that is None is as if it were not there."""
     if rot_dim < 2 or rot_dim % 2:
         raise RuntimeError("rope_frequencies: rot_dim must be even")
     if not theta > 1:
         raise RuntimeError("rope_frequencies: theta must be above 1")
-    scaling = scaling or {}
+    scaling = {name: value for name, value in (scaling or {}).items() if value is not None}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
     i = torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim
     inv, out = theta ** -i, 1.0
@@ -181,12 +181,19 @@ def rope_frequencies(rot_dim: int, theta: float, scaling: Optional[dict] = None,
     for name in needed.get(kind, ()):
         if name not in scaling:
             raise RuntimeError(f"rope_frequencies: {kind} needs {name}")
-    if scaling.get("factor") is not None and not float(scaling["factor"]) > 0:
-        raise RuntimeError("rope_frequencies: factor must be positive")
+    sizes = dict(scaling, max_position=max_position)
+    for name in ("factor", "low_freq_factor", "high_freq_factor", "original_max_position_embeddings", "max_position", "beta_fast", "beta_slow"):
+        absent = (None,) if name in ("factor", "low_freq_factor", "high_freq_factor") else (None, 0)
+        if sizes.get(name) not in absent and not 0 < float(sizes[name]) < math.inf:
+            raise RuntimeError(f"rope_frequencies: {name} must be positive")
+    if kind == "llama3" and not float(scaling.get("low_freq_factor", 1)) < float(scaling.get("high_freq_factor", 4)):
+        raise RuntimeError("rope_frequencies: low_freq_factor must be below high_freq_factor")
     if kind == "dynamic" and rot_dim == 2:
         raise RuntimeError("rope_frequencies: dynamic has no form for a single pair")
     if kind == "longrope" and not len(scaling["short_factor"]) == len(scaling["long_factor"]) == rot_dim // 2:
         raise RuntimeError("rope_frequencies: longrope needs a factor for each pair")
+    if kind == "longrope" and not (all(0 < float(f) < math.inf for f in (*scaling["short_factor"], *scaling["long_factor"])) and original > 1):
+        raise RuntimeError("rope_frequencies: longrope's factors must be positive, and its original length above 1")
     if kind == "linear":
         inv = inv / float(scaling["factor"])
     elif kind == "dynamic":

@@ -41,3 +41,30 @@ def test_trees_of_more_than_a_step_leaves_room_for_are_refused(entries):
 @pytest.mark.parametrize("field", ["num_qo", "num_kv", "num_last"])
 def test_lists_of_requests_without_room_for_a_step_are_refused(field):
     test_lists_of_tables_without_room_for_a_step_are_refused(field, MOST + 1)
+
+
+# ---- frequencies: entries of a configuration that are null, or none that a rotation has ------------------------------------------------
+@pytest.mark.parametrize("scaling,more", [
+    ({"rope_type": "linear", "factor": None}, {}), ({"rope_type": "dynamic", "factor": None}, {"max_position": 4096}), ({"rope_type": "llama3", "factor": None}, {}),
+    ({"rope_type": "yarn", "factor": None, "original_max_position_embeddings": 4096}, {}),
+    ({"rope_type": "longrope", "short_factor": None, "long_factor": [1.0] * 32}, {"max_position": 4096}),
+    ({"rope_type": "longrope", "short_factor": [1.0] * 31 + [0.0], "long_factor": [1.0] * 32}, {"max_position": 4096}),
+    ({"rope_type": "longrope", "short_factor": [1.0] * 32, "long_factor": [1.0] * 32, "original_max_position_embeddings": 1}, {"max_position": 4096}),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 4.0, "high_freq_factor": 4.0}, {}),
+    ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": 0.0}, {}), ({"rope_type": "llama3", "factor": 8.0, "original_max_position_embeddings": -1}, {}),
+    ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": 4096, "beta_fast": -32}, {}),
+    ({"rope_type": "yarn", "factor": 4.0, "original_max_position_embeddings": -4096}, {}), ({"rope_type": "linear", "factor": float("nan")}, {}),
+    ({"rope_type": "linear", "factor": float("inf")}, {}), ({"rope_type": "dynamic", "factor": 2.0}, {"max_position": -5})])
+def test_frequencies_refuse_what_is_none(scaling, more):
+    with pytest.raises(RuntimeError, match="rope_frequencies"):
+        ops.rope_frequencies(64, 10000.0, scaling, device="cpu", **more)
+
+
+def test_frequencies_take_null_for_what_has_a_default():
+    for null, plain in (({"rope_type": None}, {}), ({"rope_type": None, "type": "linear", "factor": 2.0}, {"type": "linear", "factor": 2.0}),
+                        ({"rope_type": "llama3", "factor": 8.0, "low_freq_factor": None, "high_freq_factor": None, "original_max_position_embeddings": None},
+                         {"rope_type": "llama3", "factor": 8.0}),
+                        ({"rope_type": "yarn", "factor": None, "original_max_position_embeddings": 1024, "attention_factor": None, "beta_fast": None, "truncate": None},
+                         {"rope_type": "yarn", "original_max_position_embeddings": 1024})):
+        a, b = (ops.rope_frequencies(64, 10000.0, s, max_position=4096, device="cpu") for s in (null, plain))
+        assert a[0].tolist() == b[0].tolist() and a[1] == b[1]
