@@ -72,10 +72,12 @@ const Tensor* status_word(const char* what, PyObject* o, c10::Device device) {
 }
 unsigned int* word(const Tensor* t) { return t == nullptr ? nullptr : static_cast<unsigned int*>(t->data_ptr()); }
 
-// What a kernel writes must not lie over anything else that it reads or writes. (Null: a tensor that the call goes without.)
+// What a kernel writes must not lie over anything else that it reads or writes. (Null: a tensor that the call goes without.) Rows at the same
+// distance may lie between each other: columns of one buffer.
 void apart(const char* what, std::initializer_list<const Tensor*> written, std::initializer_list<const Tensor*> read) {
   struct Span {
     const char *begin, *end;
+    int64_t row, distance;                       // bytes of a row, and from row to row; 0: no rows
   } spans[16];
   int n = 0, n_written = 0;
   const auto add = [&](const Tensor* t) {
@@ -83,7 +85,14 @@ void apart(const char* what, std::initializer_list<const Tensor*> written, std::
     int64_t last = 0;
     for (int64_t d = 0; d < t->dim(); ++d) last += (t->size(d) - 1) * t->stride(d);
     const char* begin = static_cast<const char*>(t->data_ptr());
-    spans[n++] = Span{begin, begin + (last + 1) * t->element_size()};
+    const int64_t bytes = t->element_size();
+    const bool rows = t->dim() == 2 && t->size(0) > 1 && (t->size(1) == 1 || t->stride(1) == 1) && t->stride(0) >= t->size(1);
+    spans[n++] = Span{begin, begin + (last + 1) * bytes, rows ? t->size(1) * bytes : 0, rows ? t->stride(0) * bytes : 0};
+  };
+  const auto between = [](const Span& a, const Span& b) {        // whether b's rows lie behind a's in the same columns of bytes
+    if (a.distance == 0 || a.distance != b.distance) return false;
+    const int64_t off = ((b.begin - a.begin) % a.distance + a.distance) % a.distance;
+    return off >= a.row && off + b.row <= a.distance;
   };
   if (written.size() + read.size() > 16) refuse(what, "too many tensors");
   for (const Tensor* t : written) add(t);
@@ -91,7 +100,7 @@ void apart(const char* what, std::initializer_list<const Tensor*> written, std::
   for (const Tensor* t : read) add(t);
   for (int i = 0; i < n_written; ++i)
     for (int j = i + 1; j < n; ++j)
-      if (spans[i].begin < spans[j].end && spans[j].begin < spans[i].end) refuse(what, "tensors overlap, and one of them is written");
+      if (spans[i].begin < spans[j].end && spans[j].begin < spans[i].end && !between(spans[i], spans[j])) refuse(what, "tensors overlap, and one of them is written");
 }
 
 template <class P>

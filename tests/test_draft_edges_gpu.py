@@ -184,3 +184,23 @@ def test_a_pool_that_is_not_aligned_is_refused_before_anything_moves():
         ops.kv_keep(pools, base.i32([0, 1, 2]), base.i32([[0, 2, -1]]), base.i32([2]), base.i32([0, 3]))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(before, pools))
+
+
+# ---- columns of one buffer ------------------------------------------------------------------------------------------------------
+def test_rows_that_lie_between_other_rows():
+    """Queries and outputs as columns of one buffer do not overlap; columns that both have do."""
+    b = base._batch(6, [100, 600], [7, 40], 8, 2, 128)
+    plain = ops.attn_tree(**b).clone()
+    row = 1024
+    for q_at, out_at in ((0, row), (row + 8, 0), (8, row + 16)):
+        wide = torch.full((47, 2 * row + 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        wide[:, q_at:q_at + row] = b["q"]
+        before = wide.clone()
+        ops.attn_tree(**{**b, "q": wide[:, q_at:q_at + row], "out": wide[:, out_at:out_at + row]})
+        before[:, out_at:out_at + row] = plain
+        assert torch.equal(wide, before)
+    wide = torch.zeros(48, 2 * row + 64, dtype=torch.bfloat16, device="cuda")
+    for q, out in ((wide[:47, :row], wide[:47, row - 8:2 * row - 8]), (wide[:47, 8:row + 8], wide[:47, :row]), (wide[:47, :row], wide[1:, :row]),
+                   (wide[:47, row + 64:], wide[1:, 80:row + 80]), (wide[:47, :row], wide.view(-1)[row:row + 47 * row].view(47, row))):
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.attn_tree(**{**b, "q": q, "out": out})
