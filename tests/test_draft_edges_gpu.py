@@ -204,3 +204,34 @@ def test_rows_that_lie_between_other_rows():
                    (wide[:47, row + 64:], wide[1:, 80:row + 80]), (wide[:47, :row], wide.view(-1)[row:row + 47 * row].view(47, row))):
         with pytest.raises(RuntimeError, match="overlap"):
             ops.attn_tree(**{**b, "q": q, "out": out})
+
+
+# ---- lists and paths that are partly none -----------------------------------------------------------------------------------------
+def test_rows_of_lists_that_are_partly_none():
+    """Query lists: requests beside the one that is none keep their rows, and rows of nobody are left as they were."""
+    good = base._batch(11, [100, 50, 70], [5, 6, 7], 8, 2, 128)
+    want, size = base._want(good)
+    for at, value, right in ((1, 100, slice(11, 18)), (1, -1, slice(11, 18)), (3, 10 ** 9, slice(0, 11)), (3, 10, slice(0, 11))):
+        b = {k: (v.clone() if isinstance(v, torch.Tensor) else v) for k, v in good.items()}
+        b["qo_indptr"][at] = value
+        status = ops.new_status()
+        ops.attn_tree(**b, status=status)
+        with pytest.raises(RuntimeError, match="index"):
+            ops.check_status(status)
+        base._near(b["out"], want, size, right)
+        rest = torch.ones(18, dtype=torch.bool, device="cuda")
+        rest[right] = False
+        assert (b["out"][rest] == 7).all()
+
+
+@pytest.mark.parametrize("path,counts,slots,moved", [([0, 0, 3, -1], 3, [0, 1, 2, 3], {2: 3}), ([0, 2, 5, 3], 4, [0, 1, 2, 3], {1: 2}),
+                                                     ([0, 2, 3, -1], 3, [0, 77, 2, 3], {2: 3}), ([0, -1, 3, 3], 4, [4, 5, 6, 7], {6: 7})])
+def test_moves_beside_one_that_is_none_are_made(path, counts, slots, moved):
+    pool = base.normal(base.gen(3), 1, 2, 1, 16, 64)
+    want, status = pool.clone(), ops.new_status()
+    for to, source in moved.items():
+        want[0, :, :, to] = pool[0, :, :, source]
+    ops.kv_keep([pool], base.i32(slots), base.i32([path]), base.i32([counts]), base.i32([0, 4]), status=status)
+    with pytest.raises(RuntimeError, match="index"):
+        ops.check_status(status)
+    assert torch.equal(pool, want)
