@@ -17,9 +17,9 @@ namespace {
 
 constexpr int kPage = 16;
 constexpr int kMostThreads = 1024, kMine = NFK_TABLES_REQUESTS / kMostThreads;   // requests of a thread at most
-// Threads of a CTA: barriers of many take longer, and few requests need no more (256 requests 10.2 us, with 1024 threads 11.3; 512 requests
-// the other way, 16.8, with 256 threads 20.3).
-constexpr int kFewThreads = 256;
+// Threads of a CTA: barriers of many take longer, and up to three requests a thread cost less (growth and the way back: 256 requests 11.1 us,
+// with 1024 threads 13.0; 512 11.7 and 13.0; 768 13.1 and 13.6; with a fourth it is the other way: 800 13.8, with 256 threads 14.5).
+constexpr int kFewThreads = 256, kFewRequests = 3 * kFewThreads;
 // entries of the lists that a thread writes before there are further CTAs
 constexpr int kPerThread = 2;
 
@@ -265,7 +265,7 @@ int launch(const nfk_tables_params& p, long long entries, cudaStream_t stream) {
     }
     attr = true;
   }
-  const int threads = p.requests <= kFewThreads ? kFewThreads : kMostThreads;
+  const int threads = p.requests <= kFewRequests ? kFewThreads : kMostThreads;
   long long ctas = (entries + threads * kPerThread - 1) / (threads * kPerThread);
   if (ctas > device_sm_count()) ctas = device_sm_count();
   if (ctas < 1) ctas = 1;

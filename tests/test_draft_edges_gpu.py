@@ -235,3 +235,9 @@ def test_moves_beside_one_that_is_none_are_made(path, counts, slots, moved):
     with pytest.raises(RuntimeError, match="index"):
         ops.check_status(status)
     assert torch.equal(pool, want)
+
+
+# ---- tables where the number of threads changes ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("R", [256, 257, 300, 512, 767, 768, 769, 800])
+def test_tables_of_some_hundred_requests(R):
+    base.test_grow_and_trim(R, 0, 90, 20, 3)
