@@ -193,9 +193,9 @@ PyObject* rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // q, out, kv_pool, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tree, q_heads, req_begin, req_count, sm_scale, num_ctas, workspace,
-// status, early_start
+// status, early_start, request_tokens
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 16, [&] {
+  return guarded(n, 17, [&] {
     const char* what = "attn_tree";
     const Pool c = bf16_pool(what, a[2]);
     const c10::Device device = c.pool.device();
@@ -253,6 +253,8 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.workspace_bytes = workspace.numel();
     p.status = word(status);
     p.early_start = whole(a[15], what, "early_start");
+    p.request_tokens = whole(a[16], what, "request_tokens");
+    p.listed = count(what, last, "kv_last_page_len");
     if (p.req_count > 0 && p.num_tokens > 0) launch("nfk_attn_tree", entries.attend, p, device);
   });
 }

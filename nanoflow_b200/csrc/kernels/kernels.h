@@ -382,6 +382,8 @@ typedef struct nfk_attn_tree_params {
   void* workspace;           // nfk_attn_tree_workspace bytes at 256, whatever they hold; calls that may run at the same time each
   long long workspace_bytes; // need their own
   unsigned int* status;
+  int request_tokens;        // query tokens of a request, about: chooses between forms. 0: rows of q for each of the `listed` requests
+  int listed;                // requests whose rows q has (0: req_count)
 } nfk_attn_tree_params;
 long long nfk_attn_tree_workspace(const nfk_attn_tree_params* p);   // by head_dim; 0: unsupported
 int nfk_attn_tree(const nfk_attn_tree_params* p, cudaStream_t stream);

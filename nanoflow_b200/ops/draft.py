@@ -57,7 +57,7 @@ class AttnTreeParams(Structure):
                 ("kv_indptr", c_void_p), ("kv_indices", c_void_p), ("kv_last_page_len", c_void_p), ("tree", c_void_p), ("q_heads", c_int),
                 ("kv_heads", c_int), ("head_dim", c_int), ("num_pages", c_int), ("num_tokens", c_int), ("num_indices", c_int),
                 ("req_begin", c_int), ("req_count", c_int), ("words", c_int), ("sm_scale", c_float), ("num_ctas", c_int), ("early_start", c_int),
-                ("workspace", c_void_p), ("workspace_bytes", c_longlong), ("status", c_void_p)]
+                ("workspace", c_void_p), ("workspace_bytes", c_longlong), ("status", c_void_p), ("request_tokens", c_int), ("listed", c_int)]
 
 
 class TreeMasksParams(Structure):
@@ -264,8 +264,8 @@ def tree_workspace(*, q_heads: int, kv_heads: int, head_dim: int, device="cuda")
 
 def attn_tree(q: torch.Tensor, out: torch.Tensor, kv_pool: torch.Tensor, qo_indptr: torch.Tensor, kv_indptr: torch.Tensor, kv_indices: torch.Tensor,
               kv_last_page_len: torch.Tensor, tree: Optional[torch.Tensor] = None, *, q_heads: int, workspace: torch.Tensor, req_begin: int = 0,
-              req_count: Optional[int] = None, sm_scale: Optional[float] = None, num_ctas: int = 0, status: Optional[torch.Tensor] = None,
-              early_start: int = EARLY_FIRST | EARLY_FURTHER) -> torch.Tensor:
+              req_count: Optional[int] = None, sm_scale: Optional[float] = None, num_ctas: int = 0, request_tokens: int = 0,
+              status: Optional[torch.Tensor] = None, early_start: int = EARLY_FIRST | EARLY_FURTHER) -> torch.Tensor:
     """Attention of the n_r query tokens of each request over its cached tokens, of which the last n_r are the query tokens themselves: all
     of them see what is cached in front, and token i sees token j of the request where bit j of ``tree`` (int64 ``[tokens, words]``, up to 8
     words, the row of token i) is set. ``tree=None``: a chain, i sees j up to itself.
@@ -276,9 +276,18 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, kv_pool: torch.Tensor, qo_indp
     reach it. Results do not depend on what else runs, or on the workspace's contents; they may differ in their last bits between batches.
 
     Reported in ``status``: page numbers that are none (page 0 is read instead), lists that are none (no rows, or rows of zeros), fewer
-    cached than query tokens (rows of zeros). ``workspace``: :func:`tree_workspace`. ``num_ctas``: CTA budget of each kernel."""
+    cached than query tokens (rows of zeros). ``workspace``: :func:`tree_workspace`. ``num_ctas``: CTA budget of each kernel.
+
+    ``request_tokens``: about how many query tokens a request has, for the choice between the forms for few and for many rows (any number
+    gives right results). 0: the rows of ``q`` for each listed request, which is too many where ``q`` has room for more than a step brings, as in
+    a captured graph: there short requests take up to a quarter longer.
+
+    Chains can also be run by :func:`nanoflow_b200.ops.attn_prefill`, where the host knows the tokens of each request and cuts them into items. With 32 query
+    and 8 KV heads of 128 that is the faster one for many requests of 16 tokens and more, or little in front (32 requests of 64 behind 4000:
+    157 us and 165; 4 of 512 with nothing in front: 25 and 67), and this one for few requests with long contexts, which it cuts (one of 60 behind
+    100000: 120 us and 1460; one of 26 behind 2000: 16 and 31)."""
     _calls().attend(q, out, kv_pool, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tree, q_heads, req_begin, req_count, sm_scale, num_ctas,
-                    workspace, status, early_start)
+                    workspace, status, early_start, request_tokens)
     return out
 
 

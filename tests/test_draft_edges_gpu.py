@@ -241,3 +241,34 @@ def test_moves_beside_one_that_is_none_are_made(path, counts, slots, moved):
 @pytest.mark.parametrize("R", [256, 257, 300, 512, 767, 768, 769, 800])
 def test_tables_of_some_hundred_requests(R):
     base.test_grow_and_trim(R, 0, 90, 20, 3)
+
+
+# ---- how many tokens a request has, as far as the host knows -----------------------------------------------------------------------
+@pytest.mark.parametrize("H,G,d", [(32, 8, 128), (24, 8, 64)])
+def test_rows_of_padding_and_of_other_requests_do_not_choose_the_form(H, G, d):
+    """Short chains in queries with room for 64 tokens each: with request_tokens, the bits of the call whose queries fit. A part of a batch takes
+    the batch's form."""
+    nodes = [5, 3, 1, 4] * 5
+    b = base._batch(41, [600 + 40 * k for k in range(20)], nodes, H, G, d)
+    T = sum(nodes)
+    fitting = ops.attn_tree(**b).clone()
+    q, out = (torch.full((20 * 64, H * d), 7.0, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    q[:T] = b["q"]
+    tree = torch.zeros(20 * 64, 1, dtype=torch.int64, device="cuda")
+    tree[:T] = b["tree"]
+    padded = {**b, "q": q, "out": out, "tree": tree}
+    assert torch.equal(ops.attn_tree(**padded, request_tokens=5)[:T], fitting) and (out[T:] == 7).all()
+    want, size = base._want(b)
+    for tokens in (0, 1, 64, 2 ** 31 - 1):
+        base._near(ops.attn_tree(**padded, request_tokens=tokens)[:T], want, size)
+    part = ops.attn_tree(**b, req_begin=3, req_count=2, request_tokens=5).clone()
+    assert torch.equal(ops.attn_tree(**b, req_begin=3, req_count=2), part)
+    a, e = sum(nodes[:3]), sum(nodes[:5])
+    base._near(part[a:e], want[a:e], size[a:e])
+
+
+def test_a_number_of_tokens_that_is_none_is_refused():
+    b = base._batch(1, [40, 20], [3, 2], 4, 2, 64)
+    for bad in (-1, 2 ** 31, 1.5):
+        with pytest.raises(RuntimeError, match="attn_tree|bad argument"):
+            ops.attn_tree(**b, request_tokens=bad)
