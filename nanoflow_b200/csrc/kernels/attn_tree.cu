@@ -857,7 +857,9 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 }
 
 // Rows of items that were cut: LANES lanes each, over its pieces for the weights and over head_dim, a float4 or two a lane, for the sums.
-constexpr int kJoinWarps = 8, kJoinPerSm = 4, kMostCtas = 2 * kJoinWarps * 32;
+// Three CTAs to an SM: with four, at 64 registers, rows on their way spill (1 request of 26 tokens behind 2000 15.4 us and 16.0, 32 x 64 281 and
+// 284, 64 x 128 rows 84.7 and 86.4).
+constexpr int kJoinWarps = 8, kJoinPerSm = 3, kMostCtas = 2 * kJoinWarps * 32;
 template <int HD, int SLOTS, int LANES, int AHEAD>         // AHEAD: pieces on their way at once
 __device__ __forceinline__ void join_rows(const nfk_attn_tree_params& p, const Workspace& ws, const int4* record_s, const int* rows_s, int total, int warp, int lane) {
   constexpr int V = HD / 4 / LANES, ROWS = 32 / LANES;
