@@ -3,8 +3,9 @@
 //
 // The rows of an item are those query rows of a request that share a KV head (tokens x group), in blocks of 128 (one slot) or of up to 256
 // (two). Every key and value is read once per block, 4 head_dim operations a row for 4 head_dim bytes: the cache's bytes bound it below some
-// 250 rows, the products above. In between and beyond, what a tile waits for is what counts: scores, their 2^x (16 a clock and SM, which
-// takes as long as both products at their full rate), weights, sums follow one another, and no stage of it is ever the only one.
+// 250 rows, the products above. In between and beyond, what a tile waits for is what counts: scores, their 2^x (16 a clock and SM: 1024
+// clocks for a tile of 256 rows, where both products take 1430 at the measured rate), weights, sums follow one another, and no stage of it
+// is ever the only one.
 //
 // Tiles are of 64 tokens, and a slot has two buffers of scores in tensor memory: the next tile's scores are formed while the softmax goes
 // through this one's. Weights (bf16 pairs) go over the scores that they come from and are the second product's A operand from there.
@@ -30,10 +31,10 @@
 // further tile is looked for only where its weights' sum reaches 2^14 of the first one's largest, and the reference moves (sums are rescaled,
 // the tile's weights formed anew) where that score is above it by 2^8 or more: 286 us instead of 296 with a search in every tile.
 //
-// Measured (32 query and 8 KV heads of 128, a launch of both kernels in a graph): 64 requests of 5 tokens behind up to 4000 70 us (5.2 TB/s),
-// 256 single tokens behind up to 2000 147 us (5.9 TB/s), one of 60 behind 100000 115 us; with 64 query heads 32 of 64 tokens behind up to
-// 8000 280 us (0.87 PFLOP/s; for seconds 326, at the power cap and 1610 MHz); one of 26 behind 2000 15 us, which is two launches, the scan
-// of the lists and a few tiles' way through all of it.
+// Measured (32 query and 8 KV heads of 128, a launch of both kernels in a graph): 64 requests of 5 tokens behind up to 4000 68 us (5.3 TB/s),
+// 256 single tokens behind up to 2000 146 us (5.9 TB/s), one of 60 behind 100000 116 to 122 us; with 64 query heads 32 of 64 tokens behind
+// up to 8000 281 us (0.89 PFLOP/s; for seconds 333, at the power cap and 1590 MHz); one of 26 behind 2000 14.4 us, which is two launches, the
+// scan of the lists and a few tiles' way through all of it.
 //
 // Only tiles with drafted tokens or the end of a piece need care: masks of 64 bits a row; and values that a row does not see must not
 // reach it as 0 * inf, so rows of values behind the end become zeros, as do infinities and NaN of drafted tokens, which the rows that do
@@ -610,8 +611,9 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int node = f.node + node_in, ctx = f.len - f.all;
       const uint32_t* tree = p.tree == nullptr ? nullptr : reinterpret_cast<const uint32_t*>(p.tree + static_cast<long long>(f.tok + (on ? node_in : 0)) * p.words);
       const int end = min(f.len, (f.page0 + f.pages) * kPage);           // of the piece's tokens
-      // The exponent of a weight is product * row_scale + less, which are formed where the reference moves: 32 x 64 tokens 289 us, with both
-      // formed in every tile 292, with the difference of two products taken first and the scale behind it 296, without shrink 281.
+      // The exponent of a weight is product * row_scale + less, which are formed where the reference moves (32 x 64 tokens: 3 % more than with
+      // one scale for all rows, that is without shrink; with both formed in every tile 4 %, with the difference of two products taken first
+      // and the scale behind it 5 %).
       float ref = -INFINITY, l = 0.f, row_scale = scale, less = 0.f;
       auto refer = [&](float to) {
         ref = to;

@@ -7,7 +7,7 @@
 // itself, in shared memory, and then writes its share of the lists, an entry's request found by bisection. What the call changes
 // is written by the CTA that is the last to have read it, known by a ticket.
 //
-// A step's growth and the way back together, in a graph: 1 request 6.6 us, 256 of up to 6000 tokens 10.2, 2048 of up to 4000 19.9, of which
+// A step's growth and the way back together, in a graph: 1 request 7.1 us, 512 of up to 6000 tokens 11.7, 2048 of up to 4000 17.9, of which
 // bytes need 0.3: loads of rows, lengths and pages behind one another, the barriers of the scan, eleven steps of bisection.
 #include "common.cuh"
 #include "kernels.h"

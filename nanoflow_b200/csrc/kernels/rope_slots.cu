@@ -4,7 +4,8 @@
 // what lies behind the first 2 pairs elements of a head stays as it is, as do values. All in fp32 from the bf16 inputs, rounded once.
 // Memory-bound: every element is read once and written once. In a graph, heads of 128: 8192 tokens of 32 query and 8 KV heads 36.2 us
 // (201 MB, 5.6 TB/s; floor 30.8), any number of pairs 54, by way of shared memory for each element's partner; 1215 tokens of 64 and 8 heads
-// 12.2 (floor 7.6: a token's CTA has a chain of position, angles and heads to itself, and there is one turn of them); 26 tokens 2.6.
+// 12.3 (floor 7.6: a token's CTA has a chain of position, angles and two batches of heads to itself, and 1215 of them are 31 more than fit
+// the SMs at once); 26 tokens 2.7.
 #include "cache_q8.cuh"
 #include "common.cuh"
 #include "kernels.h"
