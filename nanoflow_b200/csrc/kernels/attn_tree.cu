@@ -1041,19 +1041,20 @@ extern "C" int nfk_attn_tree(const nfk_attn_tree_params* p, cudaStream_t stream)
   if (!p->q || !p->out || !p->kv_pool || !p->qo_indptr || !p->kv_indptr || !p->kv_indices || !p->kv_last_page_len || !p->workspace || off(p->q) ||
       off(p->out) || off(p->kv_pool) || (reinterpret_cast<uintptr_t>(p->workspace) & 255) != 0 || (reinterpret_cast<uintptr_t>(p->tree) & 7) != 0)
     return NF_ERR_BAD_ARG;
-  if (p->num_tokens < 0 || p->request_tokens < 0 || p->listed < 0 || p->num_pages <= 0 || p->num_indices < 0 || p->ld_q % 8 != 0 || p->ld_out % 8 != 0 || p->ld_q < row || p->ld_out < row ||
+  if (p->num_tokens < 0 || p->request_tokens < 0 || p->listed < 0 || p->num_pages <= 0 || p->num_indices < 0 || p->ld_q % 8 != 0 ||
+      p->ld_out % 8 != 0 || p->ld_q < row || p->ld_out < row ||
       p->req_begin > 0x7fffffff - p->req_count || !(p->sm_scale > 0.f) || p->sm_scale > 2e38f ||
       p->ld_q > (1ll << 38) || p->ld_out / 8 > 0xffffffffll / p->num_tokens ||             // (places of output rows: 16 bytes each, in 32 bits)
       p->workspace_bytes < workspace_bytes(p->head_dim) ||
       (p->tree != nullptr && (p->words < 1 || p->words > NFK_TREE_NODES / 64)) ||
       static_cast<long long>(p->num_pages) * 2 * p->kv_heads * kPage > 0x7fff0000ll)
     return NF_ERR_BAD_ARG;
-  // 128 elements a head: two slots to a CTA where requests have more than 128 rows (by request_tokens; without it on average, in which rows
-  // of q that are no request's count as well), since both take every tile that has been read (32 requests of 64 tokens, 512 rows each: 279 us, by two CTAs of a slot 317; one of 240 rows behind 100000 tokens: 115 and 143;
-  // 8 of 160 rows behind 6000: 64.5 and 67.5; short contexts are the other way, 128 of 200 rows behind 350: 118 and 114; requests of one
-  // block of 128 take either form's one slot). 64 elements: always one slot, as its tiles are half as much to read and two CTAs wait less
-  // for one another than two slots (64 requests of 256 rows: 119 us against 135; 32 of 512: 211 and 243; one of 240 behind 100000: 92 and 107).
-  // With few rows it is the other way (128 requests of 20 rows behind 500 tokens 61 us, with two slots 77; 256 of four behind 1000 175 and 190).
+  // 128 elements a head: two slots to a CTA where requests have more than 128 rows (by request_tokens; without it on average, in which rows of
+  // q that are no request's count as well), since both take every tile that has been read: 32 requests of 64 tokens, 512 rows each, 279 us, by
+  // two CTAs of a slot 317; one of 240 rows behind 100000 tokens 115 and 143; 8 of 160 rows behind 6000 64.5 and 67.5. Short contexts are the
+  // other way, 128 of 200 rows behind 350 118 and 114, and so are few rows, 128 requests of 20 rows behind 500 77 and 61, 256 of four behind
+  // 1000 190 and 175. 64 elements: always one slot, as its tiles are half as much to read and two CTAs wait less for one another than two
+  // slots (64 requests of 256 rows: 119 us against 135; 32 of 512: 211 and 243; one of 240 behind 100000: 92 and 107).
   const long long tokens = p->request_tokens > 0 ? p->request_tokens : p->num_tokens;
   const long long requests = p->request_tokens > 0 ? 1 : p->listed > 0 ? p->listed : p->req_count;
   const bool wide = tokens * (p->q_heads / p->kv_heads) > 128 * requests;

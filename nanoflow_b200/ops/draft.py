@@ -154,7 +154,8 @@ def tables_grow(tables: PageTables, rows: torch.Tensor, new_tokens: torch.Tensor
 def tables_trim(tables: PageTables, rows: torch.Tensor, dropped: torch.Tensor, *, status: Optional[torch.Tensor] = None,
                 early_start: int = EARLY_FIRST) -> None:
     """The last ``dropped[i]`` tokens of row ``rows[i]`` go (all of them, if it has fewer), and pages that hold none any more are free
-    again: the first one will be taken first. Refusals as in :func:`tables_grow`."""
+    again: the first one will be taken first. ``dropped`` has an entry per row (a slice, where :func:`tree_accept` wrote one for each place
+    of longer lists). Refusals as in :func:`tables_grow`."""
     _calls().trim(tables.table, tables.lengths, tables.free_pages, tables.free_count, tables.ticket, rows, dropped, status, early_start)
 
 
@@ -282,10 +283,10 @@ def attn_tree(q: torch.Tensor, out: torch.Tensor, kv_pool: torch.Tensor, qo_indp
     gives right results). 0: the rows of ``q`` for each listed request, which is too many where ``q`` has room for more than a step brings, as in
     a captured graph: there short requests take up to a quarter longer.
 
-    Chains can also be run by :func:`nanoflow_b200.ops.attn_prefill`, where the host knows the tokens of each request and cuts them into items. With 32 query
-    and 8 KV heads of 128 that is the faster one for many requests of 16 tokens and more, or little in front (32 requests of 64 behind 4000:
-    157 us and 165; 4 of 512 with nothing in front: 25 and 67), and this one for few requests with long contexts, which it cuts (one of 60 behind
-    100000: 120 us and 1460; one of 26 behind 2000: 16 and 31)."""
+    Chains can also be run by :func:`nanoflow_b200.ops.attn_prefill`, where the host knows the tokens of each request and cuts them into items.
+    With 32 query and 8 KV heads of 128 that is the faster one for many requests of 16 tokens and more, or little in front (32 requests of 64
+    behind 4000: 157 us and 165; 4 of 512 with nothing in front: 25 and 67), and this one for few requests with long contexts, which it cuts (one
+    of 60 behind 100000: 120 us and 1460; one of 26 behind 2000: 16 and 31)."""
     _calls().attend(q, out, kv_pool, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, tree, q_heads, req_begin, req_count, sm_scale, num_ctas,
                     workspace, status, early_start, request_tokens)
     return out
